@@ -706,6 +706,118 @@ int sufb200_beaver_open_pair(const uint64_t* const* d_x, size_t sx, int ldx, con
                              const uint64_t* const* d_c, const uint64_t* r, int heads, int M, int K, int N,
                              uint64_t* d_out, size_t so, int ldo, void* stream);
 
+/* ---- attention over a paged cache of shares (both parties, one GPU) ---------
+ * The decoder's side of the layer: rotary positions, a cache of secret-shared
+ * keys and values in pages, causal attention of packed sequences of any
+ * lengths against it (whole prompts and single tokens, grouped heads), and
+ * the row max of ragged rows.  The reference holds its cache as plain share
+ * tensors per layer (include/nn/kv_cache.hpp) and masks its causal prompt as
+ * ragged rows.
+ *
+ * A cached row X is its opened E = X - B and the dealer's mask B = B_0 + B_1,
+ * which stays with the slot for the row's life (a slot that is written again
+ * needs a freshly dealt mask); pools are [pages][kv_heads][page_size][head_dim]
+ * words, 16-byte aligned, E and the B_p alike.  What multiplies a cached row
+ * is masked afresh in every call.  head_dim is even, 2..256.
+ *
+ * Wrong device-side data (a slot, position, page or length outside what the
+ * host arguments say) is skipped and reported by sufb200_ctx_sync as a bad
+ * argument; the outputs it concerns are then undefined. */
+
+/* New tokens into the cache.  Per token t and head h, with the cosines c and
+ * sines s of its position (tables [max_pos][rot_dim / 2], f = the bundle's
+ * fractional bits), every party rotates its shares,
+ *   (x1, x2) -> (x1 c - x2 s, x2 c + x1 s),
+ * pairs (i, i + rot_dim / 2), or (2i, 2i + 1) with `interleaved`; the opened
+ * sum_p (y_p + r[p]) goes through the GapARS bundle (trunc, with its tables of
+ * sufb200_trunc_tables_dev: floor(y / 2^f) for |y| < 2^62); words from rot_dim
+ * on keep their shares.  Opened results:
+ *   d_dq[t][h]      = sum_p (q'_p - A_p)
+ *   ek[slot][h]     = sum_p (k'_p - bk_p[slot][h])
+ *   ev[slot][h]     = sum_p (v_p - bv_p[slot][h])
+ * slot = page * page_size + place; a token with slot -1 is padding: nothing
+ * of it is written, its row of d_dq neither.  The slots of a call are
+ * distinct.  Shares of (t, h, d) at base + t * ts + h * hs + d.  q_heads = 0
+ * appends only (d_q, d_a, d_dq may be NULL); rot_dim = 0 rotates nothing
+ * (positions, tables and bundle unused).  Asynchronous; one launch. */
+typedef struct sufb200_rope_append {
+  const uint64_t* d_q[2];
+  const uint64_t* d_k[2];
+  const uint64_t* d_v[2];
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs; /* strides in words */
+  const int32_t* d_positions;                 /* [tokens] */
+  const int64_t* d_slots;                     /* [tokens] */
+  const int32_t* d_cos;
+  const int32_t* d_sin;
+  const uint64_t* d_a[2]; /* [tokens][q_heads][head_dim]: shares of the queries' mask A */
+  uint64_t* d_dq;         /* [tokens][q_heads][head_dim] */
+  uint64_t* d_ek;
+  const uint64_t* d_bk[2];
+  uint64_t* d_ev;
+  const uint64_t* d_bv[2];
+  int32_t tokens, q_heads, kv_heads, head_dim, rot_dim, interleaved, max_pos, pages, page_size, reserved;
+  sufb200_trunc_desc trunc[2];
+  const void* d_tables[2]; /* NULL only for a bundle without queries */
+  uint64_t r[2];           /* shares of the bundle's r_in */
+} sufb200_rope_append;
+
+int sufb200_rope_append_pair(sufb200_ctx ctx, const sufb200_rope_append* args, void* stream);
+
+/* The packed sequences of an attention call.  Sequence b has the new tokens
+ * d_cu_q[b] .. d_cu_q[b+1] (cu_q[0] = 0) and d_ctx[b] cached tokens, the new
+ * ones included, in the pages d_block_table[b][j / page_size].  Rows are
+ * packed in (sequence, head, query) order; row (b, h, i) has
+ *   len = causal ? max(0, ctx - n + i + 1) : ctx
+ * words, and sequence b's rows start at word d_row_base[b].  max_q and max_ctx
+ * bound the lengths, tokens and packed the token and word counts. */
+typedef struct sufb200_attn_seqs {
+  const int32_t* d_cu_q;        /* [batch + 1] */
+  const int32_t* d_ctx;         /* [batch] */
+  const int64_t* d_row_base;    /* [batch] */
+  const int32_t* d_block_table; /* [batch][max_pages] */
+  int64_t tokens, packed;
+  int32_t batch, max_pages, page_size, pages, q_heads, kv_heads, head_dim, causal, max_q, max_ctx;
+} sufb200_attn_seqs;
+
+/* Scores: x^ = sum_p (C_p + D B_p + A_p E (+ D E for party 0) + r[p]) for every
+ * packed (row, key): D [tokens][q_heads][head_dim] the opened queries
+ * (sufb200_rope_append_pair), A_p likewise, C_p packed shares of A B^T (query
+ * head h against key head h / (q_heads / kv_heads)), xhat packed: the masked
+ * input of the scores' truncation.
+ * Values: x^[t][h] = sum_p (C_p + sum_j (D B_p + A_p E (+ D E)) + r[p]), D = sum_p
+ * (P_p - A_p) over the packed shares P_p of the probabilities and A_p of their
+ * mask; C_p and xhat [tokens][q_heads][head_dim].  A row without keys gives
+ * C_0 + C_1 + r.  Rows behind the last sequence are left as they were.
+ * nn::matmul_beaver (src/nn/matmul_beaver.cpp) over the cached operand. */
+int sufb200_attn_scores_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, const uint64_t* d_dq,
+                             const uint64_t* const* d_a, const uint64_t* const* d_c, const uint64_t* r,
+                             const uint64_t* d_ek, const uint64_t* const* d_bk, uint64_t* d_xhat, void* stream);
+int sufb200_attn_values_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, const uint64_t* const* d_p,
+                             const uint64_t* const* d_a, const uint64_t* const* d_c, const uint64_t* r,
+                             const uint64_t* d_ev, const uint64_t* const* d_bv, uint64_t* d_xhat, void* stream);
+
+/* The row-max tournament of nn::RowMaxDiffTask over packed rows of any
+ * lengths (sufb200_relu_open_pair / _update_pair are its dense form): row r of
+ * round k has off_k[r+1] - off_k[r] values, w -> ceil(w / 2) a round, its pairs
+ * (2j, 2j + 1) packed from word off_k[r] - off_{k+1}[r]; max_width bounds the
+ * round's widths; offsets are device [rows + 1].
+ * rowmax_open_pair: x^ = sum_p (c_p[2j] - c_p[2j+1] + r[p]) of the first round.
+ * rowmax_round_pair: from c (offsets off) and the gate's shares relu_p of its
+ * pairs, next_p (offsets off1) = c_p[2j+1] + relu_p[j], an odd row's last value
+ * unchanged; with d_xhat also the open of next's pairs (off2, r).  d_relu's
+ * entries may be NULL when max_width is 1.
+ * maxdiff_ragged_pair: t_p = max_p[row] - s_p, max_p at max_off[row] (the last
+ * round's offsets: empty rows have no value). */
+int sufb200_rowmax_open_pair(sufb200_ctx ctx, const uint64_t* const* d_c, int rows, int max_width,
+                             const int32_t* d_off, const int32_t* d_off1, const uint64_t* r, uint64_t* d_xhat,
+                             void* stream);
+int sufb200_rowmax_round_pair(sufb200_ctx ctx, const uint64_t* const* d_c, const uint64_t* const* d_relu, int rows,
+                              int max_width, const int32_t* d_off, const int32_t* d_off1, const int32_t* d_off2,
+                              const uint64_t* r, uint64_t* const* d_next, uint64_t* d_xhat, void* stream);
+int sufb200_maxdiff_ragged_pair(sufb200_ctx ctx, const uint64_t* const* d_max, const uint64_t* const* d_s, int rows,
+                                int max_width, const int32_t* d_off, const int32_t* d_max_off, uint64_t* const* d_t,
+                                void* stream);
+
 /* n successive draws of mt19937_64(seed) (the reference's mask / key RNG). */
 int sufb200_host_mt19937_64(uint64_t seed, uint64_t* out, size_t n);
 

@@ -50,6 +50,35 @@ class TruncDesc(C.Structure):
     ]
 
 
+class RopeAppend(C.Structure):
+    """Mirror of sufb200_rope_append."""
+
+    _fields_ = [
+        ("d_q", C.c_void_p * 2), ("d_k", C.c_void_p * 2), ("d_v", C.c_void_p * 2),
+        ("q_ts", C.c_int64), ("q_hs", C.c_int64), ("k_ts", C.c_int64), ("k_hs", C.c_int64), ("v_ts", C.c_int64),
+        ("v_hs", C.c_int64),
+        ("d_positions", C.c_void_p), ("d_slots", C.c_void_p), ("d_cos", C.c_void_p), ("d_sin", C.c_void_p),
+        ("d_a", C.c_void_p * 2), ("d_dq", C.c_void_p),
+        ("d_ek", C.c_void_p), ("d_bk", C.c_void_p * 2), ("d_ev", C.c_void_p), ("d_bv", C.c_void_p * 2),
+        ("tokens", C.c_int32), ("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("rot_dim", C.c_int32), ("interleaved", C.c_int32), ("max_pos", C.c_int32), ("pages", C.c_int32),
+        ("page_size", C.c_int32), ("reserved", C.c_int32),
+        ("trunc", TruncDesc * 2), ("d_tables", C.c_void_p * 2), ("r", C.c_uint64 * 2),
+    ]
+
+
+class AttnSeqs(C.Structure):
+    """Mirror of sufb200_attn_seqs."""
+
+    _fields_ = [
+        ("d_cu_q", C.c_void_p), ("d_ctx", C.c_void_p), ("d_row_base", C.c_void_p), ("d_block_table", C.c_void_p),
+        ("tokens", C.c_int64), ("packed", C.c_int64),
+        ("batch", C.c_int32), ("max_pages", C.c_int32), ("page_size", C.c_int32), ("pages", C.c_int32),
+        ("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("causal", C.c_int32),
+        ("max_q", C.c_int32), ("max_ctx", C.c_int32),
+    ]
+
+
 _vp = C.c_void_p
 _sz = C.c_size_t
 _u64 = C.c_uint64
@@ -145,6 +174,12 @@ _SIGS = {
     "sufb200_relu_open_pair": (_i, [_vp, _vp, _i, _i, _u64, _u64, _vp, _vp]),
     "sufb200_relu_update_pair": (_i, [_vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp]),
     "sufb200_maxdiff_pair": (_i, [_vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp]),
+    "sufb200_rope_append_pair": (_i, [_vp, C.POINTER(RopeAppend), _vp]),
+    "sufb200_attn_scores_pair": (_i, [_vp, C.POINTER(AttnSeqs), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "sufb200_attn_values_pair": (_i, [_vp, C.POINTER(AttnSeqs), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "sufb200_rowmax_open_pair": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp]),
+    "sufb200_rowmax_round_pair": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "sufb200_maxdiff_ragged_pair": (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp]),
     "sufb200_beaver_open_pair": (_i, [_vp, _sz, _i, _vp, _sz, _i, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _sz,
                                       _i, _vp]),
 }

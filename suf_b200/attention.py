@@ -1,0 +1,559 @@
+"""Attention over a paged cache of secret-shared keys and values, for both
+parties on one GPU: rotary positions and the append into the cache, the
+scores and values of packed sequences (whole prompts and single tokens,
+causal, grouped heads), the row max of ragged rows, and the block that runs
+them with the softmax block between.
+
+A cached row X is held as the public E = X - B and the dealer's shares B_0,
+B_1 of its mask; a call's other operand Y carries a fresh mask A, and the
+Beaver product of the two, Z_p = C_p + D B_p + A_p E (+ D E for party 0) with
+D = Y - A, needs no new open of the cached side.  A slot that is written again
+needs a freshly dealt mask.  The reference keeps its cache as share tensors
+(include/nn/kv_cache.hpp) and opens both operands in every product
+(src/nn/matmul_beaver.cpp).
+
+All tensors live on the context's device; shares and opened words are int64
+tensors (the words of Z_2^64).  Calls are asynchronous on `stream` (default:
+the device's current stream).  Wrong device-side data (slots, positions,
+pages) is reported by Context.sync.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import numpy as np
+
+from . import _lib
+from ._lib import AttnSeqs, RopeAppend, check
+from .engine import Context, TruncTables
+from .layer import _CoeffGate, _Trunc, load_layer_tables
+from .softmax import SoftmaxBlock, load_tables
+
+M64 = (1 << 64) - 1
+
+
+# -- arguments ----------------------------------------------------------------
+
+def _stream(ctx: Context, stream):
+    """The stream a call runs on, on the context's device."""
+    import torch
+
+    if stream is None:
+        return torch.cuda.current_stream(ctx.device)
+    if not isinstance(stream, int) and stream.device.index != ctx.device:
+        raise ValueError(f"the stream is on {stream.device}, the context on cuda:{ctx.device}")
+    return stream
+
+
+def _raw(stream) -> int | None:
+    return (stream if isinstance(stream, int) else int(stream.cuda_stream)) or None
+
+
+def _empty(ctx: Context, shape, stream):
+    """Words on the context's device, allocated on the stream that writes them
+    and kept until the caller's current stream has passed its use of them."""
+    import torch
+
+    now = torch.cuda.current_stream(ctx.device)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=ctx.device) if stream else torch.cuda.default_stream(ctx.device)
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=torch.int64, device=torch.device("cuda", ctx.device))
+    if stream != now:
+        t.record_stream(now)
+    return t
+
+
+def _want(ctx: Context, name: str, t, shape, dtype=None):
+    """Check a dense tensor: int64 words unless `dtype`, on the device, of the shape (None: any extent)."""
+    import torch
+
+    dtype = dtype or torch.int64
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+        raise ValueError(f"{name}: expected a {dtype} tensor")
+    if t.device.type != "cuda" or t.device.index != ctx.device:
+        raise ValueError(f"{name}: on {t.device}, the context is on cuda:{ctx.device}")
+    if t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape)):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple('any' if w is None else w for w in shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: not contiguous")
+    return t
+
+
+def _pair(ctx: Context, name: str, ts, shape):
+    if not isinstance(ts, (tuple, list)) or len(ts) != 2:
+        raise ValueError(f"{name}: expected both parties' tensors")
+    return tuple(_want(ctx, f"{name}[{p}]", t, shape) for p, t in enumerate(ts))
+
+
+def _ptrs(ts):
+    return (C.c_void_p * 2)(*[int(t.data_ptr()) for t in ts])
+
+
+def _masks(r):
+    if len(r) != 2:
+        raise ValueError("r: expected both parties' shares of the mask")
+    return (C.c_uint64 * 2)(int(r[0]) & M64, int(r[1]) & M64)
+
+
+# -- rotary tables --------------------------------------------------------------
+
+def rope_table_words(max_pos: int, rot_dim: int, frac_bits: int, base: float = 10000.0, scale: float = 1.0,
+                     low_freq: float | None = None, high_freq: float | None = None, trained_pos: int | None = None):
+    """Cosines and sines of every position in fixed point: two int32 arrays
+    [max_pos][rot_dim / 2], pair i turning by pos * base^(-2i / rot_dim).
+
+    scale > 1 stretches positions for contexts longer than the model was
+    trained on: every frequency is divided by it (position interpolation), or,
+    with trained_pos and low_freq < high_freq, only those that turn fewer than
+    low_freq times over trained_pos positions; frequencies that turn more than
+    high_freq times stay, and those between are blended linearly in the number
+    of turns.  Angles are formed in 64-bit floats: those of far positions have
+    lost nothing that the rounding to frac_bits would keep."""
+    if rot_dim < 0 or rot_dim % 2 or max_pos < 1 or not 1 <= frac_bits <= 16 or not base > 0 or not scale > 0:
+        raise ValueError("rope_tables: bad size, fractional bits, base or scale")
+    half = rot_dim // 2
+    inv = base ** (-np.arange(half, dtype=np.float64) / max(half, 1))
+    if low_freq is not None or high_freq is not None or trained_pos is not None:
+        if low_freq is None or high_freq is None or trained_pos is None or not 0 <= low_freq < high_freq:
+            raise ValueError("rope_tables: the blended form takes trained_pos and low_freq < high_freq")
+        turns = trained_pos * inv / (2.0 * math.pi)
+        keep = np.clip((turns - low_freq) / (high_freq - low_freq), 0.0, 1.0)
+        inv = inv * keep + inv / scale * (1.0 - keep)
+    else:
+        inv = inv / scale
+    ang = np.arange(max_pos, dtype=np.float64)[:, None] * inv[None, :]
+    one = float(1 << frac_bits)
+    return tuple(np.rint(f(ang) * one).astype(np.int32) for f in (np.cos, np.sin))
+
+
+def rope_tables(ctx: Context, max_pos: int, rot_dim: int, frac_bits: int, **kw):
+    """rope_table_words on the context's device, as rope_append_pair takes them."""
+    import torch
+
+    dev = torch.device("cuda", ctx.device)
+    return tuple(torch.from_numpy(t).to(dev) for t in rope_table_words(max_pos, rot_dim, frac_bits, **kw))
+
+
+class TruncPair(_Trunc):
+    """A GapARS truncation bundle for both parties with its full-domain tables
+    filled (frac_bits 1..16): dealer material that stays resident."""
+
+    def __init__(self, ctx: Context, frac_bits: int, seed: int = 1, stream=None):
+        import torch
+
+        if not 1 <= frac_bits <= 16:
+            raise ValueError("TruncPair: 1..16 fractional bits")
+        dev = torch.device("cuda", ctx.device)
+        super().__init__(ctx, np.random.default_rng(seed), frac_bits, dev)
+        self.frac_bits = frac_bits
+        st = _stream(ctx, stream)
+        self._full = TruncTables(self.bundles(), dev)
+        if self._full.any():
+            with torch.cuda.device(ctx.device):
+                self._full.fill(ctx, st)
+        # the tables are read on any stream from here on
+        (torch.cuda.synchronize(dev) if isinstance(st, int) else st.synchronize())
+
+    def table_ptrs(self):
+        return self._full.ptr(0), self._full.ptr(1)
+
+    def eval_pair(self, ctx: Context, d_xhat, d_y0, d_y1, stream=None):
+        """Both parties' truncated shares of the opened x^: lookups in the
+        tables (a bundle without queries has none and is evaluated as it is)."""
+        st = _stream(ctx, stream)
+        if not self._full.any():
+            return super().eval_pair(ctx, d_xhat, d_y0, d_y1, st)
+        check(ctx._L.sufb200_trunc_bundle_eval_pair_tables_dev(
+            ctx.h, C.byref(self.desc[0]), C.cast(self.kptr[0], C.c_void_p), C.cast(self.ksz[0], C.c_void_p),
+            self._full.ptr(0), C.byref(self.desc[1]), C.cast(self.kptr[1], C.c_void_p),
+            C.cast(self.ksz[1], C.c_void_p), self._full.ptr(1), d_xhat.data_ptr(), d_xhat.numel(), d_y0.data_ptr(),
+            d_y1.data_ptr(), _raw(st)))
+
+
+# -- the cache -------------------------------------------------------------------
+
+class ShareCache:
+    """The paged cache of one layer: opened pools ek, ev and the masks' shares
+    bk, bv (pairs), each [pages][kv_heads][page_size][head_dim].  Slot = page *
+    page_size + place.  The constructor deals fresh masks for every slot."""
+
+    def __init__(self, ctx: Context, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, seed: int = 1):
+        import torch
+
+        dev = torch.device("cuda", ctx.device)
+        g = torch.Generator(device=dev)
+        g.manual_seed(seed)
+        shape = (pages, kv_heads, page_size, head_dim)
+
+        def words():
+            return torch.randint(-(2**63), 2**63 - 1, shape, dtype=torch.int64, device=dev, generator=g)
+
+        self._set(ctx, torch.zeros(shape, dtype=torch.int64, device=dev), (words(), words()),
+                  torch.zeros(shape, dtype=torch.int64, device=dev), (words(), words()))
+
+    @classmethod
+    def from_tensors(cls, ctx: Context, ek, bk, ev, bv) -> "ShareCache":
+        """A cache over pools the caller holds."""
+        self = cls.__new__(cls)
+        self._set(ctx, ek, bk, ev, bv)
+        return self
+
+    def _set(self, ctx, ek, bk, ev, bv):
+        _want(ctx, "ek", ek, (None,) * 4)
+        shape = tuple(ek.shape)
+        self.ek, self.ev = ek, _want(ctx, "ev", ev, shape)
+        self.bk, self.bv = _pair(ctx, "bk", bk, shape), _pair(ctx, "bv", bv, shape)
+        self.pages, self.kv_heads, self.page_size, self.head_dim = shape
+        if min(shape) < 1 or self.head_dim % 2 or self.head_dim > 256:
+            raise ValueError("cache: empty, or a head size that is not even, 2..256")
+
+
+def _strided(ctx: Context, name: str, ts, tokens, heads, dim):
+    """Both parties' [tokens][heads][dim] views of one stride pattern (the last axis dense)."""
+    import torch
+
+    if not isinstance(ts, (tuple, list)) or len(ts) != 2:
+        raise ValueError(f"{name}: expected both parties' tensors")
+    for p, t in enumerate(ts):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int64:
+            raise ValueError(f"{name}[{p}]: expected a torch.int64 tensor")
+        if t.device.type != "cuda" or t.device.index != ctx.device:
+            raise ValueError(f"{name}[{p}]: on {t.device}, the context is on cuda:{ctx.device}")
+        if tuple(t.shape) != (tokens, heads, dim):
+            raise ValueError(f"{name}[{p}]: shape {tuple(t.shape)}, expected {(tokens, heads, dim)}")
+        if t.numel() and dim > 1 and t.stride(2) != 1:
+            raise ValueError(f"{name}[{p}]: the head's words must be adjacent")
+        if t.stride() != ts[0].stride():
+            raise ValueError(f"{name}: the parties' strides differ")
+    return ts[0].stride(0), ts[0].stride(1)
+
+
+def rope_append_pair(ctx: Context, q, k, v, positions, slots, cos, sin, trunc: TruncPair | None, a, cache: ShareCache,
+                     d_q=None, *, interleaved: bool = False, stream=None):
+    """New tokens' queries, keys and values, both parties' shares [tokens]
+    [heads][head_dim] (views of fused rows allowed): queries and keys turned to
+    their positions (int32 [tokens]; cos, sin: rope_tables, None with trunc None
+    for no rotation) and truncated, keys and values opened against the masks of
+    their slots into `cache` (int64 [tokens]; -1: padding, nothing written, all
+    others distinct), queries opened against the mask shares a into d_q [tokens]
+    [q_heads][head_dim], which is returned.  q, a None: append only."""
+    import torch
+
+    tokens, kv, dim = int(k[0].shape[0]), cache.kv_heads, cache.head_dim
+    heads = int(q[0].shape[1]) if q is not None else 0
+    st = _stream(ctx, stream)
+    args = RopeAppend()
+    args.k_ts, args.k_hs = _strided(ctx, "k", k, tokens, kv, dim)
+    args.v_ts, args.v_hs = _strided(ctx, "v", v, tokens, kv, dim)
+    args.d_k, args.d_v = _ptrs(k), _ptrs(v)
+    if q is not None:
+        args.q_ts, args.q_hs = _strided(ctx, "q", q, tokens, heads, dim)
+        args.d_q, args.d_a = _ptrs(q), _ptrs(_pair(ctx, "a", a, (tokens, heads, dim)))
+        if d_q is None:
+            d_q = _empty(ctx, (tokens, heads, dim), st)
+        args.d_dq = _want(ctx, "d_q", d_q, (tokens, heads, dim)).data_ptr()
+    args.d_slots = _want(ctx, "slots", slots, (tokens,)).data_ptr()
+    if trunc is not None:
+        _want(ctx, "cos", cos, (None, None), torch.int32)
+        _want(ctx, "sin", sin, tuple(cos.shape), torch.int32)
+        args.max_pos, args.rot_dim = int(cos.shape[0]), 2 * int(cos.shape[1])
+        if args.rot_dim > dim:
+            raise ValueError(f"the tables turn {args.rot_dim} words of a head of {dim}")
+        args.d_positions = _want(ctx, "positions", positions, (tokens,), torch.int32).data_ptr()
+        args.d_cos, args.d_sin = cos.data_ptr(), sin.data_ptr()
+        args.trunc[0], args.trunc[1] = trunc.desc
+        args.d_tables[0], args.d_tables[1] = trunc.table_ptrs()
+        args.r[0], args.r[1] = trunc.r
+    elif cos is not None or sin is not None:
+        raise ValueError("rotation needs the truncation bundle")
+    args.d_ek, args.d_bk, args.d_ev, args.d_bv = (cache.ek.data_ptr(), _ptrs(cache.bk), cache.ev.data_ptr(),
+                                                  _ptrs(cache.bv))
+    args.tokens, args.q_heads, args.kv_heads, args.head_dim = tokens, heads, kv, dim
+    args.interleaved, args.pages, args.page_size = int(interleaved), cache.pages, cache.page_size
+    check(ctx._L.sufb200_rope_append_pair(ctx.h, C.byref(args), _raw(st)))
+    return d_q
+
+
+# -- scores and values -------------------------------------------------------------
+
+class AttnLayout:
+    """The packed sequences of an attention call, resident on the device:
+    sequence b has q_lens[b] new tokens (its queries, packed one sequence after
+    the other) and ctx_lens[b] cached tokens, the new ones included, in the
+    pages block_table[b] (int32 [batch][most pages] on the device, or lists).
+    Causal rows see what is before them: row (b, head, i) has
+    max(0, ctx - q + i + 1) keys; otherwise all ctx.  Rows are packed in
+    (sequence, head, query) order: row_lengths() is what SoftmaxBlock and
+    RowMaxPlan take, `packed` the words in all, `tokens` the queries."""
+
+    def __init__(self, ctx: Context, q_lens, ctx_lens, block_table, page_size: int, q_heads: int, kv_heads: int,
+                 causal: bool = True):
+        import torch
+
+        dev = torch.device("cuda", ctx.device)
+        q, L = np.asarray(q_lens, dtype=np.int64).reshape(-1), np.asarray(ctx_lens, dtype=np.int64).reshape(-1)
+        if q.size != L.size or (q < 0).any() or (L < 0).any():
+            raise ValueError("layout: one non-negative query and context length per sequence")
+        if kv_heads < 1 or q_heads < kv_heads or q_heads % kv_heads or page_size < 1:
+            raise ValueError("layout: query heads must be a multiple of key heads, the page size positive")
+        if not isinstance(block_table, torch.Tensor):
+            rows = [list(r) for r in block_table]
+            wide = np.zeros((len(rows), max([len(r) for r in rows] + [1])), dtype=np.int32)
+            for i, r in enumerate(rows):
+                wide[i, :len(r)] = r
+            block_table = torch.from_numpy(wide).to(dev)
+        _want(ctx, "block_table", block_table, (q.size, None), torch.int32)
+        self.q_lens, self.ctx_lens, self.causal = q, L, bool(causal)
+        self.q_heads, self.kv_heads, self.page_size = int(q_heads), int(kv_heads), int(page_size)
+        self.tokens, self.batch = int(q.sum()), int(q.size)
+        if causal:  # the lengths of a head's rows are consecutive: their sum is a difference of triangles
+            first = np.maximum(L - q, 0)
+            words = (L * (L + 1) - first * (first + 1)) // 2
+        else:
+            words = q * L
+        base = np.concatenate([[0], np.cumsum(words * q_heads)])
+        self.packed = int(base[-1])
+        if self.batch and int(L.max()) > block_table.shape[1] * page_size:
+            raise ValueError("layout: a sequence is longer than its pages")
+        if max(self.tokens, self.batch, int(L.max(initial=0))) >= 2**31:
+            raise ValueError("layout: more than 2^31 tokens")
+        self._cu = torch.from_numpy(np.concatenate([[0], np.cumsum(q)]).astype(np.int32)).to(dev)
+        self._ctx = torch.from_numpy(L.astype(np.int32)).to(dev)
+        self._base = torch.from_numpy(base[:-1].astype(np.int64)).to(dev)
+        self._table = block_table
+        s = self._seqs = AttnSeqs()
+        s.d_cu_q, s.d_ctx, s.d_row_base = self._cu.data_ptr(), self._ctx.data_ptr(), self._base.data_ptr()
+        s.d_block_table = block_table.data_ptr()
+        s.tokens, s.packed, s.batch, s.max_pages = self.tokens, self.packed, self.batch, int(block_table.shape[1])
+        s.page_size, s.q_heads, s.kv_heads, s.causal = self.page_size, self.q_heads, self.kv_heads, int(self.causal)
+        s.max_q, s.max_ctx = int(q.max(initial=0)), int(L.max(initial=0))
+
+    def row_lengths(self) -> np.ndarray:
+        """Keys of every row, in (sequence, head, query) order."""
+        out = [np.tile(np.maximum(0, L - n + 1 + np.arange(n)) if self.causal else np.full(n, L), self.q_heads)
+               for n, L in zip(self.q_lens, self.ctx_lens)]
+        return np.concatenate(out).astype(np.int64) if out else np.zeros(0, dtype=np.int64)
+
+    def _for_pool(self, ctx, name, e, b):
+        _want(ctx, name, e, (None, self.kv_heads, self.page_size, None))
+        pair = _pair(ctx, f"{name}'s masks", b, tuple(e.shape))
+        s = AttnSeqs.from_buffer_copy(self._seqs)
+        s.pages, s.head_dim = int(e.shape[0]), int(e.shape[3])
+        return s, pair
+
+
+def attn_scores_pair(ctx: Context, d_q, a, c, r, ek, bk, layout: AttnLayout, out=None, stream=None):
+    """The opened, masked scores of every packed (row, key): the opened queries
+    d_q and their mask's shares a [tokens][q_heads][head_dim], the packed shares
+    c of the triple's product, r the shares of the output's mask, ek and bk a
+    cache's keys.  Returns x^ [packed]."""
+    st = _stream(ctx, stream)
+    seqs, bk = layout._for_pool(ctx, "ek", ek, bk)
+    shape = (layout.tokens, layout.q_heads, seqs.head_dim)
+    _want(ctx, "d_q", d_q, shape)
+    a, c = _pair(ctx, "a", a, shape), _pair(ctx, "c", c, (layout.packed,))
+    if out is None:
+        out = _empty(ctx, (layout.packed,), st)
+    _want(ctx, "out", out, (layout.packed,))
+    check(ctx._L.sufb200_attn_scores_pair(ctx.h, C.byref(seqs), d_q.data_ptr(), _ptrs(a), _ptrs(c), _masks(r),
+                                          ek.data_ptr(), _ptrs(bk), out.data_ptr(), _raw(st)))
+    return out
+
+
+def attn_values_pair(ctx: Context, p, a, c, r, ev, bv, layout: AttnLayout, out=None, stream=None):
+    """The opened, masked value products of every query and head: the packed
+    shares p of the probabilities and a of their mask, the shares c of the
+    triple's product [tokens][q_heads][head_dim], ev and bv a cache's values.
+    Returns x^ [tokens][q_heads][head_dim]."""
+    st = _stream(ctx, stream)
+    seqs, bv = layout._for_pool(ctx, "ev", ev, bv)
+    shape = (layout.tokens, layout.q_heads, seqs.head_dim)
+    p, a = _pair(ctx, "p", p, (layout.packed,)), _pair(ctx, "a", a, (layout.packed,))
+    c = _pair(ctx, "c", c, shape)
+    if out is None:
+        out = _empty(ctx, shape, st)
+    _want(ctx, "out", out, shape)
+    check(ctx._L.sufb200_attn_values_pair(ctx.h, C.byref(seqs), _ptrs(p), _ptrs(a), _ptrs(c), _masks(r),
+                                          ev.data_ptr(), _ptrs(bv), out.data_ptr(), _raw(st)))
+    return out
+
+
+# -- the row max of ragged rows -----------------------------------------------------
+
+class RowMaxPlan:
+    """The rounds of the row-max tournament over packed rows of the given
+    lengths: off[k] the device row offsets of round k, pairs[k] its pairs,
+    values[k] its packed values, `rounds` how often the longest row halves."""
+
+    def __init__(self, ctx: Context, row_lengths):
+        import torch
+
+        dev = torch.device("cuda", ctx.device)
+        w = np.asarray(row_lengths, dtype=np.int64).reshape(-1)
+        if (w < 0).any() or int(w.sum()) >= 2**31:
+            raise ValueError("rowmax: row lengths must be non-negative, below 2^31 words in all")
+        self.rows = int(w.size)
+        self.off, self.values, self.pairs, self.widths = [], [], [], []
+        while True:
+            self.off.append(torch.from_numpy(np.concatenate([[0], np.cumsum(w)]).astype(np.int32)).to(dev))
+            self.values.append(int(w.sum()))
+            self.widths.append(int(w.max(initial=0)))
+            if self.widths[-1] <= 1:
+                break
+            self.pairs.append(int((w // 2).sum()))
+            w = (w + 1) // 2
+        self.rounds = len(self.pairs)
+
+
+def rowmax_open_pair(ctx: Context, plan: RowMaxPlan, c, r, out=None, stream=None):
+    """x^ [pairs[0]]: the opened differences of the first round's pairs of c (packed shares)."""
+    st = _stream(ctx, stream)
+    c = _pair(ctx, "c", c, (plan.values[0],))
+    n = plan.pairs[0] if plan.rounds else 0
+    if out is None:
+        out = _empty(ctx, (n,), st)
+    _want(ctx, "out", out, (n,))
+    if plan.rounds:
+        check(ctx._L.sufb200_rowmax_open_pair(ctx.h, _ptrs(c), plan.rows, plan.widths[0], plan.off[0].data_ptr(),
+                                              plan.off[1].data_ptr(), _masks(r), out.data_ptr(), _raw(st)))
+    return out
+
+
+def rowmax_round_pair(ctx: Context, plan: RowMaxPlan, k: int, c, relu, r_next=None, nxt=None, out=None, stream=None):
+    """Round k: its values c (packed shares) and the gate's shares relu of its
+    pairs to the next round's values, and, with r_next, the open of their
+    differences.  Returns ((next_0, next_1), x^ or None)."""
+    st = _stream(ctx, stream)
+    if not 0 <= k < plan.rounds:
+        raise ValueError(f"rowmax: round {k} of {plan.rounds}")
+    c, relu = _pair(ctx, "c", c, (plan.values[k],)), _pair(ctx, "relu", relu, (plan.pairs[k],))
+    n = plan.values[k + 1]
+    nxt = _pair(ctx, "next", nxt, (n,)) if nxt is not None else (_empty(ctx, (n,), st), _empty(ctx, (n,), st))
+    more = k + 1 < plan.rounds
+    if not more and r_next is not None:
+        raise ValueError("rowmax: the last round has no further differences to open")
+    if r_next is not None:
+        if out is None:
+            out = _empty(ctx, (plan.pairs[k + 1],), st)
+        _want(ctx, "out", out, (plan.pairs[k + 1],))
+    else:
+        out = None
+    check(ctx._L.sufb200_rowmax_round_pair(
+        ctx.h, _ptrs(c), _ptrs(relu), plan.rows, plan.widths[k], plan.off[k].data_ptr(), plan.off[k + 1].data_ptr(),
+        plan.off[k + 2].data_ptr() if more else None, _masks(r_next) if r_next is not None else None, _ptrs(nxt),
+        out.data_ptr() if out is not None else None, _raw(st)))
+    return nxt, out
+
+
+def maxdiff_ragged_pair(ctx: Context, plan: RowMaxPlan, m, s, out=None, stream=None):
+    """t_p = max_p[row] - s_p over the packed rows: m the last round's values, s the first's."""
+    st = _stream(ctx, stream)
+    m, s = _pair(ctx, "max", m, (plan.values[-1],)), _pair(ctx, "s", s, (plan.values[0],))
+    n = plan.values[0]
+    out = _pair(ctx, "out", out, (n,)) if out is not None else (_empty(ctx, (n,), st), _empty(ctx, (n,), st))
+    check(ctx._L.sufb200_maxdiff_ragged_pair(ctx.h, _ptrs(m), _ptrs(s), plan.rows, plan.widths[0],
+                                             plan.off[0].data_ptr(), plan.off[-1].data_ptr(), _ptrs(out), _raw(st)))
+    return out
+
+
+# -- the block ------------------------------------------------------------------------
+
+class CachedAttentionPair:
+    """One attention step over a cache for both parties: the new tokens
+    appended with their rotary positions, causal scores against everything
+    cached, the row max, the softmax block and the value products, every
+    truncation a GapARS bundle.  The constructor deals the step's material for
+    the layout (masks, triples, gates; f from the softmax tables); in a
+    deployment each step takes freshly dealt material.
+
+    score_shift: bits of 1/sqrt(head_dim) folded into the scores' truncation;
+    default log2(sqrt(head_dim)) for head sizes 4^k, otherwise fold the scale
+    into the query weights and pass 0."""
+
+    def __init__(self, ctx: Context, cache: ShareCache, layout: AttnLayout, seed: int = 1,
+                 score_shift: int | None = None, rope: tuple | None = None, interleaved: bool = False):
+        import torch
+
+        if layout.kv_heads != cache.kv_heads or layout.page_size != cache.page_size:
+            raise ValueError("attention: the layout's heads or pages are not the cache's")
+        dim = cache.head_dim
+        if score_shift is None:
+            score_shift = (dim.bit_length() - 1) // 2
+            if 4**score_shift != dim:
+                raise ValueError("attention: 1/sqrt(head_dim) is not a power of two: pass score_shift")
+        self.ctx, self.cache, self.layout, self.rope, self.interleaved = ctx, cache, layout, rope, interleaved
+        sm_tables = load_tables()
+        f = self.frac_bits = int(sm_tables["frac_bits"])
+        rng = np.random.default_rng(seed)
+
+        def sub():
+            return int(rng.integers(1, 2**62))
+
+        dev = torch.device("cuda", ctx.device)
+        g = torch.Generator(device=dev)
+        g.manual_seed(sub())
+
+        def words(*shape):
+            return torch.randint(-(2**63), 2**63 - 1, shape, dtype=torch.int64, device=dev, generator=g)
+
+        T, H = layout.tokens, layout.q_heads
+        self.tr_rope = TruncPair(ctx, f, sub()) if rope is not None else None
+        self.tr_s, self.tr_o = TruncPair(ctx, f + score_shift, sub()), TruncPair(ctx, f, sub())
+        self.a_q = (words(T, H, dim), words(T, H, dim))
+        self.a_p = (words(layout.packed), words(layout.packed))
+        # the triples' products A B: a product with D = A and E = 0
+        zero_e = torch.zeros_like(cache.ek)
+        z_q, z_p = torch.zeros_like(self.a_q[0]), torch.zeros_like(self.a_p[0])
+        cs = attn_scores_pair(ctx, self.a_q[0] + self.a_q[1], (z_q, z_q), (z_p, z_p), (0, 0), zero_e, cache.bk, layout)
+        cv = attn_values_pair(ctx, (self.a_p[0] + self.a_p[1], z_p), (z_p, z_p), (z_q, z_q), (0, 0), zero_e, cache.bv,
+                              layout)
+        s0, v0 = words(layout.packed), words(T, H, dim)
+        self.c_s, self.c_v = (s0, cs - s0), (v0, cv - v0)
+        if layout.packed:
+            lens = layout.row_lengths()
+            self.plan = RowMaxPlan(ctx, lens)
+            relu = load_layer_tables()["relu"]
+            self.gates = [_CoeffGate(rng, relu) for _ in range(self.plan.rounds)]
+            self.softmax = SoftmaxBlock(ctx, lens, seed=sub(), tables=sm_tables)
+        ctx.sync(_stream(ctx, None))
+
+    def run(self, q, k, v, positions, slots, stream=None, trace: dict | None = None):
+        """Both parties' shares of the new tokens' queries, keys and values
+        [tokens][heads][head_dim] (views of fused rows allowed), their positions
+        (None without rotary tables) and cache slots -> both parties' shares of
+        the attention output [tokens][q_heads][head_dim]."""
+        import torch
+
+        ctx, layout = self.ctx, self.layout
+        st = _stream(ctx, stream)
+
+        def new(n):
+            return _empty(ctx, n, st), _empty(ctx, n, st)
+
+        cos, sin = self.rope if self.rope is not None else (None, None)
+        d_q = rope_append_pair(ctx, q, k, v, positions, slots, cos, sin, self.tr_rope, self.a_q, self.cache,
+                               interleaved=self.interleaved, stream=st)
+        p = new(layout.packed)
+        if layout.packed:
+            xs = attn_scores_pair(ctx, d_q, self.a_q, self.c_s, self.tr_s.r, self.cache.ek, self.cache.bk, layout,
+                                  stream=st)
+            s = new(layout.packed)
+            self.tr_s.eval_pair(ctx, xs, *s, stream=st)
+            cur, plan = s, self.plan
+            xh = rowmax_open_pair(ctx, plan, cur, self.gates[0].r, stream=st) if plan.rounds else None
+            for i, gate in enumerate(self.gates):
+                relu = new(plan.pairs[i])
+                gate.eval_pair(ctx, xh, *relu, st)
+                nxt = self.gates[i + 1].r if i + 1 < plan.rounds else None
+                cur, xh = rowmax_round_pair(ctx, plan, i, cur, relu, nxt, stream=st)
+            t = maxdiff_ragged_pair(ctx, plan, cur, s, stream=st)
+            self.softmax.run(*t, *p, stream=st)
+            if trace is not None:
+                trace.update(d_q=d_q, scores=s, t=t, probs=p)
+        xo = attn_values_pair(ctx, p, self.a_p, self.c_v, self.tr_o.r, self.cache.ev, self.cache.bv, layout, stream=st)
+        o = new(tuple(xo.shape))
+        if xo.numel():
+            self.tr_o.eval_pair(ctx, xo, *o, stream=st)
+        return o

@@ -1,0 +1,401 @@
+// attention.cu -- the two products of attention over a paged cache of
+// secret-shared keys and values, for both parties on one GPU.
+//
+// A cached entry X (a key or value row) is held as the public E = X - B and
+// the dealer's shares B_0, B_1 of its mask B, which stays fixed for the
+// entry's life; a call's other operand Y has the fresh mask A (shares A_p),
+// D = Y - A is public, and C_p are the shares of the triple's product.  Then
+//   Z_p = C_p + D B_p + A_p E (+ D E for party 0),  Z_0 + Z_1 = Y X,
+// and what a call writes is the open of the masked result for its truncation,
+//   x^ = sum_p (Z_p + r_p)
+//      = (C_0 + C_1) + D (B_0 + B_1) + (D + A_0 + A_1) E + (r_0 + r_1).
+// The second line is what the kernels compute: sums mod 2^64 may be
+// regrouped, so a pair call spends two products per entry where the parties
+// by themselves spend two each.
+//   scores: Y = the rotated queries (D opened by the append), X = keys,
+//           contraction over the head, packed ragged rows out;
+//   values: Y = the probabilities (D = P - A opened while loading), X =
+//           values, contraction over the row's valid keys, [token][head] out.
+// Queries share key heads in groups of q_heads / kv_heads; row rho of a
+// (sequence, key head) is query rho / group of head kh * group + rho % group,
+// so rows of one tile have nearly equal causal lengths.
+#include "attention.hpp"
+
+namespace sufb200 {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+int fail(int code, const std::string& msg) { return record_error(code, msg); }
+
+// ---- few rows (single tokens): bound by the cache's three words per entry --
+// scores_rows: eight lanes per key, 16 bytes of the head each; the rows' U =
+// D + A_0 + A_1 and D sit in shared memory and are read once for two keys.
+constexpr int kKeyChunk = 128;  // keys per CTA
+
+template <int RT>
+__global__ void __launch_bounds__(kThreads) scores_rows_kernel(const __grid_constant__ AttnSeqs s,
+                                                               const __grid_constant__ AttnOperands o) {
+  extern __shared__ __align__(16) uint64_t sm[];
+  __shared__ int64_t s_key[kKeyChunk];
+  __shared__ uint64_t s_out[RT][kKeyChunk + 1];
+  const int t = threadIdx.x, dh = s.head_dim, group = s.q_heads / s.kv_heads;
+  const int b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads;
+  SeqInfo q;
+  if (!seq_info(s, b, o.status, q)) return;
+  const int R = group * q.n, rho0 = blockIdx.y * RT, k0 = blockIdx.x * kKeyChunk;
+  if (rho0 >= R) return;
+  const int last = (rho0 + RT < R ? rho0 + RT : R) - 1;
+  const int len = row_len(q.n, q.L, s.causal, last / group);  // the longest row of the tile
+  if (k0 >= len) return;
+  uint64_t* sU = sm;
+  uint64_t* sD = sm + RT * dh;
+  for (int e = t; e < RT * dh; e += kThreads) {
+    const int rr = e / dh, c = e % dh, rho = rho0 + rr;
+    uint64_t d = 0, u = 0;
+    if (rho < R) {
+      const int64_t at = (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + c;
+      d = o.x[0][at];
+      u = d + o.a[0][at] + o.a[1][at];
+    }
+    sU[e] = u;
+    sD[e] = d;
+  }
+  for (int e = t; e < kKeyChunk; e += kThreads) s_key[e] = k0 + e < len ? key_off(s, b, kh, k0 + e, o.status) : -1;
+  __syncthreads();
+  const int l8 = t & 7, grp = t >> 3;
+  for (int kk = grp; kk < kKeyChunk; kk += 64) {
+    const int64_t o0 = s_key[kk], o1 = s_key[kk + 32];
+    uint64_t acc[2][RT] = {};
+    for (int c = l8; c < dh / 2; c += 8) {
+      ulonglong2 e0 = make_ulonglong2(0, 0), w0 = e0, e1 = e0, w1 = e0;
+      if (o0 >= 0) {
+        e0 = ld_stream(o.e + o0 + 2 * c);
+        const ulonglong2 p = ld_stream(o.b[0] + o0 + 2 * c), r = ld_stream(o.b[1] + o0 + 2 * c);
+        w0 = make_ulonglong2(p.x + r.x, p.y + r.y);
+      }
+      if (o1 >= 0) {
+        e1 = ld_stream(o.e + o1 + 2 * c);
+        const ulonglong2 p = ld_stream(o.b[0] + o1 + 2 * c), r = ld_stream(o.b[1] + o1 + 2 * c);
+        w1 = make_ulonglong2(p.x + r.x, p.y + r.y);
+      }
+#pragma unroll
+      for (int rr = 0; rr < RT; rr++) {
+        const ulonglong2 u = *reinterpret_cast<const ulonglong2*>(sU + rr * dh + 2 * c);
+        const ulonglong2 d = *reinterpret_cast<const ulonglong2*>(sD + rr * dh + 2 * c);
+        acc[0][rr] += u.x * e0.x + u.y * e0.y + d.x * w0.x + d.y * w0.y;
+        acc[1][rr] += u.x * e1.x + u.y * e1.y + d.x * w1.x + d.y * w1.y;
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < 2; v++)
+#pragma unroll
+      for (int rr = 0; rr < RT; rr++) {
+        uint64_t z = acc[v][rr];
+#pragma unroll
+        for (int m = 4; m > 0; m >>= 1) z += __shfl_xor_sync(0xffffffffu, z, m);
+        if (l8 == rr % 8) s_out[rr][kk + 32 * v] = z;
+      }
+  }
+  __syncthreads();
+  for (int e = t; e < RT * kKeyChunk; e += kThreads) {
+    const int rr = e / kKeyChunk, kk = e % kKeyChunk, rho = rho0 + rr, i = rho / group;
+    if (rho >= R || k0 + kk >= row_len(q.n, q.L, s.causal, i)) continue;
+    const int64_t at = q.base + (kh * group + rho % group) * q.blk + row_off(q.n, q.L, s.causal, i) + k0 + kk;
+    o.out[at] = s_out[rr][kk] + o.c[0][at] + o.c[1][at] + o.r;
+  }
+}
+
+// out = C_0 + C_1 + r for the sequences' tokens: what the values kernels add to.
+__global__ void values_init_kernel(const __grid_constant__ AttnSeqs s, const __grid_constant__ AttnOperands o) {
+  int64_t tokens = s.d_cu_q[s.batch];
+  if (tokens < 0 || tokens > s.tokens) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(o.status, kStatusBadArgument);
+    tokens = 0;
+  }
+  const int64_t n = tokens * s.q_heads * s.head_dim;
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; i < n;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x)
+    o.out[i] = o.c[0][i] + o.c[1][i] + o.r;
+}
+
+// values_rows: a thread holds two words of the head for RT rows; the CTA's
+// key lanes walk its range of keys, whose probabilities sit in shared memory.
+// Ranges of one row meet by 64-bit atomic adds: sums mod 2^64 do not depend
+// on their order.
+constexpr int kValStage = 64;
+
+template <int RT>
+__global__ void __launch_bounds__(kThreads) values_rows_kernel(const __grid_constant__ AttnSeqs s,
+                                                               const __grid_constant__ AttnOperands o, int range) {
+  __shared__ __align__(16) uint64_t sU[kValStage][RT], sD[kValStage][RT];
+  __shared__ int64_t s_key[kValStage];
+  const int t = threadIdx.x, dh = s.head_dim, group = s.q_heads / s.kv_heads, P = dh / 2;
+  const int b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads;
+  SeqInfo q;
+  if (!seq_info(s, b, o.status, q)) return;
+  const int R = group * q.n, rho0 = blockIdx.y * RT;
+  if (rho0 >= R) return;
+  const int last = (rho0 + RT < R ? rho0 + RT : R) - 1;
+  const int len = row_len(q.n, q.L, s.causal, last / group);
+  const int beg = blockIdx.x * range, end = beg + range < len ? beg + range : len;
+  if (beg >= end) return;
+  const int lanes = kThreads / P, kl = t / P, c = t % P;
+  uint64_t ax[RT] = {}, ay[RT] = {};
+  for (int j0 = beg; j0 < end; j0 += kValStage) {
+    __syncthreads();
+    for (int e = t; e < kValStage * RT; e += kThreads) {
+      const int kk = e % kValStage, rr = e / kValStage, rho = rho0 + rr, i = rho / group, j = j0 + kk;
+      uint64_t d = 0, u = 0;
+      if (rho < R && j < end && j < row_len(q.n, q.L, s.causal, i)) {
+        const int64_t at = q.base + (kh * group + rho % group) * q.blk + row_off(q.n, q.L, s.causal, i) + j;
+        const uint64_t a0 = o.a[0][at], a1 = o.a[1][at];
+        d = (o.x[0][at] - a0) + (o.x[1][at] - a1);
+        u = d + a0 + a1;
+      }
+      sU[kk][rr] = u;
+      sD[kk][rr] = d;
+    }
+    for (int e = t; e < kValStage; e += kThreads) s_key[e] = j0 + e < end ? key_off(s, b, kh, j0 + e, o.status) : -1;
+    __syncthreads();
+    if (kl < lanes)
+      for (int kk = kl; kk < kValStage; kk += lanes) {
+        const int64_t at = s_key[kk];
+        if (at < 0) continue;
+        const ulonglong2 e = ld_stream(o.e + at + 2 * c), b0 = ld_stream(o.b[0] + at + 2 * c),
+                         b1 = ld_stream(o.b[1] + at + 2 * c);
+        const uint64_t wx = b0.x + b1.x, wy = b0.y + b1.y;
+#pragma unroll
+        for (int rr = 0; rr < RT; rr++) {
+          const uint64_t u = sU[kk][rr], d = sD[kk][rr];
+          ax[rr] += u * e.x + d * wx;
+          ay[rr] += u * e.y + d * wy;
+        }
+      }
+  }
+  if (kl >= lanes) return;
+#pragma unroll
+  for (int rr = 0; rr < RT; rr++) {
+    const int rho = rho0 + rr;
+    if (rho >= R) break;
+    unsigned long long* at = reinterpret_cast<unsigned long long*>(
+        o.out + (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + 2 * c);
+    atomicAdd(at, static_cast<unsigned long long>(ax[rr]));
+    atomicAdd(at + 1, static_cast<unsigned long long>(ay[rr]));
+  }
+}
+
+// ---- many rows: 64 x 64 output tiles on the integer pipes -------------------
+constexpr int kT = 64, kTK = 16;
+
+template <bool SCORES>
+__global__ void __launch_bounds__(kThreads) attn_tile_kernel(const __grid_constant__ AttnSeqs s,
+                                                             const __grid_constant__ AttnOperands o) {
+  __shared__ uint64_t sU[kTK][kT + 1], sD[kTK][kT + 1], sE[kTK][kT + 1], sW[kTK][kT + 1];
+  __shared__ int64_t s_key[kT];
+  const int t = threadIdx.x, dh = s.head_dim, group = s.q_heads / s.kv_heads;
+  const int b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads;
+  SeqInfo q;
+  if (!seq_info(s, b, o.status, q)) return;
+  const int R = group * q.n, rho0 = blockIdx.y * kT, n0 = blockIdx.x * kT;
+  if (rho0 >= R) return;
+  const int last = (rho0 + kT < R ? rho0 + kT : R) - 1;
+  const int len = row_len(q.n, q.L, s.causal, last / group);
+  const int cols = SCORES ? len : dh, depth = SCORES ? dh : len;
+  if (n0 >= cols || depth == 0) return;
+  if (SCORES) {
+    for (int e = t; e < kT; e += kThreads) s_key[e] = n0 + e < len ? key_off(s, b, kh, n0 + e, o.status) : -1;
+    __syncthreads();
+  }
+  const int tx = t % 16, ty = t / 16;
+  uint64_t acc[4][4] = {};
+  for (int k0 = 0; k0 < depth; k0 += kTK) {
+    if (!SCORES) {
+      if (t < kTK) s_key[t] = k0 + t < len ? key_off(s, b, kh, k0 + t, o.status) : -1;
+      __syncthreads();
+    }
+    for (int e = t; e < kT * kTK; e += kThreads) {
+      const int rr = e / kTK, kk = e % kTK, rho = rho0 + rr, i = rho / group, k = k0 + kk;
+      uint64_t d = 0, u = 0;
+      if (rho < R) {
+        const int head = kh * group + rho % group;
+        if (SCORES) {
+          if (k < dh) {
+            const int64_t at = (static_cast<int64_t>(q.t0 + i) * s.q_heads + head) * dh + k;
+            d = o.x[0][at];
+            u = d + o.a[0][at] + o.a[1][at];
+          }
+        } else if (k < row_len(q.n, q.L, s.causal, i)) {
+          const int64_t at = q.base + head * q.blk + row_off(q.n, q.L, s.causal, i) + k;
+          const uint64_t a0 = o.a[0][at], a1 = o.a[1][at];
+          d = (o.x[0][at] - a0) + (o.x[1][at] - a1);
+          u = d + a0 + a1;
+        }
+      }
+      sU[kk][rr] = u;
+      sD[kk][rr] = d;
+    }
+    for (int e = t; e < kT * kTK; e += kThreads) {
+      const int kk = SCORES ? e % kTK : e / kT, cc = SCORES ? e / kTK : e % kT;
+      const int64_t at = SCORES ? s_key[cc] : s_key[kk];
+      const int w = SCORES ? k0 + kk : n0 + cc;
+      uint64_t ev = 0, wv = 0;
+      if (at >= 0 && w < dh) {
+        ev = o.e[at + w];
+        wv = o.b[0][at + w] + o.b[1][at + w];
+      }
+      sE[kk][cc] = ev;
+      sW[kk][cc] = wv;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int kk = 0; kk < kTK; kk++) {
+      uint64_t u[4], d[4];
+#pragma unroll
+      for (int y = 0; y < 4; y++) {
+        u[y] = sU[kk][ty * 4 + y];
+        d[y] = sD[kk][ty * 4 + y];
+      }
+#pragma unroll
+      for (int x = 0; x < 4; x++) {
+        const uint64_t e = sE[kk][tx + 16 * x], w = sW[kk][tx + 16 * x];
+#pragma unroll
+        for (int y = 0; y < 4; y++) acc[y][x] += u[y] * e + d[y] * w;
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int y = 0; y < 4; y++) {
+    const int rho = rho0 + ty * 4 + y, i = rho / group, head = kh * group + rho % group;
+    if (rho >= R) continue;
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+      const int col = n0 + tx + 16 * x;
+      if (SCORES) {
+        if (col >= row_len(q.n, q.L, s.causal, i)) continue;
+        const int64_t at = q.base + head * q.blk + row_off(q.n, q.L, s.causal, i) + col;
+        o.out[at] = acc[y][x] + o.c[0][at] + o.c[1][at] + o.r;
+      } else if (col < dh) {
+        o.out[(static_cast<int64_t>(q.t0 + i) * s.q_heads + head) * dh + col] += acc[y][x];
+      }
+    }
+  }
+}
+
+int check_seqs(const sufb200_attn_seqs* s, const char* who) {
+  const std::string at = std::string(who) + ": ";
+  if (!s) return fail(SUFB200_ERR_INVALID, at + "null sequences");
+  if (s->batch < 0 || s->max_pages < 0 || s->pages < 0 || s->max_q < 0 || s->max_ctx < 0 || s->tokens < 0 || s->packed < 0)
+    return fail(SUFB200_ERR_INVALID, at + "negative size");
+  if (s->page_size < 1 || s->kv_heads < 1 || s->q_heads < s->kv_heads || s->q_heads % s->kv_heads)
+    return fail(SUFB200_ERR_INVALID, at + "page size, or query heads not a multiple of key heads");
+  if (s->head_dim < 2 || s->head_dim > 256 || s->head_dim % 2)
+    return fail(SUFB200_ERR_UNSUPPORTED, at + "head size must be even, 2..256");
+  if (static_cast<int64_t>(s->batch) * s->kv_heads > 65535)
+    return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 65535 (sequence, key head) pairs");
+  if (static_cast<int64_t>(s->q_heads / s->kv_heads) * s->max_q > 1 << 21)
+    return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^21 rows per (sequence, key head)");
+  if (static_cast<int64_t>(s->max_ctx) > static_cast<int64_t>(s->max_pages) * s->page_size)
+    return fail(SUFB200_ERR_INVALID, at + "max_ctx is more than the block table's pages hold");
+  if (static_cast<__int128>(s->q_heads) * s->max_q * s->max_ctx >= (static_cast<__int128>(1) << 60))
+    return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^60 packed words");
+  if (s->batch > 0 && (!s->d_cu_q || !s->d_ctx || !s->d_row_base || (s->max_ctx > 0 && !s->d_block_table)))
+    return fail(SUFB200_ERR_INVALID, at + "null sequence array");
+  return SUFB200_OK;
+}
+
+int check_operands(const AttnOperands& o, const char* who) {
+  const std::string at = std::string(who) + ": ";
+  const void* words[] = {o.x[0], o.x[1], o.a[0], o.a[1], o.c[0], o.c[1], o.out};
+  for (const void* p : words)
+    if (!p || !aligned_to(p, 8)) return fail(SUFB200_ERR_INVALID, at + "null or misaligned operand");
+  for (const void* p : {static_cast<const void*>(o.e), static_cast<const void*>(o.b[0]), static_cast<const void*>(o.b[1])})
+    if (!p || !aligned_to(p, 16)) return fail(SUFB200_ERR_INVALID, at + "the cache's pools must be 16-byte aligned");
+  return SUFB200_OK;
+}
+
+// Rows of a (sequence, key head) up to which the row kernels are used.
+constexpr int kFewRows = 16;
+
+}  // namespace
+
+int attn_check_ctx(sufb200_ctx ctx) {
+  if (!ctx) return fail(SUFB200_ERR_INVALID, "null context");
+  if (ctx->device < 0) return fail(SUFB200_ERR_UNSUPPORTED, "host-only context: no device to evaluate on");
+  const cudaError_t e = cudaSetDevice(ctx->device);
+  return e == cudaSuccess ? SUFB200_OK : fail(SUFB200_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(e));
+}
+
+}  // namespace sufb200
+
+using namespace sufb200;
+
+extern "C" {
+
+int sufb200_attn_scores_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, const uint64_t* d_dq,
+                             const uint64_t* const* d_a, const uint64_t* const* d_c, const uint64_t* r,
+                             const uint64_t* d_ek, const uint64_t* const* d_bk, uint64_t* d_xhat, void* stream) {
+  if (int rc = check_seqs(seqs, "attn_scores_pair")) return rc;
+  if (seqs->batch == 0 || seqs->packed == 0 || seqs->max_q == 0 || seqs->max_ctx == 0) return SUFB200_OK;
+  if (!d_a || !d_c || !r || !d_bk) return fail(SUFB200_ERR_INVALID, "attn_scores_pair: null pointer array");
+  AttnOperands o{{d_dq, d_dq}, {d_a[0], d_a[1]}, {d_c[0], d_c[1]}, d_ek, {d_bk[0], d_bk[1]}, r[0] + r[1], d_xhat,
+                 nullptr};
+  if (int rc = check_operands(o, "attn_scores_pair")) return rc;
+  if (int rc = attn_check_ctx(ctx)) return rc;
+  o.status = ctx->d_status;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int rows = seqs->q_heads / seqs->kv_heads * seqs->max_q;
+  const unsigned z = static_cast<unsigned>(seqs->batch) * seqs->kv_heads;
+  if (rows <= kFewRows) {
+    const unsigned x = (seqs->max_ctx + kKeyChunk - 1) / kKeyChunk;
+    if (rows <= 4)
+      scores_rows_kernel<4><<<dim3(x, (rows + 3) / 4, z), kThreads, 4 * seqs->head_dim * 16, st>>>(*seqs, o);
+    else
+      scores_rows_kernel<8><<<dim3(x, (rows + 7) / 8, z), kThreads, 8 * seqs->head_dim * 16, st>>>(*seqs, o);
+  } else {
+    attn_tile_kernel<true><<<dim3((seqs->max_ctx + kT - 1) / kT, (rows + kT - 1) / kT, z), kThreads, 0, st>>>(*seqs, o);
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? SUFB200_OK : fail(SUFB200_ERR_CUDA, std::string("attn_scores_pair: ") + cudaGetErrorString(e));
+}
+
+int sufb200_attn_values_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, const uint64_t* const* d_p,
+                             const uint64_t* const* d_a, const uint64_t* const* d_c, const uint64_t* r,
+                             const uint64_t* d_ev, const uint64_t* const* d_bv, uint64_t* d_xhat, void* stream) {
+  if (int rc = check_seqs(seqs, "attn_values_pair")) return rc;
+  if (seqs->batch == 0 || seqs->max_q == 0 || seqs->tokens == 0) return SUFB200_OK;
+  if (!d_p || !d_a || !d_c || !r || !d_bv) return fail(SUFB200_ERR_INVALID, "attn_values_pair: null pointer array");
+  AttnOperands o{{d_p[0], d_p[1]}, {d_a[0], d_a[1]}, {d_c[0], d_c[1]}, d_ev, {d_bv[0], d_bv[1]}, r[0] + r[1], d_xhat,
+                 nullptr};
+  if (seqs->packed == 0) {  // every row is empty: no probability is read
+    o.x[0] = o.x[1] = o.a[0] = o.a[1] = o.c[0];
+  }
+  if (int rc = check_operands(o, "attn_values_pair")) return rc;
+  if (int rc = attn_check_ctx(ctx)) return rc;
+  o.status = ctx->d_status;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int rows = seqs->q_heads / seqs->kv_heads * seqs->max_q;
+  const unsigned z = static_cast<unsigned>(seqs->batch) * seqs->kv_heads;
+  const int64_t words = seqs->tokens * seqs->q_heads * seqs->head_dim;
+  const int64_t want = (words + kThreads - 1) / kThreads, cap = static_cast<int64_t>(ctx->sm_count) * 8;
+  values_init_kernel<<<static_cast<unsigned>(want < cap ? want : cap), kThreads, 0, st>>>(*seqs, o);
+  if (seqs->packed > 0 && seqs->max_ctx > 0) {
+    if (rows <= kFewRows) {
+      const int range = 256;
+      const unsigned x = (seqs->max_ctx + range - 1) / range;
+      if (rows <= 4)
+        values_rows_kernel<4><<<dim3(x, (rows + 3) / 4, z), kThreads, 0, st>>>(*seqs, o, range);
+      else
+        values_rows_kernel<8><<<dim3(x, (rows + 7) / 8, z), kThreads, 0, st>>>(*seqs, o, range);
+    } else {
+      attn_tile_kernel<false>
+          <<<dim3((seqs->head_dim + kT - 1) / kT, (rows + kT - 1) / kT, z), kThreads, 0, st>>>(*seqs, o);
+    }
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? SUFB200_OK : fail(SUFB200_ERR_CUDA, std::string("attn_values_pair: ") + cudaGetErrorString(e));
+}
+
+}  // extern "C"

@@ -1,0 +1,105 @@
+// attention.hpp -- what the kernels of attention over a paged cache of shares
+// have in common (attention.cu, attention_rope.cu, rowmax.cu).  Internal.
+#pragma once
+
+#include <string>
+
+#include "kernels.hpp"
+#include "sufb200_internal.cuh"
+
+namespace sufb200 {
+
+// The packed sequences as the kernels see them (a copy of the public struct:
+// plain device pointers and sizes).
+using AttnSeqs = sufb200_attn_seqs;
+
+// One sequence: n new tokens (packed tokens t0 .. t0 + n), L cached tokens
+// (the new ones included), its packed rows at word `base`, `blk` words a head.
+struct SeqInfo {
+  int n, L, t0;
+  int64_t base, blk;
+};
+
+// Valid keys of query i.  Causal: query i is token L - n + i of the sequence
+// and sees itself and what is before it; with L < n the first n - L queries
+// see nothing (empty rows).
+SUFB200_HD int row_len(int n, int L, int causal, int i) {
+  if (!causal) return L;
+  const int m = L - n + i + 1;
+  return m < 0 ? 0 : m;
+}
+
+// Words in front of row i of one (sequence, head): the sum of the lengths of
+// the rows before it.
+SUFB200_HD int64_t row_off(int n, int L, int causal, int i) {
+  if (!causal) return static_cast<int64_t>(i) * L;
+  const int64_t first = L - n + 1;  // length of row 0 where it is positive
+  const int64_t skip = first < 0 ? -first : 0;  // rows 0 .. skip - 1 have lengths below 0: empty
+  const int64_t k = i - skip;
+  if (k <= 0) return 0;
+  const int64_t f = first < 0 ? 0 : first;
+  return k * f + k * (k - 1) / 2;
+}
+
+// Whether a sequence's lengths and rows lie inside what the host arguments
+// say (so every address formed from them does too); fills q.
+SUFB200_HD bool seq_fits(const AttnSeqs& s, int c0, int c1, int L, int64_t base, SeqInfo& q) {
+  q = SeqInfo{0, L, c0, base, 0};
+  if (c0 < 0 || c1 < c0 || c1 > s.tokens || c1 - c0 > s.max_q || L < 0 || L > s.max_ctx ||
+      L > static_cast<int64_t>(s.max_pages) * s.page_size || base < 0 || base > s.packed)
+    return false;
+  q.n = c1 - c0;
+  q.blk = row_off(q.n, L, s.causal, q.n);
+  return q.blk * s.q_heads <= s.packed - base;
+}
+
+// Word offset of place j % page_size of page pg, key head kh, in a pool
+// [pages][kv_heads][page_size][head_dim]; -1 when the pool has no such page.
+SUFB200_HD int64_t page_word(const AttnSeqs& s, int pg, int kh, int j) {
+  if (pg < 0 || pg >= s.pages) return -1;
+  return ((static_cast<int64_t>(pg) * s.kv_heads + kh) * s.page_size + j % s.page_size) * s.head_dim;
+}
+
+#if defined(__CUDACC__)
+// Sequence b; false (and the status word flagged) when the device arrays do
+// not fit what the host was told.
+__device__ __forceinline__ bool seq_info(const AttnSeqs& s, int b, uint32_t* status, SeqInfo& q) {
+  const bool ok = seq_fits(s, s.d_cu_q[b], s.d_cu_q[b + 1], s.d_ctx[b], s.d_row_base[b], q);
+  if (!ok) atomicOr(status, kStatusBadArgument);
+  return ok;
+}
+
+// Word offset of cached token j of sequence b, key head kh; -1 (and the
+// status word flagged) when the block table names no page of the pool.
+__device__ __forceinline__ int64_t key_off(const AttnSeqs& s, int b, int kh, int j, uint32_t* status) {
+  const int64_t at = page_word(s, s.d_block_table[static_cast<int64_t>(b) * s.max_pages + j / s.page_size], kh, j);
+  if (at < 0) atomicOr(status, kStatusBadArgument);
+  return at;
+}
+
+// A 16-byte load of cached words, which one CTA reads once: past L1.
+__device__ __forceinline__ ulonglong2 ld_stream(const uint64_t* p) {
+  ulonglong2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "l"(p));
+  return v;
+}
+#endif
+
+// Context check of the entry points (null, host-only, device made current).
+int attn_check_ctx(sufb200_ctx ctx);
+
+inline bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// The operands of one attention product, both parties.
+struct AttnOperands {
+  const uint64_t* x[2];  // scores: x[0] = opened D [tokens][q_heads][head_dim]; values: the parties' shares of P (packed)
+  const uint64_t* a[2];  // the triple's A: [tokens][q_heads][head_dim], or packed
+  const uint64_t* c[2];  // the triple's C: packed, or [tokens][q_heads][head_dim]
+  const uint64_t* e;     // opened pool [pages][kv_heads][page_size][head_dim]
+  const uint64_t* b[2];  // its masks' shares
+  uint64_t r;            // r_0 + r_1
+  uint64_t* out;
+  uint32_t* status;
+};
+
+}  // namespace sufb200

@@ -71,6 +71,7 @@ size_t prefix_min_n() {
 }
 
 constexpr size_t kAccBytes = 256;  // RangeAcc slot, keeps the frontier 256-byte aligned
+static_assert(kAccBytes == sufb200::kTruncTablesHead, "layout of the truncation tables");
 
 // Host-side per-context device buffers for the host-buffer entry points.
 struct HostIo {

@@ -102,6 +102,10 @@ cudaError_t launch_jobs_copy(const sufb200_ctx_s* ctx, const JobTable& t, uint64
 cudaError_t launch_trunc_bundle_pair(const sufb200_ctx_s* ctx, const TruncLaunch& a0, const TruncLaunch& a1,
                                      cudaStream_t st);
 
+// Bytes of a bundle's full-domain tables (sufb200_trunc_tables_dev) before its
+// first query's entries.
+constexpr size_t kTruncTablesHead = 256;
+
 // Reference GPU-backend key formats (ref_formats.cu).
 struct RefFmtLaunch {
   const uint8_t* keys;

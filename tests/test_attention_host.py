@@ -1,0 +1,272 @@
+"""CPU tests of attention over a cache of shares: the kernels' address
+arithmetic (a CPU build of the same code), the refusals of the C entries
+(a host-only context: a call with good arguments gets as far as "no device")
+and of the Python wrappers, and the rotary tables."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+import subprocess
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+ROOT = Path(__file__).resolve().parents[1]
+
+
+@pytest.fixture(scope="module")
+def emu(tmp_path_factory):
+    out = tmp_path_factory.mktemp("attn_emu") / "libattn.so"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fPIC", "-shared", "-I/usr/local/cuda/include", "-o", str(out),
+                    str(ROOT / "tests" / "hostemu" / "attn_shim.cpp")], check=True)
+    E = C.CDLL(str(out))
+    E.emu_row_off.restype = C.c_int64
+    E.emu_page_word.restype = C.c_int64
+    E.emu_sizeof.restype = C.c_size_t
+    E.emu_seq_fits.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int64, C.c_void_p]
+    E.emu_page_word.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int]
+    return E
+
+
+def test_struct_mirrors(emu):
+    from suf_b200._lib import AttnSeqs, RopeAppend
+
+    assert emu.emu_sizeof(0) == C.sizeof(RopeAppend) and emu.emu_sizeof(1) == C.sizeof(AttnSeqs)
+
+
+@pytest.mark.parametrize("causal", [0, 1])
+def test_row_offsets_match_brute_force(emu, causal):
+    for n in range(0, 9):
+        for L in range(0, 12):
+            lens = [max(0, L - n + i + 1) if causal else L for i in range(n)]
+            assert [emu.emu_row_len(n, L, causal, i) for i in range(n)] == lens
+            assert [emu.emu_row_off(n, L, causal, i) for i in range(n + 1)] == [sum(lens[:i]) for i in range(n + 1)]
+    # past 32 bits
+    n, L = 100_000, 200_000
+    want = sum(L - n + i + 1 for i in range(n)) if causal else n * L
+    assert want > 2**33 and emu.emu_row_off(n, L, causal, n) == want
+
+
+def _seqs(**kw):
+    from suf_b200._lib import AttnSeqs
+
+    s = AttnSeqs()
+    for k, v in dict(tokens=10, packed=1000, batch=2, max_pages=4, page_size=8, pages=5, q_heads=4, kv_heads=2,
+                     head_dim=64, causal=1, max_q=6, max_ctx=30).items():
+        setattr(s, k, v)
+    for k, v in kw.items():
+        setattr(s, k, v)
+    return s
+
+
+def test_sequences_outside_the_host_bounds_are_refused(emu):
+    s, blk = _seqs(), C.c_int64()
+
+    def fits(*a):
+        return emu.emu_seq_fits(C.byref(s), *a, C.byref(blk))
+
+    assert fits(0, 6, 30, 0) and blk.value == sum(range(25, 31))
+    assert fits(4, 10, 6, 1000 - 4 * 21)
+    for bad in [(-1, 3, 5, 0), (3, 2, 5, 0), (5, 11, 5, 0), (0, 7, 5, 0), (0, 3, -1, 0), (0, 3, 31, 0), (0, 3, 5, -1),
+                (0, 3, 5, 1001), (4, 10, 6, 1000 - 4 * 21 + 1), (-2**31, 2**31 - 1, 2**31 - 1, 0),
+                (0, 2**31 - 1, 2**31 - 1, 2**63 - 1)]:
+        assert not fits(*bad), bad
+    s.max_ctx = 40
+    assert not fits(0, 3, 33, 0)  # more than four pages of eight
+
+
+def test_pages_outside_the_pool_are_refused(emu):
+    s = _seqs()
+    assert emu.emu_page_word(C.byref(s), 0, 0, 0) == 0
+    assert emu.emu_page_word(C.byref(s), 4, 1, 13) == ((4 * 2 + 1) * 8 + 5) * 64
+    for pg in (-1, 5, 2**31 - 1, -2**31):
+        assert emu.emu_page_word(C.byref(s), pg, 0, 0) == -1
+    # a long cache: offsets past 32 bits
+    s.pages, s.kv_heads, s.page_size, s.head_dim = 10**6, 8, 64, 128
+    assert emu.emu_page_word(C.byref(s), 10**6 - 1, 7, 63) == 10**6 * 8 * 64 * 128 - 128
+
+
+# -- refusals of the C entries ----------------------------------------------------
+
+@pytest.fixture(scope="module")
+def host():
+    from suf_b200 import _lib
+    from suf_b200.build import build
+
+    build()
+    h = C.c_void_p()
+    _lib.check(_lib.lib().sufb200_ctx_create(-1, C.byref(h)))
+    yield h
+    _lib.lib().sufb200_ctx_destroy(h)
+
+
+P16, P8, P4 = 0x10000, 0x10008, 0x10004  # addresses the refused calls never touch
+
+
+def _arr(*v):
+    return (C.c_void_p * 2)(*v)
+
+
+def _attn(host, which, seqs, x=None, a=(P16, P16), c=(P16, P16), e=P16, b=(P16, P16), out=P16, r=(1, 2)):
+    from suf_b200 import _lib
+
+    L = _lib.lib()
+    rr = (C.c_uint64 * 2)(*r)
+    if which == "scores":
+        return L.sufb200_attn_scores_pair(host, C.byref(seqs), P16 if x is None else x, _arr(*a), _arr(*c), rr, e,
+                                          _arr(*b), out, None)
+    return L.sufb200_attn_values_pair(host, C.byref(seqs), _arr(*(x or (P16, P16))), _arr(*a), _arr(*c), rr, e,
+                                      _arr(*b), out, None)
+
+
+PTRS = dict(d_cu_q=P16, d_ctx=P16, d_row_base=P16, d_block_table=P16)
+
+
+@pytest.mark.parametrize("which", ["scores", "values"])
+def test_attention_refusals(host, which):
+    from suf_b200 import _lib
+
+    ok = _seqs(**PTRS)
+    assert _attn(host, which, ok) == _lib.ERR_UNSUPPORTED  # good arguments: only the device is missing
+    assert b"host-only" in _lib.lib().sufb200_last_error()
+    for bad, code in [(dict(head_dim=63), _lib.ERR_UNSUPPORTED), (dict(head_dim=258), _lib.ERR_UNSUPPORTED),
+                      (dict(head_dim=0), _lib.ERR_UNSUPPORTED), (dict(q_heads=3), _lib.ERR_INVALID),
+                      (dict(kv_heads=0), _lib.ERR_INVALID), (dict(page_size=0), _lib.ERR_INVALID),
+                      (dict(max_ctx=33), _lib.ERR_INVALID), (dict(batch=-1), _lib.ERR_INVALID),
+                      (dict(tokens=-1), _lib.ERR_INVALID), (dict(d_ctx=None), _lib.ERR_INVALID),
+                      (dict(d_block_table=None), _lib.ERR_INVALID), (dict(batch=40000), _lib.ERR_UNSUPPORTED),
+                      (dict(max_q=2**21), _lib.ERR_UNSUPPORTED),
+                      (dict(q_heads=2**20, kv_heads=2**16 - 1 + 1, batch=1), _lib.ERR_UNSUPPORTED)]:
+        assert _attn(host, which, _seqs(**{**PTRS, **bad})) == code, bad
+        assert b"head" in _lib.lib().sufb200_last_error() or b"attn_" in _lib.lib().sufb200_last_error()
+    for kw in [dict(a=(P16, None)), dict(c=(P4, P16)), dict(out=None), dict(out=P4), dict(e=P8), dict(b=(P16, P8)),
+               dict(e=None)]:
+        assert _attn(host, which, ok, **kw) == _lib.ERR_INVALID, kw
+    assert _attn(host, which, _seqs(**{**PTRS, "batch": 0})) == _lib.OK  # nothing to do
+
+
+def _rope(**kw):
+    from suf_b200._lib import RopeAppend
+
+    a = RopeAppend()
+    for f in ("d_q", "d_k", "d_v", "d_a", "d_bk", "d_bv", "d_tables"):
+        setattr(a, f, _arr(P16, P16))
+    for f in ("d_positions", "d_slots", "d_cos", "d_sin", "d_dq", "d_ek", "d_ev"):
+        setattr(a, f, P16)
+    for k, v in dict(tokens=3, q_heads=4, kv_heads=2, head_dim=64, rot_dim=64, max_pos=16, pages=2,
+                     page_size=8).items():
+        setattr(a, k, v)
+    for p in (0, 1):
+        d = a.trunc[p]
+        d.kind, d.frac_bits, d.party, d.nq, d.carry_a, d.carry_b = 2, 12, p, 2, 0, 1
+        d.q_bits[0] = d.q_bits[1] = 12
+        d.sign_a = d.sign_b = d.wrap_q = -1
+    for k, v in kw.items():
+        if k in ("kind", "frac_bits", "party", "carry_a", "nq"):
+            setattr(a.trunc[1], k, v)
+        else:
+            setattr(a, k, v)
+    return a
+
+
+def test_rope_append_refusals(host):
+    from suf_b200 import _lib
+
+    L = _lib.lib()
+
+    def call(**kw):
+        a = _rope(**kw)
+        return L.sufb200_rope_append_pair(host, C.byref(a), None)
+
+    assert call() == _lib.ERR_UNSUPPORTED and b"host-only" in L.sufb200_last_error()
+    assert call(tokens=0) == _lib.OK
+    assert call(carry_a=-1, nq=0, d_tables=_arr(P16, None)) == _lib.ERR_UNSUPPORTED  # no queries: no tables
+    assert call(q_heads=0, d_q=_arr(None, None), d_a=_arr(None, None), d_dq=None) == _lib.ERR_UNSUPPORTED
+    assert call(rot_dim=0, d_positions=None, d_cos=None, d_sin=None, d_tables=_arr(None, None)) == _lib.ERR_UNSUPPORTED
+    for kw in [dict(tokens=-1), dict(kv_heads=0), dict(page_size=0), dict(pages=0), dict(rot_dim=66), dict(rot_dim=3),
+               dict(d_slots=None), dict(d_k=_arr(P16, None)), dict(d_q=_arr(P16, None)), dict(d_a=_arr(P4, P16)),
+               dict(d_bv=_arr(P4, P16)), dict(d_dq=None), dict(d_ek=P4), dict(d_positions=None), dict(d_cos=None),
+               dict(max_pos=0), dict(kind=1), dict(frac_bits=11), dict(party=0), dict(carry_a=2), dict(nq=5),
+               dict(d_tables=_arr(P16, None)), dict(d_tables=_arr(P16, P8))]:
+        assert call(**kw) == _lib.ERR_INVALID, kw
+    assert call(head_dim=65) == _lib.ERR_UNSUPPORTED
+    assert L.sufb200_rope_append_pair(host, None, None) == _lib.ERR_INVALID
+
+
+def test_rowmax_refusals(host):
+    from suf_b200 import _lib
+
+    L = _lib.lib()
+    r = (C.c_uint64 * 2)(1, 2)
+    g = _arr(P16, P16)
+    assert L.sufb200_rowmax_open_pair(host, g, 4, 9, P16, P16, r, P16, None) == _lib.ERR_UNSUPPORTED
+    assert L.sufb200_rowmax_open_pair(host, g, 0, 9, P16, P16, r, P16, None) == _lib.OK
+    assert L.sufb200_rowmax_open_pair(host, g, 4, 1, P16, P16, r, P16, None) == _lib.OK
+    for args in [(None, 4, 9, P16, P16, r, P16), (g, -1, 9, P16, P16, r, P16), (g, 4, 9, None, P16, r, P16),
+                 (g, 4, 9, P16, P16, None, P16), (g, 4, 9, P16, P16, r, P4), (_arr(P16, None), 4, 9, P16, P16, r, P16)]:
+        assert L.sufb200_rowmax_open_pair(host, *args, None) == _lib.ERR_INVALID, args
+    assert L.sufb200_rowmax_round_pair(host, g, g, 4, 9, P16, P16, P16, r, g, P16, None) == _lib.ERR_UNSUPPORTED
+    assert L.sufb200_rowmax_round_pair(host, g, g, 4, 9, P16, P16, None, None, g, None, None) == _lib.ERR_UNSUPPORTED
+    for args in [(g, _arr(None, P16), 4, 9, P16, P16, P16, r, g, P16), (g, g, 4, 9, P16, P16, None, r, g, P16),
+                 (g, g, 4, 9, P16, P16, P16, None, g, P16), (g, g, 4, 9, P16, P16, P16, r, _arr(P16, P4), P16),
+                 (g, g, 4, -1, P16, P16, P16, r, g, P16)]:
+        assert L.sufb200_rowmax_round_pair(host, *args, None) == _lib.ERR_INVALID, args
+    assert L.sufb200_maxdiff_ragged_pair(host, g, g, 4, 9, P16, P16, g, None) == _lib.ERR_UNSUPPORTED
+    for args in [(g, g, 4, 9, P16, None, g), (g, _arr(None, P16), 4, 9, P16, P16, g), (g, g, -4, 9, P16, P16, g)]:
+        assert L.sufb200_maxdiff_ragged_pair(host, *args, None) == _lib.ERR_INVALID, args
+
+
+# -- refusals of the wrappers ---------------------------------------------------------
+
+class _Ctx:
+    device = 0
+
+
+def test_wrappers_refuse_wrong_tensors():
+    import torch
+
+    from suf_b200 import attention as at
+
+    x = torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(ValueError, match="cuda:0"):
+        at._want(_Ctx, "x", x, (4,))
+    with pytest.raises(ValueError, match="int64"):
+        at._want(_Ctx, "x", x.to(torch.int32), (4,))
+    with pytest.raises(ValueError, match="both parties"):
+        at._pair(_Ctx, "x", x, (4,))
+    with pytest.raises(ValueError, match="both parties"):
+        at._masks((1,))
+    with pytest.raises(ValueError, match="cuda:0"):
+        at._strided(_Ctx, "q", (torch.zeros(1, 2, 4, dtype=torch.int64),) * 2, 1, 2, 4)
+    for bad in [dict(rot_dim=3), dict(max_pos=0), dict(frac_bits=0), dict(frac_bits=17), dict(scale=0.0),
+                dict(base=-1.0), dict(low_freq=1.0), dict(low_freq=2.0, high_freq=1.0, trained_pos=64)]:
+        with pytest.raises(ValueError):
+            at.rope_table_words(**{**dict(max_pos=8, rot_dim=4, frac_bits=12), **bad})
+
+
+def test_rope_tables_are_rounded_cosines_of_the_definition():
+    """Every entry is the nearest fixed-point value of the exact cosine or sine:
+    off by at most half a unit, plus the float64 angle's own error (position
+    131071 times a frequency: 2^17 * 2^-53 in the angle, 2^-24 units at 12 bits)."""
+    from suf_b200.attention import rope_table_words
+
+    cos, sin = rope_table_words(131072, 8, 12, base=500000.0, scale=4.0)
+    for pos in (0, 1, 77, 4095, 131071):
+        for i in range(4):
+            ang = math.fmod(pos * 500000.0 ** (-i / 4) / 4.0, 2 * math.pi)
+            assert abs(cos[pos, i] - 4096 * math.cos(ang)) <= 0.5 + 2**-20
+            assert abs(sin[pos, i] - 4096 * math.sin(ang)) <= 0.5 + 2**-20
+    # blended scaling: fast pairs stay, slow pairs are stretched, between them a blend
+    plain, _ = rope_table_words(512, 16, 12)
+    all_, _ = rope_table_words(512, 16, 12, scale=8.0)
+    mix, _ = rope_table_words(512, 16, 12, scale=8.0, low_freq=1.0, high_freq=4.0, trained_pos=256)
+    turns = 256 * 10000.0 ** (-np.arange(8) / 8) / (2 * math.pi)
+    assert (turns > 4).any() and (turns < 1).any() and ((turns > 1) & (turns < 4)).any()
+    for i in range(8):
+        if turns[i] >= 4:
+            assert (mix[:, i] == plain[:, i]).all()
+        elif turns[i] <= 1:
+            assert (mix[:, i] == all_[:, i]).all()
+        else:
+            assert (mix[:, i] != plain[:, i]).any() and (mix[:, i] != all_[:, i]).any()
