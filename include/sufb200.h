@@ -764,18 +764,20 @@ typedef struct sufb200_rope_append {
 int sufb200_rope_append_pair(sufb200_ctx ctx, const sufb200_rope_append* args, void* stream);
 
 /* The packed sequences of an attention call.  Sequence b has the new tokens
- * d_cu_q[b] .. d_cu_q[b+1] (cu_q[0] = 0) and d_ctx[b] cached tokens, the new
- * ones included, in the pages d_block_table[b][j / page_size].  Rows are
- * packed in (sequence, head, query) order; row (b, h, i) has
+ * d_cu_q[b] .. d_cu_q[b+1] (cu_q[0] = 0) and ctx = d_cu_ctx[b+1] - d_cu_ctx[b]
+ * cached tokens, the new ones included, in the pages
+ * d_block_table[b][j / page_size].  Rows are packed in (sequence, head, query)
+ * order; row (b, h, i) has
  *   len = causal ? max(0, ctx - n + i + 1) : ctx
  * words, and sequence b's rows start at word d_row_base[b].  max_q and max_ctx
- * bound the lengths, tokens and packed the token and word counts. */
+ * bound the lengths; tokens, cached and packed the sums of the new tokens, the
+ * cached tokens and the words (workspaces are sized by them). */
 typedef struct sufb200_attn_seqs {
   const int32_t* d_cu_q;        /* [batch + 1] */
-  const int32_t* d_ctx;         /* [batch] */
+  const int32_t* d_cu_ctx;      /* [batch + 1] */
   const int64_t* d_row_base;    /* [batch] */
   const int32_t* d_block_table; /* [batch][max_pages] */
-  int64_t tokens, packed;
+  int64_t tokens, cached, packed;
   int32_t batch, max_pages, page_size, pages, q_heads, kv_heads, head_dim, causal, max_q, max_ctx;
 } sufb200_attn_seqs;
 

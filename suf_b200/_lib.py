@@ -71,8 +71,8 @@ class AttnSeqs(C.Structure):
     """Mirror of sufb200_attn_seqs."""
 
     _fields_ = [
-        ("d_cu_q", C.c_void_p), ("d_ctx", C.c_void_p), ("d_row_base", C.c_void_p), ("d_block_table", C.c_void_p),
-        ("tokens", C.c_int64), ("packed", C.c_int64),
+        ("d_cu_q", C.c_void_p), ("d_cu_ctx", C.c_void_p), ("d_row_base", C.c_void_p), ("d_block_table", C.c_void_p),
+        ("tokens", C.c_int64), ("cached", C.c_int64), ("packed", C.c_int64),
         ("batch", C.c_int32), ("max_pages", C.c_int32), ("page_size", C.c_int32), ("pages", C.c_int32),
         ("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("causal", C.c_int32),
         ("max_q", C.c_int32), ("max_ctx", C.c_int32),

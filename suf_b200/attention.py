@@ -23,6 +23,7 @@ import ctypes as C
 import math
 
 import numpy as np
+import torch
 
 from . import _lib
 from ._lib import AttnSeqs, RopeAppend, check
@@ -34,67 +35,72 @@ M64 = (1 << 64) - 1
 
 
 # -- arguments ----------------------------------------------------------------
+# A decode step makes a dozen of these calls on a few thousand words: what the
+# checks cost on the host counts there, so they look at one attribute after
+# the other and only a refusal formats anything.
 
-def _stream(ctx: Context, stream):
-    """The stream a call runs on, on the context's device."""
-    import torch
-
+def _stream(ctx: Context, stream) -> int | None:
+    """The raw stream a call runs on (None: the device's legacy stream)."""
     if stream is None:
-        return torch.cuda.current_stream(ctx.device)
-    if not isinstance(stream, int) and stream.device.index != ctx.device:
-        raise ValueError(f"the stream is on {stream.device}, the context on cuda:{ctx.device}")
-    return stream
+        return torch.cuda.current_stream(ctx.device).cuda_stream or None
+    if isinstance(stream, int):
+        return stream or None
+    if stream.device_index != ctx.device:
+        raise ValueError(f"the stream is on cuda:{stream.device_index}, the context on cuda:{ctx.device}")
+    return stream.cuda_stream or None
 
 
-def _raw(stream) -> int | None:
-    return (stream if isinstance(stream, int) else int(stream.cuda_stream)) or None
-
-
-def _empty(ctx: Context, shape, stream):
+def _empty(ctx: Context, shape, stream=None):
     """Words on the context's device, allocated on the stream that writes them
     and kept until the caller's current stream has passed its use of them."""
-    import torch
-
+    if stream is None:
+        return torch.empty(shape, dtype=torch.int64, device=ctx.device)
     now = torch.cuda.current_stream(ctx.device)
     if isinstance(stream, int):
         stream = torch.cuda.ExternalStream(stream, device=ctx.device) if stream else torch.cuda.default_stream(ctx.device)
+    if stream == now:
+        return torch.empty(shape, dtype=torch.int64, device=ctx.device)
     with torch.cuda.stream(stream):
-        t = torch.empty(shape, dtype=torch.int64, device=torch.device("cuda", ctx.device))
-    if stream != now:
-        t.record_stream(now)
+        t = torch.empty(shape, dtype=torch.int64, device=ctx.device)
+    t.record_stream(now)
     return t
 
 
-def _want(ctx: Context, name: str, t, shape, dtype=None):
-    """Check a dense tensor: int64 words unless `dtype`, on the device, of the shape (None: any extent)."""
-    import torch
-
-    dtype = dtype or torch.int64
+def _refuse(ctx: Context, name: str, t, shape, dtype):
     if not isinstance(t, torch.Tensor) or t.dtype != dtype:
         raise ValueError(f"{name}: expected a {dtype} tensor")
-    if t.device.type != "cuda" or t.device.index != ctx.device:
+    if t.get_device() != ctx.device:
         raise ValueError(f"{name}: on {t.device}, the context is on cuda:{ctx.device}")
     if t.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, t.shape)):
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple('any' if w is None else w for w in shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name}: not contiguous")
-    return t
+    raise ValueError(f"{name}: not contiguous")
 
 
-def _pair(ctx: Context, name: str, ts, shape):
+def _want(ctx: Context, name: str, t, shape: tuple, dtype=None) -> int:
+    """The address of a dense tensor: int64 words unless `dtype`, on the device, of the shape (None: any extent)."""
+    dtype = dtype or torch.int64
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == ctx.device and
+            (t.shape == shape or (None in shape and t.dim() == len(shape) and
+                                  all(w is None or w == g for w, g in zip(shape, t.shape)))) and t.is_contiguous()):
+        return t.data_ptr()
+    _refuse(ctx, name, t, shape, dtype)
+
+
+_Two = C.c_void_p * 2
+_TwoWords = C.c_uint64 * 2
+
+
+def _pair(ctx: Context, name: str, ts, shape: tuple):
+    """Both parties' addresses."""
     if not isinstance(ts, (tuple, list)) or len(ts) != 2:
         raise ValueError(f"{name}: expected both parties' tensors")
-    return tuple(_want(ctx, f"{name}[{p}]", t, shape) for p, t in enumerate(ts))
-
-
-def _ptrs(ts):
-    return (C.c_void_p * 2)(*[int(t.data_ptr()) for t in ts])
+    return _Two(_want(ctx, name, ts[0], shape), _want(ctx, name, ts[1], shape))
 
 
 def _masks(r):
     if len(r) != 2:
         raise ValueError("r: expected both parties' shares of the mask")
-    return (C.c_uint64 * 2)(int(r[0]) & M64, int(r[1]) & M64)
+    return _TwoWords(r[0] & M64, r[1] & M64)
 
 
 # -- rotary tables --------------------------------------------------------------
@@ -130,8 +136,6 @@ def rope_table_words(max_pos: int, rot_dim: int, frac_bits: int, base: float = 1
 
 def rope_tables(ctx: Context, max_pos: int, rot_dim: int, frac_bits: int, **kw):
     """rope_table_words on the context's device, as rope_append_pair takes them."""
-    import torch
-
     dev = torch.device("cuda", ctx.device)
     return tuple(torch.from_numpy(t).to(dev) for t in rope_table_words(max_pos, rot_dim, frac_bits, **kw))
 
@@ -141,20 +145,16 @@ class TruncPair(_Trunc):
     filled (frac_bits 1..16): dealer material that stays resident."""
 
     def __init__(self, ctx: Context, frac_bits: int, seed: int = 1, stream=None):
-        import torch
-
         if not 1 <= frac_bits <= 16:
             raise ValueError("TruncPair: 1..16 fractional bits")
         dev = torch.device("cuda", ctx.device)
         super().__init__(ctx, np.random.default_rng(seed), frac_bits, dev)
         self.frac_bits = frac_bits
-        st = _stream(ctx, stream)
         self._full = TruncTables(self.bundles(), dev)
         if self._full.any():
-            with torch.cuda.device(ctx.device):
-                self._full.fill(ctx, st)
-        # the tables are read on any stream from here on
-        (torch.cuda.synchronize(dev) if isinstance(st, int) else st.synchronize())
+            self._full.fill(ctx, _stream(ctx, stream) or 0)
+        torch.cuda.synchronize(dev)  # the tables are read on any stream from here on
+        self._args = (_lib.TruncDesc * 2)(*self.desc), _Two(*self.table_ptrs()), _masks(self.r)
 
     def table_ptrs(self):
         return self._full.ptr(0), self._full.ptr(1)
@@ -164,12 +164,12 @@ class TruncPair(_Trunc):
         tables (a bundle without queries has none and is evaluated as it is)."""
         st = _stream(ctx, stream)
         if not self._full.any():
-            return super().eval_pair(ctx, d_xhat, d_y0, d_y1, st)
+            return super().eval_pair(ctx, d_xhat, d_y0, d_y1, st or 0)
         check(ctx._L.sufb200_trunc_bundle_eval_pair_tables_dev(
             ctx.h, C.byref(self.desc[0]), C.cast(self.kptr[0], C.c_void_p), C.cast(self.ksz[0], C.c_void_p),
             self._full.ptr(0), C.byref(self.desc[1]), C.cast(self.kptr[1], C.c_void_p),
             C.cast(self.ksz[1], C.c_void_p), self._full.ptr(1), d_xhat.data_ptr(), d_xhat.numel(), d_y0.data_ptr(),
-            d_y1.data_ptr(), _raw(st)))
+            d_y1.data_ptr(), st))
 
 
 # -- the cache -------------------------------------------------------------------
@@ -180,8 +180,6 @@ class ShareCache:
     page_size + place.  The constructor deals fresh masks for every slot."""
 
     def __init__(self, ctx: Context, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, seed: int = 1):
-        import torch
-
         dev = torch.device("cuda", ctx.device)
         g = torch.Generator(device=dev)
         g.manual_seed(seed)
@@ -201,33 +199,32 @@ class ShareCache:
         return self
 
     def _set(self, ctx, ek, bk, ev, bv):
-        _want(ctx, "ek", ek, (None,) * 4)
+        args = self._args = RopeAppend()  # what every append into this cache passes
+        args.d_ek = _want(ctx, "ek", ek, (None,) * 4)
         shape = tuple(ek.shape)
-        self.ek, self.ev = ek, _want(ctx, "ev", ev, shape)
-        self.bk, self.bv = _pair(ctx, "bk", bk, shape), _pair(ctx, "bv", bv, shape)
+        args.d_ev = _want(ctx, "ev", ev, shape)
+        args.d_bk, args.d_bv = _pair(ctx, "bk", bk, shape), _pair(ctx, "bv", bv, shape)
+        self.ek, self.ev, self.bk, self.bv, self.device = ek, ev, tuple(bk), tuple(bv), ctx.device
         self.pages, self.kv_heads, self.page_size, self.head_dim = shape
         if min(shape) < 1 or self.head_dim % 2 or self.head_dim > 256:
             raise ValueError("cache: empty, or a head size that is not even, 2..256")
+        args.pages, args.kv_heads, args.page_size, args.head_dim = shape
 
 
-def _strided(ctx: Context, name: str, ts, tokens, heads, dim):
-    """Both parties' [tokens][heads][dim] views of one stride pattern (the last axis dense)."""
-    import torch
-
+def _strided(ctx: Context, name: str, ts, shape: tuple):
+    """Both parties' addresses and the common strides of [tokens][heads][dim] views (the last axis dense)."""
     if not isinstance(ts, (tuple, list)) or len(ts) != 2:
         raise ValueError(f"{name}: expected both parties' tensors")
-    for p, t in enumerate(ts):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int64:
-            raise ValueError(f"{name}[{p}]: expected a torch.int64 tensor")
-        if t.device.type != "cuda" or t.device.index != ctx.device:
-            raise ValueError(f"{name}[{p}]: on {t.device}, the context is on cuda:{ctx.device}")
-        if tuple(t.shape) != (tokens, heads, dim):
-            raise ValueError(f"{name}[{p}]: shape {tuple(t.shape)}, expected {(tokens, heads, dim)}")
-        if t.numel() and dim > 1 and t.stride(2) != 1:
-            raise ValueError(f"{name}[{p}]: the head's words must be adjacent")
-        if t.stride() != ts[0].stride():
-            raise ValueError(f"{name}: the parties' strides differ")
-    return ts[0].stride(0), ts[0].stride(1)
+    for t in ts:
+        if (not isinstance(t, torch.Tensor) or t.dtype is not torch.int64 or t.get_device() != ctx.device or
+                t.shape != shape):
+            _refuse(ctx, name, t, shape, torch.int64)
+    ld = ts[0].stride()
+    if ld != ts[1].stride():
+        raise ValueError(f"{name}: the parties' strides differ")
+    if ld[2] != 1 and ts[0].numel():
+        raise ValueError(f"{name}: the head's words must be adjacent")
+    return _Two(ts[0].data_ptr(), ts[1].data_ptr()), ld[0], ld[1]
 
 
 def rope_append_pair(ctx: Context, q, k, v, positions, slots, cos, sin, trunc: TruncPair | None, a, cache: ShareCache,
@@ -239,40 +236,34 @@ def rope_append_pair(ctx: Context, q, k, v, positions, slots, cos, sin, trunc: T
     their slots into `cache` (int64 [tokens]; -1: padding, nothing written, all
     others distinct), queries opened against the mask shares a into d_q [tokens]
     [q_heads][head_dim], which is returned.  q, a None: append only."""
-    import torch
-
-    tokens, kv, dim = int(k[0].shape[0]), cache.kv_heads, cache.head_dim
-    heads = int(q[0].shape[1]) if q is not None else 0
-    st = _stream(ctx, stream)
-    args = RopeAppend()
-    args.k_ts, args.k_hs = _strided(ctx, "k", k, tokens, kv, dim)
-    args.v_ts, args.v_hs = _strided(ctx, "v", v, tokens, kv, dim)
-    args.d_k, args.d_v = _ptrs(k), _ptrs(v)
+    if cache.device != ctx.device:
+        raise ValueError(f"the cache is on cuda:{cache.device}, the context on cuda:{ctx.device}")
+    tokens, kv, dim = k[0].shape[0], cache.kv_heads, cache.head_dim
+    args = RopeAppend.from_buffer_copy(cache._args)
+    args.d_k, args.k_ts, args.k_hs = _strided(ctx, "k", k, (tokens, kv, dim))
+    args.d_v, args.v_ts, args.v_hs = _strided(ctx, "v", v, (tokens, kv, dim))
     if q is not None:
-        args.q_ts, args.q_hs = _strided(ctx, "q", q, tokens, heads, dim)
-        args.d_q, args.d_a = _ptrs(q), _ptrs(_pair(ctx, "a", a, (tokens, heads, dim)))
+        heads = q[0].shape[1]
+        shape = (tokens, heads, dim)
+        args.d_q, args.q_ts, args.q_hs = _strided(ctx, "q", q, shape)
+        args.d_a = _pair(ctx, "a", a, shape)
         if d_q is None:
-            d_q = _empty(ctx, (tokens, heads, dim), st)
-        args.d_dq = _want(ctx, "d_q", d_q, (tokens, heads, dim)).data_ptr()
-    args.d_slots = _want(ctx, "slots", slots, (tokens,)).data_ptr()
+            d_q = _empty(ctx, shape, stream)
+        args.d_dq, args.q_heads = _want(ctx, "d_q", d_q, shape), heads
+    args.d_slots = _want(ctx, "slots", slots, (tokens,))
     if trunc is not None:
-        _want(ctx, "cos", cos, (None, None), torch.int32)
-        _want(ctx, "sin", sin, tuple(cos.shape), torch.int32)
-        args.max_pos, args.rot_dim = int(cos.shape[0]), 2 * int(cos.shape[1])
-        if args.rot_dim > dim:
-            raise ValueError(f"the tables turn {args.rot_dim} words of a head of {dim}")
-        args.d_positions = _want(ctx, "positions", positions, (tokens,), torch.int32).data_ptr()
-        args.d_cos, args.d_sin = cos.data_ptr(), sin.data_ptr()
-        args.trunc[0], args.trunc[1] = trunc.desc
-        args.d_tables[0], args.d_tables[1] = trunc.table_ptrs()
-        args.r[0], args.r[1] = trunc.r
+        args.d_cos = _want(ctx, "cos", cos, (None, None), torch.int32)
+        args.max_pos, half = cos.shape
+        args.d_sin = _want(ctx, "sin", sin, (args.max_pos, half), torch.int32)
+        args.rot_dim = 2 * half
+        if 2 * half > dim:
+            raise ValueError(f"the tables turn {2 * half} words of a head of {dim}")
+        args.d_positions = _want(ctx, "positions", positions, (tokens,), torch.int32)
+        args.trunc, args.d_tables, args.r = trunc._args
     elif cos is not None or sin is not None:
         raise ValueError("rotation needs the truncation bundle")
-    args.d_ek, args.d_bk, args.d_ev, args.d_bv = (cache.ek.data_ptr(), _ptrs(cache.bk), cache.ev.data_ptr(),
-                                                  _ptrs(cache.bv))
-    args.tokens, args.q_heads, args.kv_heads, args.head_dim = tokens, heads, kv, dim
-    args.interleaved, args.pages, args.page_size = int(interleaved), cache.pages, cache.page_size
-    check(ctx._L.sufb200_rope_append_pair(ctx.h, C.byref(args), _raw(st)))
+    args.tokens, args.interleaved = tokens, 1 if interleaved else 0
+    check(ctx._L.sufb200_rope_append_pair(ctx.h, C.byref(args), _stream(ctx, stream)))
     return d_q
 
 
@@ -290,8 +281,6 @@ class AttnLayout:
 
     def __init__(self, ctx: Context, q_lens, ctx_lens, block_table, page_size: int, q_heads: int, kv_heads: int,
                  causal: bool = True):
-        import torch
-
         dev = torch.device("cuda", ctx.device)
         q, L = np.asarray(q_lens, dtype=np.int64).reshape(-1), np.asarray(ctx_lens, dtype=np.int64).reshape(-1)
         if q.size != L.size or (q < 0).any() or (L < 0).any():
@@ -304,6 +293,8 @@ class AttnLayout:
             for i, r in enumerate(rows):
                 wide[i, :len(r)] = r
             block_table = torch.from_numpy(wide).to(dev)
+        if block_table.dim() != 2:
+            raise ValueError("layout: the block table is [batch][most pages]")
         _want(ctx, "block_table", block_table, (q.size, None), torch.int32)
         self.q_lens, self.ctx_lens, self.causal = q, L, bool(causal)
         self.q_heads, self.kv_heads, self.page_size = int(q_heads), int(kv_heads), int(page_size)
@@ -317,16 +308,17 @@ class AttnLayout:
         self.packed = int(base[-1])
         if self.batch and int(L.max()) > block_table.shape[1] * page_size:
             raise ValueError("layout: a sequence is longer than its pages")
-        if max(self.tokens, self.batch, int(L.max(initial=0))) >= 2**31:
+        if max(self.tokens, self.batch, int(L.sum())) >= 2**31:
             raise ValueError("layout: more than 2^31 tokens")
         self._cu = torch.from_numpy(np.concatenate([[0], np.cumsum(q)]).astype(np.int32)).to(dev)
-        self._ctx = torch.from_numpy(L.astype(np.int32)).to(dev)
+        self._ctx = torch.from_numpy(np.concatenate([[0], np.cumsum(L)]).astype(np.int32)).to(dev)
         self._base = torch.from_numpy(base[:-1].astype(np.int64)).to(dev)
         self._table = block_table
         s = self._seqs = AttnSeqs()
-        s.d_cu_q, s.d_ctx, s.d_row_base = self._cu.data_ptr(), self._ctx.data_ptr(), self._base.data_ptr()
+        s.d_cu_q, s.d_cu_ctx, s.d_row_base = self._cu.data_ptr(), self._ctx.data_ptr(), self._base.data_ptr()
         s.d_block_table = block_table.data_ptr()
-        s.tokens, s.packed, s.batch, s.max_pages = self.tokens, self.packed, self.batch, int(block_table.shape[1])
+        s.tokens, s.cached, s.packed = self.tokens, int(L.sum()), self.packed
+        s.batch, s.max_pages = self.batch, int(block_table.shape[1])
         s.page_size, s.q_heads, s.kv_heads, s.causal = self.page_size, self.q_heads, self.kv_heads, int(self.causal)
         s.max_q, s.max_ctx = int(q.max(initial=0)), int(L.max(initial=0))
 
@@ -337,11 +329,12 @@ class AttnLayout:
         return np.concatenate(out).astype(np.int64) if out else np.zeros(0, dtype=np.int64)
 
     def _for_pool(self, ctx, name, e, b):
-        _want(ctx, name, e, (None, self.kv_heads, self.page_size, None))
-        pair = _pair(ctx, f"{name}'s masks", b, tuple(e.shape))
+        """(the sequences with the pool's sizes, the pool's address, its masks' addresses)"""
+        e_ptr = _want(ctx, name, e, (None, self.kv_heads, self.page_size, None))
+        shape = e.shape
         s = AttnSeqs.from_buffer_copy(self._seqs)
-        s.pages, s.head_dim = int(e.shape[0]), int(e.shape[3])
-        return s, pair
+        s.pages, s.head_dim = shape[0], shape[3]
+        return s, e_ptr, _pair(ctx, f"{name}'s masks", b, shape)
 
 
 def attn_scores_pair(ctx: Context, d_q, a, c, r, ek, bk, layout: AttnLayout, out=None, stream=None):
@@ -349,16 +342,13 @@ def attn_scores_pair(ctx: Context, d_q, a, c, r, ek, bk, layout: AttnLayout, out
     d_q and their mask's shares a [tokens][q_heads][head_dim], the packed shares
     c of the triple's product, r the shares of the output's mask, ek and bk a
     cache's keys.  Returns x^ [packed]."""
-    st = _stream(ctx, stream)
-    seqs, bk = layout._for_pool(ctx, "ek", ek, bk)
-    shape = (layout.tokens, layout.q_heads, seqs.head_dim)
-    _want(ctx, "d_q", d_q, shape)
-    a, c = _pair(ctx, "a", a, shape), _pair(ctx, "c", c, (layout.packed,))
+    seqs, e, b = layout._for_pool(ctx, "ek", ek, bk)
+    shape, packed = (layout.tokens, layout.q_heads, seqs.head_dim), (layout.packed,)
     if out is None:
-        out = _empty(ctx, (layout.packed,), st)
-    _want(ctx, "out", out, (layout.packed,))
-    check(ctx._L.sufb200_attn_scores_pair(ctx.h, C.byref(seqs), d_q.data_ptr(), _ptrs(a), _ptrs(c), _masks(r),
-                                          ek.data_ptr(), _ptrs(bk), out.data_ptr(), _raw(st)))
+        out = _empty(ctx, packed, stream)
+    check(ctx._L.sufb200_attn_scores_pair(ctx.h, C.byref(seqs), _want(ctx, "d_q", d_q, shape),
+                                          _pair(ctx, "a", a, shape), _pair(ctx, "c", c, packed), _masks(r), e, b,
+                                          _want(ctx, "out", out, packed), _stream(ctx, stream)))
     return out
 
 
@@ -367,16 +357,13 @@ def attn_values_pair(ctx: Context, p, a, c, r, ev, bv, layout: AttnLayout, out=N
     shares p of the probabilities and a of their mask, the shares c of the
     triple's product [tokens][q_heads][head_dim], ev and bv a cache's values.
     Returns x^ [tokens][q_heads][head_dim]."""
-    st = _stream(ctx, stream)
-    seqs, bv = layout._for_pool(ctx, "ev", ev, bv)
-    shape = (layout.tokens, layout.q_heads, seqs.head_dim)
-    p, a = _pair(ctx, "p", p, (layout.packed,)), _pair(ctx, "a", a, (layout.packed,))
-    c = _pair(ctx, "c", c, shape)
+    seqs, e, b = layout._for_pool(ctx, "ev", ev, bv)
+    shape, packed = (layout.tokens, layout.q_heads, seqs.head_dim), (layout.packed,)
     if out is None:
-        out = _empty(ctx, shape, st)
-    _want(ctx, "out", out, shape)
-    check(ctx._L.sufb200_attn_values_pair(ctx.h, C.byref(seqs), _ptrs(p), _ptrs(a), _ptrs(c), _masks(r),
-                                          ev.data_ptr(), _ptrs(bv), out.data_ptr(), _raw(st)))
+        out = _empty(ctx, shape, stream)
+    check(ctx._L.sufb200_attn_values_pair(ctx.h, C.byref(seqs), _pair(ctx, "p", p, packed),
+                                          _pair(ctx, "a", a, packed), _pair(ctx, "c", c, shape), _masks(r), e, b,
+                                          _want(ctx, "out", out, shape), _stream(ctx, stream)))
     return out
 
 
@@ -388,8 +375,6 @@ class RowMaxPlan:
     values[k] its packed values, `rounds` how often the longest row halves."""
 
     def __init__(self, ctx: Context, row_lengths):
-        import torch
-
         dev = torch.device("cuda", ctx.device)
         w = np.asarray(row_lengths, dtype=np.int64).reshape(-1)
         if (w < 0).any() or int(w.sum()) >= 2**31:
@@ -405,19 +390,18 @@ class RowMaxPlan:
             self.pairs.append(int((w // 2).sum()))
             w = (w + 1) // 2
         self.rounds = len(self.pairs)
+        self._off = [t.data_ptr() for t in self.off]
 
 
 def rowmax_open_pair(ctx: Context, plan: RowMaxPlan, c, r, out=None, stream=None):
     """x^ [pairs[0]]: the opened differences of the first round's pairs of c (packed shares)."""
-    st = _stream(ctx, stream)
-    c = _pair(ctx, "c", c, (plan.values[0],))
     n = plan.pairs[0] if plan.rounds else 0
     if out is None:
-        out = _empty(ctx, (n,), st)
-    _want(ctx, "out", out, (n,))
-    if plan.rounds:
-        check(ctx._L.sufb200_rowmax_open_pair(ctx.h, _ptrs(c), plan.rows, plan.widths[0], plan.off[0].data_ptr(),
-                                              plan.off[1].data_ptr(), _masks(r), out.data_ptr(), _raw(st)))
+        out = _empty(ctx, (n,), stream)
+    c, o = _pair(ctx, "c", c, (plan.values[0],)), _want(ctx, "out", out, (n,))
+    if n:
+        check(ctx._L.sufb200_rowmax_open_pair(ctx.h, c, plan.rows, plan.widths[0], plan._off[0], plan._off[1],
+                                              _masks(r), o, _stream(ctx, stream)))
     return out
 
 
@@ -425,36 +409,39 @@ def rowmax_round_pair(ctx: Context, plan: RowMaxPlan, k: int, c, relu, r_next=No
     """Round k: its values c (packed shares) and the gate's shares relu of its
     pairs to the next round's values, and, with r_next, the open of their
     differences.  Returns ((next_0, next_1), x^ or None)."""
-    st = _stream(ctx, stream)
     if not 0 <= k < plan.rounds:
         raise ValueError(f"rowmax: round {k} of {plan.rounds}")
-    c, relu = _pair(ctx, "c", c, (plan.values[k],)), _pair(ctx, "relu", relu, (plan.pairs[k],))
-    n = plan.values[k + 1]
-    nxt = _pair(ctx, "next", nxt, (n,)) if nxt is not None else (_empty(ctx, (n,), st), _empty(ctx, (n,), st))
-    more = k + 1 < plan.rounds
-    if not more and r_next is not None:
-        raise ValueError("rowmax: the last round has no further differences to open")
-    if r_next is not None:
-        if out is None:
-            out = _empty(ctx, (plan.pairs[k + 1],), st)
-        _want(ctx, "out", out, (plan.pairs[k + 1],))
+    n, more = (plan.values[k + 1],), k + 1 < plan.rounds
+    if nxt is None:
+        nxt = _empty(ctx, n, stream), _empty(ctx, n, stream)
+        to = _Two(nxt[0].data_ptr(), nxt[1].data_ptr())
     else:
-        out = None
+        to = _pair(ctx, "next", nxt, n)
+    o = off2 = r = None
+    if r_next is not None:
+        if not more:
+            raise ValueError("rowmax: the last round has no further differences to open")
+        pairs = (plan.pairs[k + 1],)
+        if out is None:
+            out = _empty(ctx, pairs, stream)
+            o = out.data_ptr()
+        else:
+            o = _want(ctx, "out", out, pairs)
+        off2, r = plan._off[k + 2], _masks(r_next)
     check(ctx._L.sufb200_rowmax_round_pair(
-        ctx.h, _ptrs(c), _ptrs(relu), plan.rows, plan.widths[k], plan.off[k].data_ptr(), plan.off[k + 1].data_ptr(),
-        plan.off[k + 2].data_ptr() if more else None, _masks(r_next) if r_next is not None else None, _ptrs(nxt),
-        out.data_ptr() if out is not None else None, _raw(st)))
-    return nxt, out
+        ctx.h, _pair(ctx, "c", c, (plan.values[k],)), _pair(ctx, "relu", relu, (plan.pairs[k],)), plan.rows,
+        plan.widths[k], plan._off[k], plan._off[k + 1], off2, r, to, o, _stream(ctx, stream)))
+    return nxt, out if r_next is not None else None
 
 
 def maxdiff_ragged_pair(ctx: Context, plan: RowMaxPlan, m, s, out=None, stream=None):
     """t_p = max_p[row] - s_p over the packed rows: m the last round's values, s the first's."""
-    st = _stream(ctx, stream)
-    m, s = _pair(ctx, "max", m, (plan.values[-1],)), _pair(ctx, "s", s, (plan.values[0],))
-    n = plan.values[0]
-    out = _pair(ctx, "out", out, (n,)) if out is not None else (_empty(ctx, (n,), st), _empty(ctx, (n,), st))
-    check(ctx._L.sufb200_maxdiff_ragged_pair(ctx.h, _ptrs(m), _ptrs(s), plan.rows, plan.widths[0],
-                                             plan.off[0].data_ptr(), plan.off[-1].data_ptr(), _ptrs(out), _raw(st)))
+    n = (plan.values[0],)
+    if out is None:
+        out = _empty(ctx, n, stream), _empty(ctx, n, stream)
+    check(ctx._L.sufb200_maxdiff_ragged_pair(ctx.h, _pair(ctx, "max", m, (plan.values[-1],)), _pair(ctx, "s", s, n),
+                                             plan.rows, plan.widths[0], plan._off[0], plan._off[-1],
+                                             _pair(ctx, "out", out, n), _stream(ctx, stream)))
     return out
 
 
@@ -474,8 +461,6 @@ class CachedAttentionPair:
 
     def __init__(self, ctx: Context, cache: ShareCache, layout: AttnLayout, seed: int = 1,
                  score_shift: int | None = None, rope: tuple | None = None, interleaved: bool = False):
-        import torch
-
         if layout.kv_heads != cache.kv_heads or layout.page_size != cache.page_size:
             raise ValueError("attention: the layout's heads or pages are not the cache's")
         dim = cache.head_dim
@@ -517,21 +502,19 @@ class CachedAttentionPair:
             relu = load_layer_tables()["relu"]
             self.gates = [_CoeffGate(rng, relu) for _ in range(self.plan.rounds)]
             self.softmax = SoftmaxBlock(ctx, lens, seed=sub(), tables=sm_tables)
-        ctx.sync(_stream(ctx, None))
+        ctx.sync(_stream(ctx, None) or 0)
 
     def run(self, q, k, v, positions, slots, stream=None, trace: dict | None = None):
         """Both parties' shares of the new tokens' queries, keys and values
         [tokens][heads][head_dim] (views of fused rows allowed), their positions
         (None without rotary tables) and cache slots -> both parties' shares of
         the attention output [tokens][q_heads][head_dim]."""
-        import torch
-
-        ctx, layout = self.ctx, self.layout
-        st = _stream(ctx, stream)
+        ctx, layout, st = self.ctx, self.layout, stream
 
         def new(n):
             return _empty(ctx, n, st), _empty(ctx, n, st)
 
+        raw = _stream(ctx, stream) or 0  # the softmax block and the gates take torch's current device otherwise
         cos, sin = self.rope if self.rope is not None else (None, None)
         d_q = rope_append_pair(ctx, q, k, v, positions, slots, cos, sin, self.tr_rope, self.a_q, self.cache,
                                interleaved=self.interleaved, stream=st)
@@ -545,11 +528,11 @@ class CachedAttentionPair:
             xh = rowmax_open_pair(ctx, plan, cur, self.gates[0].r, stream=st) if plan.rounds else None
             for i, gate in enumerate(self.gates):
                 relu = new(plan.pairs[i])
-                gate.eval_pair(ctx, xh, *relu, st)
+                gate.eval_pair(ctx, xh, *relu, raw)
                 nxt = self.gates[i + 1].r if i + 1 < plan.rounds else None
                 cur, xh = rowmax_round_pair(ctx, plan, i, cur, relu, nxt, stream=st)
             t = maxdiff_ragged_pair(ctx, plan, cur, s, stream=st)
-            self.softmax.run(*t, *p, stream=st)
+            self.softmax.run(*t, *p, stream=raw)
             if trace is not None:
                 trace.update(d_q=d_q, scores=s, t=t, probs=p)
         xo = attn_values_pair(ctx, p, self.a_p, self.c_v, self.tr_o.r, self.cache.ev, self.cache.bv, layout, stream=st)

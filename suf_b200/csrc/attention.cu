@@ -287,7 +287,8 @@ __global__ void __launch_bounds__(kThreads) attn_tile_kernel(const __grid_consta
 int check_seqs(const sufb200_attn_seqs* s, const char* who) {
   const std::string at = std::string(who) + ": ";
   if (!s) return fail(SUFB200_ERR_INVALID, at + "null sequences");
-  if (s->batch < 0 || s->max_pages < 0 || s->pages < 0 || s->max_q < 0 || s->max_ctx < 0 || s->tokens < 0 || s->packed < 0)
+  if (s->batch < 0 || s->max_pages < 0 || s->pages < 0 || s->max_q < 0 || s->max_ctx < 0 || s->tokens < 0 || s->cached < 0 ||
+      s->packed < 0)
     return fail(SUFB200_ERR_INVALID, at + "negative size");
   if (s->page_size < 1 || s->kv_heads < 1 || s->q_heads < s->kv_heads || s->q_heads % s->kv_heads)
     return fail(SUFB200_ERR_INVALID, at + "page size, or query heads not a multiple of key heads");
@@ -295,13 +296,13 @@ int check_seqs(const sufb200_attn_seqs* s, const char* who) {
     return fail(SUFB200_ERR_UNSUPPORTED, at + "head size must be even, 2..256");
   if (static_cast<int64_t>(s->batch) * s->kv_heads > 65535)
     return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 65535 (sequence, key head) pairs");
-  if (static_cast<int64_t>(s->q_heads / s->kv_heads) * s->max_q > 1 << 21)
-    return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^21 rows per (sequence, key head)");
+  if (static_cast<int64_t>(s->q_heads / s->kv_heads) * s->max_q > 1 << 20)
+    return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^20 rows per (sequence, key head)");
   if (static_cast<int64_t>(s->max_ctx) > static_cast<int64_t>(s->max_pages) * s->page_size)
     return fail(SUFB200_ERR_INVALID, at + "max_ctx is more than the block table's pages hold");
   if (static_cast<__int128>(s->q_heads) * s->max_q * s->max_ctx >= (static_cast<__int128>(1) << 60))
     return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^60 packed words");
-  if (s->batch > 0 && (!s->d_cu_q || !s->d_ctx || !s->d_row_base || (s->max_ctx > 0 && !s->d_block_table)))
+  if (s->batch > 0 && (!s->d_cu_q || !s->d_cu_ctx || !s->d_row_base || (s->max_ctx > 0 && !s->d_block_table)))
     return fail(SUFB200_ERR_INVALID, at + "null sequence array");
   return SUFB200_OK;
 }
@@ -354,6 +355,9 @@ int sufb200_attn_scores_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
       scores_rows_kernel<4><<<dim3(x, (rows + 3) / 4, z), kThreads, 4 * seqs->head_dim * 16, st>>>(*seqs, o);
     else
       scores_rows_kernel<8><<<dim3(x, (rows + 7) / 8, z), kThreads, 8 * seqs->head_dim * 16, st>>>(*seqs, o);
+  } else if (scores_tc_fits(*seqs)) {
+    const cudaError_t e = launch_scores_tc(ctx, *seqs, o, st);
+    if (e != cudaSuccess) return fail(SUFB200_ERR_CUDA, std::string("attn_scores_pair: ") + cudaGetErrorString(e));
   } else {
     attn_tile_kernel<true><<<dim3((seqs->max_ctx + kT - 1) / kT, (rows + kT - 1) / kT, z), kThreads, 0, st>>>(*seqs, o);
   }
@@ -390,8 +394,8 @@ int sufb200_attn_values_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
       else
         values_rows_kernel<8><<<dim3(x, (rows + 7) / 8, z), kThreads, 0, st>>>(*seqs, o, range);
     } else {
-      attn_tile_kernel<false>
-          <<<dim3((seqs->head_dim + kT - 1) / kT, (rows + kT - 1) / kT, z), kThreads, 0, st>>>(*seqs, o);
+      const cudaError_t e = launch_values_tc(ctx, *seqs, o, st);
+      if (e != cudaSuccess) return fail(SUFB200_ERR_CUDA, std::string("attn_values_pair: ") + cudaGetErrorString(e));
     }
   }
   const cudaError_t e = cudaGetLastError();

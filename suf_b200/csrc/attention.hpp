@@ -16,7 +16,7 @@ using AttnSeqs = sufb200_attn_seqs;
 // One sequence: n new tokens (packed tokens t0 .. t0 + n), L cached tokens
 // (the new ones included), its packed rows at word `base`, `blk` words a head.
 struct SeqInfo {
-  int n, L, t0;
+  int n, L, t0, l0;  // l0: cached tokens of the sequences before it
   int64_t base, blk;
 };
 
@@ -43,9 +43,11 @@ SUFB200_HD int64_t row_off(int n, int L, int causal, int i) {
 
 // Whether a sequence's lengths and rows lie inside what the host arguments
 // say (so every address formed from them does too); fills q.
-SUFB200_HD bool seq_fits(const AttnSeqs& s, int c0, int c1, int L, int64_t base, SeqInfo& q) {
-  q = SeqInfo{0, L, c0, base, 0};
-  if (c0 < 0 || c1 < c0 || c1 > s.tokens || c1 - c0 > s.max_q || L < 0 || L > s.max_ctx ||
+SUFB200_HD bool seq_fits(const AttnSeqs& s, int c0, int c1, int l0, int l1, int64_t base, SeqInfo& q) {
+  q = SeqInfo{0, 0, c0, l0, base, 0};
+  if (l0 < 0 || l1 < l0 || l1 > s.cached) return false;
+  const int L = q.L = l1 - l0;
+  if (c0 < 0 || c1 < c0 || c1 > s.tokens || c1 - c0 > s.max_q || L > s.max_ctx ||
       L > static_cast<int64_t>(s.max_pages) * s.page_size || base < 0 || base > s.packed)
     return false;
   q.n = c1 - c0;
@@ -64,7 +66,7 @@ SUFB200_HD int64_t page_word(const AttnSeqs& s, int pg, int kh, int j) {
 // Sequence b; false (and the status word flagged) when the device arrays do
 // not fit what the host was told.
 __device__ __forceinline__ bool seq_info(const AttnSeqs& s, int b, uint32_t* status, SeqInfo& q) {
-  const bool ok = seq_fits(s, s.d_cu_q[b], s.d_cu_q[b + 1], s.d_ctx[b], s.d_row_base[b], q);
+  const bool ok = seq_fits(s, s.d_cu_q[b], s.d_cu_q[b + 1], s.d_cu_ctx[b], s.d_cu_ctx[b + 1], s.d_row_base[b], q);
   if (!ok) atomicOr(status, kStatusBadArgument);
   return ok;
 }
@@ -101,5 +103,11 @@ struct AttnOperands {
   uint64_t* out;
   uint32_t* status;
 };
+
+// The products on the tensor cores (attention_tc.cu), for sequences with many
+// rows per key head; the values form adds to o.out.
+bool scores_tc_fits(const AttnSeqs& s);
+cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st);
+cudaError_t launch_values_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st);
 
 }  // namespace sufb200

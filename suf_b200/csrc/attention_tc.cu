@@ -1,0 +1,557 @@
+// attention_tc.cu -- the two products of attention over a cache of shares
+// (attention.cu has the formula) on the tensor cores, for sequences with many
+// rows per key head (prompts).
+//
+// A product mod 2^64 is 36 limb products of bytes, twelve tcgen05 kind::i8
+// MMAs a 32-deep step into eight diagonals of int32 in tensor memory
+// (umma_i8.cuh; exact up to depth 8192).  The cached operand is the M = 128
+// side, the query rows the N = 64 side:
+//   scores: out[key][row] = sum_k E[key][k] U[row][k] + W[key][k] D[row][k]
+//   values: out[d][row]   = sum_j E[j][d]   U[row][j] + W[j][d]   D[row][j]
+// with W = B_0 + B_1, U = D + A_0 + A_1: two steps per 32 of depth, one
+// accumulator.  A thread of the epilogue holds one key (or word of the head)
+// for 32 rows, so a warp's stores and its loads of C are 256 adjacent bytes
+// whatever the packed rows' offsets are.
+//
+// The cached operand is read by every row tile of its group of heads, so a
+// pre-pass writes its byte planes once, one contiguous 32 KB block per step
+// (bulk copies, no multicast).  The rows' planes are made inside: for the
+// scores once per CTA (they stay in shared memory while the keys stream past),
+// for the values chunk by chunk from the packed shares, which are read
+// nowhere else.
+#include "attention.hpp"
+#include "umma_i8.cuh"
+
+namespace sufb200 {
+
+namespace {
+
+constexpr int kThreads = 384;     // warp 0 copies A, warp 1 issues MMAs, warps 4-11 make B planes and store
+constexpr int kWorkers = 256;
+constexpr uint32_t kAStage = 8 * kPlaneX;  // 32 KB: A planes of one step
+constexpr uint32_t kBStage = 8 * kPlaneY;  // 16 KB: B planes of one step
+constexpr int kAStages = 3;
+constexpr uint32_t kBOff = kAStages * kAStage;
+constexpr int kBStages = 4;  // values: two chunks of 32 keys, U and D each
+constexpr uint32_t kCtrlBytes = 2048;
+constexpr int kMaxDepthKeys = 4096;  // values: two products deep, 8192 in all
+
+struct AttnTc {
+  AttnSeqs s;
+  AttnOperands o;
+  uint8_t* planes;
+  int64_t tiles;  // blocks of rows (scores: 128 keys; values: 32 keys) per key head in `planes`
+  int chunks;     // scores: 32-word chunks of the head; values: 128-word tiles of the head
+  int span;       // scores: key tiles per CTA; values: keys per CTA
+};
+
+// First block of a sequence with l0 cached tokens before it, blocks of `per`
+// tokens: a sequence of L tokens has at most (l0 + L) / per + 1 - l0 / per.
+__device__ __forceinline__ int64_t first_block(int l0, int b, int per) { return l0 / per + b; }
+
+// Byte i of four K-consecutive words into plane i at `at`, for all planes.
+__device__ __forceinline__ void put4(uint8_t* at, uint32_t plane, const uint64_t (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const uint32_t a0 = static_cast<uint32_t>(v[0] >> (i < 4 ? 0 : 32)), a1 = static_cast<uint32_t>(v[1] >> (i < 4 ? 0 : 32));
+    const uint32_t a2 = static_cast<uint32_t>(v[2] >> (i < 4 ? 0 : 32)), a3 = static_cast<uint32_t>(v[3] >> (i < 4 ? 0 : 32));
+    const uint32_t sel = static_cast<uint32_t>(i & 3) | (static_cast<uint32_t>(4 + (i & 3)) << 4);
+    *reinterpret_cast<uint32_t*>(at + i * plane) = __byte_perm(__byte_perm(a0, a1, sel), __byte_perm(a2, a3, sel), 0x5410);
+  }
+}
+
+// The cached operand's byte planes.  KEYS: block (128-key tile, chunk of 32
+// words), rows = keys; else block (32 keys, 128-word tile), rows = words of
+// the head.  Out-of-range rows and depths are zero.
+template <bool KEYS>
+__global__ void __launch_bounds__(256) cache_planes_kernel(const __grid_constant__ AttnTc a) {
+  pdl_trigger();
+  __shared__ int64_t s_key[kTM];
+  const AttnSeqs& s = a.s;
+  const int t = threadIdx.x, b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads;
+  constexpr int kPer = KEYS ? kTM : kTK;
+  SeqInfo q;
+  if (!seq_info(s, b, a.o.status, q)) return;
+  const int j0 = blockIdx.x * kPer;
+  if (j0 >= q.L) return;
+  for (int e = t; e < kPer; e += 256) s_key[e] = j0 + e < q.L ? key_off(s, b, kh, j0 + e, a.o.status) : -1;
+  __syncthreads();
+  const int64_t block = ((kh * a.tiles + first_block(q.l0, b, kPer) + blockIdx.x) * a.chunks + blockIdx.y) * 2;
+  uint8_t* dst = a.planes + block * kAStage;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int u = t + 256 * i, kq = u & 3, r = (u >> 2) & (kTM - 1), h = u >> 9;
+    uint64_t e[4], w[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int deep = 16 * h + 4 * kq + j;
+      const int64_t at = s_key[KEYS ? r : deep];
+      const int word = KEYS ? static_cast<int>(blockIdx.y) * kTK + deep : static_cast<int>(blockIdx.y) * kTM + r;
+      const bool in = at >= 0 && word < s.head_dim;
+      e[j] = in ? a.o.e[at + word] : 0;
+      w[j] = in ? a.o.b[0][at + word] + a.o.b[1][at + word] : 0;
+    }
+    uint8_t* at = dst + core_off(r, h) + 4 * kq;
+    put4(at, kPlaneX, e);
+    put4(at + kAStage, kPlaneX, w);
+  }
+}
+
+// The mbarriers and flags behind the stages.
+struct Ctrl {
+  uint32_t afull, aempty, bfull, bempty, tfull, tempty, done, slot;
+  volatile uint32_t* err;
+  uint32_t* tmem_slot;
+  int64_t* row;  // [64] scores: first word of a row; values: its first packed word
+  int* len;      // [64] its keys
+};
+
+__device__ __forceinline__ Ctrl ctrl_at(uint8_t* smem, uint32_t off) {
+  Ctrl c;
+  const uint32_t base = smem_u32(smem) + off;
+  c.afull = base;
+  c.aempty = base + 8 * kAStages;
+  c.bfull = base + 16 * kAStages;
+  c.bempty = c.bfull + 8 * kBStages;
+  c.tfull = c.bempty + 8 * kBStages;
+  c.tempty = c.tfull + 8;
+  c.done = c.tempty + 8;
+  c.slot = c.done + 8;
+  uint8_t* p = smem + off + (c.slot - base);
+  c.tmem_slot = reinterpret_cast<uint32_t*>(p);
+  c.err = reinterpret_cast<volatile uint32_t*>(p + 4);
+  c.row = reinterpret_cast<int64_t*>(smem + off + 512);
+  c.len = reinterpret_cast<int*>(smem + off + 512 + 8 * kTN);
+  return c;
+}
+static_assert(16 * kAStages + 16 * kBStages + 32 <= 512 && 512 + 12 * kTN <= kCtrlBytes, "control block");
+
+// Tensor memory and barriers; every thread of the CTA.  Returns the columns' base.
+__device__ __forceinline__ uint32_t start(const Ctrl& c, int warp, int t) {
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(c.slot), "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (t == 0) {
+    for (int i = 0; i < kAStages; i++) {
+      mbar_init(c.afull + 8 * i, 1);
+      mbar_init(c.aempty + 8 * i, 1);
+    }
+    for (int i = 0; i < kBStages; i++) {
+      mbar_init(c.bfull + 8 * i, kWorkers / 32);
+      mbar_init(c.bempty + 8 * i, 1);
+    }
+    mbar_init(c.tfull, 1);
+    mbar_init(c.tempty, kWorkers / 32);
+    mbar_init(c.done, 1);
+    *c.err = 0;
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // B planes written so far -> tensor core reads
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  return *c.tmem_slot;
+}
+
+// All threads: report a wait that gave up, let what was issued finish (again
+// with a limit) and free the tensor memory.  `copies` = A copies issued.
+__device__ __forceinline__ void stop(const Ctrl& c, uint32_t tmem, uint32_t* status, int warp, int lane, int copies) {
+  __syncthreads();
+  if (*c.err) {
+    if (warp == 0 && lane == 0) {
+      atomicOr(status, kStatusTimeout);
+      for (int i = copies > kAStages ? copies - kAStages : 0; i < copies; i++)
+        mbar_wait(c.afull + 8 * (i % kAStages), static_cast<uint32_t>((i / kAStages) & 1));
+    }
+    if (warp == 1 && lane == 0) {
+      umma_commit(c.done);
+      mbar_wait(c.done, 0);
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 0) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// Lane 0 of the producer warp: the A planes of one step into the ring.
+__device__ __forceinline__ bool load_a(const Ctrl& c, uint32_t sbase, int li, const uint8_t* src) {
+  const int st = li % kAStages;
+  if (li >= kAStages && !mbar_wait(c.aempty + 8 * st, static_cast<uint32_t>(((li / kAStages) - 1) & 1))) return false;
+  mbar_expect_tx(c.afull + 8 * st, kAStage);
+  bulk_copy(sbase + static_cast<uint32_t>(st) * kAStage, src, kAStage, c.afull + 8 * st);
+  return true;
+}
+
+// 8 columns of this warp's 32 lanes; the registers are valid after tmem_wait8.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_wait8(uint32_t (&v)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])
+               :
+               : "memory");
+}
+
+// sum_s (P_s mod 2^32) << 8s of 32 columns from `col` on, for this thread's lane.
+__device__ __forceinline__ void fold32(uint32_t tmem, int quarter, int col, uint64_t (&z)[32]) {
+#pragma unroll
+  for (int cb = 0; cb < 4; cb++) {
+    uint32_t v[8][8];
+#pragma unroll
+    for (int sd = 0; sd < 8; sd++)
+      tmem_ld8(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(sd * kTN + col + cb * 8), v[sd]);
+#pragma unroll
+    for (int sd = 0; sd < 8; sd++) tmem_wait8(v[sd]);
+#pragma unroll
+    for (int x = 0; x < 8; x++) {
+      uint64_t lo = v[0][x];
+#pragma unroll
+      for (int sd = 1; sd < 4; sd++) lo += static_cast<uint64_t>(v[sd][x]) << (8 * sd);
+      const uint32_t hi = v[4][x] + (v[5][x] << 8) + (v[6][x] << 16) + (v[7][x] << 24);
+      z[cb * 8 + x] = lo + (static_cast<uint64_t>(hi) << 32);
+    }
+  }
+}
+
+// The MMAs of one step: A stage li, B planes at byte offset boff, then the commits.
+__device__ __forceinline__ void issue(const uint32_t (&dt)[8], const uint64_t (&ad)[8], const uint64_t (&bd)[8], int st,
+                                      uint32_t boff, uint32_t accumulate) {
+  const uint64_t ao = static_cast<uint64_t>((static_cast<uint32_t>(st) * kAStage) >> 4);
+  const uint64_t bo = static_cast<uint64_t>(boff >> 4);
+  uint64_t as[8], bs[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    as[i] = ad[i] + ao;
+    bs[i] = bd[i] + bo;
+  }
+  mma_step(dt, as, bs, accumulate);
+}
+
+__global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_constant__ AttnTc a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const AttnSeqs& s = a.s;
+  const AttnOperands& o = a.o;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, dh = s.head_dim, group = s.q_heads / s.kv_heads;
+  const int b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads;
+  SeqInfo q;
+  const bool fits = seq_info(s, b, o.status, q);
+  const int R = group * q.n, rho0 = blockIdx.y * kTN;
+  const int last = (rho0 + kTN < R ? rho0 + kTN : R) - 1;
+  const int len = fits && rho0 < R ? row_len(q.n, q.L, s.causal, last / group) : 0;
+  const int nt = (len + kTM - 1) / kTM, tile0 = blockIdx.x * a.span;
+  const int tiles = nt - tile0 < a.span ? nt - tile0 : a.span;
+  if (tiles <= 0) {
+    pdl_wait();
+    return;
+  }
+  const int steps = 2 * a.chunks;
+  const uint32_t sbase = smem_u32(smem);
+  const Ctrl c = ctrl_at(smem, kBOff + static_cast<uint32_t>(steps) * kBStage);
+
+  // this tile's rows: where they go, and their planes [U | D]
+  if (t < kTN) {
+    const int rho = rho0 + t, i = rho / group;
+    c.row[t] = rho < R ? q.base + (kh * group + rho % group) * q.blk + row_off(q.n, q.L, s.causal, i) : 0;
+    c.len[t] = rho < R ? row_len(q.n, q.L, s.causal, i) : 0;
+  }
+  for (int u = t; u < a.chunks * 512; u += kThreads) {
+    const int kq = u & 3, r = (u >> 2) & (kTN - 1), h = (u >> 8) & 1, ch = u >> 9, rho = rho0 + r;
+    uint64_t d[4] = {0, 0, 0, 0}, w[4] = {0, 0, 0, 0};
+    const int k = ch * kTK + 16 * h + 4 * kq;
+    if (rho < R) {
+      const int64_t at = (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + k;
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (k + j < dh) {
+          d[j] = o.x[0][at + j];
+          w[j] = d[j] + o.a[0][at + j] + o.a[1][at + j];
+        }
+    }
+    uint8_t* at = smem + kBOff + static_cast<uint32_t>(2 * ch) * kBStage + core_off(r, h) + 4 * kq;
+    put4(at, kPlaneY, w);
+    put4(at + kBStage, kPlaneY, d);
+  }
+  const uint32_t tmem = start(c, warp, t);
+  int copies = 0;
+
+  if (warp == 0) {  // A planes: every step of every key tile
+    pdl_wait();  // written by the pre-pass
+    const uint8_t* src = a.planes + (kh * a.tiles + first_block(q.l0, b, kTM) + tile0) * steps * static_cast<int64_t>(kAStage);
+    for (int li = 0; li < tiles * steps; li++) {
+      int go = 1;
+      if (lane == 0) {
+        go = load_a(c, sbase, li, src + static_cast<int64_t>(li) * kAStage);
+        if (!go) *c.err = 1;
+      }
+      if (!__shfl_sync(0xffffffffu, go, 0)) break;
+      copies++;
+    }
+  } else if (warp == 1) {  // MMAs
+    uint64_t ad[8], bd[8];
+    uint32_t dt[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      ad[i] = umma_desc(sbase + static_cast<uint32_t>(i) * kPlaneX);
+      bd[i] = umma_desc(sbase + kBOff + static_cast<uint32_t>(i) * kPlaneY);
+      dt[i] = tmem + static_cast<uint32_t>(i * kTN);
+    }
+    for (int tl = 0; tl < tiles; tl++) {
+      int go = 1;
+      if (lane == 0) {
+        go = tl == 0 || mbar_wait(c.tempty, static_cast<uint32_t>((tl - 1) & 1));  // the last tile is out of tensor memory
+        for (int st = 0; st < steps && go; st++) {
+          const int li = tl * steps + st, as = li % kAStages;
+          go = mbar_wait(c.afull + 8 * as, static_cast<uint32_t>((li / kAStages) & 1));
+          if (!go) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          issue(dt, ad, bd, as, static_cast<uint32_t>(st) * kBStage, st > 0 ? 1u : 0u);
+          umma_commit(c.aempty + 8 * as);
+        }
+        if (go)
+          umma_commit(c.tfull);
+        else
+          *c.err = 1;
+      }
+      if (!__shfl_sync(0xffffffffu, go, 0)) break;
+    }
+  } else if (warp >= 4) {  // epilogue: while the next tile's MMAs run
+    const int quarter = warp & 3, col = ((warp - 4) >> 2) * 32;
+    for (int tl = 0; tl < tiles; tl++) {
+      int go = 1;
+      if (lane == 0) go = mbar_wait(c.tfull, static_cast<uint32_t>(tl & 1));
+      if (!__shfl_sync(0xffffffffu, go, 0)) {
+        if (lane == 0) *c.err = 1;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      uint64_t z[32];
+      fold32(tmem, quarter, col, z);
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(c.tempty);
+      const int key = (tile0 + tl) * kTM + quarter * 32 + lane;
+#pragma unroll
+      for (int x0 = 0; x0 < 32; x0 += 8) {
+        uint64_t add[8];
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+          const int64_t at = c.row[col + x0 + x] + key;
+          add[x] = key < c.len[col + x0 + x] ? o.c[0][at] + o.c[1][at] : 0;
+        }
+#pragma unroll
+        for (int x = 0; x < 8; x++)
+          if (key < c.len[col + x0 + x]) o.out[c.row[col + x0 + x] + key] = z[x0 + x] + add[x] + o.r;
+      }
+    }
+  }
+  stop(c, tmem, o.status, warp, lane, copies);
+}
+
+__global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_constant__ AttnTc a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const AttnSeqs& s = a.s;
+  const AttnOperands& o = a.o;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, dh = s.head_dim, group = s.q_heads / s.kv_heads;
+  const int b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads, dt0 = blockIdx.y % a.chunks;
+  SeqInfo q;
+  const bool fits = seq_info(s, b, o.status, q);
+  const int R = group * q.n, rho0 = static_cast<int>(blockIdx.y / a.chunks) * kTN;
+  const int last = (rho0 + kTN < R ? rho0 + kTN : R) - 1;
+  const int len = fits && rho0 < R ? row_len(q.n, q.L, s.causal, last / group) : 0;
+  const int beg = blockIdx.x * a.span, end = len < beg + a.span ? len : beg + a.span;
+  const int nch = end > beg ? (end - beg + kTK - 1) / kTK : 0;
+  if (nch == 0) {
+    pdl_wait();
+    return;
+  }
+  const uint32_t sbase = smem_u32(smem);
+  const Ctrl c = ctrl_at(smem, kBOff + kBStages * kBStage);
+  if (t < kTN) {
+    const int rho = rho0 + t, i = rho / group;
+    c.row[t] = rho < R ? q.base + (kh * group + rho % group) * q.blk + row_off(q.n, q.L, s.causal, i) : 0;
+    c.len[t] = rho < R ? row_len(q.n, q.L, s.causal, i) : 0;
+  }
+  const uint32_t tmem = start(c, warp, t);
+  int copies = 0;
+
+  if (warp == 0) {
+    pdl_wait();
+    const int64_t block0 = kh * a.tiles + first_block(q.l0, b, kTK) + beg / kTK;
+    for (int li = 0; li < 2 * nch; li++) {
+      int go = 1;
+      if (lane == 0) {
+        go = load_a(c, sbase, li, a.planes + (((block0 + li / 2) * a.chunks + dt0) * 2 + (li & 1)) * kAStage);
+        if (!go) *c.err = 1;
+      }
+      if (!__shfl_sync(0xffffffffu, go, 0)) break;
+      copies++;
+    }
+  } else if (warp == 1) {
+    uint64_t ad[8], bd[8];
+    uint32_t dt[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      ad[i] = umma_desc(sbase + static_cast<uint32_t>(i) * kPlaneX);
+      bd[i] = umma_desc(sbase + kBOff + static_cast<uint32_t>(i) * kPlaneY);
+      dt[i] = tmem + static_cast<uint32_t>(i * kTN);
+    }
+    int go = 1;
+    for (int li = 0; li < 2 * nch; li++) {
+      if (lane == 0) {
+        const int as = li % kAStages, bs = li % kBStages;
+        go = mbar_wait(c.afull + 8 * as, static_cast<uint32_t>((li / kAStages) & 1)) &&
+             mbar_wait(c.bfull + 8 * bs, static_cast<uint32_t>((li / kBStages) & 1));
+        if (go) {
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          issue(dt, ad, bd, as, static_cast<uint32_t>(bs) * kBStage, li > 0 ? 1u : 0u);
+          umma_commit(c.aempty + 8 * as);
+          umma_commit(c.bempty + 8 * bs);
+        } else {
+          *c.err = 1;
+        }
+      }
+      if (!__shfl_sync(0xffffffffu, go, 0)) break;
+    }
+    if (lane == 0 && go) umma_commit(c.tfull);
+    __syncwarp();
+  } else if (warp >= 4) {
+    // A worker's two units of a chunk: row r, words 16 h + 4 q ... + 3 of its
+    // keys, for h = 0, 1.  The next chunk's shares are in flight while this
+    // one's are split.
+    const int kq = lane & 3, r = (warp - 4) * 8 + (lane >> 2);
+    const int64_t row = c.row[r];
+    const int rlen = c.len[r];
+    uint64_t p0[2][4], p1[2][4], a0[2][4], a1[2][4];
+    const auto fetch = [&](int ch) {
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int key = beg + ch * kTK + 16 * h + 4 * kq + j;
+          const bool in = key < rlen && key < end;
+          p0[h][j] = in ? o.x[0][row + key] : 0;
+          p1[h][j] = in ? o.x[1][row + key] : 0;
+          a0[h][j] = in ? o.a[0][row + key] : 0;
+          a1[h][j] = in ? o.a[1][row + key] : 0;
+        }
+    };
+    fetch(0);
+    int go = 1;
+    for (int ch = 0; ch < nch; ch++) {
+      uint64_t d[2][4], u[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          d[h][j] = (p0[h][j] - a0[h][j]) + (p1[h][j] - a1[h][j]);
+          u[h][j] = d[h][j] + a0[h][j] + a1[h][j];
+        }
+      if (ch + 1 < nch) fetch(ch + 1);
+      const int su = (2 * ch) % kBStages, sd = su + 1;
+      if (lane == 0 && 2 * ch >= kBStages)
+        go = mbar_wait(c.bempty + 8 * su, static_cast<uint32_t>(((2 * ch / kBStages) - 1) & 1)) &&
+             mbar_wait(c.bempty + 8 * sd, static_cast<uint32_t>(((2 * ch / kBStages) - 1) & 1));
+      if (!__shfl_sync(0xffffffffu, go, 0)) {
+        if (lane == 0) *c.err = 1;
+        break;
+      }
+      uint8_t* at = smem + kBOff + static_cast<uint32_t>(su) * kBStage + 4 * kq;
+#pragma unroll
+      for (int h = 0; h < 2; h++) put4(at + core_off(r, h), kPlaneY, u[h]);
+#pragma unroll
+      for (int h = 0; h < 2; h++) put4(at + kBStage + core_off(r, h), kPlaneY, d[h]);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // generic writes -> tensor core reads
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(c.bfull + 8 * su);
+        mbar_arrive(c.bfull + 8 * sd);
+      }
+    }
+    if (lane == 0 && go) go = mbar_wait(c.tfull, 0);
+    if (__shfl_sync(0xffffffffu, go, 0)) {
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int quarter = warp & 3, col = ((warp - 4) >> 2) * 32;
+      uint64_t z[32];
+      fold32(tmem, quarter, col, z);
+      const int word = dt0 * kTM + quarter * 32 + lane;
+#pragma unroll
+      for (int x = 0; x < 32; x++) {
+        const int rho = rho0 + col + x;
+        if (rho < R && word < dh)
+          atomicAdd(reinterpret_cast<unsigned long long*>(
+                        o.out + (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + word),
+                    static_cast<unsigned long long>(z[x]));
+      }
+    } else if (lane == 0) {
+      *c.err = 1;
+    }
+  }
+  stop(c, tmem, o.status, warp, lane, copies);
+}
+
+template <typename K>
+cudaError_t launch(K kernel, dim3 grid, size_t smem, cudaStream_t st, const AttnTc& a) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  return launch_pdl(kernel, grid, dim3(kThreads), smem, st, a);
+}
+
+}  // namespace
+
+// Head sizes whose row planes stay in shared memory beside three A stages.
+bool scores_tc_fits(const AttnSeqs& s) { return s.head_dim <= 128; }
+
+cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st) {
+  const int rows = s.q_heads / s.kv_heads * s.max_q;
+  const unsigned z = static_cast<unsigned>(s.batch) * s.kv_heads;
+  const int nt = (s.max_ctx + kTM - 1) / kTM, rt = (rows + kTN - 1) / kTN;
+  AttnTc a{s, o, nullptr, s.cached / kTM + s.batch, (s.head_dim + kTK - 1) / kTK, 0};
+  const int64_t bytes = a.tiles * s.kv_heads * a.chunks * 2 * static_cast<int64_t>(kAStage);
+  cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&a.planes), bytes, ctx->pool, st);
+  if (e != cudaSuccess) return e;
+  // key tiles per CTA: long runs reuse the rows' planes and hide the epilogue
+  // behind the next tile, as long as every SM has a few CTAs to take
+  const int64_t all = static_cast<int64_t>(nt) * rt * z, want = all / (static_cast<int64_t>(ctx->sm_count) * 4);
+  a.span = static_cast<int>(want < 1 ? 1 : (want > 8 ? 8 : want));
+  cache_planes_kernel<true><<<dim3(nt, a.chunks, z), 256, 0, st>>>(a);
+  e = cudaGetLastError();
+  const size_t smem = kBOff + static_cast<size_t>(2 * a.chunks) * kBStage + kCtrlBytes;
+  if (e == cudaSuccess) e = launch(scores_tc_kernel, dim3((nt + a.span - 1) / a.span, rt, z), smem, st, a);
+  const cudaError_t f = cudaFreeAsync(a.planes, st);
+  return e == cudaSuccess ? f : e;
+}
+
+// Adds to o.out, which holds C_0 + C_1 + r.
+cudaError_t launch_values_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st) {
+  const int rows = s.q_heads / s.kv_heads * s.max_q;
+  const int nch = (s.max_ctx + kTK - 1) / kTK, rt = (rows + kTN - 1) / kTN;
+  AttnTc a{s, o, nullptr, s.cached / kTK + s.batch, (s.head_dim + kTM - 1) / kTM, 0};
+  const unsigned z = static_cast<unsigned>(s.batch) * s.kv_heads;
+  const int64_t bytes = a.tiles * s.kv_heads * a.chunks * 2 * static_cast<int64_t>(kAStage);
+  cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&a.planes), bytes, ctx->pool, st);
+  if (e != cudaSuccess) return e;
+  // keys per CTA: at most the exact depth; shorter while that leaves SMs idle
+  const int64_t units = static_cast<int64_t>(rt) * z * a.chunks;
+  int64_t parts = (static_cast<int64_t>(ctx->sm_count) * 4 + units - 1) / units;
+  const int64_t most = (nch + 7) / 8;  // eight chunks at least
+  parts = parts > most ? most : (parts < 1 ? 1 : parts);
+  a.span = static_cast<int>((nch + parts - 1) / parts) * kTK;
+  if (a.span > kMaxDepthKeys) a.span = kMaxDepthKeys;
+  cache_planes_kernel<false><<<dim3(nch, a.chunks, z), 256, 0, st>>>(a);
+  e = cudaGetLastError();
+  const size_t smem = kBOff + kBStages * kBStage + kCtrlBytes;
+  if (e == cudaSuccess)
+    e = launch(values_tc_kernel, dim3((s.max_ctx + a.span - 1) / a.span, rt * a.chunks, z), smem, st, a);
+  const cudaError_t f = cudaFreeAsync(a.planes, st);
+  return e == cudaSuccess ? f : e;
+}
+
+}  // namespace sufb200

@@ -41,121 +41,17 @@
 
 #include "kernels.hpp"
 #include "ring_common.cuh"
+#include "umma_i8.cuh"
 
 namespace sufb200 {
 
 namespace {
 
-constexpr int kTM = 128;  // output rows per tile (TMEM lanes)
-constexpr int kTN = 64;   // output columns per tile (per diagonal)
-constexpr int kTK = 32;   // K per MMA (8-bit operands)
 constexpr int kThreads = 128;
 constexpr int kStages = 4;
-constexpr uint32_t kPlaneX = kTM * kTK;                    // 4 KB: one plane of the A tile
-constexpr uint32_t kPlaneY = kTN * kTK;                    // 2 KB: one plane of the B tile
 constexpr uint32_t kStageBytes = 8 * (kPlaneX + kPlaneY);  // 48 KB
 constexpr uint32_t kCtrlOffset = kStages * kStageBytes;    // mbarriers, error flag, TMEM slot
 constexpr uint32_t kSmemBytes = kCtrlOffset + 256;         // 192 KB: one CTA per SM, all 512 TMEM columns
-constexpr uint32_t kTmemCols = 512;
-// idesc for kind::i8 with M = 128 and the given N: D s32 (bits 4-5 = 2), A
-// and B unsigned 8-bit, both K-major, N >> 3 at bits 17-22, M >> 4 at 24-28.
-__host__ __device__ constexpr uint32_t idesc_n(int n) { return (2u << 4) | (uint32_t(n >> 3) << 17) | (uint32_t(kTM >> 4) << 24); }
-constexpr uint32_t kWaitIters = 1u << 26;
-constexpr uint64_t kWaitNs = 2000000000ull;  // give up after 2 s of wall time
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-// K-major, no swizzle: start >> 4, LBO 128 B, SBO 256 B, version 1.
-__device__ __forceinline__ uint64_t umma_desc(uint32_t saddr) {
-  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128 >> 4) << 16) |
-         (static_cast<uint64_t>(256 >> 4) << 32) | (1ull << 46);
-}
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ uint64_t global_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  return t;
-}
-
-// Bounded wait for the phase with the given parity (iterations and wall
-// time, since one try_wait may suspend for an implementation-defined while);
-// false on timeout.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-  const uint64_t t0 = global_ns();
-  for (uint32_t it = 0; it < kWaitIters; it++) {
-    if ((it & 255u) == 255u && global_ns() - t0 > kWaitNs) return false;
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return true;
-  }
-  return false;
-}
-
-__device__ __forceinline__ void umma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                        uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-      :
-      : "r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u));
-}
-
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-
-// 16 columns of this warp's 32 lanes; the registers are valid after tmem_wait.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-      "[%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr));
-}
-
-// Waits for this thread's outstanding tensor-memory loads; taking the
-// registers as operands keeps every use of them after the wait.
-__device__ __forceinline__ void tmem_wait(uint32_t (&v)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
-                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
-               :
-               : "memory");
-}
-
-// Offset of (row r, K half h) inside a plane slab (core-matrix order).
-__device__ __forceinline__ uint32_t core_off(int r, int h) {
-  return static_cast<uint32_t>((r >> 3) * 256 + h * 128 + (r & 7) * 16);
-}
-
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
 // Plane i (byte i of every word) of 16 K-consecutive words: 16 bytes.
 __device__ __forceinline__ uint4 plane_bytes(const uint64_t (&v)[16], int i) {
   uint32_t w[4];
@@ -169,22 +65,6 @@ __device__ __forceinline__ uint4 plane_bytes(const uint64_t (&v)[16], int i) {
     w[q] = __byte_perm(__byte_perm(a0, a1, sel), __byte_perm(a2, a3, sel), 0x5410);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// The B planes of a stage are consecutive 64-row blocks in core-matrix
-// order, so [y_0 | y_1 | y_2 | y_3] is one N = 256 operand.  x_i times it,
-// accumulated at column 64 i, lands product (i, j) on column 64 (i + j):
-// diagonal i + j.  Twelve MMAs (N = 256 except where the 512 columns end)
-// cover the 36 limb pairs; the first two write all 512 columns, so on the
-// first step (accumulate = 0) they alone start from zero.
-__device__ __forceinline__ void mma_step(const uint32_t (&dt)[8], const uint64_t (&as)[8], const uint64_t (&bs)[8],
-                                         uint32_t accumulate) {
-  umma_i8(dt[0], as[0], bs[0], idesc_n(256), accumulate);
-  umma_i8(dt[4], as[0], bs[4], idesc_n(256), accumulate);
-#pragma unroll
-  for (int i = 1; i < 8; i++) umma_i8(dt[i], as[i], bs[0], idesc_n(i <= 4 ? 256 : 64 * (8 - i)), 1u);
-#pragma unroll
-  for (int i = 1; i < 4; i++) umma_i8(dt[i + 4], as[i], bs[4], idesc_n(256 - 64 * i), 1u);
 }
 
 // ---- Epilogue: the K-split CTAs of a tile are one thread-block cluster ----

@@ -10,9 +10,9 @@ extern "C" {
 int emu_row_len(int n, int L, int causal, int i) { return row_len(n, L, causal, i); }
 int64_t emu_row_off(int n, int L, int causal, int i) { return row_off(n, L, causal, i); }
 
-int emu_seq_fits(const sufb200_attn_seqs* s, int c0, int c1, int L, int64_t base, int64_t* blk) {
+int emu_seq_fits(const sufb200_attn_seqs* s, int c0, int c1, int l0, int l1, int64_t base, int64_t* blk) {
   SeqInfo q;
-  const bool ok = seq_fits(*s, c0, c1, L, base, q);
+  const bool ok = seq_fits(*s, c0, c1, l0, l1, base, q);
   *blk = q.blk;
   return ok ? 1 : 0;
 }

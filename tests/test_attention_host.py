@@ -24,7 +24,7 @@ def emu(tmp_path_factory):
     E.emu_row_off.restype = C.c_int64
     E.emu_page_word.restype = C.c_int64
     E.emu_sizeof.restype = C.c_size_t
-    E.emu_seq_fits.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int64, C.c_void_p]
+    E.emu_seq_fits.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64, C.c_void_p]
     E.emu_page_word.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int]
     return E
 
@@ -52,7 +52,7 @@ def _seqs(**kw):
     from suf_b200._lib import AttnSeqs
 
     s = AttnSeqs()
-    for k, v in dict(tokens=10, packed=1000, batch=2, max_pages=4, page_size=8, pages=5, q_heads=4, kv_heads=2,
+    for k, v in dict(tokens=10, cached=60, packed=1000, batch=2, max_pages=4, page_size=8, pages=5, q_heads=4, kv_heads=2,
                      head_dim=64, causal=1, max_q=6, max_ctx=30).items():
         setattr(s, k, v)
     for k, v in kw.items():
@@ -66,14 +66,14 @@ def test_sequences_outside_the_host_bounds_are_refused(emu):
     def fits(*a):
         return emu.emu_seq_fits(C.byref(s), *a, C.byref(blk))
 
-    assert fits(0, 6, 30, 0) and blk.value == sum(range(25, 31))
-    assert fits(4, 10, 6, 1000 - 4 * 21)
-    for bad in [(-1, 3, 5, 0), (3, 2, 5, 0), (5, 11, 5, 0), (0, 7, 5, 0), (0, 3, -1, 0), (0, 3, 31, 0), (0, 3, 5, -1),
-                (0, 3, 5, 1001), (4, 10, 6, 1000 - 4 * 21 + 1), (-2**31, 2**31 - 1, 2**31 - 1, 0),
-                (0, 2**31 - 1, 2**31 - 1, 2**63 - 1)]:
+    assert fits(0, 6, 0, 30, 0) and blk.value == sum(range(25, 31))
+    assert fits(4, 10, 54, 60, 1000 - 4 * 21)
+    for bad in [(-1, 3, 0, 5, 0), (3, 2, 0, 5, 0), (5, 11, 0, 5, 0), (0, 7, 0, 5, 0), (0, 3, 5, 4, 0), (0, 3, 0, 31, 0),
+                (0, 3, 0, 5, -1), (0, 3, 0, 5, 1001), (4, 10, 0, 6, 1000 - 4 * 21 + 1), (0, 3, 56, 61, 0),
+                (0, 3, -1, 4, 0), (-2**31, 2**31 - 1, -2**31, 2**31 - 1, 0), (0, 2**31 - 1, 0, 2**31 - 1, 2**63 - 1)]:
         assert not fits(*bad), bad
     s.max_ctx = 40
-    assert not fits(0, 3, 33, 0)  # more than four pages of eight
+    assert not fits(0, 3, 0, 33, 0)  # more than four pages of eight
 
 
 def test_pages_outside_the_pool_are_refused(emu):
@@ -120,7 +120,7 @@ def _attn(host, which, seqs, x=None, a=(P16, P16), c=(P16, P16), e=P16, b=(P16, 
                                       _arr(*b), out, None)
 
 
-PTRS = dict(d_cu_q=P16, d_ctx=P16, d_row_base=P16, d_block_table=P16)
+PTRS = dict(d_cu_q=P16, d_cu_ctx=P16, d_row_base=P16, d_block_table=P16)
 
 
 @pytest.mark.parametrize("which", ["scores", "values"])
@@ -134,9 +134,9 @@ def test_attention_refusals(host, which):
                       (dict(head_dim=0), _lib.ERR_UNSUPPORTED), (dict(q_heads=3), _lib.ERR_INVALID),
                       (dict(kv_heads=0), _lib.ERR_INVALID), (dict(page_size=0), _lib.ERR_INVALID),
                       (dict(max_ctx=33), _lib.ERR_INVALID), (dict(batch=-1), _lib.ERR_INVALID),
-                      (dict(tokens=-1), _lib.ERR_INVALID), (dict(d_ctx=None), _lib.ERR_INVALID),
+                      (dict(tokens=-1), _lib.ERR_INVALID), (dict(cached=-1), _lib.ERR_INVALID), (dict(d_cu_ctx=None), _lib.ERR_INVALID),
                       (dict(d_block_table=None), _lib.ERR_INVALID), (dict(batch=40000), _lib.ERR_UNSUPPORTED),
-                      (dict(max_q=2**21), _lib.ERR_UNSUPPORTED),
+                      (dict(max_q=2**20), _lib.ERR_UNSUPPORTED),
                       (dict(q_heads=2**20, kv_heads=2**16 - 1 + 1, batch=1), _lib.ERR_UNSUPPORTED)]:
         assert _attn(host, which, _seqs(**{**PTRS, **bad})) == code, bad
         assert b"head" in _lib.lib().sufb200_last_error() or b"attn_" in _lib.lib().sufb200_last_error()
@@ -238,7 +238,7 @@ def test_wrappers_refuse_wrong_tensors():
     with pytest.raises(ValueError, match="both parties"):
         at._masks((1,))
     with pytest.raises(ValueError, match="cuda:0"):
-        at._strided(_Ctx, "q", (torch.zeros(1, 2, 4, dtype=torch.int64),) * 2, 1, 2, 4)
+        at._strided(_Ctx, "q", (torch.zeros(1, 2, 4, dtype=torch.int64),) * 2, (1, 2, 4))
     for bad in [dict(rot_dim=3), dict(max_pos=0), dict(frac_bits=0), dict(frac_bits=17), dict(scale=0.0),
                 dict(base=-1.0), dict(low_freq=1.0), dict(low_freq=2.0, high_freq=1.0, trained_pos=64)]:
         with pytest.raises(ValueError):
