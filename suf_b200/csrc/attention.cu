@@ -382,21 +382,22 @@ int sufb200_attn_values_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int rows = seqs->q_heads / seqs->kv_heads * seqs->max_q;
   const unsigned z = static_cast<unsigned>(seqs->batch) * seqs->kv_heads;
-  const int64_t words = seqs->tokens * seqs->q_heads * seqs->head_dim;
-  const int64_t want = (words + kThreads - 1) / kThreads, cap = static_cast<int64_t>(ctx->sm_count) * 8;
-  values_init_kernel<<<static_cast<unsigned>(want < cap ? want : cap), kThreads, 0, st>>>(*seqs, o);
-  if (seqs->packed > 0 && seqs->max_ctx > 0) {
-    if (rows <= kFewRows) {
-      const int range = 256;
-      const unsigned x = (seqs->max_ctx + range - 1) / range;
-      if (rows <= 4)
-        values_rows_kernel<4><<<dim3(x, (rows + 3) / 4, z), kThreads, 0, st>>>(*seqs, o, range);
-      else
-        values_rows_kernel<8><<<dim3(x, (rows + 7) / 8, z), kThreads, 0, st>>>(*seqs, o, range);
-    } else {
-      const cudaError_t e = launch_values_tc(ctx, *seqs, o, st);
-      if (e != cudaSuccess) return fail(SUFB200_ERR_CUDA, std::string("attn_values_pair: ") + cudaGetErrorString(e));
-    }
+  const bool any = seqs->packed > 0 && seqs->max_ctx > 0, few = rows <= kFewRows;
+  if (!any || few || !values_tc_solo(ctx, *seqs)) {
+    const int64_t words = seqs->tokens * seqs->q_heads * seqs->head_dim;
+    const int64_t want = (words + kThreads - 1) / kThreads, cap = static_cast<int64_t>(ctx->sm_count) * 8;
+    values_init_kernel<<<static_cast<unsigned>(want < cap ? want : cap), kThreads, 0, st>>>(*seqs, o);
+  }
+  if (any && few) {
+    const int range = 256;
+    const unsigned x = (seqs->max_ctx + range - 1) / range;
+    if (rows <= 4)
+      values_rows_kernel<4><<<dim3(x, (rows + 3) / 4, z), kThreads, 0, st>>>(*seqs, o, range);
+    else
+      values_rows_kernel<8><<<dim3(x, (rows + 7) / 8, z), kThreads, 0, st>>>(*seqs, o, range);
+  } else if (any) {
+    const cudaError_t e = launch_values_tc(ctx, *seqs, o, st);
+    if (e != cudaSuccess) return fail(SUFB200_ERR_CUDA, std::string("attn_values_pair: ") + cudaGetErrorString(e));
   }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SUFB200_OK : fail(SUFB200_ERR_CUDA, std::string("attn_values_pair: ") + cudaGetErrorString(e));

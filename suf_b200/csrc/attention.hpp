@@ -85,6 +85,20 @@ __device__ __forceinline__ ulonglong2 ld_stream(const uint64_t* p) {
   asm volatile("ld.global.nc.L1::no_allocate.v2.u64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "l"(p));
   return v;
 }
+
+// *p where `in`, else 0, as one predicated load: a batch of them stays a
+// batch, where a conditional load may become a branch that waits.
+__device__ __forceinline__ uint64_t ld_if(const uint64_t* p, bool in) {
+  uint64_t v;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %2, 0;\n\t"
+      "mov.u64 %0, 0;\n\t"
+      "@p ld.global.nc.u64 %0, [%1];\n\t}"
+      : "=l"(v)
+      : "l"(p), "r"(static_cast<int>(in)));
+  return v;
+}
 #endif
 
 // Context check of the entry points (null, host-only, device made current).
@@ -105,9 +119,11 @@ struct AttnOperands {
 };
 
 // The products on the tensor cores (attention_tc.cu), for sequences with many
-// rows per key head; the values form adds to o.out.
+// rows per key head.  The values form adds to o.out unless values_tc_solo: then
+// it stores whole results.
 bool scores_tc_fits(const AttnSeqs& s);
 cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st);
+bool values_tc_solo(const sufb200_ctx_s* ctx, const AttnSeqs& s);
 cudaError_t launch_values_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st);
 
 }  // namespace sufb200

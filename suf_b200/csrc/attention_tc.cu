@@ -60,6 +60,32 @@ __device__ __forceinline__ void put4(uint8_t* at, uint32_t plane, const uint64_t
   }
 }
 
+// Words of four rows, lane = depth, turned so that a lane holds row lane % 4
+// of the four depths of its group of four lanes (a 4 x 4 transpose by halves).
+__device__ __forceinline__ void turn4(uint64_t (&v)[4], int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const uint64_t got = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[i] : v[i + 1], 1);
+    if (lane & 1)
+      v[i] = got;
+    else
+      v[i + 1] = got;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const uint64_t got = __shfl_xor_sync(0xffffffffu, lane & 2 ? v[i] : v[i + 2], 2);
+    if (lane & 2)
+      v[i] = got;
+    else
+      v[i + 2] = got;
+  }
+}
+
+// Where a lane of turn4 puts its four depths of row r0 + lane % 4.
+__device__ __forceinline__ uint32_t turned_off(int r0, int lane) {
+  return core_off(r0 + (lane & 3), lane >> 4) + 4 * ((lane >> 2) & 3);
+}
+
 // The cached operand's byte planes.  KEYS: block (128-key tile, chunk of 32
 // words), rows = keys; else block (32 keys, 128-word tile), rows = words of
 // the head.  Out-of-range rows and depths are zero.
@@ -127,7 +153,7 @@ __device__ __forceinline__ Ctrl ctrl_at(uint8_t* smem, uint32_t off) {
 static_assert(16 * kAStages + 16 * kBStages + 32 <= 512 && 512 + 12 * kTN <= kCtrlBytes, "control block");
 
 // Tensor memory and barriers; every thread of the CTA.  Returns the columns' base.
-__device__ __forceinline__ uint32_t start(const Ctrl& c, int warp, int t) {
+__device__ __forceinline__ uint32_t start(const Ctrl& c, int warp, int t, int bwarps) {
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(c.slot), "r"(kTmemCols)
                  : "memory");
@@ -139,7 +165,7 @@ __device__ __forceinline__ uint32_t start(const Ctrl& c, int warp, int t) {
       mbar_init(c.aempty + 8 * i, 1);
     }
     for (int i = 0; i < kBStages; i++) {
-      mbar_init(c.bfull + 8 * i, kWorkers / 32);
+      mbar_init(c.bfull + 8 * i, bwarps);
       mbar_init(c.bempty + 8 * i, 1);
     }
     mbar_init(c.tfull, 1);
@@ -147,7 +173,6 @@ __device__ __forceinline__ uint32_t start(const Ctrl& c, int warp, int t) {
     mbar_init(c.done, 1);
     *c.err = 0;
   }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // B planes written so far -> tensor core reads
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -243,7 +268,8 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
   const int b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads;
   SeqInfo q;
   const bool fits = seq_info(s, b, o.status, q);
-  const int R = group * q.n, rho0 = blockIdx.y * kTN;
+  // the longest causal rows first
+  const int R = group * q.n, rho0 = static_cast<int>(gridDim.y - 1 - blockIdx.y) * kTN;
   const int last = (rho0 + kTN < R ? rho0 + kTN : R) - 1;
   const int len = fits && rho0 < R ? row_len(q.n, q.L, s.causal, last / group) : 0;
   const int nt = (len + kTM - 1) / kTM, tile0 = blockIdx.x * a.span;
@@ -255,31 +281,12 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
   const int steps = 2 * a.chunks;
   const uint32_t sbase = smem_u32(smem);
   const Ctrl c = ctrl_at(smem, kBOff + static_cast<uint32_t>(steps) * kBStage);
-
-  // this tile's rows: where they go, and their planes [U | D]
   if (t < kTN) {
     const int rho = rho0 + t, i = rho / group;
     c.row[t] = rho < R ? q.base + (kh * group + rho % group) * q.blk + row_off(q.n, q.L, s.causal, i) : 0;
     c.len[t] = rho < R ? row_len(q.n, q.L, s.causal, i) : 0;
   }
-  for (int u = t; u < a.chunks * 512; u += kThreads) {
-    const int kq = u & 3, r = (u >> 2) & (kTN - 1), h = (u >> 8) & 1, ch = u >> 9, rho = rho0 + r;
-    uint64_t d[4] = {0, 0, 0, 0}, w[4] = {0, 0, 0, 0};
-    const int k = ch * kTK + 16 * h + 4 * kq;
-    if (rho < R) {
-      const int64_t at = (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + k;
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        if (k + j < dh) {
-          d[j] = o.x[0][at + j];
-          w[j] = d[j] + o.a[0][at + j] + o.a[1][at + j];
-        }
-    }
-    uint8_t* at = smem + kBOff + static_cast<uint32_t>(2 * ch) * kBStage + core_off(r, h) + 4 * kq;
-    put4(at, kPlaneY, w);
-    put4(at + kBStage, kPlaneY, d);
-  }
-  const uint32_t tmem = start(c, warp, t);
+  const uint32_t tmem = start(c, warp, t, kThreads / 32 - 2);
   int copies = 0;
 
   if (warp == 0) {  // A planes: every step of every key tile
@@ -306,7 +313,8 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
     for (int tl = 0; tl < tiles; tl++) {
       int go = 1;
       if (lane == 0) {
-        go = tl == 0 || mbar_wait(c.tempty, static_cast<uint32_t>((tl - 1) & 1));  // the last tile is out of tensor memory
+        // the rows' planes are written, the last tile is out of tensor memory
+        go = tl == 0 ? mbar_wait(c.bfull, 0) : mbar_wait(c.tempty, static_cast<uint32_t>((tl - 1) & 1));
         for (int st = 0; st < steps && go; st++) {
           const int li = tl * steps + st, as = li % kAStages;
           go = mbar_wait(c.afull + 8 * as, static_cast<uint32_t>((li / kAStages) & 1));
@@ -321,6 +329,43 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
           *c.err = 1;
       }
       if (!__shfl_sync(0xffffffffu, go, 0)) break;
+    }
+  } else {
+    // the rows' planes [U | D]: four rows of a chunk at a time
+    for (int u = warp - 2; u < a.chunks * (kTN / 4); u += kThreads / 32 - 2) {
+      const int ch = u / (kTN / 4), r0 = (u % (kTN / 4)) * 4, k = ch * kTK + lane;
+      uint64_t d[4], w[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int rho = rho0 + r0 + j;
+        const bool in = rho < R && k < dh;
+        const int64_t at = (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + k;
+        d[j] = ld_if(o.x[0] + at, in);
+        w[j] = d[j] + ld_if(o.a[0] + at, in) + ld_if(o.a[1] + at, in);
+      }
+      turn4(w, lane);
+      turn4(d, lane);
+      uint8_t* at = smem + kBOff + static_cast<uint32_t>(2 * ch) * kBStage + turned_off(r0, lane);
+      put4(at, kPlaneY, w);
+      put4(at + kBStage, kPlaneY, d);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // generic writes -> tensor core reads
+    __syncwarp();
+    if (lane == 0) mbar_arrive(c.bfull);
+  }
+  if (warp == 2 || warp == 3) {  // C of the coming tiles into L2, about a tile ahead of the epilogue
+    for (int tl = 0; tl < tiles; tl++) {
+      int go = 1;
+      if (lane == 0 && tl > 1) go = mbar_wait(c.tfull, static_cast<uint32_t>((tl - 2) & 1));
+      if (!__shfl_sync(0xffffffffu, go, 0)) break;  // the MMA warp reports it
+      const int k0 = (tile0 + tl) * kTM;
+      for (int u = (warp - 2) * 32 + lane; u < kTN * 9; u += 64) {
+        const int r = u / 9, k = k0 + (u % 9) * 16 < k0 + kTM ? k0 + (u % 9) * 16 : k0 + kTM - 1;
+        if (k < c.len[r]) {
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(o.c[0] + c.row[r] + k));
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(o.c[1] + c.row[r] + k));
+        }
+      }
     }
   } else if (warp >= 4) {  // epilogue: while the next tile's MMAs run
     const int quarter = warp & 3, col = ((warp - 4) >> 2) * 32;
@@ -340,21 +385,26 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
       const int key = (tile0 + tl) * kTM + quarter * 32 + lane;
 #pragma unroll
       for (int x0 = 0; x0 < 32; x0 += 8) {
-        uint64_t add[8];
+        uint64_t c0[8], c1[8];
 #pragma unroll
         for (int x = 0; x < 8; x++) {
           const int64_t at = c.row[col + x0 + x] + key;
-          add[x] = key < c.len[col + x0 + x] ? o.c[0][at] + o.c[1][at] : 0;
+          const bool in = key < c.len[col + x0 + x];
+          c0[x] = ld_if(o.c[0] + at, in);
+          c1[x] = ld_if(o.c[1] + at, in);
         }
 #pragma unroll
         for (int x = 0; x < 8; x++)
-          if (key < c.len[col + x0 + x]) o.out[c.row[col + x0 + x] + key] = z[x0 + x] + add[x] + o.r;
+          if (key < c.len[col + x0 + x]) o.out[c.row[col + x0 + x] + key] = z[x0 + x] + c0[x] + c1[x] + o.r;
       }
     }
   }
   stop(c, tmem, o.status, warp, lane, copies);
 }
 
+// SOLO: one CTA has all keys of a row tile and stores; else the ranges add to
+// out, which holds C_0 + C_1 + r.
+template <bool SOLO>
 __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_constant__ AttnTc a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const AttnSeqs& s = a.s;
@@ -363,23 +413,35 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
   const int b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads, dt0 = blockIdx.y % a.chunks;
   SeqInfo q;
   const bool fits = seq_info(s, b, o.status, q);
-  const int R = group * q.n, rho0 = static_cast<int>(blockIdx.y / a.chunks) * kTN;
+  // the longest causal rows first
+  const int R = fits ? group * q.n : 0, rho0 = static_cast<int>((gridDim.y - 1 - blockIdx.y) / a.chunks) * kTN;
   const int last = (rho0 + kTN < R ? rho0 + kTN : R) - 1;
-  const int len = fits && rho0 < R ? row_len(q.n, q.L, s.causal, last / group) : 0;
+  const int len = rho0 < R ? row_len(q.n, q.L, s.causal, last / group) : 0;
   const int beg = blockIdx.x * a.span, end = len < beg + a.span ? len : beg + a.span;
   const int nch = end > beg ? (end - beg + kTK - 1) / kTK : 0;
+  const int word0 = dt0 * kTM;
+  // word `word` of the output of row rho
+  const auto place = [&](int rho, int word) {
+    return (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + word;
+  };
   if (nch == 0) {
     pdl_wait();
+    if (SOLO && rho0 < R)  // rows without keys: C_0 + C_1 + r
+      for (int e = t; e < kTN * kTM; e += kThreads) {
+        const int rho = rho0 + e / kTM, word = word0 + e % kTM;
+        if (rho < R && word < dh) o.out[place(rho, word)] = o.c[0][place(rho, word)] + o.c[1][place(rho, word)] + o.r;
+      }
     return;
   }
   const uint32_t sbase = smem_u32(smem);
   const Ctrl c = ctrl_at(smem, kBOff + kBStages * kBStage);
   if (t < kTN) {
     const int rho = rho0 + t, i = rho / group;
+    const int m = rho < R ? row_len(q.n, q.L, s.causal, i) : 0;
     c.row[t] = rho < R ? q.base + (kh * group + rho % group) * q.blk + row_off(q.n, q.L, s.causal, i) : 0;
-    c.len[t] = rho < R ? row_len(q.n, q.L, s.causal, i) : 0;
+    c.len[t] = m < end ? m : end;
   }
-  const uint32_t tmem = start(c, warp, t);
+  const uint32_t tmem = start(c, warp, t, kWorkers / 32);
   int copies = 0;
 
   if (warp == 0) {
@@ -423,36 +485,32 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
     if (lane == 0 && go) umma_commit(c.tfull);
     __syncwarp();
   } else if (warp >= 4) {
-    // A worker's two units of a chunk: row r, words 16 h + 4 q ... + 3 of its
-    // keys, for h = 0, 1.  The next chunk's shares are in flight while this
-    // one's are split.
-    const int kq = lane & 3, r = (warp - 4) * 8 + (lane >> 2);
-    const int64_t row = c.row[r];
-    const int rlen = c.len[r];
-    uint64_t p0[2][4], p1[2][4], a0[2][4], a1[2][4];
+    // A worker warp's eight rows of a chunk, lane = key: 256 adjacent bytes a
+    // load.  The next chunk's shares are in flight while this one's are split.
+    const int r0 = (warp - 4) * 8;
+    uint64_t p0[8], p1[8], a0[8], a1[8];
     const auto fetch = [&](int ch) {
+      const int key = beg + ch * kTK + lane;
 #pragma unroll
-      for (int h = 0; h < 2; h++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int key = beg + ch * kTK + 16 * h + 4 * kq + j;
-          const bool in = key < rlen && key < end;
-          p0[h][j] = in ? o.x[0][row + key] : 0;
-          p1[h][j] = in ? o.x[1][row + key] : 0;
-          a0[h][j] = in ? o.a[0][row + key] : 0;
-          a1[h][j] = in ? o.a[1][row + key] : 0;
-        }
+      for (int j = 0; j < 8; j++) {
+        const int64_t at = c.row[r0 + j] + key;
+        const bool in = key < c.len[r0 + j];
+        p0[j] = ld_if(o.x[0] + at, in);
+        p1[j] = ld_if(o.x[1] + at, in);
+        a0[j] = ld_if(o.a[0] + at, in);
+        a1[j] = ld_if(o.a[1] + at, in);
+      }
     };
     fetch(0);
     int go = 1;
     for (int ch = 0; ch < nch; ch++) {
       uint64_t d[2][4], u[2][4];
 #pragma unroll
-      for (int h = 0; h < 2; h++)
+      for (int g = 0; g < 2; g++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          d[h][j] = (p0[h][j] - a0[h][j]) + (p1[h][j] - a1[h][j]);
-          u[h][j] = d[h][j] + a0[h][j] + a1[h][j];
+          d[g][j] = (p0[4 * g + j] - a0[4 * g + j]) + (p1[4 * g + j] - a1[4 * g + j]);
+          u[g][j] = d[g][j] + a0[4 * g + j] + a1[4 * g + j];
         }
       if (ch + 1 < nch) fetch(ch + 1);
       const int su = (2 * ch) % kBStages, sd = su + 1;
@@ -463,11 +521,17 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
         if (lane == 0) *c.err = 1;
         break;
       }
-      uint8_t* at = smem + kBOff + static_cast<uint32_t>(su) * kBStage + 4 * kq;
+      uint8_t* at = smem + kBOff + static_cast<uint32_t>(su) * kBStage;
 #pragma unroll
-      for (int h = 0; h < 2; h++) put4(at + core_off(r, h), kPlaneY, u[h]);
+      for (int g = 0; g < 2; g++) {
+        turn4(u[g], lane);
+        put4(at + turned_off(r0 + 4 * g, lane), kPlaneY, u[g]);
+      }
 #pragma unroll
-      for (int h = 0; h < 2; h++) put4(at + kBStage + core_off(r, h), kPlaneY, d[h]);
+      for (int g = 0; g < 2; g++) {
+        turn4(d[g], lane);
+        put4(at + kBStage + turned_off(r0 + 4 * g, lane), kPlaneY, d[g]);
+      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // generic writes -> tensor core reads
       __syncwarp();
       if (lane == 0) {
@@ -481,14 +545,31 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
       const int quarter = warp & 3, col = ((warp - 4) >> 2) * 32;
       uint64_t z[32];
       fold32(tmem, quarter, col, z);
-      const int word = dt0 * kTM + quarter * 32 + lane;
+      const int word = word0 + quarter * 32 + lane;
+      if (SOLO) {
 #pragma unroll
-      for (int x = 0; x < 32; x++) {
-        const int rho = rho0 + col + x;
-        if (rho < R && word < dh)
-          atomicAdd(reinterpret_cast<unsigned long long*>(
-                        o.out + (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + word),
-                    static_cast<unsigned long long>(z[x]));
+        for (int x0 = 0; x0 < 32; x0 += 8) {
+          uint64_t c0[8], c1[8];
+#pragma unroll
+          for (int x = 0; x < 8; x++) {
+            const int rho = rho0 + col + x0 + x;
+            const bool in = rho < R && word < dh;
+            c0[x] = ld_if(o.c[0] + place(rho, word), in);
+            c1[x] = ld_if(o.c[1] + place(rho, word), in);
+          }
+#pragma unroll
+          for (int x = 0; x < 8; x++) {
+            const int rho = rho0 + col + x0 + x;
+            if (rho < R && word < dh) o.out[place(rho, word)] = z[x0 + x] + c0[x] + c1[x] + o.r;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 32; x++) {
+          const int rho = rho0 + col + x;
+          if (rho < R && word < dh)
+            atomicAdd(reinterpret_cast<unsigned long long*>(o.out + place(rho, word)), static_cast<unsigned long long>(z[x]));
+        }
       }
     } else if (lane == 0) {
       *c.err = 1;
@@ -529,27 +610,36 @@ cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const 
   return e == cudaSuccess ? f : e;
 }
 
-// Adds to o.out, which holds C_0 + C_1 + r.
+// Keys per CTA of the values form, and whether one CTA takes whole rows.
+int values_span(const sufb200_ctx_s* ctx, const AttnSeqs& s) {
+  const int rows = s.q_heads / s.kv_heads * s.max_q;
+  const int nch = (s.max_ctx + kTK - 1) / kTK, rt = (rows + kTN - 1) / kTN, words = (s.head_dim + kTM - 1) / kTM;
+  const int64_t units = static_cast<int64_t>(rt) * words * s.batch * s.kv_heads;
+  // at most the exact depth; shorter, down to eight chunks, while that leaves SMs idle
+  int64_t parts = (static_cast<int64_t>(ctx->sm_count) * 4 + units - 1) / units;
+  const int64_t most = (nch + 7) / 8;
+  parts = parts > most ? most : (parts < 1 ? 1 : parts);
+  const int span = static_cast<int>((nch + parts - 1) / parts) * kTK;
+  return span > kMaxDepthKeys ? kMaxDepthKeys : span;
+}
+
+bool values_tc_solo(const sufb200_ctx_s* ctx, const AttnSeqs& s) { return values_span(ctx, s) >= s.max_ctx; }
+
 cudaError_t launch_values_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st) {
   const int rows = s.q_heads / s.kv_heads * s.max_q;
   const int nch = (s.max_ctx + kTK - 1) / kTK, rt = (rows + kTN - 1) / kTN;
-  AttnTc a{s, o, nullptr, s.cached / kTK + s.batch, (s.head_dim + kTM - 1) / kTM, 0};
+  AttnTc a{s, o, nullptr, s.cached / kTK + s.batch, (s.head_dim + kTM - 1) / kTM, values_span(ctx, s)};
   const unsigned z = static_cast<unsigned>(s.batch) * s.kv_heads;
   const int64_t bytes = a.tiles * s.kv_heads * a.chunks * 2 * static_cast<int64_t>(kAStage);
   cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&a.planes), bytes, ctx->pool, st);
   if (e != cudaSuccess) return e;
-  // keys per CTA: at most the exact depth; shorter while that leaves SMs idle
-  const int64_t units = static_cast<int64_t>(rt) * z * a.chunks;
-  int64_t parts = (static_cast<int64_t>(ctx->sm_count) * 4 + units - 1) / units;
-  const int64_t most = (nch + 7) / 8;  // eight chunks at least
-  parts = parts > most ? most : (parts < 1 ? 1 : parts);
-  a.span = static_cast<int>((nch + parts - 1) / parts) * kTK;
-  if (a.span > kMaxDepthKeys) a.span = kMaxDepthKeys;
   cache_planes_kernel<false><<<dim3(nch, a.chunks, z), 256, 0, st>>>(a);
   e = cudaGetLastError();
   const size_t smem = kBOff + kBStages * kBStage + kCtrlBytes;
+  const dim3 grid((s.max_ctx + a.span - 1) / a.span, rt * a.chunks, z);
   if (e == cudaSuccess)
-    e = launch(values_tc_kernel, dim3((s.max_ctx + a.span - 1) / a.span, rt * a.chunks, z), smem, st, a);
+    e = a.span >= s.max_ctx ? launch(values_tc_kernel<true>, grid, smem, st, a)
+                            : launch(values_tc_kernel<false>, grid, smem, st, a);
   const cudaError_t f = cudaFreeAsync(a.planes, st);
   return e == cudaSuccess ? f : e;
 }
