@@ -26,8 +26,8 @@ namespace sufb200 {
 
 namespace {
 
-constexpr int kThreads = 384;     // warp 0 copies A, warp 1 issues MMAs, warps 4-11 make B planes and store
-constexpr int kWorkers = 256;
+constexpr int kThreads = 640;  // warp 0 copies A, warp 1 issues MMAs, warps 4-19 make B planes and store
+constexpr int kWorkers = 512;
 constexpr uint32_t kAStage = 8 * kPlaneX;  // 32 KB: A planes of one step
 constexpr uint32_t kBStage = 8 * kPlaneY;  // 16 KB: B planes of one step
 constexpr int kAStages = 3;
@@ -60,30 +60,31 @@ __device__ __forceinline__ void put4(uint8_t* at, uint32_t plane, const uint64_t
   }
 }
 
-// Words of four rows, lane = depth, turned so that a lane holds row lane % 4
-// of the four depths of its group of four lanes (a 4 x 4 transpose by halves).
+// A warp's unit of the rows' planes is eight rows x 16 depths.  It is loaded
+// with lane = (row parity, depth), register j = row 2 j + parity (128 adjacent
+// bytes of two rows a load), and turned by a 4 x 4 transpose in every group of
+// four lanes: then a lane holds row 2 (lane % 4) + parity of the four depths
+// 4 (lane % 16 / 4) ..., and a warp's four-byte stores of one plane cover all 32
+// banks.
 __device__ __forceinline__ void turn4(uint64_t (&v)[4], int lane) {
+  const bool odd = lane & 1, high = lane & 2;
 #pragma unroll
   for (int i = 0; i < 4; i += 2) {
-    const uint64_t got = __shfl_xor_sync(0xffffffffu, lane & 1 ? v[i] : v[i + 1], 1);
-    if (lane & 1)
-      v[i] = got;
-    else
-      v[i + 1] = got;
+    const uint64_t got = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 1], 1);
+    v[i] = odd ? got : v[i];
+    v[i + 1] = odd ? v[i + 1] : got;
   }
 #pragma unroll
   for (int i = 0; i < 2; i++) {
-    const uint64_t got = __shfl_xor_sync(0xffffffffu, lane & 2 ? v[i] : v[i + 2], 2);
-    if (lane & 2)
-      v[i] = got;
-    else
-      v[i + 2] = got;
+    const uint64_t got = __shfl_xor_sync(0xffffffffu, high ? v[i] : v[i + 2], 2);
+    v[i] = high ? got : v[i];
+    v[i + 2] = high ? v[i + 2] : got;
   }
 }
 
-// Where a lane of turn4 puts its four depths of row r0 + lane % 4.
-__device__ __forceinline__ uint32_t turned_off(int r0, int lane) {
-  return core_off(r0 + (lane & 3), lane >> 4) + 4 * ((lane >> 2) & 3);
+// Where a lane of a turned unit (rows r0 ..., half h of the step) puts its bytes.
+__device__ __forceinline__ uint32_t turned_off(int r0, int h, int lane) {
+  return core_off(r0 + 2 * (lane & 3) + (lane >> 4), h) + 4 * ((lane & 15) >> 2);
 }
 
 // The cached operand's byte planes.  KEYS: block (128-key tile, chunk of 32
@@ -121,6 +122,13 @@ __global__ void __launch_bounds__(256) cache_planes_kernel(const __grid_constant
     put4(at, kPlaneX, e);
     put4(at + kAStage, kPlaneX, w);
   }
+}
+
+// True in one lane of the (converged) warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 
 // The mbarriers and flags behind the stages.
@@ -189,8 +197,9 @@ __device__ __forceinline__ void stop(const Ctrl& c, uint32_t tmem, uint32_t* sta
       for (int i = copies > kAStages ? copies - kAStages : 0; i < copies; i++)
         mbar_wait(c.afull + 8 * (i % kAStages), static_cast<uint32_t>((i / kAStages) & 1));
     }
-    if (warp == 1 && lane == 0) {
-      umma_commit(c.done);
+    if (warp == 1) {
+      if (elect_one()) umma_commit(c.done);
+      __syncwarp();
       mbar_wait(c.done, 0);
     }
   }
@@ -225,10 +234,10 @@ __device__ __forceinline__ void tmem_wait8(uint32_t (&v)[8]) {
                : "memory");
 }
 
-// sum_s (P_s mod 2^32) << 8s of 32 columns from `col` on, for this thread's lane.
-__device__ __forceinline__ void fold32(uint32_t tmem, int quarter, int col, uint64_t (&z)[32]) {
+// sum_s (P_s mod 2^32) << 8s of 16 columns from `col` on, for this thread's lane.
+__device__ __forceinline__ void fold16(uint32_t tmem, int quarter, int col, uint64_t (&z)[16]) {
 #pragma unroll
-  for (int cb = 0; cb < 4; cb++) {
+  for (int cb = 0; cb < 2; cb++) {
     uint32_t v[8][8];
 #pragma unroll
     for (int sd = 0; sd < 8; sd++)
@@ -265,14 +274,14 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
   const AttnSeqs& s = a.s;
   const AttnOperands& o = a.o;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, dh = s.head_dim, group = s.q_heads / s.kv_heads;
-  const int b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads;
+  const int b = blockIdx.x / s.kv_heads, kh = blockIdx.x % s.kv_heads;
   SeqInfo q;
   const bool fits = seq_info(s, b, o.status, q);
-  // the longest causal rows first
-  const int R = group * q.n, rho0 = static_cast<int>(gridDim.y - 1 - blockIdx.y) * kTN;
+  // every sequence's longest causal rows first
+  const int R = fits ? group * q.n : 0, rho0 = ((R + kTN - 1) / kTN - 1 - static_cast<int>(blockIdx.y)) * kTN;
   const int last = (rho0 + kTN < R ? rho0 + kTN : R) - 1;
-  const int len = fits && rho0 < R ? row_len(q.n, q.L, s.causal, last / group) : 0;
-  const int nt = (len + kTM - 1) / kTM, tile0 = blockIdx.x * a.span;
+  const int len = rho0 >= 0 && rho0 < R ? row_len(q.n, q.L, s.causal, last / group) : 0;
+  const int nt = (len + kTM - 1) / kTM, tile0 = blockIdx.z * a.span;
   const int tiles = nt - tile0 < a.span ? nt - tile0 : a.span;
   if (tiles <= 0) {
     pdl_wait();
@@ -310,42 +319,45 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
       bd[i] = umma_desc(sbase + kBOff + static_cast<uint32_t>(i) * kPlaneY);
       dt[i] = tmem + static_cast<uint32_t>(i * kTN);
     }
-    for (int tl = 0; tl < tiles; tl++) {
-      int go = 1;
-      if (lane == 0) {
-        // the rows' planes are written, the last tile is out of tensor memory
-        go = tl == 0 ? mbar_wait(c.bfull, 0) : mbar_wait(c.tempty, static_cast<uint32_t>((tl - 1) & 1));
-        for (int st = 0; st < steps && go; st++) {
-          const int li = tl * steps + st, as = li % kAStages;
-          go = mbar_wait(c.afull + 8 * as, static_cast<uint32_t>((li / kAStages) & 1));
-          if (!go) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    // The whole warp waits and steps, one elected lane issues: step, stage and
+    // descriptors stay warp-uniform.
+    bool go = true;
+    for (int tl = 0; tl < tiles && go; tl++) {
+      // the rows' planes are written, the last tile is out of tensor memory
+      go = __all_sync(0xffffffffu, tl == 0 ? mbar_wait(c.bfull, 0) : mbar_wait(c.tempty, static_cast<uint32_t>((tl - 1) & 1)));
+      for (int st = 0; st < steps && go; st++) {
+        const int li = tl * steps + st, as = li % kAStages;
+        go = __all_sync(0xffffffffu, mbar_wait(c.afull + 8 * as, static_cast<uint32_t>((li / kAStages) & 1)));
+        if (!go) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (elect_one()) {
           issue(dt, ad, bd, as, static_cast<uint32_t>(st) * kBStage, st > 0 ? 1u : 0u);
           umma_commit(c.aempty + 8 * as);
+          if (st + 1 == steps) umma_commit(c.tfull);
         }
-        if (go)
-          umma_commit(c.tfull);
-        else
-          *c.err = 1;
+        __syncwarp();
       }
-      if (!__shfl_sync(0xffffffffu, go, 0)) break;
     }
+    if (!go && lane == 0) *c.err = 1;
   } else {
-    // the rows' planes [U | D]: four rows of a chunk at a time
+    // the rows' planes [U | D]
     for (int u = warp - 2; u < a.chunks * (kTN / 4); u += kThreads / 32 - 2) {
-      const int ch = u / (kTN / 4), r0 = (u % (kTN / 4)) * 4, k = ch * kTK + lane;
-      uint64_t d[4], w[4];
+      const int ch = u / (kTN / 4), h = u & 1, r0 = (u % (kTN / 4)) / 2 * 8, k = ch * kTK + 16 * h + (lane & 15);
+      uint64_t d[4], w[4], x[4];
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const int rho = rho0 + r0 + j;
+        const int rho = rho0 + r0 + 2 * j + (lane >> 4);
         const bool in = rho < R && k < dh;
         const int64_t at = (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + k;
         d[j] = ld_if(o.x[0] + at, in);
-        w[j] = d[j] + ld_if(o.a[0] + at, in) + ld_if(o.a[1] + at, in);
+        w[j] = ld_if(o.a[0] + at, in);
+        x[j] = ld_if(o.a[1] + at, in);
       }
+#pragma unroll
+      for (int j = 0; j < 4; j++) w[j] += d[j] + x[j];
       turn4(w, lane);
       turn4(d, lane);
-      uint8_t* at = smem + kBOff + static_cast<uint32_t>(2 * ch) * kBStage + turned_off(r0, lane);
+      uint8_t* at = smem + kBOff + static_cast<uint32_t>(2 * ch) * kBStage + turned_off(r0, h, lane);
       put4(at, kPlaneY, w);
       put4(at + kBStage, kPlaneY, d);
     }
@@ -368,7 +380,9 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
       }
     }
   } else if (warp >= 4) {  // epilogue: while the next tile's MMAs run
-    const int quarter = warp & 3, col = ((warp - 4) >> 2) * 32;
+    // The MMAs take most of the shared-memory bandwidth, so the rows' places
+    // are worked out again for every column instead of being kept there.
+    const int quarter = warp & 3, col = ((warp - 4) >> 2) * 16;
     for (int tl = 0; tl < tiles; tl++) {
       int go = 1;
       if (lane == 0) go = mbar_wait(c.tfull, static_cast<uint32_t>(tl & 1));
@@ -377,25 +391,33 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
         break;
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      uint64_t z[32];
-      fold32(tmem, quarter, col, z);
+      uint64_t z[16];
+      fold16(tmem, quarter, col, z);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(c.tempty);
       const int key = (tile0 + tl) * kTM + quarter * 32 + lane;
+      int i = (rho0 + col) / group, g = (rho0 + col) % group;  // column col's query and head of the group
+      const int64_t head0 = q.base + static_cast<int64_t>(kh * group) * q.blk + key;
 #pragma unroll
-      for (int x0 = 0; x0 < 32; x0 += 8) {
+      for (int x0 = 0; x0 < 16; x0 += 8) {
         uint64_t c0[8], c1[8];
+        int64_t at[8];
+        bool in[8];
 #pragma unroll
         for (int x = 0; x < 8; x++) {
-          const int64_t at = c.row[col + x0 + x] + key;
-          const bool in = key < c.len[col + x0 + x];
-          c0[x] = ld_if(o.c[0] + at, in);
-          c1[x] = ld_if(o.c[1] + at, in);
+          at[x] = head0 + g * q.blk + row_off(q.n, q.L, s.causal, i);
+          in[x] = rho0 + col + x0 + x < R && key < row_len(q.n, q.L, s.causal, i);
+          c0[x] = ld_if(o.c[0] + at[x], in[x]);
+          c1[x] = ld_if(o.c[1] + at[x], in[x]);
+          if (++g == group) {
+            g = 0;
+            i++;
+          }
         }
 #pragma unroll
         for (int x = 0; x < 8; x++)
-          if (key < c.len[col + x0 + x]) o.out[c.row[col + x0 + x] + key] = z[x0 + x] + c0[x] + c1[x] + o.r;
+          if (in[x]) o.out[at[x]] = z[x0 + x] + c0[x] + c1[x] + o.r;
       }
     }
   }
@@ -410,14 +432,15 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
   const AttnSeqs& s = a.s;
   const AttnOperands& o = a.o;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, dh = s.head_dim, group = s.q_heads / s.kv_heads;
-  const int b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads, dt0 = blockIdx.y % a.chunks;
+  const int b = blockIdx.x / s.kv_heads, kh = blockIdx.x % s.kv_heads, dt0 = blockIdx.y % a.chunks;
   SeqInfo q;
   const bool fits = seq_info(s, b, o.status, q);
-  // the longest causal rows first
-  const int R = fits ? group * q.n : 0, rho0 = static_cast<int>((gridDim.y - 1 - blockIdx.y) / a.chunks) * kTN;
+  // every sequence's longest causal rows first
+  const int R = fits ? group * q.n : 0;
+  const int rho0 = ((R + kTN - 1) / kTN - 1 - static_cast<int>(blockIdx.y / a.chunks)) * kTN;
   const int last = (rho0 + kTN < R ? rho0 + kTN : R) - 1;
-  const int len = rho0 < R ? row_len(q.n, q.L, s.causal, last / group) : 0;
-  const int beg = blockIdx.x * a.span, end = len < beg + a.span ? len : beg + a.span;
+  const int len = rho0 >= 0 && rho0 < R ? row_len(q.n, q.L, s.causal, last / group) : 0;
+  const int beg = blockIdx.z * a.span, end = len < beg + a.span ? len : beg + a.span;
   const int nch = end > beg ? (end - beg + kTK - 1) / kTK : 0;
   const int word0 = dt0 * kTM;
   // word `word` of the output of row rho
@@ -426,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
   };
   if (nch == 0) {
     pdl_wait();
-    if (SOLO && rho0 < R)  // rows without keys: C_0 + C_1 + r
+    if (SOLO && rho0 >= 0 && rho0 < R)  // rows without keys: C_0 + C_1 + r
       for (int e = t; e < kTN * kTM; e += kThreads) {
         const int rho = rho0 + e / kTM, word = word0 + e % kTM;
         if (rho < R && word < dh) o.out[place(rho, word)] = o.c[0][place(rho, word)] + o.c[1][place(rho, word)] + o.r;
@@ -465,54 +488,58 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
       bd[i] = umma_desc(sbase + kBOff + static_cast<uint32_t>(i) * kPlaneY);
       dt[i] = tmem + static_cast<uint32_t>(i * kTN);
     }
-    int go = 1;
+    bool go = true;
     for (int li = 0; li < 2 * nch; li++) {
-      if (lane == 0) {
-        const int as = li % kAStages, bs = li % kBStages;
-        go = mbar_wait(c.afull + 8 * as, static_cast<uint32_t>((li / kAStages) & 1)) &&
-             mbar_wait(c.bfull + 8 * bs, static_cast<uint32_t>((li / kBStages) & 1));
-        if (go) {
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          issue(dt, ad, bd, as, static_cast<uint32_t>(bs) * kBStage, li > 0 ? 1u : 0u);
-          umma_commit(c.aempty + 8 * as);
-          umma_commit(c.bempty + 8 * bs);
-        } else {
-          *c.err = 1;
-        }
+      const int as = li % kAStages, bs = li % kBStages;
+      go = __all_sync(0xffffffffu, mbar_wait(c.afull + 8 * as, static_cast<uint32_t>((li / kAStages) & 1)) &&
+                                       mbar_wait(c.bfull + 8 * bs, static_cast<uint32_t>((li / kBStages) & 1)));
+      if (!go) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (elect_one()) {
+        issue(dt, ad, bd, as, static_cast<uint32_t>(bs) * kBStage, li > 0 ? 1u : 0u);
+        umma_commit(c.aempty + 8 * as);
+        umma_commit(c.bempty + 8 * bs);
+        if (li + 1 == 2 * nch) umma_commit(c.tfull);
       }
-      if (!__shfl_sync(0xffffffffu, go, 0)) break;
+      __syncwarp();
     }
-    if (lane == 0 && go) umma_commit(c.tfull);
-    __syncwarp();
+    if (!go && lane == 0) *c.err = 1;
   } else if (warp >= 4) {
-    // A worker warp's eight rows of a chunk, lane = key: 256 adjacent bytes a
-    // load.  The next chunk's shares are in flight while this one's are split.
-    const int r0 = (warp - 4) * 8;
-    uint64_t p0[8], p1[8], a0[8], a1[8];
-    const auto fetch = [&](int ch) {
-      const int key = beg + ch * kTK + lane;
+    // A worker warp has one unit of every chunk.  The next chunk's shares are in
+    // flight while this one's are split.
+    const int r0 = ((warp - 4) >> 1) * 8, h = warp & 1;
+    int64_t row[4];
+    int m[4];
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const int64_t at = c.row[r0 + j] + key;
-        const bool in = key < c.len[r0 + j];
-        p0[j] = ld_if(o.x[0] + at, in);
-        p1[j] = ld_if(o.x[1] + at, in);
-        a0[j] = ld_if(o.a[0] + at, in);
-        a1[j] = ld_if(o.a[1] + at, in);
+    for (int j = 0; j < 4; j++) {
+      row[j] = c.row[r0 + 2 * j + (lane >> 4)];
+      m[j] = c.len[r0 + 2 * j + (lane >> 4)];
+    }
+    uint64_t p0[4], p1[4], a0[4], a1[4];
+    const auto fetch = [&](int ch) {
+      const int key = beg + ch * kTK + 16 * h + (lane & 15);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const bool in = key < m[j];
+        p0[j] = ld_if(o.x[0] + row[j] + key, in);
+        p1[j] = ld_if(o.x[1] + row[j] + key, in);
+        a0[j] = ld_if(o.a[0] + row[j] + key, in);
+        a1[j] = ld_if(o.a[1] + row[j] + key, in);
       }
     };
     fetch(0);
     int go = 1;
+    const uint32_t mine = turned_off(r0, h, lane);
     for (int ch = 0; ch < nch; ch++) {
-      uint64_t d[2][4], u[2][4];
+      uint64_t d[4], u[4];
 #pragma unroll
-      for (int g = 0; g < 2; g++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          d[g][j] = (p0[4 * g + j] - a0[4 * g + j]) + (p1[4 * g + j] - a1[4 * g + j]);
-          u[g][j] = d[g][j] + a0[4 * g + j] + a1[4 * g + j];
-        }
+      for (int j = 0; j < 4; j++) {
+        d[j] = (p0[j] - a0[j]) + (p1[j] - a1[j]);
+        u[j] = d[j] + a0[j] + a1[j];
+      }
       if (ch + 1 < nch) fetch(ch + 1);
+      turn4(u, lane);
+      turn4(d, lane);
       const int su = (2 * ch) % kBStages, sd = su + 1;
       if (lane == 0 && 2 * ch >= kBStages)
         go = mbar_wait(c.bempty + 8 * su, static_cast<uint32_t>(((2 * ch / kBStages) - 1) & 1)) &&
@@ -521,17 +548,9 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
         if (lane == 0) *c.err = 1;
         break;
       }
-      uint8_t* at = smem + kBOff + static_cast<uint32_t>(su) * kBStage;
-#pragma unroll
-      for (int g = 0; g < 2; g++) {
-        turn4(u[g], lane);
-        put4(at + turned_off(r0 + 4 * g, lane), kPlaneY, u[g]);
-      }
-#pragma unroll
-      for (int g = 0; g < 2; g++) {
-        turn4(d[g], lane);
-        put4(at + kBStage + turned_off(r0 + 4 * g, lane), kPlaneY, d[g]);
-      }
+      uint8_t* at = smem + kBOff + static_cast<uint32_t>(su) * kBStage + mine;
+      put4(at, kPlaneY, u);
+      put4(at + kBStage, kPlaneY, d);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // generic writes -> tensor core reads
       __syncwarp();
       if (lane == 0) {
@@ -542,13 +561,13 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
     if (lane == 0 && go) go = mbar_wait(c.tfull, 0);
     if (__shfl_sync(0xffffffffu, go, 0)) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int quarter = warp & 3, col = ((warp - 4) >> 2) * 32;
-      uint64_t z[32];
-      fold32(tmem, quarter, col, z);
+      const int quarter = warp & 3, col = ((warp - 4) >> 2) * 16;
+      uint64_t z[16];
+      fold16(tmem, quarter, col, z);
       const int word = word0 + quarter * 32 + lane;
       if (SOLO) {
 #pragma unroll
-        for (int x0 = 0; x0 < 32; x0 += 8) {
+        for (int x0 = 0; x0 < 16; x0 += 8) {
           uint64_t c0[8], c1[8];
 #pragma unroll
           for (int x = 0; x < 8; x++) {
@@ -565,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
         }
       } else {
 #pragma unroll
-        for (int x = 0; x < 32; x++) {
+        for (int x = 0; x < 16; x++) {
           const int rho = rho0 + col + x;
           if (rho < R && word < dh)
             atomicAdd(reinterpret_cast<unsigned long long*>(o.out + place(rho, word)), static_cast<unsigned long long>(z[x]));
@@ -601,11 +620,11 @@ cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const 
   // key tiles per CTA: long runs reuse the rows' planes and hide the epilogue
   // behind the next tile, as long as every SM has a few CTAs to take
   const int64_t all = static_cast<int64_t>(nt) * rt * z, want = all / (static_cast<int64_t>(ctx->sm_count) * 4);
-  a.span = static_cast<int>(want < 1 ? 1 : (want > 8 ? 8 : want));
+  a.span = static_cast<int>(want < 1 ? 1 : (want > 16 ? 16 : want));
   cache_planes_kernel<true><<<dim3(nt, a.chunks, z), 256, 0, st>>>(a);
   e = cudaGetLastError();
   const size_t smem = kBOff + static_cast<size_t>(2 * a.chunks) * kBStage + kCtrlBytes;
-  if (e == cudaSuccess) e = launch(scores_tc_kernel, dim3((nt + a.span - 1) / a.span, rt, z), smem, st, a);
+  if (e == cudaSuccess) e = launch(scores_tc_kernel, dim3(z, rt, (nt + a.span - 1) / a.span), smem, st, a);
   const cudaError_t f = cudaFreeAsync(a.planes, st);
   return e == cudaSuccess ? f : e;
 }
@@ -636,7 +655,7 @@ cudaError_t launch_values_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const 
   cache_planes_kernel<false><<<dim3(nch, a.chunks, z), 256, 0, st>>>(a);
   e = cudaGetLastError();
   const size_t smem = kBOff + kBStages * kBStage + kCtrlBytes;
-  const dim3 grid((s.max_ctx + a.span - 1) / a.span, rt * a.chunks, z);
+  const dim3 grid(z, rt * a.chunks, (s.max_ctx + a.span - 1) / a.span);
   if (e == cudaSuccess)
     e = a.span >= s.max_ctx ? launch(values_tc_kernel<true>, grid, smem, st, a)
                             : launch(values_tc_kernel<false>, grid, smem, st, a);
