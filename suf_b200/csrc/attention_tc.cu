@@ -365,21 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
     __syncwarp();
     if (lane == 0) mbar_arrive(c.bfull);
   }
-  if (warp == 2 || warp == 3) {  // C of the coming tiles into L2, about a tile ahead of the epilogue
-    for (int tl = 0; tl < tiles; tl++) {
-      int go = 1;
-      if (lane == 0 && tl > 1) go = mbar_wait(c.tfull, static_cast<uint32_t>((tl - 2) & 1));
-      if (!__shfl_sync(0xffffffffu, go, 0)) break;  // the MMA warp reports it
-      const int k0 = (tile0 + tl) * kTM;
-      for (int u = (warp - 2) * 32 + lane; u < kTN * 9; u += 64) {
-        const int r = u / 9, k = k0 + (u % 9) * 16 < k0 + kTM ? k0 + (u % 9) * 16 : k0 + kTM - 1;
-        if (k < c.len[r]) {
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(o.c[0] + c.row[r] + k));
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(o.c[1] + c.row[r] + k));
-        }
-      }
-    }
-  } else if (warp >= 4) {  // epilogue: while the next tile's MMAs run
+  if (warp >= 4) {  // epilogue: while the next tile's MMAs run
     // The MMAs take most of the shared-memory bandwidth, so the rows' places
     // are worked out again for every column instead of being kept there.
     const int quarter = warp & 3, col = ((warp - 4) >> 2) * 16;

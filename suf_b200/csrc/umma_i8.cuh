@@ -42,11 +42,18 @@ __device__ __forceinline__ uint64_t global_ns() {
 
 // Bounded wait for the phase with the given parity (iterations and wall
 // time, since one try_wait may suspend for an implementation-defined while);
-// false on timeout.
+// false on timeout.  The clock is read from the 256th try on: reading it costs
+// more than the wait of a phase that is already complete.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-  const uint64_t t0 = global_ns();
+  uint64_t t0 = 0;
   for (uint32_t it = 0; it < kWaitIters; it++) {
-    if ((it & 255u) == 255u && global_ns() - t0 > kWaitNs) return false;
+    if ((it & 255u) == 255u) {
+      const uint64_t now = global_ns();
+      if (t0 == 0)
+        t0 = now;
+      else if (now - t0 > kWaitNs)
+        return false;
+    }
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
