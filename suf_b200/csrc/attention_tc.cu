@@ -160,8 +160,10 @@ __device__ __forceinline__ Ctrl ctrl_at(uint8_t* smem, uint32_t off) {
 }
 static_assert(16 * kAStages + 16 * kBStages + 32 <= 512 && 512 + 12 * kTN <= kCtrlBytes, "control block");
 
-// Tensor memory and barriers; every thread of the CTA.  Returns the columns' base.
-__device__ __forceinline__ uint32_t start(const Ctrl& c, int warp, int t, int bwarps) {
+// Tensor memory and barriers; every thread of the CTA.  A CTA takes all 512
+// columns, so they start at column 0 and the accumulators' addresses are
+// constants; false (and *err set) should they not.
+__device__ __forceinline__ bool start(const Ctrl& c, int warp, int t, int bwarps) {
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(c.slot), "r"(kTmemCols)
                  : "memory");
@@ -184,12 +186,13 @@ __device__ __forceinline__ uint32_t start(const Ctrl& c, int warp, int t, int bw
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  return *c.tmem_slot;
+  if (*c.tmem_slot != 0) *c.err = 1;
+  return *c.tmem_slot == 0;
 }
 
 // All threads: report a wait that gave up, let what was issued finish (again
 // with a limit) and free the tensor memory.  `copies` = A copies issued.
-__device__ __forceinline__ void stop(const Ctrl& c, uint32_t tmem, uint32_t* status, int warp, int lane, int copies) {
+__device__ __forceinline__ void stop(const Ctrl& c, uint32_t* status, int warp, int lane, int copies) {
   __syncthreads();
   if (*c.err) {
     if (warp == 0 && lane == 0) {
@@ -207,7 +210,7 @@ __device__ __forceinline__ void stop(const Ctrl& c, uint32_t tmem, uint32_t* sta
   __syncthreads();
   if (warp == 0) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*c.tmem_slot), "r"(kTmemCols) : "memory");
   }
 }
 
@@ -220,53 +223,59 @@ __device__ __forceinline__ bool load_a(const Ctrl& c, uint32_t sbase, int li, co
   return true;
 }
 
-// 8 columns of this warp's 32 lanes; the registers are valid after tmem_wait8.
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+// 4 columns of this warp's 32 lanes; the registers are valid after tmem_wait4.
+__device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t (&v)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
                : "r"(taddr));
 }
 
-__device__ __forceinline__ void tmem_wait8(uint32_t (&v)[8]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])
-               :
-               : "memory");
+__device__ __forceinline__ void tmem_wait4(uint32_t (&v)[4]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]) : : "memory");
 }
 
-// sum_s (P_s mod 2^32) << 8s of 16 columns from `col` on, for this thread's lane.
-__device__ __forceinline__ void fold16(uint32_t tmem, int quarter, int col, uint64_t (&z)[16]) {
+// sum_s (P_s mod 2^32) << 8s of 16 columns from `col` on, for this thread's
+// lane; four columns at a time (all eight diagonals of more would spill).
+__device__ __forceinline__ void fold16(int quarter, int col, uint64_t (&z)[16]) {
 #pragma unroll
-  for (int cb = 0; cb < 2; cb++) {
-    uint32_t v[8][8];
+  for (int cb = 0; cb < 4; cb++) {
+    uint32_t v[8][4];
 #pragma unroll
     for (int sd = 0; sd < 8; sd++)
-      tmem_ld8(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(sd * kTN + col + cb * 8), v[sd]);
+      tmem_ld4((static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(sd * kTN + col + cb * 4), v[sd]);
 #pragma unroll
-    for (int sd = 0; sd < 8; sd++) tmem_wait8(v[sd]);
+    for (int sd = 0; sd < 8; sd++) tmem_wait4(v[sd]);
 #pragma unroll
-    for (int x = 0; x < 8; x++) {
+    for (int x = 0; x < 4; x++) {
       uint64_t lo = v[0][x];
 #pragma unroll
       for (int sd = 1; sd < 4; sd++) lo += static_cast<uint64_t>(v[sd][x]) << (8 * sd);
       const uint32_t hi = v[4][x] + (v[5][x] << 8) + (v[6][x] << 16) + (v[7][x] << 24);
-      z[cb * 8 + x] = lo + (static_cast<uint64_t>(hi) << 32);
+      z[cb * 4 + x] = lo + (static_cast<uint64_t>(hi) << 32);
     }
   }
 }
 
-// The MMAs of one step: A stage li, B planes at byte offset boff, then the commits.
-__device__ __forceinline__ void issue(const uint32_t (&dt)[8], const uint64_t (&ad)[8], const uint64_t (&bd)[8], int st,
-                                      uint32_t boff, uint32_t accumulate) {
-  const uint64_t ao = static_cast<uint64_t>((static_cast<uint32_t>(st) * kAStage) >> 4);
-  const uint64_t bo = static_cast<uint64_t>(boff >> 4);
-  uint64_t as[8], bs[8];
+// The twelve MMAs of one step (umma_i8.cuh's mma_step) on the A planes at
+// shared address a and the B planes at b.  One thread issues them, and its
+// instructions bound a step once the copies keep up (the twelve take about
+// 1,210 cycles of the tensor core): accumulators, shapes and the descriptors'
+// high words are constants, only two 32-bit bases vary.
+__device__ __forceinline__ uint64_t plane_desc(uint32_t base_lo, uint32_t planes_off) {
+  return static_cast<uint64_t>(base_lo + (planes_off >> 4)) | (static_cast<uint64_t>((1u << 14) | (256u >> 4)) << 32);
+}
+__device__ __forceinline__ uint32_t desc_base(uint32_t saddr) { return (saddr >> 4) | ((128u >> 4) << 16); }
+
+__device__ __forceinline__ void issue(uint32_t a, uint32_t b, uint32_t accumulate) {
+  const uint32_t al = desc_base(a), bl = desc_base(b);
+  umma_i8(0, plane_desc(al, 0), plane_desc(bl, 0), idesc_n(256), accumulate);
+  umma_i8(4 * kTN, plane_desc(al, 0), plane_desc(bl, 4 * kPlaneY), idesc_n(256), accumulate);
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    as[i] = ad[i] + ao;
-    bs[i] = bd[i] + bo;
-  }
-  mma_step(dt, as, bs, accumulate);
+  for (int i = 1; i < 8; i++)
+    umma_i8(i * kTN, plane_desc(al, i * kPlaneX), plane_desc(bl, 0), idesc_n(i <= 4 ? 256 : 64 * (8 - i)), 1u);
+#pragma unroll
+  for (int i = 1; i < 4; i++)
+    umma_i8((i + 4) * kTN, plane_desc(al, i * kPlaneX), plane_desc(bl, 4 * kPlaneY), idesc_n(256 - 64 * i), 1u);
 }
 
 __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_constant__ AttnTc a) {
@@ -295,10 +304,11 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
     c.row[t] = rho < R ? q.base + (kh * group + rho % group) * q.blk + row_off(q.n, q.L, s.causal, i) : 0;
     c.len[t] = rho < R ? row_len(q.n, q.L, s.causal, i) : 0;
   }
-  const uint32_t tmem = start(c, warp, t, kThreads / 32 - 2);
+  const bool ready = start(c, warp, t, kThreads / 32 - 2);
   int copies = 0;
 
-  if (warp == 0) {  // A planes: every step of every key tile
+  if (!ready) {
+  } else if (warp == 0) {  // A planes: every step of every key tile
     pdl_wait();  // written by the pre-pass
     const uint8_t* src = a.planes + (kh * a.tiles + first_block(q.l0, b, kTM) + tile0) * steps * static_cast<int64_t>(kAStage);
     for (int li = 0; li < tiles * steps; li++) {
@@ -311,14 +321,6 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
       copies++;
     }
   } else if (warp == 1) {  // MMAs
-    uint64_t ad[8], bd[8];
-    uint32_t dt[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      ad[i] = umma_desc(sbase + static_cast<uint32_t>(i) * kPlaneX);
-      bd[i] = umma_desc(sbase + kBOff + static_cast<uint32_t>(i) * kPlaneY);
-      dt[i] = tmem + static_cast<uint32_t>(i * kTN);
-    }
     // The whole warp waits and steps, one elected lane issues: step, stage and
     // descriptors stay warp-uniform.
     bool go = true;
@@ -331,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
         if (!go) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (elect_one()) {
-          issue(dt, ad, bd, as, static_cast<uint32_t>(st) * kBStage, st > 0 ? 1u : 0u);
+          issue(sbase + static_cast<uint32_t>(as) * kAStage, sbase + kBOff + static_cast<uint32_t>(st) * kBStage, st > 0 ? 1u : 0u);
           umma_commit(c.aempty + 8 * as);
           if (st + 1 == steps) umma_commit(c.tfull);
         }
@@ -365,10 +367,15 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
     __syncwarp();
     if (lane == 0) mbar_arrive(c.bfull);
   }
-  if (warp >= 4) {  // epilogue: while the next tile's MMAs run
-    // The MMAs take most of the shared-memory bandwidth, so the rows' places
-    // are worked out again for every column instead of being kept there.
+  if (ready && warp >= 4) {  // epilogue: while the next tile's MMAs run
+    // The MMAs take most of the shared-memory bandwidth and every multiply of
+    // an address would stand in this warp's chain, so the rows' places are
+    // stepped from one row to the next (row_off, row_len by differences).
     const int quarter = warp & 3, col = ((warp - 4) >> 2) * 16;
+    const int i0 = (rho0 + col) / group, g0 = (rho0 + col) % group;  // the first row's query and head of the group
+    const int rows = R - rho0 - col;                                 // rows there are, from there on
+    const int64_t at0 = q.base + static_cast<int64_t>(kh * group) * q.blk + row_off(q.n, q.L, s.causal, i0);
+    const int len0 = s.causal ? q.L - q.n + i0 + 1 : q.L;
     for (int tl = 0; tl < tiles; tl++) {
       int go = 1;
       if (lane == 0) go = mbar_wait(c.tfull, static_cast<uint32_t>(tl & 1));
@@ -378,36 +385,48 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       uint64_t z[16];
-      fold16(tmem, quarter, col, z);
+      fold16(quarter, col, z);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(c.tempty);
       const int key = (tile0 + tl) * kTM + quarter * 32 + lane;
-      int i = (rho0 + col) / group, g = (rho0 + col) % group;  // column col's query and head of the group
-      const int64_t head0 = q.base + static_cast<int64_t>(kh * group) * q.blk + key;
+      // this query's row of the group's first head, and this row
+      int g = g0, len = len0;
+      int64_t row = at0 + key, at = row + g0 * q.blk;
+      const auto next = [&] {
+        at += q.blk;
+        if (++g == group) {
+          g = 0;
+          row += len > 0 ? len : 0;
+          at = row;
+          len += s.causal ? 1 : 0;
+        }
+      };
 #pragma unroll
       for (int x0 = 0; x0 < 16; x0 += 8) {
         uint64_t c0[8], c1[8];
-        int64_t at[8];
-        bool in[8];
+        const int g1 = g, len1 = len;
+        const int64_t row1 = row, at1 = at;
 #pragma unroll
         for (int x = 0; x < 8; x++) {
-          at[x] = head0 + g * q.blk + row_off(q.n, q.L, s.causal, i);
-          in[x] = rho0 + col + x0 + x < R && key < row_len(q.n, q.L, s.causal, i);
-          c0[x] = ld_if(o.c[0] + at[x], in[x]);
-          c1[x] = ld_if(o.c[1] + at[x], in[x]);
-          if (++g == group) {
-            g = 0;
-            i++;
-          }
+          const bool in = x0 + x < rows && key < len;
+          c0[x] = ld_if(o.c[0] + at, in);
+          c1[x] = ld_if(o.c[1] + at, in);
+          next();
         }
+        g = g1;  // the same eight rows again: stepping costs less than keeping their places
+        len = len1;
+        row = row1;
+        at = at1;
 #pragma unroll
-        for (int x = 0; x < 8; x++)
-          if (in[x]) o.out[at[x]] = z[x0 + x] + c0[x] + c1[x] + o.r;
+        for (int x = 0; x < 8; x++) {
+          if (x0 + x < rows && key < len) o.out[at] = z[x0 + x] + c0[x] + c1[x] + o.r;
+          next();
+        }
       }
     }
   }
-  stop(c, tmem, o.status, warp, lane, copies);
+  stop(c, o.status, warp, lane, copies);
 }
 
 // SOLO: one CTA has all keys of a row tile and stores; else the ranges add to
@@ -450,10 +469,11 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
     c.row[t] = rho < R ? q.base + (kh * group + rho % group) * q.blk + row_off(q.n, q.L, s.causal, i) : 0;
     c.len[t] = m < end ? m : end;
   }
-  const uint32_t tmem = start(c, warp, t, kWorkers / 32);
+  const bool ready = start(c, warp, t, kWorkers / 32);
   int copies = 0;
 
-  if (warp == 0) {
+  if (!ready) {
+  } else if (warp == 0) {
     pdl_wait();
     const int64_t block0 = kh * a.tiles + first_block(q.l0, b, kTK) + beg / kTK;
     for (int li = 0; li < 2 * nch; li++) {
@@ -466,14 +486,6 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
       copies++;
     }
   } else if (warp == 1) {
-    uint64_t ad[8], bd[8];
-    uint32_t dt[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      ad[i] = umma_desc(sbase + static_cast<uint32_t>(i) * kPlaneX);
-      bd[i] = umma_desc(sbase + kBOff + static_cast<uint32_t>(i) * kPlaneY);
-      dt[i] = tmem + static_cast<uint32_t>(i * kTN);
-    }
     bool go = true;
     for (int li = 0; li < 2 * nch; li++) {
       const int as = li % kAStages, bs = li % kBStages;
@@ -482,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
       if (!go) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (elect_one()) {
-        issue(dt, ad, bd, as, static_cast<uint32_t>(bs) * kBStage, li > 0 ? 1u : 0u);
+        issue(sbase + static_cast<uint32_t>(as) * kAStage, sbase + kBOff + static_cast<uint32_t>(bs) * kBStage, li > 0 ? 1u : 0u);
         umma_commit(c.aempty + 8 * as);
         umma_commit(c.bempty + 8 * bs);
         if (li + 1 == 2 * nch) umma_commit(c.tfull);
@@ -549,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int quarter = warp & 3, col = ((warp - 4) >> 2) * 16;
       uint64_t z[16];
-      fold16(tmem, quarter, col, z);
+      fold16(quarter, col, z);
       const int word = word0 + quarter * 32 + lane;
       if (SOLO) {
 #pragma unroll
@@ -580,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
       *c.err = 1;
     }
   }
-  stop(c, tmem, o.status, warp, lane, copies);
+  stop(c, o.status, warp, lane, copies);
 }
 
 template <typename K>
