@@ -39,10 +39,14 @@ M64 = (1 << 64) - 1
 # checks cost on the host counts there, so they look at one attribute after
 # the other and only a refusal formats anything.
 
+_current_raw = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def _stream(ctx: Context, stream) -> int | None:
     """The raw stream a call runs on (None: the device's legacy stream)."""
     if stream is None:
-        return torch.cuda.current_stream(ctx.device).cuda_stream or None
+        return _current_raw(ctx.device) or None
     if isinstance(stream, int):
         return stream or None
     if stream.device_index != ctx.device:
@@ -76,13 +80,15 @@ def _refuse(ctx: Context, name: str, t, shape, dtype):
     raise ValueError(f"{name}: not contiguous")
 
 
-def _want(ctx: Context, name: str, t, shape: tuple, dtype=None) -> int:
+def _want(ctx: Context, name: str, t, shape: tuple, dtype=torch.int64) -> int:
     """The address of a dense tensor: int64 words unless `dtype`, on the device, of the shape (None: any extent)."""
-    dtype = dtype or torch.int64
-    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == ctx.device and
-            (t.shape == shape or (None in shape and t.dim() == len(shape) and
-                                  all(w is None or w == g for w, g in zip(shape, t.shape)))) and t.is_contiguous()):
-        return t.data_ptr()
+    try:
+        if t.dtype is dtype and t.get_device() == ctx.device and t.is_contiguous() and (
+                t.shape == shape or (None in shape and t.dim() == len(shape) and
+                                     all(w is None or w == g for w, g in zip(shape, t.shape)))):
+            return t.data_ptr()
+    except AttributeError:
+        pass
     _refuse(ctx, name, t, shape, dtype)
 
 
@@ -94,7 +100,8 @@ def _pair(ctx: Context, name: str, ts, shape: tuple):
     """Both parties' addresses."""
     if not isinstance(ts, (tuple, list)) or len(ts) != 2:
         raise ValueError(f"{name}: expected both parties' tensors")
-    return _Two(_want(ctx, name, ts[0], shape), _want(ctx, name, ts[1], shape))
+    x, y = ts
+    return _Two(_want(ctx, name, x, shape), _want(ctx, name, y, shape))
 
 
 def _masks(r):
@@ -215,16 +222,17 @@ def _strided(ctx: Context, name: str, ts, shape: tuple):
     """Both parties' addresses and the common strides of [tokens][heads][dim] views (the last axis dense)."""
     if not isinstance(ts, (tuple, list)) or len(ts) != 2:
         raise ValueError(f"{name}: expected both parties' tensors")
-    for t in ts:
+    x, y = ts
+    for t in (x, y):
         if (not isinstance(t, torch.Tensor) or t.dtype is not torch.int64 or t.get_device() != ctx.device or
                 t.shape != shape):
             _refuse(ctx, name, t, shape, torch.int64)
-    ld = ts[0].stride()
-    if ld != ts[1].stride():
+    ld = x.stride()
+    if ld != y.stride():
         raise ValueError(f"{name}: the parties' strides differ")
-    if ld[2] != 1 and ts[0].numel():
+    if ld[2] != 1 and x.numel():
         raise ValueError(f"{name}: the head's words must be adjacent")
-    return _Two(ts[0].data_ptr(), ts[1].data_ptr()), ld[0], ld[1]
+    return _Two(x.data_ptr(), y.data_ptr()), ld[0], ld[1]
 
 
 def rope_append_pair(ctx: Context, q, k, v, positions, slots, cos, sin, trunc: TruncPair | None, a, cache: ShareCache,

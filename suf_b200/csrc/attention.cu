@@ -32,25 +32,26 @@ int fail(int code, const std::string& msg) { return record_error(code, msg); }
 // ---- few rows (single tokens): bound by the cache's three words per entry --
 // scores_rows: eight lanes per key, 16 bytes of the head each; the rows' U =
 // D + A_0 + A_1 and D sit in shared memory and are read once for two keys.
-constexpr int kKeyChunk = 128;  // keys per CTA
+constexpr int kKeyChunk = 256;  // most keys per CTA
 
 template <int RT>
-__global__ void __launch_bounds__(kThreads) scores_rows_kernel(const __grid_constant__ AttnSeqs s,
-                                                               const __grid_constant__ AttnOperands o) {
+__global__ void __launch_bounds__(kThreads, RT == 4 ? 4 : 3) scores_rows_kernel(const __grid_constant__ AttnSeqs s,
+                                                                                const __grid_constant__ AttnOperands o,
+                                                                                int chunk) {
   extern __shared__ __align__(16) uint64_t sm[];
-  __shared__ int64_t s_key[kKeyChunk];
-  __shared__ uint64_t s_out[RT][kKeyChunk + 1];
   const int t = threadIdx.x, dh = s.head_dim, group = s.q_heads / s.kv_heads;
   const int b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads;
   SeqInfo q;
   if (!seq_info(s, b, o.status, q)) return;
-  const int R = group * q.n, rho0 = blockIdx.y * RT, k0 = blockIdx.x * kKeyChunk;
+  const int R = group * q.n, rho0 = blockIdx.y * RT, k0 = blockIdx.x * chunk;
   if (rho0 >= R) return;
   const int last = (rho0 + RT < R ? rho0 + RT : R) - 1;
   const int len = row_len(q.n, q.L, s.causal, last / group);  // the longest row of the tile
   if (k0 >= len) return;
-  uint64_t* sU = sm;
-  uint64_t* sD = sm + RT * dh;
+  uint64_t* sU = sm;                    // [RT][dh]
+  uint64_t* sD = sU + RT * dh;          // [RT][dh]
+  uint64_t* s_out = sD + RT * dh;       // [RT][chunk + 1]
+  int64_t* s_key = reinterpret_cast<int64_t*>(s_out + RT * (chunk + 1));  // [chunk]
   for (int e = t; e < RT * dh; e += kThreads) {
     const int rr = e / dh, c = e % dh, rho = rho0 + rr;
     uint64_t d = 0, u = 0;
@@ -62,10 +63,10 @@ __global__ void __launch_bounds__(kThreads) scores_rows_kernel(const __grid_cons
     sU[e] = u;
     sD[e] = d;
   }
-  for (int e = t; e < kKeyChunk; e += kThreads) s_key[e] = k0 + e < len ? key_off(s, b, kh, k0 + e, o.status) : -1;
+  for (int e = t; e < chunk; e += kThreads) s_key[e] = k0 + e < len ? key_off(s, b, kh, k0 + e, o.status) : -1;
   __syncthreads();
   const int l8 = t & 7, grp = t >> 3;
-  for (int kk = grp; kk < kKeyChunk; kk += 64) {
+  for (int kk = grp; kk < chunk; kk += 64) {
     const int64_t o0 = s_key[kk], o1 = s_key[kk + 32];
     uint64_t acc[2][RT] = {};
     for (int c = l8; c < dh / 2; c += 8) {
@@ -95,15 +96,15 @@ __global__ void __launch_bounds__(kThreads) scores_rows_kernel(const __grid_cons
         uint64_t z = acc[v][rr];
 #pragma unroll
         for (int m = 4; m > 0; m >>= 1) z += __shfl_xor_sync(0xffffffffu, z, m);
-        if (l8 == rr % 8) s_out[rr][kk + 32 * v] = z;
+        if (l8 == rr % 8) s_out[rr * (chunk + 1) + kk + 32 * v] = z;
       }
   }
   __syncthreads();
-  for (int e = t; e < RT * kKeyChunk; e += kThreads) {
-    const int rr = e / kKeyChunk, kk = e % kKeyChunk, rho = rho0 + rr, i = rho / group;
+  for (int e = t; e < RT * chunk; e += kThreads) {
+    const int rr = e / chunk, kk = e % chunk, rho = rho0 + rr, i = rho / group;
     if (rho >= R || k0 + kk >= row_len(q.n, q.L, s.causal, i)) continue;
     const int64_t at = q.base + (kh * group + rho % group) * q.blk + row_off(q.n, q.L, s.causal, i) + k0 + kk;
-    o.out[at] = s_out[rr][kk] + o.c[0][at] + o.c[1][at] + o.r;
+    o.out[at] = s_out[rr * (chunk + 1) + kk] + o.c[0][at] + o.c[1][at] + o.r;
   }
 }
 
@@ -320,6 +321,19 @@ int check_operands(const AttnOperands& o, const char* who) {
 // Rows of a (sequence, key head) up to which the row kernels are used.
 constexpr int kFewRows = 16;
 
+// Keys a CTA of the row kernels walks: the longest run (least, doubled up to
+// most) that still leaves `per_sm` CTAs per SM.  A long run pays its set-up
+// once, a short cache wants every SM.  One step over 73,279 cached tokens of
+// 8 x 128 words: scores 332 us in runs of 256 (eight CTAs per SM asked for),
+// 348 us in runs of 128; values 315 us in runs of 1,024 (three asked for),
+// 322 of 512, 331 of 256.
+int keys_per_cta(const sufb200_ctx_s* ctx, const AttnSeqs& s, int rows, int least, int most, int per_sm) {
+  const int64_t keys = s.cached * s.kv_heads * ((rows + 7) / 8), ctas = static_cast<int64_t>(ctx->sm_count) * per_sm;
+  int run = least;
+  while (run < most && keys / (2 * run) >= ctas) run *= 2;
+  return run;
+}
+
 }  // namespace
 
 int attn_check_ctx(sufb200_ctx ctx) {
@@ -350,11 +364,15 @@ int sufb200_attn_scores_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
   const int rows = seqs->q_heads / seqs->kv_heads * seqs->max_q;
   const unsigned z = static_cast<unsigned>(seqs->batch) * seqs->kv_heads;
   if (rows <= kFewRows) {
-    const unsigned x = (seqs->max_ctx + kKeyChunk - 1) / kKeyChunk;
-    if (rows <= 4)
-      scores_rows_kernel<4><<<dim3(x, (rows + 3) / 4, z), kThreads, 4 * seqs->head_dim * 16, st>>>(*seqs, o);
+    const int rt = rows <= 4 ? 4 : 8;
+    // rows of 8 x 256 words and 256 keys would pass 48 KB of shared memory
+    const int chunk = keys_per_cta(ctx, *seqs, rows, 64, rt * seqs->head_dim > 1024 ? kKeyChunk / 2 : kKeyChunk, 8);
+    const size_t smem = sizeof(uint64_t) * (2 * rt * seqs->head_dim + rt * (chunk + 1) + chunk);
+    const dim3 grid((seqs->max_ctx + chunk - 1) / chunk, (rows + rt - 1) / rt, z);
+    if (rt == 4)
+      scores_rows_kernel<4><<<grid, kThreads, smem, st>>>(*seqs, o, chunk);
     else
-      scores_rows_kernel<8><<<dim3(x, (rows + 7) / 8, z), kThreads, 8 * seqs->head_dim * 16, st>>>(*seqs, o);
+      scores_rows_kernel<8><<<grid, kThreads, smem, st>>>(*seqs, o, chunk);
   } else if (scores_tc_fits(*seqs)) {
     const cudaError_t e = launch_scores_tc(ctx, *seqs, o, st);
     if (e != cudaSuccess) return fail(SUFB200_ERR_CUDA, std::string("attn_scores_pair: ") + cudaGetErrorString(e));
@@ -389,7 +407,7 @@ int sufb200_attn_values_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
     values_init_kernel<<<static_cast<unsigned>(want < cap ? want : cap), kThreads, 0, st>>>(*seqs, o);
   }
   if (any && few) {
-    const int range = 256;
+    const int range = keys_per_cta(ctx, *seqs, rows, kValStage, 1024, 3);
     const unsigned x = (seqs->max_ctx + range - 1) / range;
     if (rows <= 4)
       values_rows_kernel<4><<<dim3(x, (rows + 3) / 4, z), kThreads, 0, st>>>(*seqs, o, range);

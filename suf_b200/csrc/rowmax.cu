@@ -72,9 +72,20 @@ __global__ void __launch_bounds__(kThreads)
     const int at = off[r], w = off[r + 1] - at;
     if (w <= 0) continue;
     const uint64_t a = m0[moff[r]], b = m1[moff[r]];
-    for (int j = blockIdx.y * tpr + lane; j < w; j += gridDim.y * tpr) {
-      t0[at + j] = a - s0[at + j];
-      t1[at + j] = b - s1[at + j];
+    const int step = gridDim.y * tpr;
+    for (int j = blockIdx.y * tpr + lane; j < w; j += 4 * step) {  // four words' loads before their first use
+      uint64_t v0[4], v1[4];
+#pragma unroll
+      for (int x = 0; x < 4; x++) {
+        v0[x] = ld_if(s0 + at + j + x * step, j + x * step < w);
+        v1[x] = ld_if(s1 + at + j + x * step, j + x * step < w);
+      }
+#pragma unroll
+      for (int x = 0; x < 4; x++)
+        if (j + x * step < w) {
+          t0[at + j + x * step] = a - v0[x];
+          t1[at + j + x * step] = b - v1[x];
+        }
     }
   }
 }
