@@ -127,10 +127,12 @@ __global__ void values_init_kernel(const __grid_constant__ AttnSeqs s, const __g
 // on their order.
 constexpr int kValStage = 64;
 
-template <int RT>
+// SOLO: one CTA has every key of its rows and stores whole results.
+template <int RT, bool SOLO>
 __global__ void __launch_bounds__(kThreads) values_rows_kernel(const __grid_constant__ AttnSeqs s,
                                                                const __grid_constant__ AttnOperands o, int range) {
   __shared__ __align__(16) uint64_t sU[kValStage][RT], sD[kValStage][RT];
+  __shared__ ulonglong2 s_sum[SOLO ? kThreads : 1];
   __shared__ int64_t s_key[kValStage];
   const int t = threadIdx.x, dh = s.head_dim, group = s.q_heads / s.kv_heads, P = dh / 2;
   const int b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads;
@@ -141,7 +143,7 @@ __global__ void __launch_bounds__(kThreads) values_rows_kernel(const __grid_cons
   const int last = (rho0 + RT < R ? rho0 + RT : R) - 1;
   const int len = row_len(q.n, q.L, s.causal, last / group);
   const int beg = blockIdx.x * range, end = beg + range < len ? beg + range : len;
-  if (beg >= end) return;
+  if (!SOLO && beg >= end) return;
   const int lanes = kThreads / P, kl = t / P, c = t % P;
   uint64_t ax[RT] = {}, ay[RT] = {};
   for (int j0 = beg; j0 < end; j0 += kValStage) {
@@ -175,24 +177,36 @@ __global__ void __launch_bounds__(kThreads) values_rows_kernel(const __grid_cons
         }
       }
   }
-  if (kl >= lanes) return;
 #pragma unroll
   for (int rr = 0; rr < RT; rr++) {
     const int rho = rho0 + rr;
     if (rho >= R) break;
-    unsigned long long* at = reinterpret_cast<unsigned long long*>(
-        o.out + (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + 2 * c);
-    atomicAdd(at, static_cast<unsigned long long>(ax[rr]));
-    atomicAdd(at + 1, static_cast<unsigned long long>(ay[rr]));
+    const int64_t at = (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + 2 * c;
+    if (SOLO) {
+      __syncthreads();
+      s_sum[t] = make_ulonglong2(ax[rr], ay[rr]);
+      __syncthreads();
+      if (kl > 0) continue;
+      uint64_t x = o.c[0][at] + o.c[1][at] + o.r, y = o.c[0][at + 1] + o.c[1][at + 1] + o.r;
+      for (int l = 0; l < lanes; l++) {
+        x += s_sum[l * P + c].x;
+        y += s_sum[l * P + c].y;
+      }
+      o.out[at] = x;
+      o.out[at + 1] = y;
+    } else if (kl < lanes) {
+      unsigned long long* to = reinterpret_cast<unsigned long long*>(o.out + at);
+      atomicAdd(to, static_cast<unsigned long long>(ax[rr]));
+      atomicAdd(to + 1, static_cast<unsigned long long>(ay[rr]));
+    }
   }
 }
 
-// ---- many rows: 64 x 64 output tiles on the integer pipes -------------------
+// ---- scores, many rows of wide heads: 64 x 64 tiles on the integer pipes ----
 constexpr int kT = 64, kTK = 16;
 
-template <bool SCORES>
-__global__ void __launch_bounds__(kThreads) attn_tile_kernel(const __grid_constant__ AttnSeqs s,
-                                                             const __grid_constant__ AttnOperands o) {
+__global__ void __launch_bounds__(kThreads) scores_tile_kernel(const __grid_constant__ AttnSeqs s,
+                                                               const __grid_constant__ AttnOperands o) {
   __shared__ uint64_t sU[kTK][kT + 1], sD[kTK][kT + 1], sE[kTK][kT + 1], sW[kTK][kT + 1];
   __shared__ int64_t s_key[kT];
   const int t = threadIdx.x, dh = s.head_dim, group = s.q_heads / s.kv_heads;
@@ -203,51 +217,29 @@ __global__ void __launch_bounds__(kThreads) attn_tile_kernel(const __grid_consta
   if (rho0 >= R) return;
   const int last = (rho0 + kT < R ? rho0 + kT : R) - 1;
   const int len = row_len(q.n, q.L, s.causal, last / group);
-  const int cols = SCORES ? len : dh, depth = SCORES ? dh : len;
-  if (n0 >= cols || depth == 0) return;
-  if (SCORES) {
-    for (int e = t; e < kT; e += kThreads) s_key[e] = n0 + e < len ? key_off(s, b, kh, n0 + e, o.status) : -1;
-    __syncthreads();
-  }
+  if (n0 >= len) return;
+  for (int e = t; e < kT; e += kThreads) s_key[e] = n0 + e < len ? key_off(s, b, kh, n0 + e, o.status) : -1;
+  __syncthreads();
   const int tx = t % 16, ty = t / 16;
   uint64_t acc[4][4] = {};
-  for (int k0 = 0; k0 < depth; k0 += kTK) {
-    if (!SCORES) {
-      if (t < kTK) s_key[t] = k0 + t < len ? key_off(s, b, kh, k0 + t, o.status) : -1;
-      __syncthreads();
-    }
+  for (int k0 = 0; k0 < dh; k0 += kTK) {
     for (int e = t; e < kT * kTK; e += kThreads) {
-      const int rr = e / kTK, kk = e % kTK, rho = rho0 + rr, i = rho / group, k = k0 + kk;
-      uint64_t d = 0, u = 0;
-      if (rho < R) {
-        const int head = kh * group + rho % group;
-        if (SCORES) {
-          if (k < dh) {
-            const int64_t at = (static_cast<int64_t>(q.t0 + i) * s.q_heads + head) * dh + k;
-            d = o.x[0][at];
-            u = d + o.a[0][at] + o.a[1][at];
-          }
-        } else if (k < row_len(q.n, q.L, s.causal, i)) {
-          const int64_t at = q.base + head * q.blk + row_off(q.n, q.L, s.causal, i) + k;
-          const uint64_t a0 = o.a[0][at], a1 = o.a[1][at];
-          d = (o.x[0][at] - a0) + (o.x[1][at] - a1);
-          u = d + a0 + a1;
-        }
+      const int rr = e / kTK, kk = e % kTK, rho = rho0 + rr, k = k0 + kk;
+      uint64_t d = 0, u = 0, ev = 0, wv = 0;
+      if (rho < R && k < dh) {
+        const int64_t at = (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + k;
+        d = o.x[0][at];
+        u = d + o.a[0][at] + o.a[1][at];
+      }
+      if (s_key[rr] >= 0 && k < dh) {
+        const int64_t at = s_key[rr] + k;
+        ev = o.e[at];
+        wv = o.b[0][at] + o.b[1][at];
       }
       sU[kk][rr] = u;
       sD[kk][rr] = d;
-    }
-    for (int e = t; e < kT * kTK; e += kThreads) {
-      const int kk = SCORES ? e % kTK : e / kT, cc = SCORES ? e / kTK : e % kT;
-      const int64_t at = SCORES ? s_key[cc] : s_key[kk];
-      const int w = SCORES ? k0 + kk : n0 + cc;
-      uint64_t ev = 0, wv = 0;
-      if (at >= 0 && w < dh) {
-        ev = o.e[at + w];
-        wv = o.b[0][at + w] + o.b[1][at + w];
-      }
-      sE[kk][cc] = ev;
-      sW[kk][cc] = wv;
+      sE[kk][rr] = ev;
+      sW[kk][rr] = wv;
     }
     __syncthreads();
 #pragma unroll 4
@@ -269,18 +261,14 @@ __global__ void __launch_bounds__(kThreads) attn_tile_kernel(const __grid_consta
   }
 #pragma unroll
   for (int y = 0; y < 4; y++) {
-    const int rho = rho0 + ty * 4 + y, i = rho / group, head = kh * group + rho % group;
+    const int rho = rho0 + ty * 4 + y, i = rho / group;
     if (rho >= R) continue;
 #pragma unroll
     for (int x = 0; x < 4; x++) {
-      const int col = n0 + tx + 16 * x;
-      if (SCORES) {
-        if (col >= row_len(q.n, q.L, s.causal, i)) continue;
-        const int64_t at = q.base + head * q.blk + row_off(q.n, q.L, s.causal, i) + col;
-        o.out[at] = acc[y][x] + o.c[0][at] + o.c[1][at] + o.r;
-      } else if (col < dh) {
-        o.out[(static_cast<int64_t>(q.t0 + i) * s.q_heads + head) * dh + col] += acc[y][x];
-      }
+      const int key = n0 + tx + 16 * x;
+      if (key >= row_len(q.n, q.L, s.causal, i)) continue;
+      const int64_t at = q.base + (kh * group + rho % group) * q.blk + row_off(q.n, q.L, s.causal, i) + key;
+      o.out[at] = acc[y][x] + o.c[0][at] + o.c[1][at] + o.r;
     }
   }
 }
@@ -318,8 +306,15 @@ int check_operands(const AttnOperands& o, const char* who) {
   return SUFB200_OK;
 }
 
-// Rows of a (sequence, key head) up to which the row kernels are used.
-constexpr int kFewRows = 16;
+// Rows of a (sequence, key head) up to which the row kernels are used; above,
+// the tensor cores (whose pre-pass reads the cache once and writes its planes).
+// Four sequences of 8,192 tokens, 32 / 8 heads of 128, row kernels against
+// tensor cores: scores of 8 rows 238 and 407 us, 16 rows 455 and 419 us; values
+// of 8 rows 291 and 346 us, 16 rows 568 and 354 us.
+constexpr int kFewRows = 8;
+// Longest context whose values one CTA per (row tile, key head) takes whole,
+// in one launch instead of an init pass and adds.
+constexpr int kSoloKeys = 256;
 
 // Keys a CTA of the row kernels walks: the longest run (least, doubled up to
 // most) that still leaves `per_sm` CTAs per SM.  A long run pays its set-up
@@ -327,8 +322,8 @@ constexpr int kFewRows = 16;
 // 8 x 128 words: scores 332 us in runs of 256 (eight CTAs per SM asked for),
 // 348 us in runs of 128; values 315 us in runs of 1,024 (three asked for),
 // 322 of 512, 331 of 256.
-int keys_per_cta(const sufb200_ctx_s* ctx, const AttnSeqs& s, int rows, int least, int most, int per_sm) {
-  const int64_t keys = s.cached * s.kv_heads * ((rows + 7) / 8), ctas = static_cast<int64_t>(ctx->sm_count) * per_sm;
+int keys_per_cta(const sufb200_ctx_s* ctx, const AttnSeqs& s, int least, int most, int per_sm) {
+  const int64_t keys = s.cached * s.kv_heads, ctas = static_cast<int64_t>(ctx->sm_count) * per_sm;
   int run = least;
   while (run < most && keys / (2 * run) >= ctas) run *= 2;
   return run;
@@ -366,7 +361,7 @@ int sufb200_attn_scores_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
   if (rows <= kFewRows) {
     const int rt = rows <= 4 ? 4 : 8;
     // rows of 8 x 256 words and 256 keys would pass 48 KB of shared memory
-    const int chunk = keys_per_cta(ctx, *seqs, rows, 64, rt * seqs->head_dim > 1024 ? kKeyChunk / 2 : kKeyChunk, 8);
+    const int chunk = keys_per_cta(ctx, *seqs, 64, rt * seqs->head_dim > 1024 ? kKeyChunk / 2 : kKeyChunk, 8);
     const size_t smem = sizeof(uint64_t) * (2 * rt * seqs->head_dim + rt * (chunk + 1) + chunk);
     const dim3 grid((seqs->max_ctx + chunk - 1) / chunk, (rows + rt - 1) / rt, z);
     if (rt == 4)
@@ -377,7 +372,9 @@ int sufb200_attn_scores_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
     const cudaError_t e = launch_scores_tc(ctx, *seqs, o, st);
     if (e != cudaSuccess) return fail(SUFB200_ERR_CUDA, std::string("attn_scores_pair: ") + cudaGetErrorString(e));
   } else {
-    attn_tile_kernel<true><<<dim3((seqs->max_ctx + kT - 1) / kT, (rows + kT - 1) / kT, z), kThreads, 0, st>>>(*seqs, o);
+    // row planes of head sizes above 128 do not fit beside the stages (16 / 4
+    // heads of 128, 2,048 tokens: 3,402 us here against 368 us)
+    scores_tile_kernel<<<dim3((seqs->max_ctx + kT - 1) / kT, (rows + kT - 1) / kT, z), kThreads, 0, st>>>(*seqs, o);
   }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SUFB200_OK : fail(SUFB200_ERR_CUDA, std::string("attn_scores_pair: ") + cudaGetErrorString(e));
@@ -401,18 +398,18 @@ int sufb200_attn_values_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
   const int rows = seqs->q_heads / seqs->kv_heads * seqs->max_q;
   const unsigned z = static_cast<unsigned>(seqs->batch) * seqs->kv_heads;
   const bool any = seqs->packed > 0 && seqs->max_ctx > 0, few = rows <= kFewRows;
-  if (!any || few || !values_tc_solo(ctx, *seqs)) {
+  const bool solo = any && (few ? seqs->max_ctx <= kSoloKeys : values_tc_solo(ctx, *seqs));
+  if (!solo) {
     const int64_t words = seqs->tokens * seqs->q_heads * seqs->head_dim;
     const int64_t want = (words + kThreads - 1) / kThreads, cap = static_cast<int64_t>(ctx->sm_count) * 8;
     values_init_kernel<<<static_cast<unsigned>(want < cap ? want : cap), kThreads, 0, st>>>(*seqs, o);
   }
   if (any && few) {
-    const int range = keys_per_cta(ctx, *seqs, rows, kValStage, 1024, 3);
-    const unsigned x = (seqs->max_ctx + range - 1) / range;
-    if (rows <= 4)
-      values_rows_kernel<4><<<dim3(x, (rows + 3) / 4, z), kThreads, 0, st>>>(*seqs, o, range);
-    else
-      values_rows_kernel<8><<<dim3(x, (rows + 7) / 8, z), kThreads, 0, st>>>(*seqs, o, range);
+    const int range = solo ? kSoloKeys : keys_per_cta(ctx, *seqs, kValStage, 1024, 3), rt = rows <= 4 ? 4 : 8;
+    const dim3 grid((seqs->max_ctx + range - 1) / range, (rows + rt - 1) / rt, z);
+    const auto kernel = rt == 4 ? (solo ? values_rows_kernel<4, true> : values_rows_kernel<4, false>)
+                                : (solo ? values_rows_kernel<8, true> : values_rows_kernel<8, false>);
+    kernel<<<grid, kThreads, 0, st>>>(*seqs, o, range);
   } else if (any) {
     const cudaError_t e = launch_values_tc(ctx, *seqs, o, st);
     if (e != cudaSuccess) return fail(SUFB200_ERR_CUDA, std::string("attn_values_pair: ") + cudaGetErrorString(e));

@@ -56,27 +56,20 @@ __global__ void carry_table_kernel(const __grid_constant__ sufb200_rope_append a
     table[x] = carry_both(a, x);
 }
 
-// Where the carries come from.
-enum { kCarryBundle, kCarryGlobal, kCarryShared };
-
 // A warp per (token, head): its lanes hold the head's pairs, two neighbouring
 // pairs a lane with 16-byte accesses when VEC (every row 16-byte aligned and
 // the pairs' halves at even words), one pair with 8-byte accesses otherwise.
-template <int CARRY, bool VEC>
+// PACKED: the carries come from carry_table_kernel's table (32 KB at 12 bits:
+// L1 holds it), else from the bundle's own tables.
+template <bool PACKED, bool VEC>
 __global__ void __launch_bounds__(kThreads) rope_append_kernel(const __grid_constant__ sufb200_rope_append a,
                                                                const GapArs g, const uint64_t* __restrict__ table,
                                                                uint32_t* status) {
-  extern __shared__ __align__(16) uint64_t s_carry[];
-  if (CARRY != kCarryBundle) pdl_wait();
-  if (CARRY == kCarryShared) {
-    for (int i = threadIdx.x; i < 1 << (g.f - 1); i += kThreads)
-      reinterpret_cast<ulonglong2*>(s_carry)[i] = reinterpret_cast<const ulonglong2*>(table)[i];
-    __syncthreads();
-  }
+  if (PACKED) pdl_wait();
   const auto open = [&](uint64_t y0, uint64_t y1) {  // sum_p of the truncated shares of y
     const uint64_t yhat = y0 + y1 + g.r, h = yhat + (1ull << 62);
     const uint32_t x = static_cast<uint32_t>(yhat) & ((1u << g.f) - 1);
-    const uint64_t carry = CARRY == kCarryShared ? s_carry[x] : (CARRY == kCarryGlobal ? __ldg(table + x) : carry_both(a, x));
+    const uint64_t carry = PACKED ? __ldg(table + x) : carry_both(a, x);
     return g.base + (h >> g.f) - carry + ((h >> 63) == 0 ? g.m : 0);
   };
   const int half = a.rot_dim / 2, heads = a.q_heads + 2 * a.kv_heads, lane = threadIdx.x & 31;
@@ -224,31 +217,22 @@ bool paired(const sufb200_rope_append& a) {
 }
 
 // Fewest turned words for which the carries are packed into a table first: a
-// launch of its own, and 8 bytes of table per element read instead of four
-// 32-byte entries.
-constexpr int64_t kPackWords = 1 << 17;
-constexpr int kSharedCarryBits = 13;  // widest table held in shared memory (64 KB)
+// launch of its own, then 8 bytes of a 32 KB table per word instead of four
+// 32-byte entries of 512 KB.  40 turned heads of 128 words: 64 tokens 20 us
+// unpacked, 29 us packed; 128 tokens 29 and 28 us; 4,133 tokens 321 and 165 us.
+// (The packed table in shared memory took the same 165 us.)
+constexpr int64_t kPackWords = 1 << 19;
 
-template <int CARRY>
+template <bool PACKED>
 cudaError_t launch_rope(const sufb200_ctx_s* ctx, const sufb200_rope_append& a, const GapArs& g, const uint64_t* table,
                         cudaStream_t st) {
   const int64_t rows = static_cast<int64_t>(a.tokens) * (a.q_heads + 2 * a.kv_heads);
-  const size_t smem = CARRY == kCarryShared ? sizeof(uint64_t) << g.f : 0;
-  const auto kernel = paired(a) ? rope_append_kernel<CARRY, true> : rope_append_kernel<CARRY, false>;
-  int per_sm = 8;
-  if (CARRY == kCarryShared) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
-    per_sm = static_cast<int>((224u << 10) / (smem + 1024));
-    per_sm = per_sm > 8 ? 8 : per_sm;
-  }
-  const int64_t want = (rows + kThreads / 32 - 1) / (kThreads / 32), cap = static_cast<int64_t>(ctx->sm_count) * per_sm;
-  const dim3 grid(static_cast<unsigned>(CARRY == kCarryShared && want > cap ? cap : (want > 1 << 20 ? 1 << 20 : want)));
-  if (CARRY == kCarryBundle) {
-    kernel<<<grid, kThreads, smem, st>>>(a, g, table, ctx->d_status);
-    return cudaGetLastError();
-  }
-  return launch_pdl(kernel, grid, dim3(kThreads), smem, st, a, g, table, ctx->d_status);
+  const auto kernel = paired(a) ? rope_append_kernel<PACKED, true> : rope_append_kernel<PACKED, false>;
+  const int64_t want = (rows + kThreads / 32 - 1) / (kThreads / 32);
+  const dim3 grid(static_cast<unsigned>(want > 1 << 20 ? 1 << 20 : want));
+  if (PACKED) return launch_pdl(kernel, grid, dim3(kThreads), 0, st, a, g, table, ctx->d_status);
+  kernel<<<grid, kThreads, 0, st>>>(a, g, table, ctx->d_status);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -276,16 +260,14 @@ extern "C" int sufb200_rope_append_pair(sufb200_ctx ctx, const sufb200_rope_appe
   const int64_t turned = static_cast<int64_t>(args->tokens) * (args->q_heads + args->kv_heads) * args->rot_dim;
   cudaError_t e;
   if (turned < kPackWords) {
-    e = launch_rope<kCarryBundle>(ctx, *args, g, nullptr, st);
+    e = launch_rope<false>(ctx, *args, g, nullptr, st);
   } else {
     uint64_t* table = nullptr;
     e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&table), sizeof(uint64_t) << g.f, ctx->pool, st);
     if (e == cudaSuccess) {
       carry_table_kernel<<<((1 << g.f) + 127) / 128, 128, 0, st>>>(*args, table);
       e = cudaGetLastError();
-      if (e == cudaSuccess)
-        e = g.f <= kSharedCarryBits ? launch_rope<kCarryShared>(ctx, *args, g, table, st)
-                                    : launch_rope<kCarryGlobal>(ctx, *args, g, table, st);
+      if (e == cudaSuccess) e = launch_rope<true>(ctx, *args, g, table, st);
       const cudaError_t f = cudaFreeAsync(table, st);
       if (e == cudaSuccess) e = f;
     }
