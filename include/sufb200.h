@@ -771,7 +771,9 @@ int sufb200_rope_append_pair(sufb200_ctx ctx, const sufb200_rope_append* args, v
  *   len = causal ? max(0, ctx - n + i + 1) : ctx
  * words, and sequence b's rows start at word d_row_base[b].  max_q and max_ctx
  * bound the lengths; tokens, cached and packed the sums of the new tokens, the
- * cached tokens and the words (workspaces are sized by them). */
+ * cached tokens and the words (workspaces are sized by them).  At most 2^26
+ * cached tokens in a sequence, 65,535 (sequence, key head) pairs and 2^20 rows
+ * (queries of its heads) per pair. */
 typedef struct sufb200_attn_seqs {
   const int32_t* d_cu_q;        /* [batch + 1] */
   const int32_t* d_cu_ctx;      /* [batch + 1] */

@@ -211,11 +211,18 @@ class ShareCache:
         shape = tuple(ek.shape)
         args.d_ev = _want(ctx, "ev", ev, shape)
         args.d_bk, args.d_bv = _pair(ctx, "bk", bk, shape), _pair(ctx, "bv", bv, shape)
-        self.ek, self.ev, self.bk, self.bv, self.device = ek, ev, tuple(bk), tuple(bv), ctx.device
+        self._pools, self.device = (ek, tuple(bk), ev, tuple(bv)), ctx.device
         self.pages, self.kv_heads, self.page_size, self.head_dim = shape
         if min(shape) < 1 or self.head_dim % 2 or self.head_dim > 256:
             raise ValueError("cache: empty, or a head size that is not even, 2..256")
         args.pages, args.kv_heads, args.page_size, args.head_dim = shape
+
+
+    # the pools are fixed: appends keep their addresses
+    ek = property(lambda self: self._pools[0])
+    bk = property(lambda self: self._pools[1])
+    ev = property(lambda self: self._pools[2])
+    bv = property(lambda self: self._pools[3])
 
 
 def _strided(ctx: Context, name: str, ts, shape: tuple):

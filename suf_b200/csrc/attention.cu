@@ -287,6 +287,7 @@ int check_seqs(const sufb200_attn_seqs* s, const char* who) {
     return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 65535 (sequence, key head) pairs");
   if (static_cast<int64_t>(s->q_heads / s->kv_heads) * s->max_q > 1 << 20)
     return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^20 rows per (sequence, key head)");
+  if (s->max_ctx > 1 << 26) return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^26 cached tokens in a sequence");
   if (static_cast<int64_t>(s->max_ctx) > static_cast<int64_t>(s->max_pages) * s->page_size)
     return fail(SUFB200_ERR_INVALID, at + "max_ctx is more than the block table's pages hold");
   if (static_cast<__int128>(s->q_heads) * s->max_q * s->max_ctx >= (static_cast<__int128>(1) << 60))

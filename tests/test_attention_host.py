@@ -137,6 +137,7 @@ def test_attention_refusals(host, which):
                       (dict(tokens=-1), _lib.ERR_INVALID), (dict(cached=-1), _lib.ERR_INVALID), (dict(d_cu_ctx=None), _lib.ERR_INVALID),
                       (dict(d_block_table=None), _lib.ERR_INVALID), (dict(batch=40000), _lib.ERR_UNSUPPORTED),
                       (dict(max_q=2**20), _lib.ERR_UNSUPPORTED),
+                      (dict(max_ctx=2**26 + 1, max_pages=2**26), _lib.ERR_UNSUPPORTED),
                       (dict(q_heads=2**20, kv_heads=2**16 - 1 + 1, batch=1), _lib.ERR_UNSUPPORTED)]:
         assert _attn(host, which, _seqs(**{**PTRS, **bad})) == code, bad
         assert b"head" in _lib.lib().sufb200_last_error() or b"attn_" in _lib.lib().sufb200_last_error()

@@ -165,6 +165,10 @@ ATTN = [  # (new tokens, context) per sequence, q heads, kv heads, dim, page, ca
     ([(33, 260)], 2, 1, 256, 64, False),
     ([(1, 5000), (1, 4097)], 4, 4, 80, 64, True),                 # long rows, split
     ([(40, 2100)], 4, 2, 32, 64, True),
+    ([(20, 4500), (1, 4097)], 2, 1, 64, 64, True),                # tiles over more keys than one exact accumulation
+    ([(9, 130), (10, 9)], 3, 3, 34, 16, True),                    # just past the row kernels, empty rows
+    ([(1, 256), (1, 255)], 4, 1, 128, 64, True),                  # one CTA's whole context
+    ([(1, 257)], 8, 1, 62, 64, True),
 ]
 
 
@@ -442,3 +446,135 @@ def test_block_prompt_then_single_tokens_matches_model(ctx, torch_cuda):
             want = _model(turned[:, :hq], have[b], vals[b], lambda i: L - n + i + 1, hq // hkv, f, 3, relu, sm)
             assert (got[t0:t0 + n] == want).all(), (step, b)
             t0 += n
+
+
+def test_block_runs_on_a_side_stream_and_in_a_graph(ctx, torch_cuda):
+    """A decode step captured once and replayed on new shares gives the words
+    of the eager call on the same material."""
+    from suf_b200.attention import AttnLayout, CachedAttentionPair, ShareCache, rope_tables
+
+    torch = torch_cuda
+    rng = np.random.default_rng(4)
+    hq, hkv, dim, page = 4, 2, 64, 8
+    cache = ShareCache(ctx, 8, hkv, dim, page, seed=5)
+    layout = AttnLayout(ctx, [3, 1], [19, 30], [[0, 2, 4], [1, 3, 5, 7]], page, hq, hkv)
+    blk = CachedAttentionPair(ctx, cache, layout, seed=6, rope=rope_tables(ctx, 64, dim, 12), interleaved=True)
+    pos = torch.tensor([16, 17, 18, 29], dtype=torch.int32, device="cuda")
+    slots = torch.tensor([4 * 8 + 0, 4 * 8 + 1, 4 * 8 + 2, 7 * 8 + 5], dtype=torch.int64, device="cuda")
+    cache.ek.copy_(-cache.bk[0] - cache.bk[1] + 4096)  # cached keys and values of one
+    cache.ev.copy_(-cache.bv[0] - cache.bv[1] + 4096)
+
+    def shares():
+        x = np.rint(rng.normal(0.0, 1.0, (4, hq + 2 * hkv, dim)) * 4096).astype(np.int64)
+        s0 = _words(rng, *x.shape)
+        return [_dev(torch, s0), _dev(torch, x.view(U) - s0)]
+
+    buf = shares()
+    q, k, v = (tuple(b[:, i:j] for b in buf) for i, j in ((0, hq), (hq, hq + hkv), (hq + hkv, hq + 2 * hkv)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    blk.run(q, k, v, pos, slots, stream=side)  # warm-up outside the capture
+    ctx.sync(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side, capture_error_mode="relaxed"):
+        o = blk.run(q, k, v, pos, slots, stream=side)
+    for _ in range(2):
+        for b, n in zip(buf, shares()):
+            b.copy_(n)
+        g.replay()
+        torch.cuda.synchronize()
+        ctx.sync()
+        e = blk.run(q, k, v, pos, slots)
+        ctx.sync()
+        assert all((from_dev(x) == from_dev(y)).all() for x, y in zip(o, e))
+
+
+def test_block_without_new_tokens(ctx, torch_cuda):
+    from suf_b200.attention import AttnLayout, CachedAttentionPair, ShareCache
+
+    cache = ShareCache(ctx, 4, 2, 64, 8, seed=1)
+    blk = CachedAttentionPair(ctx, cache, AttnLayout(ctx, [0, 0], [9, 0], [[0, 1], []], 8, 4, 2), seed=2)
+    none = tuple(torch_cuda.zeros((0, n, 64), dtype=torch_cuda.int64, device="cuda") for n in (4, 2, 2))
+    o = blk.run(*((x, x) for x in none), None, torch_cuda.zeros(0, dtype=torch_cuda.int64, device="cuda"))
+    ctx.sync()
+    assert o[0].shape == (0, 4, 64)
+
+
+def test_truncation_pair_with_and_without_queries(ctx, torch_cuda):
+    from suf_b200.attention import TruncPair
+
+    torch = torch_cuda
+    rng = np.random.default_rng(8)
+    x = rng.integers(-(2**61), 2**61, 5000, dtype=np.int64)
+    bare = next(s for s in range(200) if int(TruncPair(ctx, 1, seed=s).desc[0].nq) == 0)
+    for f, seed in ((12, 3), (16, 4), (1, bare)):
+        tr = TruncPair(ctx, f, seed=seed)
+        xh = _dev(torch, x.view(U) + U(tr.r[0]) + U(tr.r[1]))
+        y = torch.empty_like(xh), torch.empty_like(xh)
+        tr.eval_pair(ctx, xh, *y)
+        ctx.sync()
+        assert ((from_dev(y[0]) + from_dev(y[1])).view(np.int64) == x >> f).all()
+
+
+def test_products_are_exact_at_full_depth(ctx, torch_cuda):
+    """Every operand word all ones: the largest sums the int32 diagonals of the
+    tensor-core path can meet, over 4,096 keys (the exact depth) and 5,000."""
+    from suf_b200.attention import AttnLayout, attn_scores_pair, attn_values_pair
+
+    torch = torch_cuda
+    n, dh, page = 64, 128, 64
+    for L in (4096, 5000):
+        pages = -(-L // page)
+        lay = AttnLayout(ctx, [n], [L], [list(range(pages))], page, 1, 1, causal=False)
+        ones = torch.full((pages, 1, page, dh), -1, dtype=torch.int64, device="cuda")
+        zero = torch.zeros_like(ones)
+        pool = (ones, (ones, zero))  # E and W all ones
+        z_q, z_p = torch.zeros((n, 1, dh), dtype=torch.int64, device="cuda"), torch.zeros(n * L, dtype=torch.int64,
+                                                                                         device="cuda")
+        out = attn_values_pair(ctx, (z_p - 1, z_p), (z_p, z_p), (z_q, z_q), (0, 0), *pool, lay)
+        ctx.sync()
+        assert (from_dev(out) == U(2 * L)).all()  # (-1)(-1) twice per key
+        out = attn_scores_pair(ctx, z_q - 1, (z_q, z_q), (z_p, z_p), (0, 0), *pool, lay)
+        ctx.sync()
+        assert (from_dev(out) == U(2 * dh)).all()
+
+
+def test_pages_past_32_bit_offsets(ctx, torch_cuda):
+    """Pages whose words lie past 2^32 in the pool (one pool stands for the
+    opened words and both masks: it is only read)."""
+    from suf_b200.attention import AttnLayout, attn_scores_pair, attn_values_pair
+
+    torch = torch_cuda
+    hkv, dh, page = 8, 128, 64
+    words = hkv * dh * page
+    pages = 2**32 // words + 4
+    if torch.cuda.mem_get_info()[0] < 8 * words * pages + 2**31:
+        pytest.skip("needs 37 GB of free device memory")
+    pool = torch.empty((pages, hkv, page, dh), dtype=torch.int64, device="cuda")
+    rng = np.random.default_rng(1)
+    ids = [pages - 1, 3, pages - 3]
+    small = _words(rng, 3, hkv, page, dh)
+    for i, p in enumerate(ids):
+        pool[p] = _dev(torch, small[i])
+    for n in (1, 12):  # row kernels, tensor cores
+        L = 150
+        lay = AttnLayout(ctx, [n], [L], [ids], page, hkv, hkv)
+        lens = [L - n + i + 1 for i in range(n)]
+        k = small.transpose(1, 0, 2, 3).reshape(hkv, -1, dh)[:, :L]
+        d, c = _words(rng, n, hkv, dh), _words(rng, hkv * sum(lens))
+        z_q, z_p = np.zeros_like(d), np.zeros_like(c)
+        dz_q, dz_p = _dev(torch, z_q), _dev(torch, z_p)
+        got = attn_scores_pair(ctx, _dev(torch, d), (dz_q, dz_q), (_dev(torch, c), dz_p), (0, 0), pool, (pool, pool), lay)
+        ctx.sync()
+        want = np.concatenate([U(3) * (k[h, :lens[i]] @ d[i, h]) for h in range(hkv) for i in range(n)]) + c
+        assert (from_dev(got) == want).all()
+        got = attn_values_pair(ctx, (_dev(torch, c), dz_p), (dz_p, dz_p), (dz_q, dz_q), (0, 0), pool, (pool, pool), lay)
+        ctx.sync()
+        want, at = np.zeros_like(d), 0
+        for h in range(hkv):
+            for i in range(n):
+                want[i, h] = U(3) * (c[at:at + lens[i]] @ k[h, :lens[i]])
+                at += lens[i]
+        assert (from_dev(got) == want).all()
+    del pool
+    torch.cuda.empty_cache()
