@@ -256,26 +256,44 @@ __device__ __forceinline__ void fold16(int quarter, int col, uint64_t (&z)[16]) 
   }
 }
 
-// The twelve MMAs of one step (umma_i8.cuh's mma_step) on the A planes at
-// shared address a and the B planes at b.  One thread issues them, and its
-// instructions bound a step once the copies keep up (the twelve take about
-// 1,210 cycles of the tensor core): accumulators, shapes and the descriptors'
-// high words are constants, only two 32-bit bases vary.
+// The twelve MMAs of one step (umma_i8.cuh's products in another order) on the
+// A planes at shared address a and the B planes at b.  The tensor core's queue
+// is short: it runs dry whenever the issuing warp is held up for longer than
+// the last MMAs it was given take, and a wait for the next step's planes holds
+// it up by about 200 cycles even when they are there.  So a step is issued in
+// two parts, the small MMAs in the first and four of the widest last, and the
+// next step's wait stands between them (a step took 0.90 us with the wait in
+// front, 0.63 us of it MMAs).  For the same reason accumulators, shapes and the
+// descriptors' high words are constants; only two 32-bit bases vary.
 __device__ __forceinline__ uint64_t plane_desc(uint32_t base_lo, uint32_t planes_off) {
   return static_cast<uint64_t>(base_lo + (planes_off >> 4)) | (static_cast<uint64_t>((1u << 14) | (256u >> 4)) << 32);
 }
 __device__ __forceinline__ uint32_t desc_base(uint32_t saddr) { return (saddr >> 4) | ((128u >> 4) << 16); }
 
-__device__ __forceinline__ void issue(uint32_t a, uint32_t b, uint32_t accumulate) {
+// x_i times [y_j ...] for N = 256, fewer where the 512 columns end.
+__device__ __forceinline__ void issue_one(uint32_t al, uint32_t bl, int i, int j, uint32_t accumulate) {
+  const int n = 64 * (8 - i - j);
+  umma_i8((i + j) * kTN, plane_desc(al, i * kPlaneX), plane_desc(bl, j * kPlaneY), idesc_n(n < 256 ? n : 256), accumulate);
+}
+
+__device__ __forceinline__ void issue_first(uint32_t a, uint32_t b, uint32_t accumulate) {
   const uint32_t al = desc_base(a), bl = desc_base(b);
-  umma_i8(0, plane_desc(al, 0), plane_desc(bl, 0), idesc_n(256), accumulate);
-  umma_i8(4 * kTN, plane_desc(al, 0), plane_desc(bl, 4 * kPlaneY), idesc_n(256), accumulate);
-#pragma unroll
-  for (int i = 1; i < 8; i++)
-    umma_i8(i * kTN, plane_desc(al, i * kPlaneX), plane_desc(bl, 0), idesc_n(i <= 4 ? 256 : 64 * (8 - i)), 1u);
-#pragma unroll
-  for (int i = 1; i < 4; i++)
-    umma_i8((i + 4) * kTN, plane_desc(al, i * kPlaneX), plane_desc(bl, 4 * kPlaneY), idesc_n(256 - 64 * i), 1u);
+  issue_one(al, bl, 0, 0, accumulate);  // these two write all 512 columns
+  issue_one(al, bl, 0, 4, accumulate);
+  issue_one(al, bl, 7, 0, 1u);
+  issue_one(al, bl, 3, 4, 1u);
+  issue_one(al, bl, 6, 0, 1u);
+  issue_one(al, bl, 2, 4, 1u);
+  issue_one(al, bl, 5, 0, 1u);
+  issue_one(al, bl, 1, 4, 1u);
+}
+
+__device__ __forceinline__ void issue_last(uint32_t a, uint32_t b) {
+  const uint32_t al = desc_base(a), bl = desc_base(b);
+  issue_one(al, bl, 1, 0, 1u);
+  issue_one(al, bl, 2, 0, 1u);
+  issue_one(al, bl, 3, 0, 1u);
+  issue_one(al, bl, 4, 0, 1u);
 }
 
 __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_constant__ AttnTc a) {
@@ -323,17 +341,26 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
   } else if (warp == 1) {  // MMAs
     // The whole warp waits and steps, one elected lane issues: step, stage and
     // descriptors stay warp-uniform.
-    bool go = true;
-    for (int tl = 0; tl < tiles && go; tl++) {
-      // the rows' planes are written, the last tile is out of tensor memory
-      go = __all_sync(0xffffffffu, tl == 0 ? mbar_wait(c.bfull, 0) : mbar_wait(c.tempty, static_cast<uint32_t>((tl - 1) & 1)));
-      for (int st = 0; st < steps && go; st++) {
-        const int li = tl * steps + st, as = li % kAStages;
-        go = __all_sync(0xffffffffu, mbar_wait(c.afull + 8 * as, static_cast<uint32_t>((li / kAStages) & 1)));
+    const auto landed = [&](int li) {
+      const bool ok = mbar_wait(c.afull + 8 * (li % kAStages), static_cast<uint32_t>((li / kAStages) & 1));
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      return __all_sync(0xffffffffu, ok) != 0;
+    };
+    bool go = __all_sync(0xffffffffu, mbar_wait(c.bfull, 0)) && landed(0);  // the rows' planes, the first keys'
+    for (int tl = 0, li = 0; tl < tiles && go; tl++) {
+      if (tl > 0) {  // the last tile is out of tensor memory
+        go = __all_sync(0xffffffffu, mbar_wait(c.tempty, static_cast<uint32_t>((tl - 1) & 1)));
         if (!go) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      }
+      for (int st = 0; st < steps && go; st++, li++) {
+        const int as = li % kAStages;
+        const uint32_t at = sbase + static_cast<uint32_t>(as) * kAStage, bt = sbase + kBOff + static_cast<uint32_t>(st) * kBStage;
+        if (elect_one()) issue_first(at, bt, st > 0 ? 1u : 0u);
+        __syncwarp();
+        if (li + 1 < tiles * steps) go = landed(li + 1);
         if (elect_one()) {
-          issue(sbase + static_cast<uint32_t>(as) * kAStage, sbase + kBOff + static_cast<uint32_t>(st) * kBStage, st > 0 ? 1u : 0u);
+          issue_last(at, bt);
           umma_commit(c.aempty + 8 * as);
           if (st + 1 == steps) umma_commit(c.tfull);
         }
@@ -486,15 +513,21 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
       copies++;
     }
   } else if (warp == 1) {
-    bool go = true;
-    for (int li = 0; li < 2 * nch; li++) {
-      const int as = li % kAStages, bs = li % kBStages;
-      go = __all_sync(0xffffffffu, mbar_wait(c.afull + 8 * as, static_cast<uint32_t>((li / kAStages) & 1)) &&
-                                       mbar_wait(c.bfull + 8 * bs, static_cast<uint32_t>((li / kBStages) & 1)));
-      if (!go) break;
+    const auto landed = [&](int li) {
+      const bool ok = mbar_wait(c.afull + 8 * (li % kAStages), static_cast<uint32_t>((li / kAStages) & 1)) &&
+                      mbar_wait(c.bfull + 8 * (li % kBStages), static_cast<uint32_t>((li / kBStages) & 1));
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      return __all_sync(0xffffffffu, ok) != 0;
+    };
+    bool go = landed(0);
+    for (int li = 0; li < 2 * nch && go; li++) {
+      const int as = li % kAStages, bs = li % kBStages;
+      const uint32_t at = sbase + static_cast<uint32_t>(as) * kAStage, bt = sbase + kBOff + static_cast<uint32_t>(bs) * kBStage;
+      if (elect_one()) issue_first(at, bt, li > 0 ? 1u : 0u);
+      __syncwarp();
+      if (li + 1 < 2 * nch) go = landed(li + 1);
       if (elect_one()) {
-        issue(sbase + static_cast<uint32_t>(as) * kAStage, sbase + kBOff + static_cast<uint32_t>(bs) * kBStage, li > 0 ? 1u : 0u);
+        issue_last(at, bt);
         umma_commit(c.aempty + 8 * as);
         umma_commit(c.bempty + 8 * bs);
         if (li + 1 == 2 * nch) umma_commit(c.tfull);
