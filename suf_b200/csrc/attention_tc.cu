@@ -397,13 +397,40 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
   if (ready && warp >= 4) {  // epilogue: while the next tile's MMAs run
     // The MMAs take most of the shared-memory bandwidth and every multiply of
     // an address would stand in this warp's chain, so the rows' places are
-    // stepped from one row to the next (row_off, row_len by differences).
+    // stepped from one row to the next (row_off, row_len by differences).  C is
+    // fetched four rows ahead of the stores, the first four while the tile's
+    // MMAs still run; more in flight would spill.
     const int quarter = warp & 3, col = ((warp - 4) >> 2) * 16;
     const int i0 = (rho0 + col) / group, g0 = (rho0 + col) % group;  // the first row's query and head of the group
     const int rows = R - rho0 - col;                                 // rows there are, from there on
     const int64_t at0 = q.base + static_cast<int64_t>(kh * group) * q.blk + row_off(q.n, q.L, s.causal, i0);
     const int len0 = s.causal ? q.L - q.n + i0 + 1 : q.L;
     for (int tl = 0; tl < tiles; tl++) {
+      const int key = (tile0 + tl) * kTM + quarter * 32 + lane;
+      // this query's row of the group's first head, and this row: one walk for
+      // the loads of C, four rows ahead, one for the stores
+      int lg = g0, llen = len0, sg = g0, slen = len0;
+      int64_t lrow = at0 + key, lat = lrow + g0 * q.blk, srow = lrow, sat = lat;
+      const auto next = [&](int& g, int& len, int64_t& row, int64_t& at) {
+        at += q.blk;
+        if (++g == group) {
+          g = 0;
+          row += len > 0 ? len : 0;
+          at = row;
+          len += s.causal ? 1 : 0;
+        }
+      };
+      uint64_t c0[2][4], c1[2][4];
+      const auto fetch = [&](int x0) {
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          const bool in = x0 + x < rows && key < llen;
+          c0[(x0 >> 2) & 1][x] = ld_if(o.c[0] + lat, in);
+          c1[(x0 >> 2) & 1][x] = ld_if(o.c[1] + lat, in);
+          next(lg, llen, lrow, lat);
+        }
+      };
+      fetch(0);
       int go = 1;
       if (lane == 0) go = mbar_wait(c.tfull, static_cast<uint32_t>(tl & 1));
       if (!__shfl_sync(0xffffffffu, go, 0)) {
@@ -416,39 +443,13 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(c.tempty);
-      const int key = (tile0 + tl) * kTM + quarter * 32 + lane;
-      // this query's row of the group's first head, and this row
-      int g = g0, len = len0;
-      int64_t row = at0 + key, at = row + g0 * q.blk;
-      const auto next = [&] {
-        at += q.blk;
-        if (++g == group) {
-          g = 0;
-          row += len > 0 ? len : 0;
-          at = row;
-          len += s.causal ? 1 : 0;
-        }
-      };
 #pragma unroll
-      for (int x0 = 0; x0 < 16; x0 += 8) {
-        uint64_t c0[8], c1[8];
-        const int g1 = g, len1 = len;
-        const int64_t row1 = row, at1 = at;
+      for (int x0 = 0; x0 < 16; x0 += 4) {
+        if (x0 < 12) fetch(x0 + 4);
 #pragma unroll
-        for (int x = 0; x < 8; x++) {
-          const bool in = x0 + x < rows && key < len;
-          c0[x] = ld_if(o.c[0] + at, in);
-          c1[x] = ld_if(o.c[1] + at, in);
-          next();
-        }
-        g = g1;  // the same eight rows again: stepping costs less than keeping their places
-        len = len1;
-        row = row1;
-        at = at1;
-#pragma unroll
-        for (int x = 0; x < 8; x++) {
-          if (x0 + x < rows && key < len) o.out[at] = z[x0 + x] + c0[x] + c1[x] + o.r;
-          next();
+        for (int x = 0; x < 4; x++) {
+          if (x0 + x < rows && key < slen) o.out[sat] = z[x0 + x] + c0[(x0 >> 2) & 1][x] + c1[(x0 >> 2) & 1][x] + o.r;
+          next(sg, slen, srow, sat);
         }
       }
     }
@@ -595,30 +596,43 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
       const int quarter = warp & 3, col = ((warp - 4) >> 2) * 16;
       uint64_t z[16];
       fold16(quarter, col, z);
-      const int word = word0 + quarter * 32 + lane;
+      const int word = word0 + quarter * 32 + lane, left = R - rho0 - col;  // rows there are from column 0 on
+      int g = (rho0 + col) % group;
+      int64_t at = left > 0 ? place(rho0 + col, word) : 0;
+      const auto next = [&] {  // the row after: the group's next head, or the next token's first
+        at += dh;
+        if (++g == group) {
+          g = 0;
+          at += static_cast<int64_t>(s.q_heads - group) * dh;
+        }
+      };
       if (SOLO) {
 #pragma unroll
         for (int x0 = 0; x0 < 16; x0 += 8) {
           uint64_t c0[8], c1[8];
+          const int g1 = g;
+          const int64_t at1 = at;
 #pragma unroll
           for (int x = 0; x < 8; x++) {
-            const int rho = rho0 + col + x0 + x;
-            const bool in = rho < R && word < dh;
-            c0[x] = ld_if(o.c[0] + place(rho, word), in);
-            c1[x] = ld_if(o.c[1] + place(rho, word), in);
+            const bool in = x0 + x < left && word < dh;
+            c0[x] = ld_if(o.c[0] + at, in);
+            c1[x] = ld_if(o.c[1] + at, in);
+            next();
           }
+          g = g1;
+          at = at1;
 #pragma unroll
           for (int x = 0; x < 8; x++) {
-            const int rho = rho0 + col + x0 + x;
-            if (rho < R && word < dh) o.out[place(rho, word)] = z[x0 + x] + c0[x] + c1[x] + o.r;
+            if (x0 + x < left && word < dh) o.out[at] = z[x0 + x] + c0[x] + c1[x] + o.r;
+            next();
           }
         }
       } else {
 #pragma unroll
         for (int x = 0; x < 16; x++) {
-          const int rho = rho0 + col + x;
-          if (rho < R && word < dh)
-            atomicAdd(reinterpret_cast<unsigned long long*>(o.out + place(rho, word)), static_cast<unsigned long long>(z[x]));
+          if (x < left && word < dh)
+            atomicAdd(reinterpret_cast<unsigned long long*>(o.out + at), static_cast<unsigned long long>(z[x]));
+          next();
         }
       }
     } else if (lane == 0) {
