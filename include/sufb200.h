@@ -770,7 +770,8 @@ int sufb200_rope_append_pair(sufb200_ctx ctx, const sufb200_rope_append* args, v
  * order; row (b, h, i) has
  *   len = causal ? max(0, ctx - n + i + 1) : ctx
  * words, and sequence b's rows start at word d_row_base[b].  max_q and max_ctx
- * bound the lengths; tokens, cached and packed the sums of the new tokens, the
+ * bound the lengths, min_q the new tokens of the sequences that have any (from
+ * below: short and long ones are computed by different kernels); tokens, cached and packed the sums of the new tokens, the
  * cached tokens and the words (workspaces are sized by them).  At most 2^26
  * cached tokens in a sequence, 65,535 (sequence, key head) pairs and 2^20 rows
  * (queries of its heads) per pair. */
@@ -780,7 +781,7 @@ typedef struct sufb200_attn_seqs {
   const int64_t* d_row_base;    /* [batch] */
   const int32_t* d_block_table; /* [batch][max_pages] */
   int64_t tokens, cached, packed;
-  int32_t batch, max_pages, page_size, pages, q_heads, kv_heads, head_dim, causal, max_q, max_ctx;
+  int32_t batch, max_pages, page_size, pages, q_heads, kv_heads, head_dim, causal, min_q, max_q, max_ctx, reserved;
 } sufb200_attn_seqs;
 
 /* Scores: x^ = sum_p (C_p + D B_p + A_p E (+ D E for party 0) + r[p]) for every

@@ -75,7 +75,7 @@ class AttnSeqs(C.Structure):
         ("tokens", C.c_int64), ("cached", C.c_int64), ("packed", C.c_int64),
         ("batch", C.c_int32), ("max_pages", C.c_int32), ("page_size", C.c_int32), ("pages", C.c_int32),
         ("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("causal", C.c_int32),
-        ("max_q", C.c_int32), ("max_ctx", C.c_int32),
+        ("min_q", C.c_int32), ("max_q", C.c_int32), ("max_ctx", C.c_int32), ("reserved", C.c_int32),
     ]
 
 

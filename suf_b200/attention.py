@@ -335,7 +335,8 @@ class AttnLayout:
         s.tokens, s.cached, s.packed = self.tokens, int(L.sum()), self.packed
         s.batch, s.max_pages = self.batch, int(block_table.shape[1])
         s.page_size, s.q_heads, s.kv_heads, s.causal = self.page_size, self.q_heads, self.kv_heads, int(self.causal)
-        s.max_q, s.max_ctx = int(q.max(initial=0)), int(L.max(initial=0))
+        s.min_q, s.max_q, s.max_ctx = int(q[q > 0].min(initial=2**31 - 1)), int(q.max(initial=0)), int(L.max(initial=0))
+        s.min_q = min(s.min_q, s.max_q)
 
     def row_lengths(self) -> np.ndarray:
         """Keys of every row, in (sequence, head, query) order."""

@@ -27,11 +27,23 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Rows of a (sequence, key head) up to which the row kernels are used; above,
+// the tensor cores (whose pre-pass reads the cache once and writes its planes).
+// Four sequences of 8,192 tokens, 32 / 8 heads of 128, row kernels against
+// tensor cores: scores of 8 rows 238 and 407 us, 16 rows 455 and 419 us; values
+// of 8 rows 291 and 346 us, 16 rows 568 and 354 us.
+constexpr int kFewRows = 8;
+
 int fail(int code, const std::string& msg) { return record_error(code, msg); }
 
 // ---- few rows (single tokens): bound by the cache's three words per entry --
 // scores_rows: eight lanes per key, 16 bytes of the head each; the rows' U =
-// D + A_0 + A_1 and D sit in shared memory and are read once for two keys.
+// D + A_0 + A_1 and D sit in shared memory and are read once for two keys.  Up
+// to four rows the multiplies (two per word and row, three integer
+// instructions each) stay below the memory's time.  One decode step over
+// 73,279 cached tokens, 32 / 8 heads of 128: 341 us cold, 5.4 TB/s of 6.5; what
+// is left is waiting on memory with 32 warps an SM (long_scoreboard 11 per
+// issue, DRAM 83 %).
 constexpr int kKeyChunk = 256;  // most keys per CTA
 
 template <int RT>
@@ -44,7 +56,7 @@ __global__ void __launch_bounds__(kThreads, RT == 4 ? 4 : 3) scores_rows_kernel(
   SeqInfo q;
   if (!seq_info(s, b, o.status, q)) return;
   const int R = group * q.n, rho0 = blockIdx.y * RT, k0 = blockIdx.x * chunk;
-  if (rho0 >= R) return;
+  if (rho0 >= R || R > kFewRows) return;
   const int last = (rho0 + RT < R ? rho0 + RT : R) - 1;
   const int len = row_len(q.n, q.L, s.causal, last / group);  // the longest row of the tile
   if (k0 >= len) return;
@@ -124,7 +136,8 @@ __global__ void values_init_kernel(const __grid_constant__ AttnSeqs s, const __g
 // values_rows: a thread holds two words of the head for RT rows; the CTA's
 // key lanes walk its range of keys, whose probabilities sit in shared memory.
 // Ranges of one row meet by 64-bit atomic adds: sums mod 2^64 do not depend
-// on their order.
+// on their order.  The same decode step: 332 us cold, 5.7 TB/s.  (Two and four
+// keys a thread at a time, for more loads in flight: 387 us, for fewer warps.)
 constexpr int kValStage = 64;
 
 // SOLO: one CTA has every key of its rows and stores whole results.
@@ -139,7 +152,7 @@ __global__ void __launch_bounds__(kThreads) values_rows_kernel(const __grid_cons
   SeqInfo q;
   if (!seq_info(s, b, o.status, q)) return;
   const int R = group * q.n, rho0 = blockIdx.y * RT;
-  if (rho0 >= R) return;
+  if (rho0 >= R || R > kFewRows) return;
   const int last = (rho0 + RT < R ? rho0 + RT : R) - 1;
   const int len = row_len(q.n, q.L, s.causal, last / group);
   const int beg = blockIdx.x * range, end = beg + range < len ? beg + range : len;
@@ -214,7 +227,7 @@ __global__ void __launch_bounds__(kThreads) scores_tile_kernel(const __grid_cons
   SeqInfo q;
   if (!seq_info(s, b, o.status, q)) return;
   const int R = group * q.n, rho0 = blockIdx.y * kT, n0 = blockIdx.x * kT;
-  if (rho0 >= R) return;
+  if (rho0 >= R || R <= o.few) return;
   const int last = (rho0 + kT < R ? rho0 + kT : R) - 1;
   const int len = row_len(q.n, q.L, s.causal, last / group);
   if (n0 >= len) return;
@@ -273,10 +286,24 @@ __global__ void __launch_bounds__(kThreads) scores_tile_kernel(const __grid_cons
   }
 }
 
+// The most rows of a (sequence, key head), and the most the row kernels take
+// (0: every sequence has more): a batch of prompts and single tokens runs both
+// kinds of kernel, each on its own sequences.
+struct Rows {
+  int most, few;
+};
+
+Rows rows_of(const AttnSeqs& s) {
+  const int group = s.q_heads / s.kv_heads;
+  Rows r{group * s.max_q, 0};
+  if (group * s.min_q <= kFewRows) r.few = r.most <= kFewRows ? r.most : kFewRows;
+  return r;
+}
+
 int check_seqs(const sufb200_attn_seqs* s, const char* who) {
   const std::string at = std::string(who) + ": ";
   if (!s) return fail(SUFB200_ERR_INVALID, at + "null sequences");
-  if (s->batch < 0 || s->max_pages < 0 || s->pages < 0 || s->max_q < 0 || s->max_ctx < 0 || s->tokens < 0 || s->cached < 0 ||
+  if (s->batch < 0 || s->max_pages < 0 || s->pages < 0 || s->min_q < 0 || s->max_q < s->min_q || s->max_ctx < 0 || s->tokens < 0 || s->cached < 0 ||
       s->packed < 0)
     return fail(SUFB200_ERR_INVALID, at + "negative size");
   if (s->page_size < 1 || s->kv_heads < 1 || s->q_heads < s->kv_heads || s->q_heads % s->kv_heads)
@@ -307,12 +334,6 @@ int check_operands(const AttnOperands& o, const char* who) {
   return SUFB200_OK;
 }
 
-// Rows of a (sequence, key head) up to which the row kernels are used; above,
-// the tensor cores (whose pre-pass reads the cache once and writes its planes).
-// Four sequences of 8,192 tokens, 32 / 8 heads of 128, row kernels against
-// tensor cores: scores of 8 rows 238 and 407 us, 16 rows 455 and 419 us; values
-// of 8 rows 291 and 346 us, 16 rows 568 and 354 us.
-constexpr int kFewRows = 8;
 // Longest context whose values one CTA per (row tile, key head) takes whole,
 // in one launch instead of an init pass and adds.
 constexpr int kSoloKeys = 256;
@@ -351,31 +372,33 @@ int sufb200_attn_scores_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
   if (int rc = check_seqs(seqs, "attn_scores_pair")) return rc;
   if (seqs->batch == 0 || seqs->packed == 0 || seqs->max_q == 0 || seqs->max_ctx == 0) return SUFB200_OK;
   if (!d_a || !d_c || !r || !d_bk) return fail(SUFB200_ERR_INVALID, "attn_scores_pair: null pointer array");
-  AttnOperands o{{d_dq, d_dq}, {d_a[0], d_a[1]}, {d_c[0], d_c[1]}, d_ek, {d_bk[0], d_bk[1]}, r[0] + r[1], d_xhat,
+  AttnOperands o{{d_dq, d_dq}, {d_a[0], d_a[1]}, {d_c[0], d_c[1]}, d_ek, {d_bk[0], d_bk[1]}, r[0] + r[1], 0, d_xhat,
                  nullptr};
   if (int rc = check_operands(o, "attn_scores_pair")) return rc;
   if (int rc = attn_check_ctx(ctx)) return rc;
   o.status = ctx->d_status;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int rows = seqs->q_heads / seqs->kv_heads * seqs->max_q;
+  const Rows rows = rows_of(*seqs);
   const unsigned z = static_cast<unsigned>(seqs->batch) * seqs->kv_heads;
-  if (rows <= kFewRows) {
-    const int rt = rows <= 4 ? 4 : 8;
+  if (rows.few > 0) {
+    const int rt = rows.few <= 4 ? 4 : 8;
     // rows of 8 x 256 words and 256 keys would pass 48 KB of shared memory
     const int chunk = keys_per_cta(ctx, *seqs, 64, rt * seqs->head_dim > 1024 ? kKeyChunk / 2 : kKeyChunk, 8);
     const size_t smem = sizeof(uint64_t) * (2 * rt * seqs->head_dim + rt * (chunk + 1) + chunk);
-    const dim3 grid((seqs->max_ctx + chunk - 1) / chunk, (rows + rt - 1) / rt, z);
+    const dim3 grid((seqs->max_ctx + chunk - 1) / chunk, 1, z);
     if (rt == 4)
       scores_rows_kernel<4><<<grid, kThreads, smem, st>>>(*seqs, o, chunk);
     else
       scores_rows_kernel<8><<<grid, kThreads, smem, st>>>(*seqs, o, chunk);
-  } else if (scores_tc_fits(*seqs)) {
+  }
+  o.few = rows.few;
+  if (rows.most > kFewRows && scores_tc_fits(*seqs)) {
     const cudaError_t e = launch_scores_tc(ctx, *seqs, o, st);
     if (e != cudaSuccess) return fail(SUFB200_ERR_CUDA, std::string("attn_scores_pair: ") + cudaGetErrorString(e));
-  } else {
+  } else if (rows.most > kFewRows) {
     // row planes of head sizes above 128 do not fit beside the stages (16 / 4
     // heads of 128, 2,048 tokens: 3,402 us here against 368 us)
-    scores_tile_kernel<<<dim3((seqs->max_ctx + kT - 1) / kT, (rows + kT - 1) / kT, z), kThreads, 0, st>>>(*seqs, o);
+    scores_tile_kernel<<<dim3((seqs->max_ctx + kT - 1) / kT, (rows.most + kT - 1) / kT, z), kThreads, 0, st>>>(*seqs, o);
   }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SUFB200_OK : fail(SUFB200_ERR_CUDA, std::string("attn_scores_pair: ") + cudaGetErrorString(e));
@@ -387,7 +410,7 @@ int sufb200_attn_values_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
   if (int rc = check_seqs(seqs, "attn_values_pair")) return rc;
   if (seqs->batch == 0 || seqs->max_q == 0 || seqs->tokens == 0) return SUFB200_OK;
   if (!d_p || !d_a || !d_c || !r || !d_bv) return fail(SUFB200_ERR_INVALID, "attn_values_pair: null pointer array");
-  AttnOperands o{{d_p[0], d_p[1]}, {d_a[0], d_a[1]}, {d_c[0], d_c[1]}, d_ev, {d_bv[0], d_bv[1]}, r[0] + r[1], d_xhat,
+  AttnOperands o{{d_p[0], d_p[1]}, {d_a[0], d_a[1]}, {d_c[0], d_c[1]}, d_ev, {d_bv[0], d_bv[1]}, r[0] + r[1], 0, d_xhat,
                  nullptr};
   if (seqs->packed == 0) {  // every row is empty: no probability is read
     o.x[0] = o.x[1] = o.a[0] = o.a[1] = o.c[0];
@@ -396,22 +419,24 @@ int sufb200_attn_values_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
   if (int rc = attn_check_ctx(ctx)) return rc;
   o.status = ctx->d_status;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int rows = seqs->q_heads / seqs->kv_heads * seqs->max_q;
+  const Rows rows = rows_of(*seqs);
   const unsigned z = static_cast<unsigned>(seqs->batch) * seqs->kv_heads;
-  const bool any = seqs->packed > 0 && seqs->max_ctx > 0, few = rows <= kFewRows;
-  const bool solo = any && (few ? seqs->max_ctx <= kSoloKeys : values_tc_solo(ctx, *seqs));
-  if (!solo) {
+  const bool any = seqs->packed > 0 && seqs->max_ctx > 0;
+  const bool few_solo = seqs->max_ctx <= kSoloKeys, many_solo = rows.most > kFewRows && values_tc_solo(ctx, *seqs);
+  if (!any || (rows.few > 0 && !few_solo) || (rows.most > kFewRows && !many_solo)) {
     const int64_t words = seqs->tokens * seqs->q_heads * seqs->head_dim;
     const int64_t want = (words + kThreads - 1) / kThreads, cap = static_cast<int64_t>(ctx->sm_count) * 8;
     values_init_kernel<<<static_cast<unsigned>(want < cap ? want : cap), kThreads, 0, st>>>(*seqs, o);
   }
-  if (any && few) {
-    const int range = solo ? kSoloKeys : keys_per_cta(ctx, *seqs, kValStage, 1024, 3), rt = rows <= 4 ? 4 : 8;
-    const dim3 grid((seqs->max_ctx + range - 1) / range, (rows + rt - 1) / rt, z);
-    const auto kernel = rt == 4 ? (solo ? values_rows_kernel<4, true> : values_rows_kernel<4, false>)
-                                : (solo ? values_rows_kernel<8, true> : values_rows_kernel<8, false>);
+  if (any && rows.few > 0) {
+    const int range = few_solo ? kSoloKeys : keys_per_cta(ctx, *seqs, kValStage, 1024, 3);
+    const dim3 grid((seqs->max_ctx + range - 1) / range, 1, z);
+    const auto kernel = rows.few <= 4 ? (few_solo ? values_rows_kernel<4, true> : values_rows_kernel<4, false>)
+                                      : (few_solo ? values_rows_kernel<8, true> : values_rows_kernel<8, false>);
     kernel<<<grid, kThreads, 0, st>>>(*seqs, o, range);
-  } else if (any) {
+  }
+  o.few = rows.few;
+  if (any && rows.most > kFewRows) {
     const cudaError_t e = launch_values_tc(ctx, *seqs, o, st);
     if (e != cudaSuccess) return fail(SUFB200_ERR_CUDA, std::string("attn_values_pair: ") + cudaGetErrorString(e));
   }

@@ -114,6 +114,7 @@ struct AttnOperands {
   const uint64_t* e;     // opened pool [pages][kv_heads][page_size][head_dim]
   const uint64_t* b[2];  // its masks' shares
   uint64_t r;            // r_0 + r_1
+  int few;               // sequences of at most this many rows per key head are another kernel's
   uint64_t* out;
   uint32_t* status;
 };

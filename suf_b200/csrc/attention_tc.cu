@@ -10,7 +10,7 @@
 //   values: out[d][row]   = sum_j E[j][d]   U[row][j] + W[j][d]   D[row][j]
 // with W = B_0 + B_1, U = D + A_0 + A_1: two steps per 32 of depth, one
 // accumulator.  A thread of the epilogue holds one key (or word of the head)
-// for 32 rows, so a warp's stores and its loads of C are 256 adjacent bytes
+// for 16 rows, so a warp's stores and its loads of C are 256 adjacent bytes
 // whatever the packed rows' offsets are.
 //
 // The cached operand is read by every row tile of its group of heads, so a
@@ -19,6 +19,15 @@
 // scores once per CTA (they stay in shared memory while the keys stream past),
 // for the values chunk by chunk from the packed shares, which are read
 // nowhere else.
+//
+// What bounds them (packed prompts of 2,048, 700 behind 1,024 and one token, 16
+// / 4 heads of 128; 49 M scores): a step's MMAs alone take 1,210 cycles, 211 us
+// in all, with the clock near 1.65 - 1.8 GHz under them.  The scores take 488 us
+// (2.8 TB/s): their epilogue moves 24 bytes a score beside MMAs that use most of
+// the shared memory's bandwidth, and a tile's epilogue is slower than its MMAs.
+// The values take 428 us: 1,580 cycles a step, the tensor core sharing shared
+// memory with the splitting of the shares.  On the integer pipes the two took
+// 5,030 and 5,293 us.
 #include "attention.hpp"
 #include "umma_i8.cuh"
 
@@ -98,7 +107,7 @@ __global__ void __launch_bounds__(256) cache_planes_kernel(const __grid_constant
   const int t = threadIdx.x, b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads;
   constexpr int kPer = KEYS ? kTM : kTK;
   SeqInfo q;
-  if (!seq_info(s, b, a.o.status, q)) return;
+  if (!seq_info(s, b, a.o.status, q) || s.q_heads / s.kv_heads * q.n <= a.o.few) return;
   const int j0 = blockIdx.x * kPer;
   if (j0 >= q.L) return;
   for (int e = t; e < kPer; e += 256) s_key[e] = j0 + e < q.L ? key_off(s, b, kh, j0 + e, a.o.status) : -1;
@@ -303,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, dh = s.head_dim, group = s.q_heads / s.kv_heads;
   const int b = blockIdx.x / s.kv_heads, kh = blockIdx.x % s.kv_heads;
   SeqInfo q;
-  const bool fits = seq_info(s, b, o.status, q);
+  const bool fits = seq_info(s, b, o.status, q) && group * q.n > o.few;
   // every sequence's longest causal rows first
   const int R = fits ? group * q.n : 0, rho0 = ((R + kTN - 1) / kTN - 1 - static_cast<int>(blockIdx.y)) * kTN;
   const int last = (rho0 + kTN < R ? rho0 + kTN : R) - 1;
@@ -467,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, dh = s.head_dim, group = s.q_heads / s.kv_heads;
   const int b = blockIdx.x / s.kv_heads, kh = blockIdx.x % s.kv_heads, dt0 = blockIdx.y % a.chunks;
   SeqInfo q;
-  const bool fits = seq_info(s, b, o.status, q);
+  const bool fits = seq_info(s, b, o.status, q) && group * q.n > o.few;
   // every sequence's longest causal rows first
   const int R = fits ? group * q.n : 0;
   const int rho0 = ((R + kTN - 1) / kTN - 1 - static_cast<int>(blockIdx.y / a.chunks)) * kTN;

@@ -7,7 +7,10 @@
 // 2j, 2j + 1, and the last value of an odd row moves on as it is.  With off_k
 // the packed row offsets of round k, row r has off_k[r+1] - off_k[r] values,
 // and its pairs start at word off_k[r] - off_{k+1}[r] of the packed pairs
-// (values minus survivors of the rows before it).
+// (values minus survivors of the rows before it).  Rows may start at any word,
+// so accesses are 8 bytes wide and a warp's are adjacent; a round of 14.7 M
+// values in 21,712 rows runs at 5.5 - 6 TB/s (91 us for the first merge), below
+// some 10,000 values a round is one launch's latency (5.5 us).
 #include "attention.hpp"
 
 namespace sufb200 {

@@ -53,7 +53,7 @@ def _seqs(**kw):
 
     s = AttnSeqs()
     for k, v in dict(tokens=10, cached=60, packed=1000, batch=2, max_pages=4, page_size=8, pages=5, q_heads=4, kv_heads=2,
-                     head_dim=64, causal=1, max_q=6, max_ctx=30).items():
+                     head_dim=64, causal=1, min_q=1, max_q=6, max_ctx=30).items():
         setattr(s, k, v)
     for k, v in kw.items():
         setattr(s, k, v)

@@ -169,6 +169,8 @@ ATTN = [  # (new tokens, context) per sequence, q heads, kv heads, dim, page, ca
     ([(9, 130), (10, 9)], 3, 3, 34, 16, True),                    # just past the row kernels, empty rows
     ([(1, 256), (1, 255)], 4, 1, 128, 64, True),                  # one CTA's whole context
     ([(1, 257)], 8, 1, 62, 64, True),
+    ([(40, 60), (1, 300), (2, 1)], 4, 2, 160, 16, True),          # prompts and single tokens, wide heads
+    ([(1, 300), (40, 60), (0, 5), (3, 0), (20, 7)], 6, 2, 64, 32, False),
 ]
 
 
