@@ -775,13 +775,20 @@ int sufb200_rope_append_pair(sufb200_ctx ctx, const sufb200_rope_append* args, v
  * cached tokens and the words (workspaces are sized by them).  At most 2^26
  * cached tokens in a sequence, 65,535 (sequence, key head) pairs and 2^20 rows
  * (queries of its heads) per pair. */
+#define SUFB200_ATTN_FEW_ROWS 8  /* rows of a (sequence, key head) up to which it counts as short */
+#define SUFB200_ATTN_ROW_TILE 64 /* rows of a row tile */
 typedef struct sufb200_attn_seqs {
   const int32_t* d_cu_q;        /* [batch + 1] */
   const int32_t* d_cu_ctx;      /* [batch + 1] */
   const int64_t* d_row_base;    /* [batch] */
   const int32_t* d_block_table; /* [batch][max_pages] */
+  /* Order of work, or NULL (in order of the sequences, with idle blocks for
+   * those that are not long): (sequence, tile) pairs of every row tile of every
+   * sequence with more than SUFB200_ATTN_FEW_ROWS rows per key head, the longest
+   * rows first.  Tile i holds rows 64 i .. 64 i + 63 of query * group + head. */
+  const int32_t* d_tiles; /* [n_tiles][2] */
   int64_t tokens, cached, packed;
-  int32_t batch, max_pages, page_size, pages, q_heads, kv_heads, head_dim, causal, min_q, max_q, max_ctx, reserved;
+  int32_t batch, max_pages, page_size, pages, q_heads, kv_heads, head_dim, causal, min_q, max_q, max_ctx, n_tiles;
 } sufb200_attn_seqs;
 
 /* Scores: x^ = sum_p (C_p + D B_p + A_p E (+ D E for party 0) + r[p]) for every

@@ -28,6 +28,9 @@ TRUNC_FAITHFUL_TR = 0
 TRUNC_FAITHFUL_ARS = 1
 TRUNC_GAPARS = 2
 
+ATTN_FEW_ROWS = 8  # SUFB200_ATTN_FEW_ROWS
+ATTN_ROW_TILE = 64  # SUFB200_ATTN_ROW_TILE
+
 NOALLOC_KEY_BYTES = 16384  # SUFB200_NOALLOC_KEY_BYTES
 
 
@@ -72,10 +75,11 @@ class AttnSeqs(C.Structure):
 
     _fields_ = [
         ("d_cu_q", C.c_void_p), ("d_cu_ctx", C.c_void_p), ("d_row_base", C.c_void_p), ("d_block_table", C.c_void_p),
+        ("d_tiles", C.c_void_p),
         ("tokens", C.c_int64), ("cached", C.c_int64), ("packed", C.c_int64),
         ("batch", C.c_int32), ("max_pages", C.c_int32), ("page_size", C.c_int32), ("pages", C.c_int32),
         ("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("causal", C.c_int32),
-        ("min_q", C.c_int32), ("max_q", C.c_int32), ("max_ctx", C.c_int32), ("reserved", C.c_int32),
+        ("min_q", C.c_int32), ("max_q", C.c_int32), ("max_ctx", C.c_int32), ("n_tiles", C.c_int32),
     ]
 
 

@@ -337,6 +337,25 @@ class AttnLayout:
         s.page_size, s.q_heads, s.kv_heads, s.causal = self.page_size, self.q_heads, self.kv_heads, int(self.causal)
         s.min_q, s.max_q, s.max_ctx = int(q[q > 0].min(initial=2**31 - 1)), int(q.max(initial=0)), int(L.max(initial=0))
         s.min_q = min(s.min_q, s.max_q)
+        tiles = self._tile_list()
+        if len(tiles):
+            self._tiles = torch.from_numpy(tiles).to(dev)
+            s.d_tiles, s.n_tiles = self._tiles.data_ptr(), len(tiles)
+
+    def _tile_list(self) -> np.ndarray:
+        """(sequence, row tile) of the sequences with many rows, the longest rows first."""
+        group = self.q_heads // self.kv_heads
+        rows = self.q_lens * group
+        long_ = np.flatnonzero(rows > _lib.ATTN_FEW_ROWS)
+        if not len(long_):
+            return np.zeros((0, 2), dtype=np.int32)
+        count = -(-rows[long_] // _lib.ATTN_ROW_TILE)
+        seq = np.repeat(long_, count)
+        tile = np.arange(len(seq)) - np.repeat(np.cumsum(count) - count, count)
+        last = (np.minimum((tile + 1) * _lib.ATTN_ROW_TILE, rows[seq]) - 1) // group  # the tile's last query
+        length = self.ctx_lens[seq] + (last + 1 - self.q_lens[seq] if self.causal else 0)
+        order = np.argsort(-length, kind="stable")
+        return np.stack([seq, tile], axis=1)[order].astype(np.int32)
 
     def row_lengths(self) -> np.ndarray:
         """Keys of every row, in (sequence, head, query) order."""

@@ -32,7 +32,7 @@ constexpr int kThreads = 256;
 // Four sequences of 8,192 tokens, 32 / 8 heads of 128, row kernels against
 // tensor cores: scores of 8 rows 238 and 407 us, 16 rows 455 and 419 us; values
 // of 8 rows 291 and 346 us, 16 rows 568 and 354 us.
-constexpr int kFewRows = 8;
+constexpr int kFewRows = SUFB200_ATTN_FEW_ROWS;
 
 int fail(int code, const std::string& msg) { return record_error(code, msg); }
 
@@ -319,6 +319,7 @@ int check_seqs(const sufb200_attn_seqs* s, const char* who) {
     return fail(SUFB200_ERR_INVALID, at + "max_ctx is more than the block table's pages hold");
   if (static_cast<__int128>(s->q_heads) * s->max_q * s->max_ctx >= (static_cast<__int128>(1) << 60))
     return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^60 packed words");
+  if (s->n_tiles < 0 || (s->n_tiles > 0 && !s->d_tiles)) return fail(SUFB200_ERR_INVALID, at + "null tile list");
   if (s->batch > 0 && (!s->d_cu_q || !s->d_cu_ctx || !s->d_row_base || (s->max_ctx > 0 && !s->d_block_table)))
     return fail(SUFB200_ERR_INVALID, at + "null sequence array");
   return SUFB200_OK;

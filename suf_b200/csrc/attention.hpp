@@ -41,6 +41,12 @@ SUFB200_HD int64_t row_off(int n, int L, int causal, int i) {
   return k * f + k * (k - 1) / 2;
 }
 
+// Blocks of `per` items over packed sequences, as one list: the sequence with
+// c items before it starts at block c / per + b, which leaves room for every
+// sequence's last, partly filled block; blocks_of bounds them all.
+SUFB200_HD int64_t first_block(int64_t c, int b, int per) { return c / per + b; }
+inline int64_t blocks_of(int64_t items, int batch, int per) { return items / per + batch; }
+
 // Whether a sequence's lengths and rows lie inside what the host arguments
 // say (so every address formed from them does too); fills q.
 SUFB200_HD bool seq_fits(const AttnSeqs& s, int c0, int c1, int l0, int l1, int64_t base, SeqInfo& q) {
@@ -63,6 +69,21 @@ SUFB200_HD int64_t page_word(const AttnSeqs& s, int pg, int kh, int j) {
 }
 
 #if defined(__CUDACC__)
+// The sequence block g of the list belongs to (m items per entry of cu, [batch
+// + 1]): the last one that starts at or before g.  A whole warp searches, 32
+// sequences a round.
+__device__ __forceinline__ int block_seq(const int32_t* cu, int batch, int m, int per, int64_t g) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = batch;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, i = lo + (lane + 1) * step;
+    const bool before = i < hi && first_block(static_cast<int64_t>(m) * cu[i], i, per) <= g;
+    lo += __popc(__ballot_sync(0xffffffffu, before)) * step;
+    hi = lo + step < hi ? lo + step : hi;
+  }
+  return lo;
+}
+
 // Sequence b; false (and the status word flagged) when the device arrays do
 // not fit what the host was told.
 __device__ __forceinline__ bool seq_info(const AttnSeqs& s, int b, uint32_t* status, SeqInfo& q) {

@@ -35,6 +35,7 @@ namespace sufb200 {
 
 namespace {
 
+static_assert(kTN == SUFB200_ATTN_ROW_TILE, "row tile");
 constexpr int kThreads = 640;  // warp 0 copies A, warp 1 issues MMAs, warps 4-19 make B planes and store
 constexpr int kWorkers = 512;
 constexpr uint32_t kAStage = 8 * kPlaneX;  // 32 KB: A planes of one step
@@ -49,14 +50,10 @@ struct AttnTc {
   AttnSeqs s;
   AttnOperands o;
   uint8_t* planes;
-  int64_t tiles;  // blocks of rows (scores: 128 keys; values: 32 keys) per key head in `planes`
+  int64_t tiles;  // blocks (scores: 128 keys; values: 32 keys) per key head in `planes`
   int chunks;     // scores: 32-word chunks of the head; values: 128-word tiles of the head
   int span;       // scores: key tiles per CTA; values: keys per CTA
 };
-
-// First block of a sequence with l0 cached tokens before it, blocks of `per`
-// tokens: a sequence of L tokens has at most (l0 + L) / per + 1 - l0 / per.
-__device__ __forceinline__ int64_t first_block(int l0, int b, int per) { return l0 / per + b; }
 
 // Byte i of four K-consecutive words into plane i at `at`, for all planes.
 __device__ __forceinline__ void put4(uint8_t* at, uint32_t plane, const uint64_t (&v)[4]) {
@@ -104,15 +101,16 @@ __global__ void __launch_bounds__(256) cache_planes_kernel(const __grid_constant
   pdl_trigger();
   __shared__ int64_t s_key[kTM];
   const AttnSeqs& s = a.s;
-  const int t = threadIdx.x, b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads;
   constexpr int kPer = KEYS ? kTM : kTK;
+  const int t = threadIdx.x, b = block_seq(s.d_cu_ctx, s.batch, 1, kPer, blockIdx.x), kh = blockIdx.z;
   SeqInfo q;
   if (!seq_info(s, b, a.o.status, q) || s.q_heads / s.kv_heads * q.n <= a.o.few) return;
-  const int j0 = blockIdx.x * kPer;
-  if (j0 >= q.L) return;
+  const int64_t first = blockIdx.x - first_block(q.l0, b, kPer);  // this block in its sequence
+  if (first < 0 || first * kPer >= q.L) return;
+  const int j0 = static_cast<int>(first) * kPer;
   for (int e = t; e < kPer; e += 256) s_key[e] = j0 + e < q.L ? key_off(s, b, kh, j0 + e, a.o.status) : -1;
   __syncthreads();
-  const int64_t block = ((kh * a.tiles + first_block(q.l0, b, kPer) + blockIdx.x) * a.chunks + blockIdx.y) * 2;
+  const int64_t block = ((kh * a.tiles + blockIdx.x) * a.chunks + blockIdx.y) * 2;
   uint8_t* dst = a.planes + block * kAStage;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
@@ -305,19 +303,50 @@ __device__ __forceinline__ void issue_last(uint32_t a, uint32_t b) {
   issue_one(al, bl, 4, 0, 1u);
 }
 
+// Row tile `tile` of the call: its sequence and its first row, rho0 = -1 when
+// there is none.  From the list of tiles, or counting through the sequences,
+// each from its last (longest) rows on.
+struct TileOf {
+  SeqInfo q;
+  int b, R, rho0;
+};
+
+__device__ __forceinline__ TileOf tile_of(const AttnTc& a, int tile) {
+  const AttnSeqs& s = a.s;
+  const int group = s.q_heads / s.kv_heads;
+  TileOf t{};
+  t.rho0 = -1;
+  const bool list = s.d_tiles != nullptr;
+  t.b = list ? s.d_tiles[2 * tile] : block_seq(s.d_cu_q, s.batch, group, kTN, tile);
+  if (t.b < 0 || t.b >= s.batch) {
+    atomicOr(a.o.status, kStatusBadArgument);
+    return t;
+  }
+  if (!seq_info(s, t.b, a.o.status, t.q) || group * t.q.n <= a.o.few) return t;
+  t.R = group * t.q.n;
+  const int64_t tiles = (t.R + kTN - 1) / kTN;
+  const int64_t i = list ? s.d_tiles[2 * tile + 1] : tiles - 1 - (tile - first_block(static_cast<int64_t>(group) * t.q.t0, t.b, kTN));
+  if (i >= 0 && i < tiles) t.rho0 = static_cast<int>(i) * kTN;
+  return t;
+}
+
+// Row tiles a launch enumerates.
+int64_t row_tiles(const AttnSeqs& s) {
+  return s.d_tiles ? s.n_tiles : blocks_of(s.q_heads / s.kv_heads * s.tokens, s.batch, kTN);
+}
+
 __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_constant__ AttnTc a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const AttnSeqs& s = a.s;
   const AttnOperands& o = a.o;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, dh = s.head_dim, group = s.q_heads / s.kv_heads;
-  const int b = blockIdx.x / s.kv_heads, kh = blockIdx.x % s.kv_heads;
-  SeqInfo q;
-  const bool fits = seq_info(s, b, o.status, q) && group * q.n > o.few;
-  // every sequence's longest causal rows first
-  const int R = fits ? group * q.n : 0, rho0 = ((R + kTN - 1) / kTN - 1 - static_cast<int>(blockIdx.y)) * kTN;
+  const int kh = blockIdx.x % s.kv_heads;
+  const TileOf tile = tile_of(a, blockIdx.x / s.kv_heads);
+  const SeqInfo& q = tile.q;
+  const int b = tile.b, R = tile.R, rho0 = tile.rho0;
   const int last = (rho0 + kTN < R ? rho0 + kTN : R) - 1;
   const int len = rho0 >= 0 && rho0 < R ? row_len(q.n, q.L, s.causal, last / group) : 0;
-  const int nt = (len + kTM - 1) / kTM, tile0 = blockIdx.z * a.span;
+  const int nt = (len + kTM - 1) / kTM, tile0 = blockIdx.y * a.span;
   const int tiles = nt - tile0 < a.span ? nt - tile0 : a.span;
   if (tiles <= 0) {
     pdl_wait();
@@ -474,15 +503,13 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
   const AttnSeqs& s = a.s;
   const AttnOperands& o = a.o;
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, dh = s.head_dim, group = s.q_heads / s.kv_heads;
-  const int b = blockIdx.x / s.kv_heads, kh = blockIdx.x % s.kv_heads, dt0 = blockIdx.y % a.chunks;
-  SeqInfo q;
-  const bool fits = seq_info(s, b, o.status, q) && group * q.n > o.few;
-  // every sequence's longest causal rows first
-  const int R = fits ? group * q.n : 0;
-  const int rho0 = ((R + kTN - 1) / kTN - 1 - static_cast<int>(blockIdx.y / a.chunks)) * kTN;
+  const int kh = blockIdx.x % s.kv_heads, dt0 = blockIdx.x / s.kv_heads % a.chunks;
+  const TileOf tile = tile_of(a, blockIdx.x / s.kv_heads / a.chunks);
+  const SeqInfo& q = tile.q;
+  const int b = tile.b, R = tile.R, rho0 = tile.rho0;
   const int last = (rho0 + kTN < R ? rho0 + kTN : R) - 1;
   const int len = rho0 >= 0 && rho0 < R ? row_len(q.n, q.L, s.causal, last / group) : 0;
-  const int beg = blockIdx.z * a.span, end = len < beg + a.span ? len : beg + a.span;
+  const int beg = blockIdx.y * a.span, end = len < beg + a.span ? len : beg + a.span;
   const int nch = end > beg ? (end - beg + kTK - 1) / kTK : 0;
   const int word0 = dt0 * kTM;
   // word `word` of the output of row rho
@@ -664,30 +691,31 @@ cudaError_t launch(K kernel, dim3 grid, size_t smem, cudaStream_t st, const Attn
 bool scores_tc_fits(const AttnSeqs& s) { return s.head_dim <= 128; }
 
 cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st) {
-  const int rows = s.q_heads / s.kv_heads * s.max_q;
-  const unsigned z = static_cast<unsigned>(s.batch) * s.kv_heads;
-  const int nt = (s.max_ctx + kTM - 1) / kTM, rt = (rows + kTN - 1) / kTN;
-  AttnTc a{s, o, nullptr, s.cached / kTM + s.batch, (s.head_dim + kTK - 1) / kTK, 0};
+  const int64_t rts = row_tiles(s);
+  const int nt = (s.max_ctx + kTM - 1) / kTM;
+  AttnTc a{s, o, nullptr, blocks_of(s.cached, s.batch, kTM), (s.head_dim + kTK - 1) / kTK, 0};
   const int64_t bytes = a.tiles * s.kv_heads * a.chunks * 2 * static_cast<int64_t>(kAStage);
   cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&a.planes), bytes, ctx->pool, st);
   if (e != cudaSuccess) return e;
   // key tiles per CTA: long runs reuse the rows' planes and hide the epilogue
-  // behind the next tile, as long as every SM has a few CTAs to take
-  const int64_t all = static_cast<int64_t>(nt) * rt * z, want = all / (static_cast<int64_t>(ctx->sm_count) * 4);
+  // behind the next tile, as long as every SM has a few CTAs to take (a
+  // 2,048-token prompt, 16 / 4 heads of 128, first form: 738 us for runs of one
+  // tile, 510 of two, 410 of four, 363 of eight, 346 of sixteen)
+  const int64_t all = nt * rts * s.kv_heads, want = all / (static_cast<int64_t>(ctx->sm_count) * 4);
   a.span = static_cast<int>(want < 1 ? 1 : (want > 16 ? 16 : want));
-  cache_planes_kernel<true><<<dim3(nt, a.chunks, z), 256, 0, st>>>(a);
+  cache_planes_kernel<true><<<dim3(static_cast<unsigned>(a.tiles), a.chunks, s.kv_heads), 256, 0, st>>>(a);
   e = cudaGetLastError();
   const size_t smem = kBOff + static_cast<size_t>(2 * a.chunks) * kBStage + kCtrlBytes;
-  if (e == cudaSuccess) e = launch(scores_tc_kernel, dim3(z, rt, (nt + a.span - 1) / a.span), smem, st, a);
+  const dim3 grid(static_cast<unsigned>(rts * s.kv_heads), (nt + a.span - 1) / a.span);
+  if (e == cudaSuccess) e = launch(scores_tc_kernel, grid, smem, st, a);
   const cudaError_t f = cudaFreeAsync(a.planes, st);
   return e == cudaSuccess ? f : e;
 }
 
 // Keys per CTA of the values form, and whether one CTA takes whole rows.
 int values_span(const sufb200_ctx_s* ctx, const AttnSeqs& s) {
-  const int rows = s.q_heads / s.kv_heads * s.max_q;
-  const int nch = (s.max_ctx + kTK - 1) / kTK, rt = (rows + kTN - 1) / kTN, words = (s.head_dim + kTM - 1) / kTM;
-  const int64_t units = static_cast<int64_t>(rt) * words * s.batch * s.kv_heads;
+  const int nch = (s.max_ctx + kTK - 1) / kTK, words = (s.head_dim + kTM - 1) / kTM;
+  const int64_t units = row_tiles(s) * words * s.kv_heads;
   // at most the exact depth; shorter, down to eight chunks, while that leaves SMs idle
   int64_t parts = (static_cast<int64_t>(ctx->sm_count) * 4 + units - 1) / units;
   const int64_t most = (nch + 7) / 8;
@@ -699,17 +727,14 @@ int values_span(const sufb200_ctx_s* ctx, const AttnSeqs& s) {
 bool values_tc_solo(const sufb200_ctx_s* ctx, const AttnSeqs& s) { return values_span(ctx, s) >= s.max_ctx; }
 
 cudaError_t launch_values_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st) {
-  const int rows = s.q_heads / s.kv_heads * s.max_q;
-  const int nch = (s.max_ctx + kTK - 1) / kTK, rt = (rows + kTN - 1) / kTN;
-  AttnTc a{s, o, nullptr, s.cached / kTK + s.batch, (s.head_dim + kTM - 1) / kTM, values_span(ctx, s)};
-  const unsigned z = static_cast<unsigned>(s.batch) * s.kv_heads;
+  AttnTc a{s, o, nullptr, blocks_of(s.cached, s.batch, kTK), (s.head_dim + kTM - 1) / kTM, values_span(ctx, s)};
   const int64_t bytes = a.tiles * s.kv_heads * a.chunks * 2 * static_cast<int64_t>(kAStage);
   cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&a.planes), bytes, ctx->pool, st);
   if (e != cudaSuccess) return e;
-  cache_planes_kernel<false><<<dim3(nch, a.chunks, z), 256, 0, st>>>(a);
+  cache_planes_kernel<false><<<dim3(static_cast<unsigned>(a.tiles), a.chunks, s.kv_heads), 256, 0, st>>>(a);
   e = cudaGetLastError();
   const size_t smem = kBOff + kBStages * kBStage + kCtrlBytes;
-  const dim3 grid(z, rt * a.chunks, (s.max_ctx + a.span - 1) / a.span);
+  const dim3 grid(static_cast<unsigned>(row_tiles(s) * a.chunks * s.kv_heads), (s.max_ctx + a.span - 1) / a.span);
   if (e == cudaSuccess)
     e = a.span >= s.max_ctx ? launch(values_tc_kernel<true>, grid, smem, st, a)
                             : launch(values_tc_kernel<false>, grid, smem, st, a);

@@ -21,3 +21,6 @@ int64_t emu_page_word(const sufb200_attn_seqs* s, int pg, int kh, int j) { retur
 
 size_t emu_sizeof(int which) { return which == 0 ? sizeof(sufb200_rope_append) : sizeof(sufb200_attn_seqs); }
 }
+
+extern "C" int64_t emu_first_block(int64_t c, int b, int per) { return first_block(c, b, per); }
+extern "C" int64_t emu_blocks_of(int64_t items, int batch, int per) { return blocks_of(items, batch, per); }

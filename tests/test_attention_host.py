@@ -87,6 +87,24 @@ def test_pages_outside_the_pool_are_refused(emu):
     assert emu.emu_page_word(C.byref(s), 10**6 - 1, 7, 63) == 10**6 * 8 * 64 * 128 - 128
 
 
+def test_blocks_of_packed_sequences_never_overlap(emu):
+    """Every sequence has room for all its blocks before the next one starts,
+    and the last one within the bound that sizes grids and workspaces."""
+    emu.emu_first_block.restype = emu.emu_blocks_of.restype = C.c_int64
+    emu.emu_first_block.argtypes, emu.emu_blocks_of.argtypes = [C.c_int64, C.c_int, C.c_int], [C.c_int64, C.c_int, C.c_int]
+    rng = np.random.default_rng(1)
+    for _ in range(300):
+        per, m = int(rng.choice([32, 64, 128])), int(rng.choice([1, 4, 5]))
+        lens = rng.choice([0, 1, 7, 31, 32, 33, 64, 127, 128, 129, 500], rng.integers(1, 9)) * m
+        at = np.concatenate([[0], np.cumsum(lens)])
+        end = 0
+        for b, n in enumerate(lens):
+            first = emu.emu_first_block(int(at[b]), b, per)
+            assert first >= end
+            end = first + -(-int(n) // per)
+        assert end <= emu.emu_blocks_of(int(at[-1]), len(lens), per)
+
+
 # -- refusals of the C entries ----------------------------------------------------
 
 @pytest.fixture(scope="module")
@@ -134,7 +152,8 @@ def test_attention_refusals(host, which):
                       (dict(head_dim=0), _lib.ERR_UNSUPPORTED), (dict(q_heads=3), _lib.ERR_INVALID),
                       (dict(kv_heads=0), _lib.ERR_INVALID), (dict(page_size=0), _lib.ERR_INVALID),
                       (dict(max_ctx=33), _lib.ERR_INVALID), (dict(batch=-1), _lib.ERR_INVALID),
-                      (dict(tokens=-1), _lib.ERR_INVALID), (dict(cached=-1), _lib.ERR_INVALID), (dict(d_cu_ctx=None), _lib.ERR_INVALID),
+                      (dict(tokens=-1), _lib.ERR_INVALID), (dict(n_tiles=3), _lib.ERR_INVALID),
+                      (dict(min_q=7), _lib.ERR_INVALID), (dict(cached=-1), _lib.ERR_INVALID), (dict(d_cu_ctx=None), _lib.ERR_INVALID),
                       (dict(d_block_table=None), _lib.ERR_INVALID), (dict(batch=40000), _lib.ERR_UNSUPPORTED),
                       (dict(max_q=2**20), _lib.ERR_UNSUPPORTED),
                       (dict(max_ctx=2**26 + 1, max_pages=2**26), _lib.ERR_UNSUPPORTED),

@@ -275,6 +275,39 @@ def test_values_match_definition(ctx, torch_cuda, case):
 
 
 @pytest.mark.parametrize("which", ["scores", "values"])
+@pytest.mark.parametrize("case", [ATTN[7], ATTN[12], ATTN[20], ATTN[21]])
+def test_attention_without_a_tile_list(ctx, torch_cuda, which, case):
+    """The C entry's form without an order of work: the same words."""
+    from suf_b200 import attention as at
+
+    A = _Attn(ctx, torch_cuda, case, 14)
+    args, want = getattr(A, which)()
+    assert A.layout._seqs.n_tiles > 0
+    A.layout._seqs.d_tiles, A.layout._seqs.n_tiles = None, 0
+    got = getattr(at, f"attn_{which}_pair")(ctx, *args)
+    ctx.sync()
+    assert (from_dev(got) == want).all()
+
+
+@pytest.mark.parametrize("which", ["scores", "values"])
+def test_attention_reports_a_bad_tile_list(ctx, torch_cuda, which):
+    from suf_b200 import SufB200Error
+    from suf_b200 import attention as at
+
+    A = _Attn(ctx, torch_cuda, ATTN[12], 15)
+    args, _ = getattr(A, which)()
+    for bad in (-1, 3, 2**31 - 1):
+        A.layout._tiles[0, 0] = bad
+        getattr(at, f"attn_{which}_pair")(ctx, *args)
+        with pytest.raises(SufB200Error):
+            ctx.sync()
+    A.layout._tiles[0, 0] = 0
+    A.layout._tiles[0, 1] = 10**9  # a tile past the sequence's last: nothing to do
+    getattr(at, f"attn_{which}_pair")(ctx, *args)
+    ctx.sync()
+
+
+@pytest.mark.parametrize("which", ["scores", "values"])
 @pytest.mark.parametrize("case", [ATTN[2], ATTN[9]])
 def test_attention_reports_bad_pages(ctx, torch_cuda, which, case):
     from suf_b200 import SufB200Error
