@@ -784,8 +784,8 @@ typedef struct sufb200_attn_seqs {
   const int32_t* d_block_table; /* [batch][max_pages] */
   /* Order of work, or NULL (in order of the sequences, with idle blocks for
    * those that are not long): (sequence, tile) pairs of every row tile of every
-   * sequence with more than SUFB200_ATTN_FEW_ROWS rows per key head, the longest
-   * rows first.  Tile i holds rows 64 i .. 64 i + 63 of query * group + head. */
+   * sequence with more than SUFB200_ATTN_FEW_ROWS rows per key head, each once, the
+   * longest rows first.  Tile i holds rows 64 i .. 64 i + 63 of query * group + head. */
   const int32_t* d_tiles; /* [n_tiles][2] */
   int64_t tokens, cached, packed;
   int32_t batch, max_pages, page_size, pages, q_heads, kv_heads, head_dim, causal, min_q, max_q, max_ctx, n_tiles;

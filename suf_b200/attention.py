@@ -14,8 +14,9 @@ needs a freshly dealt mask.  The reference keeps its cache as share tensors
 
 All tensors live on the context's device; shares and opened words are int64
 tensors (the words of Z_2^64).  Calls are asynchronous on `stream` (default:
-the device's current stream).  Wrong device-side data (slots, positions,
-pages) is reported by Context.sync.
+the device's current stream); what they are given has to stay allocated until
+that stream has passed them.  Wrong device-side data (slots, positions, pages)
+is reported by Context.sync.
 """
 from __future__ import annotations
 
@@ -169,6 +170,11 @@ class TruncPair(_Trunc):
     def eval_pair(self, ctx: Context, d_xhat, d_y0, d_y1, stream=None):
         """Both parties' truncated shares of the opened x^: lookups in the
         tables (a bundle without queries has none and is evaluated as it is)."""
+        shape = d_xhat.shape
+        for name, t in (("x^", d_xhat), ("y0", d_y0), ("y1", d_y1)):
+            _want(ctx, name, t, shape)
+        if d_xhat.numel() == 0:
+            return
         st = _stream(ctx, stream)
         if not self._full.any():
             return super().eval_pair(ctx, d_xhat, d_y0, d_y1, st or 0)

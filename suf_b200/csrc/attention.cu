@@ -314,6 +314,10 @@ int check_seqs(const sufb200_attn_seqs* s, const char* who) {
     return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 65535 (sequence, key head) pairs");
   if (static_cast<int64_t>(s->q_heads / s->kv_heads) * s->max_q > 1 << 20)
     return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^20 rows per (sequence, key head)");
+  // grids count row tiles x key heads x 128-word tiles of the head
+  const int64_t tiles = s->tokens / SUFB200_ATTN_ROW_TILE * (s->q_heads / s->kv_heads + 1) + s->n_tiles + s->batch;
+  if (s->tokens > INT32_MAX || s->cached > INT32_MAX || tiles > INT32_MAX / 2 / s->kv_heads)
+    return fail(SUFB200_ERR_UNSUPPORTED, at + "too many tokens for one call");
   if (s->max_ctx > 1 << 26) return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^26 cached tokens in a sequence");
   if (static_cast<int64_t>(s->max_ctx) > static_cast<int64_t>(s->max_pages) * s->page_size)
     return fail(SUFB200_ERR_INVALID, at + "max_ctx is more than the block table's pages hold");

@@ -263,8 +263,10 @@ __device__ __forceinline__ void fold16(int quarter, int col, uint64_t (&z)[16]) 
   }
 }
 
-// The twelve MMAs of one step (umma_i8.cuh's products in another order) on the
-// A planes at shared address a and the B planes at b.  The tensor core's queue
+// The twelve MMAs of one step (the products of ring_gemm_tc.cu's mma_step in
+// another order) on the A planes at shared address a and the B planes at b:
+// x_i times [y_j ...] for N = 256, accumulated at column 64 (i + j), lands every
+// product (i, j) on its diagonal i + j.  The tensor core's queue
 // is short: it runs dry whenever the issuing warp is held up for longer than
 // the last MMAs it was given take, and a wait for the next step's planes holds
 // it up by about 200 cycles even when they are there.  So a step is issued in

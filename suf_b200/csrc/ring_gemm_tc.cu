@@ -67,6 +67,22 @@ __device__ __forceinline__ uint4 plane_bytes(const uint64_t (&v)[16], int i) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// The B planes of a stage are consecutive 64-row blocks in core-matrix
+// order, so [y_0 | y_1 | y_2 | y_3] is one N = 256 operand.  x_i times it,
+// accumulated at column 64 i, lands product (i, j) on column 64 (i + j):
+// diagonal i + j.  Twelve MMAs (N = 256 except where the 512 columns end)
+// cover the 36 limb pairs; the first two write all 512 columns, so on the
+// first step (accumulate = 0) they alone start from zero.
+__device__ __forceinline__ void mma_step(const uint32_t (&dt)[8], const uint64_t (&as)[8], const uint64_t (&bs)[8],
+                                         uint32_t accumulate) {
+  umma_i8(dt[0], as[0], bs[0], idesc_n(256), accumulate);
+  umma_i8(dt[4], as[0], bs[4], idesc_n(256), accumulate);
+#pragma unroll
+  for (int i = 1; i < 8; i++) umma_i8(dt[i], as[i], bs[0], idesc_n(i <= 4 ? 256 : 64 * (8 - i)), 1u);
+#pragma unroll
+  for (int i = 1; i < 4; i++) umma_i8(dt[i + 4], as[i], bs[4], idesc_n(256 - 64 * i), 1u);
+}
+
 // ---- Epilogue: the K-split CTAs of a tile are one thread-block cluster ----
 // Every CTA folds its 8 diagonals into a 128 x 64 word tile in its own shared
 // memory (the pipeline stages are idle by then); after a cluster barrier each

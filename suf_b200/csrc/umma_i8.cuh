@@ -1,7 +1,6 @@
 // umma_i8.cuh -- tcgen05 kind::i8 building blocks of the exact Z_2^64 products
 // (ring_gemm_tc.cu, attention_tc.cu): mbarriers with bounded waits, bulk
-// copies, descriptors of byte-plane operands, the twelve MMAs of a step and
-// tensor-memory loads.
+// copies, descriptors of byte-plane operands and tensor-memory loads.
 #pragma once
 
 #include <cstdint>
@@ -118,22 +117,6 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
-// The B planes of a stage are consecutive 64-row blocks in core-matrix
-// order, so [y_0 | y_1 | y_2 | y_3] is one N = 256 operand.  x_i times it,
-// accumulated at column 64 i, lands product (i, j) on column 64 (i + j):
-// diagonal i + j.  Twelve MMAs (N = 256 except where the 512 columns end)
-// cover the 36 limb pairs; the first two write all 512 columns, so on the
-// first step (accumulate = 0) they alone start from zero.
-__device__ __forceinline__ void mma_step(const uint32_t (&dt)[8], const uint64_t (&as)[8], const uint64_t (&bs)[8],
-                                         uint32_t accumulate) {
-  umma_i8(dt[0], as[0], bs[0], idesc_n(256), accumulate);
-  umma_i8(dt[4], as[0], bs[4], idesc_n(256), accumulate);
-#pragma unroll
-  for (int i = 1; i < 8; i++) umma_i8(dt[i], as[i], bs[0], idesc_n(i <= 4 ? 256 : 64 * (8 - i)), 1u);
-#pragma unroll
-  for (int i = 1; i < 4; i++) umma_i8(dt[i + 4], as[i], bs[4], idesc_n(256 - 64 * i), 1u);
 }
 
 }  // namespace sufb200

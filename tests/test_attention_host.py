@@ -155,7 +155,8 @@ def test_attention_refusals(host, which):
                       (dict(tokens=-1), _lib.ERR_INVALID), (dict(n_tiles=3), _lib.ERR_INVALID),
                       (dict(min_q=7), _lib.ERR_INVALID), (dict(cached=-1), _lib.ERR_INVALID), (dict(d_cu_ctx=None), _lib.ERR_INVALID),
                       (dict(d_block_table=None), _lib.ERR_INVALID), (dict(batch=40000), _lib.ERR_UNSUPPORTED),
-                      (dict(max_q=2**20), _lib.ERR_UNSUPPORTED),
+                      (dict(max_q=2**20), _lib.ERR_UNSUPPORTED), (dict(tokens=2**31), _lib.ERR_UNSUPPORTED),
+                      (dict(cached=2**31), _lib.ERR_UNSUPPORTED),
                       (dict(max_ctx=2**26 + 1, max_pages=2**26), _lib.ERR_UNSUPPORTED),
                       (dict(q_heads=2**20, kv_heads=2**16 - 1 + 1, batch=1), _lib.ERR_UNSUPPORTED)]:
         assert _attn(host, which, _seqs(**{**PTRS, **bad})) == code, bad
@@ -290,3 +291,23 @@ def test_rope_tables_are_rounded_cosines_of_the_definition():
             assert (mix[:, i] == all_[:, i]).all()
         else:
             assert (mix[:, i] != plain[:, i]).any() and (mix[:, i] != all_[:, i]).any()
+
+
+def test_mma_order_covers_every_limb_pair_once():
+    """The tensor-core kernels' twelve MMAs of a step (attention_tc.cu): every
+    limb pair (i, j), i + j <= 7, once on its diagonal, within the 512 columns,
+    the two that start from zero first and covering all of them."""
+    import re
+
+    src = (ROOT / "suf_b200" / "csrc" / "attention_tc.cu").read_text()
+    calls = [(int(i), int(j), acc) for i, j, acc in re.findall(r"issue_one\(al, bl, (\d), (\d), (accumulate|1u)\);", src)]
+    assert "const int n = 64 * (8 - i - j);" in src and "idesc_n(n < 256 ? n : 256)" in src and len(calls) == 12
+    seen = {}
+    for i, j, _ in calls:
+        n = min(64 * (8 - i - j), 256)
+        assert (i + j) * 64 + n <= 512 and j * 64 + n <= 512
+        for q in range(n // 64):
+            seen[(i, j + q)] = seen.get((i, j + q), 0) + 1
+    assert seen == {(i, j): 1 for i in range(8) for j in range(8) if i + j <= 7}
+    assert [c[2] for c in calls[:2]] == ["accumulate"] * 2 and {c[2] for c in calls[2:]} == {"1u"}
+    assert [(c[0], c[1]) for c in calls[:2]] == [(0, 0), (0, 4)]
