@@ -101,15 +101,26 @@ __global__ void __launch_bounds__(kThreads, RT == 4 ? 4 : 3) scores_rows_kernel(
         acc[1][rr] += u.x * e1.x + u.y * e1.y + d.x * w1.x + d.y * w1.y;
       }
     }
+    // sums over the key's eight lanes, halving the rows a lane holds in every
+    // exchange: RT - 1 exchanges (and log2(8 / RT) more) instead of 3 RT
 #pragma unroll
-    for (int v = 0; v < 2; v++)
+    for (int v = 0; v < 2; v++) {
+      int row = 0;
 #pragma unroll
-      for (int rr = 0; rr < RT; rr++) {
-        uint64_t z = acc[v][rr];
+      for (int m = 1; m < RT; m *= 2) {
+        const bool up = l8 & m;
 #pragma unroll
-        for (int m = 4; m > 0; m >>= 1) z += __shfl_xor_sync(0xffffffffu, z, m);
-        if (l8 == rr % 8) s_out[rr * (chunk + 1) + kk + 32 * v] = z;
+        for (int rr = 0; rr < RT / (2 * m); rr++) {
+          const uint64_t keep = up ? acc[v][2 * rr + 1] : acc[v][2 * rr];
+          const uint64_t give = up ? acc[v][2 * rr] : acc[v][2 * rr + 1];
+          acc[v][rr] = keep + __shfl_xor_sync(0xffffffffu, give, m);
+        }
+        row += up ? m : 0;
       }
+#pragma unroll
+      for (int m = RT; m < 8; m *= 2) acc[v][0] += __shfl_xor_sync(0xffffffffu, acc[v][0], m);
+      if (l8 < RT) s_out[row * (chunk + 1) + kk + 32 * v] = acc[v][0];
+    }
   }
   __syncthreads();
   for (int e = t; e < RT * chunk; e += kThreads) {

@@ -28,6 +28,8 @@
 // The values take 428 us: 1,580 cycles a step, the tensor core sharing shared
 // memory with the splitting of the shares.  On the integer pipes the two took
 // 5,030 and 5,293 us.
+#include <atomic>
+
 #include "attention.hpp"
 #include "umma_i8.cuh"
 
@@ -680,10 +682,19 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
   stop(c, o.status, warp, lane, copies);
 }
 
-template <typename K>
-cudaError_t launch(K kernel, dim3 grid, size_t smem, cudaStream_t st, const AttnTc& a) {
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (e != cudaSuccess) return e;
+// Launch as the pre-pass's programmatic dependent; the kernel may take all
+// shared memory, said once per kernel and device.
+template <int WHICH>
+cudaError_t launch(const sufb200_ctx_s* ctx, void (*kernel)(AttnTc), dim3 grid, size_t smem, cudaStream_t st,
+                   const AttnTc& a) {
+  constexpr int kMaxDevices = 64;
+  static std::atomic<bool> ready[kMaxDevices];
+  const bool known = ctx->device < kMaxDevices;
+  if (!known || !ready[ctx->device].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    if (e != cudaSuccess) return e;
+    if (known) ready[ctx->device].store(true, std::memory_order_release);
+  }
   return launch_pdl(kernel, grid, dim3(kThreads), smem, st, a);
 }
 
@@ -709,7 +720,7 @@ cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const 
   e = cudaGetLastError();
   const size_t smem = kBOff + static_cast<size_t>(2 * a.chunks) * kBStage + kCtrlBytes;
   const dim3 grid(static_cast<unsigned>(rts * s.kv_heads), (nt + a.span - 1) / a.span);
-  if (e == cudaSuccess) e = launch(scores_tc_kernel, grid, smem, st, a);
+  if (e == cudaSuccess) e = launch<0>(ctx, scores_tc_kernel, grid, smem, st, a);
   const cudaError_t f = cudaFreeAsync(a.planes, st);
   return e == cudaSuccess ? f : e;
 }
@@ -738,8 +749,8 @@ cudaError_t launch_values_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const 
   const size_t smem = kBOff + kBStages * kBStage + kCtrlBytes;
   const dim3 grid(static_cast<unsigned>(row_tiles(s) * a.chunks * s.kv_heads), (s.max_ctx + a.span - 1) / a.span);
   if (e == cudaSuccess)
-    e = a.span >= s.max_ctx ? launch(values_tc_kernel<true>, grid, smem, st, a)
-                            : launch(values_tc_kernel<false>, grid, smem, st, a);
+    e = a.span >= s.max_ctx ? launch<1>(ctx, values_tc_kernel<true>, grid, smem, st, a)
+                            : launch<2>(ctx, values_tc_kernel<false>, grid, smem, st, a);
   const cudaError_t f = cudaFreeAsync(a.planes, st);
   return e == cudaSuccess ? f : e;
 }
