@@ -22,10 +22,10 @@
 //
 // What bounds them (packed prompts of 2,048, 700 behind 1,024 and one token, 16
 // / 4 heads of 128; 49 M scores): a step's MMAs alone take 1,210 cycles, 211 us
-// in all, with the clock near 1.65 - 1.8 GHz under them.  The scores take 488 us
-// (2.8 TB/s): their epilogue moves 24 bytes a score beside MMAs that use most of
+// in all, with the clock near 1.65 - 1.8 GHz under them.  The scores take 493 us
+// (2.7 TB/s): their epilogue moves 24 bytes a score beside MMAs that use most of
 // the shared memory's bandwidth, and a tile's epilogue is slower than its MMAs.
-// The values take 428 us: 1,580 cycles a step, the tensor core sharing shared
+// The values take 436 us: 1,580 - 1,600 cycles a step, the tensor core sharing shared
 // memory with the splitting of the shares.  On the integer pipes the two took
 // 5,030 and 5,293 us.
 #include <atomic>
