@@ -312,6 +312,10 @@ class AttnLayout:
             rows = [list(r) for r in block_table]
             wide = np.zeros((len(rows), max([len(r) for r in rows] + [1])), dtype=np.int32)
             for i, r in enumerate(rows):
+                if i < q.size and len(r) * page_size < L[i]:
+                    raise ValueError("layout: a sequence is longer than its pages")
+                if any(not 0 <= pg < 2**31 for pg in r):
+                    raise ValueError("layout: pages are numbers from 0 on")
                 wide[i, :len(r)] = r
             block_table = torch.from_numpy(wide).to(dev)
         if block_table.dim() != 2:

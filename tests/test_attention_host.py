@@ -311,3 +311,13 @@ def test_mma_order_covers_every_limb_pair_once():
     assert seen == {(i, j): 1 for i in range(8) for j in range(8) if i + j <= 7}
     assert [c[2] for c in calls[:2]] == ["accumulate"] * 2 and {c[2] for c in calls[2:]} == {"1u"}
     assert [(c[0], c[1]) for c in calls[:2]] == [(0, 0), (0, 4)]
+
+
+def test_layout_refuses_lists_shorter_than_their_sequences():
+    """A sequence whose own list of pages is too short is refused, although
+    another sequence's list is long enough to widen the table."""
+    from suf_b200 import attention as at
+
+    for pages in ([[1], [2, 3]], [[], [2]], [[1, 2], [3, 2**31]], [[1, -1], [3]]):
+        with pytest.raises(ValueError, match="pages"):
+            at.AttnLayout(_Ctx, [1, 1], [20, 10], pages, 16, 4, 2)
