@@ -314,8 +314,8 @@ Rows rows_of(const AttnSeqs& s) {
 int check_seqs(const sufb200_attn_seqs* s, const char* who) {
   const std::string at = std::string(who) + ": ";
   if (!s) return fail(SUFB200_ERR_INVALID, at + "null sequences");
-  if (s->batch < 0 || s->max_pages < 0 || s->pages < 0 || s->min_q < 0 || s->max_q < s->min_q || s->max_ctx < 0 || s->tokens < 0 || s->cached < 0 ||
-      s->packed < 0)
+  if (s->batch < 0 || s->max_pages < 0 || s->pages < 0 || s->min_q < 0 || s->max_q < s->min_q || s->max_ctx < 0 ||
+      s->tokens < 0 || s->cached < 0 || s->packed < 0)
     return fail(SUFB200_ERR_INVALID, at + "negative size");
   if (s->page_size < 1 || s->kv_heads < 1 || s->q_heads < s->kv_heads || s->q_heads % s->kv_heads)
     return fail(SUFB200_ERR_INVALID, at + "page size, or query heads not a multiple of key heads");
@@ -326,7 +326,7 @@ int check_seqs(const sufb200_attn_seqs* s, const char* who) {
   if (static_cast<int64_t>(s->q_heads / s->kv_heads) * s->max_q > 1 << 20)
     return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^20 rows per (sequence, key head)");
   // grids count row tiles x key heads x 128-word tiles of the head
-  const int64_t tiles = s->tokens / SUFB200_ATTN_ROW_TILE * (s->q_heads / s->kv_heads + 1) + s->n_tiles + s->batch;
+  const int64_t tiles = s->q_heads / s->kv_heads * s->tokens / SUFB200_ATTN_ROW_TILE + s->n_tiles + s->batch;
   if (s->tokens > INT32_MAX || s->cached > INT32_MAX || tiles > INT32_MAX / 2 / s->kv_heads)
     return fail(SUFB200_ERR_UNSUPPORTED, at + "too many tokens for one call");
   if (s->max_ctx > 1 << 26) return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^26 cached tokens in a sequence");
@@ -334,7 +334,8 @@ int check_seqs(const sufb200_attn_seqs* s, const char* who) {
     return fail(SUFB200_ERR_INVALID, at + "max_ctx is more than the block table's pages hold");
   if (static_cast<__int128>(s->q_heads) * s->max_q * s->max_ctx >= (static_cast<__int128>(1) << 60))
     return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^60 packed words");
-  if (s->n_tiles < 0 || (s->n_tiles > 0 && !s->d_tiles)) return fail(SUFB200_ERR_INVALID, at + "null tile list");
+  if (s->n_tiles < 0 || (s->n_tiles > 0) != (s->d_tiles != nullptr))
+    return fail(SUFB200_ERR_INVALID, at + "null or empty tile list");
   if (s->batch > 0 && (!s->d_cu_q || !s->d_cu_ctx || !s->d_row_base || (s->max_ctx > 0 && !s->d_block_table)))
     return fail(SUFB200_ERR_INVALID, at + "null sequence array");
   return SUFB200_OK;

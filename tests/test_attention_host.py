@@ -321,3 +321,25 @@ def test_layout_refuses_lists_shorter_than_their_sequences():
     for pages in ([[1], [2, 3]], [[], [2]], [[1, 2], [3, 2**31]], [[1, -1], [3]]):
         with pytest.raises(ValueError, match="pages"):
             at.AttnLayout(_Ctx, [1, 1], [20, 10], pages, 16, 4, 2)
+
+
+@pytest.mark.parametrize("which", ["scores", "values"])
+def test_an_empty_tile_list_is_refused(host, which):
+    """A list without entries would be a launch without blocks."""
+    from suf_b200 import _lib
+
+    assert _attn(host, which, _seqs(**PTRS, d_tiles=P16, n_tiles=0)) == _lib.ERR_INVALID
+    assert _attn(host, which, _seqs(**PTRS, d_tiles=P16, n_tiles=1)) == _lib.ERR_UNSUPPORTED
+    assert b"host-only" in _lib.lib().sufb200_last_error()
+
+
+@pytest.mark.parametrize("which", ["scores", "values"])
+def test_grids_past_31_bits_are_refused(host, which):
+    """Few tokens of very many heads: row tiles times key heads count the grid."""
+    from suf_b200 import _lib
+
+    wide = dict(batch=1, tokens=63, max_q=1, min_q=1, kv_heads=2**15)
+    assert _attn(host, which, _seqs(**PTRS, **{**wide, "q_heads": 2**20})) == _lib.ERR_UNSUPPORTED
+    assert b"host-only" in _lib.lib().sufb200_last_error()
+    assert _attn(host, which, _seqs(**PTRS, **{**wide, "q_heads": 2**31 - 2**15})) == _lib.ERR_UNSUPPORTED
+    assert b"too many" in _lib.lib().sufb200_last_error()
