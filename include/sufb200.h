@@ -722,7 +722,8 @@ int sufb200_beaver_open_pair(const uint64_t* const* d_x, size_t sx, int ldx, con
  *
  * Wrong device-side data (a slot, position, page or length outside what the
  * host arguments say) is skipped and reported by sufb200_ctx_sync as a bad
- * argument; the outputs it concerns are then undefined. */
+ * argument; the outputs it concerns are then undefined.  Outputs overlap no
+ * input of their call. */
 
 /* New tokens into the cache.  Per token t and head h, with the cosines c and
  * sines s of its position (tables [max_pos][rot_dim / 2], f = the bundle's
@@ -811,8 +812,9 @@ int sufb200_attn_values_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
 /* The row-max tournament of nn::RowMaxDiffTask over packed rows of any
  * lengths (sufb200_relu_open_pair / _update_pair are its dense form): row r of
  * round k has off_k[r+1] - off_k[r] values, w -> ceil(w / 2) a round, its pairs
- * (2j, 2j + 1) packed from word off_k[r] - off_{k+1}[r]; max_width bounds the
- * round's widths; offsets are device [rows + 1].
+ * (2j, 2j + 1) packed from word off_k[r] - off_{k+1}[r]; max_width (at most
+ * 2^30) bounds the round's widths; offsets are device [rows + 1] and are taken
+ * as they are: they have to lie within the arrays.
  * rowmax_open_pair: x^ = sum_p (c_p[2j] - c_p[2j+1] + r[p]) of the first round.
  * rowmax_round_pair: from c (offsets off) and the gate's shares relu_p of its
  * pairs, next_p (offsets off1) = c_p[2j+1] + relu_p[j], an odd row's last value

@@ -15,8 +15,8 @@ needs a freshly dealt mask.  The reference keeps its cache as share tensors
 All tensors live on the context's device; shares and opened words are int64
 tensors (the words of Z_2^64).  Calls are asynchronous on `stream` (default:
 the device's current stream); what they are given has to stay allocated until
-that stream has passed them.  Wrong device-side data (slots, positions, pages)
-is reported by Context.sync.
+that stream has passed them, and outputs overlap no input.  Wrong device-side
+data (slots, positions, pages) is reported by Context.sync.
 """
 from __future__ import annotations
 
@@ -108,7 +108,7 @@ def _pair(ctx: Context, name: str, ts, shape: tuple):
 def _masks(r):
     if len(r) != 2:
         raise ValueError("r: expected both parties' shares of the mask")
-    return _TwoWords(r[0] & M64, r[1] & M64)
+    return _TwoWords(int(r[0]) & M64, int(r[1]) & M64)
 
 
 # -- rotary tables --------------------------------------------------------------
@@ -422,8 +422,8 @@ class RowMaxPlan:
     def __init__(self, ctx: Context, row_lengths):
         dev = torch.device("cuda", ctx.device)
         w = np.asarray(row_lengths, dtype=np.int64).reshape(-1)
-        if (w < 0).any() or int(w.sum()) >= 2**31:
-            raise ValueError("rowmax: row lengths must be non-negative, below 2^31 words in all")
+        if (w < 0).any() or int(w.max(initial=0)) > 2**30 or int(w.sum()) >= 2**31:
+            raise ValueError("rowmax: row lengths must be 0..2^30, below 2^31 words in all")
         self.rows = int(w.size)
         self.off, self.values, self.pairs, self.widths = [], [], [], []
         while True:

@@ -116,6 +116,14 @@ Shape shape_for(const sufb200_ctx_s* ctx, int rows, int width) {
   return s;
 }
 
+// Rows stop at 2^30 words: places are 32 bits wide and a row's threads step past
+// its end by up to four strides of the grid (at most 16 blocks of kThreads an SM: below 2^20).
+int check_rows(int rows, int max_width, const char* who) {
+  if (rows < 0 || max_width < 0) return fail(SUFB200_ERR_INVALID, std::string(who) + ": negative size");
+  if (max_width > 1 << 30) return fail(SUFB200_ERR_UNSUPPORTED, std::string(who) + ": rows of more than 2^30 words");
+  return SUFB200_OK;
+}
+
 int check_words(std::initializer_list<const void*> ps, const char* who) {
   for (const void* p : ps)
     if (!p || !aligned_to(p, 8)) return fail(SUFB200_ERR_INVALID, std::string(who) + ": null or misaligned device pointer");
@@ -138,7 +146,7 @@ extern "C" {
 int sufb200_rowmax_open_pair(sufb200_ctx ctx, const uint64_t* const* d_c, int rows, int max_width,
                              const int32_t* d_off, const int32_t* d_off1, const uint64_t* r, uint64_t* d_xhat,
                              void* stream) {
-  if (rows < 0 || max_width < 0) return fail(SUFB200_ERR_INVALID, "rowmax_open_pair: negative size");
+  if (int rc = check_rows(rows, max_width, "rowmax_open_pair")) return rc;
   if (rows == 0 || max_width < 2) return SUFB200_OK;
   if (!d_c || !r || !d_off || !d_off1) return fail(SUFB200_ERR_INVALID, "rowmax_open_pair: null argument");
   if (int rc = check_words({d_c[0], d_c[1], d_xhat}, "rowmax_open_pair")) return rc;
@@ -152,7 +160,7 @@ int sufb200_rowmax_open_pair(sufb200_ctx ctx, const uint64_t* const* d_c, int ro
 int sufb200_rowmax_round_pair(sufb200_ctx ctx, const uint64_t* const* d_c, const uint64_t* const* d_relu, int rows,
                               int max_width, const int32_t* d_off, const int32_t* d_off1, const int32_t* d_off2,
                               const uint64_t* r, uint64_t* const* d_next, uint64_t* d_xhat, void* stream) {
-  if (rows < 0 || max_width < 0) return fail(SUFB200_ERR_INVALID, "rowmax_round_pair: negative size");
+  if (int rc = check_rows(rows, max_width, "rowmax_round_pair")) return rc;
   if (rows == 0 || max_width == 0) return SUFB200_OK;
   if (!d_c || !d_relu || !d_off || !d_off1 || !d_next) return fail(SUFB200_ERR_INVALID, "rowmax_round_pair: null argument");
   if (int rc = check_words({d_c[0], d_c[1], d_next[0], d_next[1]}, "rowmax_round_pair")) return rc;
@@ -171,7 +179,7 @@ int sufb200_rowmax_round_pair(sufb200_ctx ctx, const uint64_t* const* d_c, const
 int sufb200_maxdiff_ragged_pair(sufb200_ctx ctx, const uint64_t* const* d_max, const uint64_t* const* d_s, int rows,
                                 int max_width, const int32_t* d_off, const int32_t* d_max_off, uint64_t* const* d_t,
                                 void* stream) {
-  if (rows < 0 || max_width < 0) return fail(SUFB200_ERR_INVALID, "maxdiff_ragged_pair: negative size");
+  if (int rc = check_rows(rows, max_width, "maxdiff_ragged_pair")) return rc;
   if (rows == 0 || max_width == 0) return SUFB200_OK;
   if (!d_max || !d_s || !d_t || !d_off || !d_max_off) return fail(SUFB200_ERR_INVALID, "maxdiff_ragged_pair: null argument");
   if (int rc = check_words({d_max[0], d_max[1], d_s[0], d_s[1], d_t[0], d_t[1]}, "maxdiff_ragged_pair")) return rc;

@@ -343,3 +343,22 @@ def test_grids_past_31_bits_are_refused(host, which):
     assert b"host-only" in _lib.lib().sufb200_last_error()
     assert _attn(host, which, _seqs(**PTRS, **{**wide, "q_heads": 2**31 - 2**15})) == _lib.ERR_UNSUPPORTED
     assert b"too many" in _lib.lib().sufb200_last_error()
+
+
+def test_rowmax_refuses_rows_whose_steps_pass_32_bits(host):
+    """Threads step through a row by up to 2^22 words past its end in 32-bit
+    places: rows stop at 2^30 words."""
+    from suf_b200 import _lib
+    from suf_b200 import attention as at
+
+    L, r, g = _lib.lib(), (C.c_uint64 * 2)(1, 2), _arr(P16, P16)
+    for w, said in [(2**30, b"host-only"), (2**30 + 1, b"2^30")]:
+        assert L.sufb200_rowmax_open_pair(host, g, 1, w, P16, P16, r, P16, None) == _lib.ERR_UNSUPPORTED
+        assert said in L.sufb200_last_error()
+        assert L.sufb200_rowmax_round_pair(host, g, g, 1, w, P16, P16, P16, r, g, P16, None) == _lib.ERR_UNSUPPORTED
+        assert said in L.sufb200_last_error()
+        assert L.sufb200_maxdiff_ragged_pair(host, g, g, 1, w, P16, P16, g, None) == _lib.ERR_UNSUPPORTED
+        assert said in L.sufb200_last_error()
+    for lens in ([2**30 + 1], [3, -1], [2**30, 2**30]):
+        with pytest.raises(ValueError, match="row lengths"):
+            at.RowMaxPlan(_Ctx, lens)
