@@ -29,9 +29,9 @@ constexpr int kThreads = 256;
 
 // Rows of a (sequence, key head) up to which the row kernels are used; above,
 // the tensor cores (whose pre-pass reads the cache once and writes its planes).
-// Four sequences of 8,192 tokens, 32 / 8 heads of 128, row kernels against
-// tensor cores: scores of 8 rows 238 and 407 us, 16 rows 455 and 419 us; values
-// of 8 rows 291 and 346 us, 16 rows 568 and 354 us.
+// Four sequences of 8,192 tokens, 32 / 8 heads of 128, row kernels (16 rows in two
+// passes over the cache) against tensor cores: scores of 8 rows 238 and 407 us, 16
+// rows 455 and 419 us; values of 8 rows 291 and 346 us, 16 rows 568 and 354 us.
 constexpr int kFewRows = SUFB200_ATTN_FEW_ROWS;
 
 int fail(int code, const std::string& msg) { return record_error(code, msg); }
@@ -41,10 +41,44 @@ int fail(int code, const std::string& msg) { return record_error(code, msg); }
 // D + A_0 + A_1 and D sit in shared memory and are read once for two keys.  Up
 // to four rows the multiplies (two per word and row, three integer
 // instructions each) stay below the memory's time.  One decode step over
-// 73,279 cached tokens, 32 / 8 heads of 128: 341 us cold, 5.4 TB/s of 6.5; what
+// 73,279 cached tokens, 32 / 8 heads of 128: 350 us cold, 5.3 TB/s of 6.5; what
 // is left is waiting on memory with 32 warps an SM (long_scoreboard 11 per
 // issue, DRAM 83 %).
 constexpr int kKeyChunk = 256;  // most keys per CTA
+
+// The run of `per` cached tokens that this block has, of which sequence and key
+// head; false: none, or the sequence has more rows than the row kernels take.
+// Runs are listed sequence after sequence, so that short caches beside a long
+// one leave no idle blocks (200 caches of 50 - 400 tokens beside one of 40,000,
+// 32 / 8 heads of 128: scores 438 us, 883 by a grid of every sequence's longest
+// possible cache), and by key heads within a run, whose rows of a page lie one
+// behind the other (eight rows, 73,279 tokens: 467 us, 541 with the heads outside).
+// Where one run holds any cache (ONE, or by the lengths) a block is a sequence.
+template <bool ONE>
+__device__ __forceinline__ bool run_of(const AttnSeqs& s, int per, uint32_t* status, int& b, int& kh, int& beg,
+                                       SeqInfo& q) {
+  const unsigned g = blockIdx.x / static_cast<unsigned>(s.kv_heads);
+  kh = static_cast<int>(blockIdx.x - g * s.kv_heads);
+  beg = 0;
+  if (ONE || s.max_ctx <= per) {
+    b = static_cast<int>(g);
+    if (!seq_info(s, b, status, q)) return false;
+  } else {
+    // every sequence is looked at, also where wrong lengths hide it from the search
+    if (g < static_cast<unsigned>(s.batch) && kh == 0) seq_info(s, static_cast<int>(g), status, q);
+    b = block_seq(s.d_cu_ctx, s.batch, 1, per, g);
+    if (!seq_info(s, b, status, q)) return false;
+    const int64_t first = g - first_block(q.l0, b, per);
+    if (first < 0 || first * per >= q.L) return false;
+    beg = static_cast<int>(first) * per;
+  }
+  return q.n > 0 && s.q_heads / s.kv_heads * q.n <= kFewRows;
+}
+
+dim3 runs_grid(const AttnSeqs& s, int per) {
+  const int64_t runs = s.max_ctx <= per ? s.batch : blocks_of(s.cached, s.batch, per);
+  return dim3(static_cast<unsigned>(runs * s.kv_heads));
+}
 
 template <int RT>
 __global__ void __launch_bounds__(kThreads, RT == 4 ? 4 : 3) scores_rows_kernel(const __grid_constant__ AttnSeqs s,
@@ -52,20 +86,16 @@ __global__ void __launch_bounds__(kThreads, RT == 4 ? 4 : 3) scores_rows_kernel(
                                                                                 int chunk) {
   extern __shared__ __align__(16) uint64_t sm[];
   const int t = threadIdx.x, dh = s.head_dim, group = s.q_heads / s.kv_heads;
-  const int b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads;
+  int b, kh, k0;
   SeqInfo q;
-  if (!seq_info(s, b, o.status, q)) return;
-  const int R = group * q.n, rho0 = blockIdx.y * RT, k0 = blockIdx.x * chunk;
-  if (rho0 >= R || R > kFewRows) return;
-  const int last = (rho0 + RT < R ? rho0 + RT : R) - 1;
-  const int len = row_len(q.n, q.L, s.causal, last / group);  // the longest row of the tile
-  if (k0 >= len) return;
+  if (!run_of<false>(s, chunk, o.status, b, kh, k0, q)) return;
+  const int R = group * q.n, len = q.L;  // the last row has every key
   uint64_t* sU = sm;                    // [RT][dh]
   uint64_t* sD = sU + RT * dh;          // [RT][dh]
   uint64_t* s_out = sD + RT * dh;       // [RT][chunk + 1]
   int64_t* s_key = reinterpret_cast<int64_t*>(s_out + RT * (chunk + 1));  // [chunk]
   for (int e = t; e < RT * dh; e += kThreads) {
-    const int rr = e / dh, c = e % dh, rho = rho0 + rr;
+    const int rho = e / dh, c = e % dh;
     uint64_t d = 0, u = 0;
     if (rho < R) {
       const int64_t at = (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + c;
@@ -124,10 +154,10 @@ __global__ void __launch_bounds__(kThreads, RT == 4 ? 4 : 3) scores_rows_kernel(
   }
   __syncthreads();
   for (int e = t; e < RT * chunk; e += kThreads) {
-    const int rr = e / chunk, kk = e % chunk, rho = rho0 + rr, i = rho / group;
+    const int rho = e / chunk, kk = e % chunk, i = rho / group;
     if (rho >= R || k0 + kk >= row_len(q.n, q.L, s.causal, i)) continue;
     const int64_t at = q.base + (kh * group + rho % group) * q.blk + row_off(q.n, q.L, s.causal, i) + k0 + kk;
-    o.out[at] = s_out[rr * (chunk + 1) + kk] + o.c[0][at] + o.c[1][at] + o.r;
+    o.out[at] = s_out[rho * (chunk + 1) + kk] + o.c[0][at] + o.c[1][at] + o.r;
   }
 }
 
@@ -147,33 +177,29 @@ __global__ void values_init_kernel(const __grid_constant__ AttnSeqs s, const __g
 // values_rows: a thread holds two words of the head for RT rows; the CTA's
 // key lanes walk its range of keys, whose probabilities sit in shared memory.
 // Ranges of one row meet by 64-bit atomic adds: sums mod 2^64 do not depend
-// on their order.  The same decode step: 332 us cold, 5.7 TB/s.  (Two and four
+// on their order.  The same decode step: 351 us cold, 5.3 TB/s.  (Two and four
 // keys a thread at a time, for more loads in flight: 387 us, for fewer warps.)
 constexpr int kValStage = 64;
 
 // SOLO: one CTA has every key of its rows and stores whole results.
 template <int RT, bool SOLO>
-__global__ void __launch_bounds__(kThreads) values_rows_kernel(const __grid_constant__ AttnSeqs s,
-                                                               const __grid_constant__ AttnOperands o, int range) {
+__global__ void __launch_bounds__(kThreads, RT == 4 ? 4 : 3) values_rows_kernel(const __grid_constant__ AttnSeqs s,
+                                                                                const __grid_constant__ AttnOperands o,
+                                                                                int range) {
   __shared__ __align__(16) uint64_t sU[kValStage][RT], sD[kValStage][RT];
   __shared__ ulonglong2 s_sum[SOLO ? kThreads : 1];
   __shared__ int64_t s_key[kValStage];
   const int t = threadIdx.x, dh = s.head_dim, group = s.q_heads / s.kv_heads, P = dh / 2;
-  const int b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads;
+  int b, kh, beg;
   SeqInfo q;
-  if (!seq_info(s, b, o.status, q)) return;
-  const int R = group * q.n, rho0 = blockIdx.y * RT;
-  if (rho0 >= R || R > kFewRows) return;
-  const int last = (rho0 + RT < R ? rho0 + RT : R) - 1;
-  const int len = row_len(q.n, q.L, s.causal, last / group);
-  const int beg = blockIdx.x * range, end = beg + range < len ? beg + range : len;
-  if (!SOLO && beg >= end) return;
+  if (!run_of<SOLO>(s, range, o.status, b, kh, beg, q)) return;
+  const int R = group * q.n, len = q.L, end = range < len - beg ? beg + range : len;
   const int lanes = kThreads / P, kl = t / P, c = t % P;
   uint64_t ax[RT] = {}, ay[RT] = {};
   for (int j0 = beg; j0 < end; j0 += kValStage) {
     __syncthreads();
     for (int e = t; e < kValStage * RT; e += kThreads) {
-      const int kk = e % kValStage, rr = e / kValStage, rho = rho0 + rr, i = rho / group, j = j0 + kk;
+      const int kk = e % kValStage, rho = e / kValStage, i = rho / group, j = j0 + kk;
       uint64_t d = 0, u = 0;
       if (rho < R && j < end && j < row_len(q.n, q.L, s.causal, i)) {
         const int64_t at = q.base + (kh * group + rho % group) * q.blk + row_off(q.n, q.L, s.causal, i) + j;
@@ -181,8 +207,8 @@ __global__ void __launch_bounds__(kThreads) values_rows_kernel(const __grid_cons
         d = (o.x[0][at] - a0) + (o.x[1][at] - a1);
         u = d + a0 + a1;
       }
-      sU[kk][rr] = u;
-      sD[kk][rr] = d;
+      sU[kk][rho] = u;
+      sD[kk][rho] = d;
     }
     for (int e = t; e < kValStage; e += kThreads) s_key[e] = j0 + e < end ? key_off(s, b, kh, j0 + e, o.status) : -1;
     __syncthreads();
@@ -202,13 +228,12 @@ __global__ void __launch_bounds__(kThreads) values_rows_kernel(const __grid_cons
       }
   }
 #pragma unroll
-  for (int rr = 0; rr < RT; rr++) {
-    const int rho = rho0 + rr;
+  for (int rho = 0; rho < RT; rho++) {
     if (rho >= R) break;
     const int64_t at = (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + 2 * c;
     if (SOLO) {
       __syncthreads();
-      s_sum[t] = make_ulonglong2(ax[rr], ay[rr]);
+      s_sum[t] = make_ulonglong2(ax[rho], ay[rho]);
       __syncthreads();
       if (kl > 0) continue;
       uint64_t x = o.c[0][at] + o.c[1][at] + o.r, y = o.c[0][at + 1] + o.c[1][at + 1] + o.r;
@@ -220,8 +245,8 @@ __global__ void __launch_bounds__(kThreads) values_rows_kernel(const __grid_cons
       o.out[at + 1] = y;
     } else if (kl < lanes) {
       unsigned long long* to = reinterpret_cast<unsigned long long*>(o.out + at);
-      atomicAdd(to, static_cast<unsigned long long>(ax[rr]));
-      atomicAdd(to + 1, static_cast<unsigned long long>(ay[rr]));
+      atomicAdd(to, static_cast<unsigned long long>(ax[rho]));
+      atomicAdd(to + 1, static_cast<unsigned long long>(ay[rho]));
     }
   }
 }
@@ -327,7 +352,8 @@ int check_seqs(const sufb200_attn_seqs* s, const char* who) {
     return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^20 rows per (sequence, key head)");
   // grids count row tiles x key heads x 128-word tiles of the head
   const int64_t tiles = s->q_heads / s->kv_heads * s->tokens / SUFB200_ATTN_ROW_TILE + s->n_tiles + s->batch;
-  if (s->tokens > INT32_MAX || s->cached > INT32_MAX || tiles > INT32_MAX / 2 / s->kv_heads)
+  const int64_t runs = blocks_of(s->cached, s->batch, kValStage);  // the row kernels' shortest runs
+  if (s->tokens > INT32_MAX || s->cached > INT32_MAX || tiles > INT32_MAX / 2 / s->kv_heads || runs > INT32_MAX / s->kv_heads)
     return fail(SUFB200_ERR_UNSUPPORTED, at + "too many tokens for one call");
   if (s->max_ctx > 1 << 26) return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^26 cached tokens in a sequence");
   if (static_cast<int64_t>(s->max_ctx) > static_cast<int64_t>(s->max_pages) * s->page_size)
@@ -357,10 +383,13 @@ constexpr int kSoloKeys = 256;
 
 // Keys a CTA of the row kernels walks: the longest run (least, doubled up to
 // most) that still leaves `per_sm` CTAs per SM.  A long run pays its set-up
-// once, a short cache wants every SM.  One step over 73,279 cached tokens of
-// 8 x 128 words: scores 332 us in runs of 256 (eight CTAs per SM asked for),
-// 348 us in runs of 128; values 315 us in runs of 1,024 (three asked for),
-// 322 of 512, 331 of 256.
+// once, a short cache wants every SM, and many short runs end more evenly.  One
+// step over 73,279 cached tokens of 8 x 128 words: scores 328 us in runs of 256
+// (eight CTAs per SM asked for), 333 of 128, with eight rows 467 and 483 us;
+// values 321 us in runs of 512 (three asked for), 322 of 1,024, 325 of 256, with
+// eight rows 544, 667 (two uneven waves) and 531 us.  200 caches of 50 - 400
+// tokens beside one of 40,000: scores 438 us of 256, 409 of 128, 539 of 512;
+// values 402 of 512, 396 of 256, 528 of 2,048.
 int keys_per_cta(const sufb200_ctx_s* ctx, const AttnSeqs& s, int least, int most, int per_sm) {
   const int64_t keys = s.cached * s.kv_heads, ctas = static_cast<int64_t>(ctx->sm_count) * per_sm;
   int run = least;
@@ -402,7 +431,7 @@ int sufb200_attn_scores_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
     // rows of 8 x 256 words and 256 keys would pass 48 KB of shared memory
     const int chunk = keys_per_cta(ctx, *seqs, 64, rt * seqs->head_dim > 1024 ? kKeyChunk / 2 : kKeyChunk, 8);
     const size_t smem = sizeof(uint64_t) * (2 * rt * seqs->head_dim + rt * (chunk + 1) + chunk);
-    const dim3 grid((seqs->max_ctx + chunk - 1) / chunk, 1, z);
+    const dim3 grid = runs_grid(*seqs, chunk);
     if (rt == 4)
       scores_rows_kernel<4><<<grid, kThreads, smem, st>>>(*seqs, o, chunk);
     else
@@ -437,7 +466,6 @@ int sufb200_attn_values_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
   o.status = ctx->d_status;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const Rows rows = rows_of(*seqs);
-  const unsigned z = static_cast<unsigned>(seqs->batch) * seqs->kv_heads;
   const bool any = seqs->packed > 0 && seqs->max_ctx > 0;
   const bool few_solo = seqs->max_ctx <= kSoloKeys, many_solo = rows.most > kFewRows && values_tc_solo(ctx, *seqs);
   if (!any || (rows.few > 0 && !few_solo) || (rows.most > kFewRows && !many_solo)) {
@@ -446,8 +474,8 @@ int sufb200_attn_values_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
     values_init_kernel<<<static_cast<unsigned>(want < cap ? want : cap), kThreads, 0, st>>>(*seqs, o);
   }
   if (any && rows.few > 0) {
-    const int range = few_solo ? kSoloKeys : keys_per_cta(ctx, *seqs, kValStage, 1024, 3);
-    const dim3 grid((seqs->max_ctx + range - 1) / range, 1, z);
+    const int range = few_solo ? kSoloKeys : keys_per_cta(ctx, *seqs, kValStage, rows.few <= 4 ? 512 : 256, 3);
+    const dim3 grid = runs_grid(*seqs, range);
     const auto kernel = rows.few <= 4 ? (few_solo ? values_rows_kernel<4, true> : values_rows_kernel<4, false>)
                                       : (few_solo ? values_rows_kernel<8, true> : values_rows_kernel<8, false>);
     kernel<<<grid, kThreads, 0, st>>>(*seqs, o, range);

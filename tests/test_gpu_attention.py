@@ -613,3 +613,51 @@ def test_pages_past_32_bit_offsets(ctx, torch_cuda):
         assert (from_dev(got) == want).all()
     del pool
     torch.cuda.empty_cache()
+
+
+def _many_sequences(prompts):
+    """A batch whose search for a block's sequence takes several steps: empty
+    caches, runs of every length, one long cache, with `prompts` whole prompts
+    between the single tokens."""
+    rng = np.random.default_rng(31)
+    seqs = [(1, int(L)) for L in rng.choice([0, 1, 2, 31, 63, 64, 65, 127, 200, 257], 1100)]
+    seqs[700] = (1, 1500)
+    seqs[3] = seqs[40] = (0, 90)
+    if prompts:
+        for i in (0, 33, 500, 1099):
+            seqs[i] = (12, 80 + i % 7)
+    return (seqs, 2, 1, 6, 16, True)
+
+
+@pytest.mark.parametrize("which", ["scores", "values"])
+@pytest.mark.parametrize("prompts", [False, True])
+def test_many_sequences_match_definition(ctx, torch_cuda, which, prompts):
+    from suf_b200 import attention as at
+
+    A = _Attn(ctx, torch_cuda, _many_sequences(prompts), 33)
+    args, want = getattr(A, which)()
+    got = getattr(at, f"attn_{which}_pair")(ctx, *args)
+    ctx.sync()
+    assert (from_dev(got) == want).all()
+
+
+@pytest.mark.parametrize("which", ["scores", "values"])
+@pytest.mark.parametrize("case", [ATTN[3], ATTN[12], ATTN[14]])
+def test_attention_reports_bad_lengths(ctx, torch_cuda, which, case):
+    """Cached lengths that fall, or pass what the host was told: reported, also
+    where no block's search finds the sequence."""
+    from suf_b200 import SufB200Error
+    from suf_b200 import attention as at
+
+    A = _Attn(ctx, torch_cuda, case, 34)
+    args, want = getattr(A, which)()
+    call, good = getattr(at, f"attn_{which}_pair"), A.layout._ctx.clone()
+    for at_, bad in [(-1, 0), (1, -5), (1, 2**31 - 1), (-1, 2**31 - 1)]:
+        A.layout._ctx[at_] = bad
+        call(ctx, *args)
+        with pytest.raises(SufB200Error):
+            ctx.sync()
+        A.layout._ctx.copy_(good)
+    got = call(ctx, *args)
+    ctx.sync()
+    assert (from_dev(got) == want).all()
