@@ -95,6 +95,18 @@ __device__ __forceinline__ uint32_t turned_off(int r0, int h, int lane) {
   return core_off(r0 + 2 * (lane & 3) + (lane >> 4), h) + 4 * ((lane & 15) >> 2);
 }
 
+// Two words at p (16-byte aligned) where `in`, else 0.
+__device__ __forceinline__ void ld2_if(const uint64_t* p, bool in, uint64_t& x, uint64_t& y) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %3, 0;\n\t"
+      "mov.u64 %0, 0;\n\t"
+      "mov.u64 %1, 0;\n\t"
+      "@p ld.global.nc.v2.u64 {%0, %1}, [%2];\n\t}"
+      : "=&l"(x), "=&l"(y)
+      : "l"(p), "r"(static_cast<int>(in)));
+}
+
 // The cached operand's byte planes.  KEYS: block (128-key tile, chunk of 32
 // words), rows = keys; else block (32 keys, 128-word tile), rows = words of
 // the head.  Out-of-range rows and depths are zero.
@@ -114,22 +126,44 @@ __global__ void __launch_bounds__(256) cache_planes_kernel(const __grid_constant
   __syncthreads();
   const int64_t block = ((kh * a.tiles + blockIdx.x) * a.chunks + blockIdx.y) * 2;
   uint8_t* dst = a.planes + block * kAStage;
+  // two units of four words at a time: their loads before the first use
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int u = t + 256 * i, kq = u & 3, r = (u >> 2) & (kTM - 1), h = u >> 9;
-    uint64_t e[4], w[4];
+  for (int i = 0; i < 4; i += 2) {
+    uint64_t e[2][4], w[2][4], v[2][4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int deep = 16 * h + 4 * kq + j;
-      const int64_t at = s_key[KEYS ? r : deep];
-      const int word = KEYS ? static_cast<int>(blockIdx.y) * kTK + deep : static_cast<int>(blockIdx.y) * kTM + r;
-      const bool in = at >= 0 && word < s.head_dim;
-      e[j] = in ? a.o.e[at + word] : 0;
-      w[j] = in ? a.o.b[0][at + word] + a.o.b[1][at + word] : 0;
+    for (int y = 0; y < 2; y++) {
+      const int u = t + 256 * (i + y), deep = 16 * (u >> 9) + 4 * (u & 3), r = (u >> 2) & (kTM - 1);
+      if (KEYS) {  // four words of a key; the head's size is even
+        const int64_t at = s_key[r];
+        const int word = static_cast<int>(blockIdx.y) * kTK + deep;
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          const bool in = at >= 0 && word + j < s.head_dim;
+          ld2_if(a.o.e + at + word + j, in, e[y][j], e[y][j + 1]);
+          ld2_if(a.o.b[0] + at + word + j, in, w[y][j], w[y][j + 1]);
+          ld2_if(a.o.b[1] + at + word + j, in, v[y][j], v[y][j + 1]);
+        }
+      } else {  // a word of four keys
+        const int word = static_cast<int>(blockIdx.y) * kTM + r;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int64_t at = s_key[deep + j];
+          const bool in = at >= 0 && word < s.head_dim;
+          e[y][j] = ld_if(a.o.e + at + word, in);
+          w[y][j] = ld_if(a.o.b[0] + at + word, in);
+          v[y][j] = ld_if(a.o.b[1] + at + word, in);
+        }
+      }
     }
-    uint8_t* at = dst + core_off(r, h) + 4 * kq;
-    put4(at, kPlaneX, e);
-    put4(at + kAStage, kPlaneX, w);
+#pragma unroll
+    for (int y = 0; y < 2; y++) {
+      const int u = t + 256 * (i + y);
+      uint8_t* at = dst + core_off((u >> 2) & (kTM - 1), u >> 9) + 4 * (u & 3);
+#pragma unroll
+      for (int j = 0; j < 4; j++) w[y][j] += v[y][j];
+      put4(at, kPlaneX, e[y]);
+      put4(at + kAStage, kPlaneX, w[y]);
+    }
   }
 }
 
@@ -272,7 +306,7 @@ __device__ __forceinline__ void fold16(int quarter, int col, uint64_t (&z)[16]) 
 // is short: it runs dry whenever the issuing warp is held up for longer than
 // the last MMAs it was given take, and a wait for the next step's planes holds
 // it up by about 200 cycles even when they are there.  So a step is issued in
-// two parts, the small MMAs in the first and four of the widest last, and the
+// two parts, 416 cycles of MMAs in the last, and the
 // next step's wait stands between them (a step took 0.90 us with the wait in
 // front, 0.63 us of it MMAs).  For the same reason accumulators, shapes and the
 // descriptors' high words are constants; only two 32-bit bases vary.
@@ -292,19 +326,19 @@ __device__ __forceinline__ void issue_first(uint32_t a, uint32_t b, uint32_t acc
   issue_one(al, bl, 0, 0, accumulate);  // these two write all 512 columns
   issue_one(al, bl, 0, 4, accumulate);
   issue_one(al, bl, 7, 0, 1u);
-  issue_one(al, bl, 3, 4, 1u);
   issue_one(al, bl, 6, 0, 1u);
-  issue_one(al, bl, 2, 4, 1u);
   issue_one(al, bl, 5, 0, 1u);
-  issue_one(al, bl, 1, 4, 1u);
+  issue_one(al, bl, 4, 0, 1u);
+  issue_one(al, bl, 3, 4, 1u);
+  issue_one(al, bl, 3, 0, 1u);
 }
 
 __device__ __forceinline__ void issue_last(uint32_t a, uint32_t b) {
   const uint32_t al = desc_base(a), bl = desc_base(b);
-  issue_one(al, bl, 1, 0, 1u);
+  issue_one(al, bl, 2, 4, 1u);
   issue_one(al, bl, 2, 0, 1u);
-  issue_one(al, bl, 3, 0, 1u);
-  issue_one(al, bl, 4, 0, 1u);
+  issue_one(al, bl, 1, 4, 1u);
+  issue_one(al, bl, 1, 0, 1u);
 }
 
 // Row tile `tile` of the call: its sequence and its first row, rho0 = -1 when
@@ -360,9 +394,8 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
   const uint32_t sbase = smem_u32(smem);
   const Ctrl c = ctrl_at(smem, kBOff + static_cast<uint32_t>(steps) * kBStage);
   if (t < kTN) {
-    const int rho = rho0 + t, i = rho / group;
-    c.row[t] = rho < R ? q.base + (kh * group + rho % group) * q.blk + row_off(q.n, q.L, s.causal, i) : 0;
-    c.len[t] = rho < R ? row_len(q.n, q.L, s.causal, i) : 0;
+    const int rho = rho0 + t;
+    c.row[t] = rho < R ? (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh : -1;
   }
   const bool ready = start(c, warp, t, kThreads / 32 - 2);
   int copies = 0;
@@ -411,26 +444,35 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
     }
     if (!go && lane == 0) *c.err = 1;
   } else {
-    // the rows' planes [U | D]
-    for (int u = warp - 2; u < a.chunks * (kTN / 4); u += kThreads / 32 - 2) {
-      const int ch = u / (kTN / 4), h = u & 1, r0 = (u % (kTN / 4)) / 2 * 8, k = ch * kTK + 16 * h + (lane & 15);
-      uint64_t d[4], w[4], x[4];
+    // the rows' planes [U | D]: the loads of two units, then their splitting
+    const int units = a.chunks * (kTN / 4);
+    for (int u0 = warp - 2; u0 < units; u0 += 2 * (kThreads / 32 - 2)) {
+      uint64_t d[2][4], w[2][4], x[2][4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int rho = rho0 + r0 + 2 * j + (lane >> 4);
-        const bool in = rho < R && k < dh;
-        const int64_t at = (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + k;
-        d[j] = ld_if(o.x[0] + at, in);
-        w[j] = ld_if(o.a[0] + at, in);
-        x[j] = ld_if(o.a[1] + at, in);
+      for (int y = 0; y < 2; y++) {
+        const int u = u0 + y * (kThreads / 32 - 2), k = u / (kTN / 4) * kTK + 16 * (u & 1) + (lane & 15);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int64_t row = c.row[u % (kTN / 4) / 2 * 8 + 2 * j + (lane >> 4)];
+          const bool in = row >= 0 && u < units && k < dh;
+          d[y][j] = ld_if(o.x[0] + row + k, in);
+          w[y][j] = ld_if(o.a[0] + row + k, in);
+          x[y][j] = ld_if(o.a[1] + row + k, in);
+        }
       }
 #pragma unroll
-      for (int j = 0; j < 4; j++) w[j] += d[j] + x[j];
-      turn4(w, lane);
-      turn4(d, lane);
-      uint8_t* at = smem + kBOff + static_cast<uint32_t>(2 * ch) * kBStage + turned_off(r0, h, lane);
-      put4(at, kPlaneY, w);
-      put4(at + kBStage, kPlaneY, d);
+      for (int y = 0; y < 2; y++) {
+        const int u = u0 + y * (kThreads / 32 - 2);
+        if (u >= units) break;
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[y][j] += d[y][j] + x[y][j];
+        turn4(w[y], lane);
+        turn4(d[y], lane);
+        uint8_t* at = smem + kBOff + static_cast<uint32_t>(2 * (u / (kTN / 4))) * kBStage +
+                      turned_off(u % (kTN / 4) / 2 * 8, u & 1, lane);
+        put4(at, kPlaneY, w[y]);
+        put4(at + kBStage, kPlaneY, d[y]);
+      }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // generic writes -> tensor core reads
     __syncwarp();
@@ -630,37 +672,41 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
         mbar_arrive(c.bfull + 8 * sd);
       }
     }
+    const int quarter = warp & 3, col = ((warp - 4) >> 2) * 16;
+    const int word = word0 + quarter * 32 + lane, left = R - rho0 - col;  // rows there are from column 0 on
+    int g = (rho0 + col) % group;
+    int64_t at = left > 0 ? place(rho0 + col, word) : 0;
+    const auto next = [&] {  // the row after: the group's next head, or the next token's first
+      at += dh;
+      if (++g == group) {
+        g = 0;
+        at += static_cast<int64_t>(s.q_heads - group) * dh;
+      }
+    };
+    uint64_t c0[8], c1[8];
+    const auto fetch_c = [&](int x0) {  // C of eight rows; leaves the walk where it was
+      const int g1 = g;
+      const int64_t at1 = at;
+#pragma unroll
+      for (int x = 0; x < 8; x++) {
+        const bool in = x0 + x < left && word < dh;
+        c0[x] = ld_if(o.c[0] + at, in);
+        c1[x] = ld_if(o.c[1] + at, in);
+        next();
+      }
+      g = g1;
+      at = at1;
+    };
+    if (SOLO) fetch_c(0);  // while the last MMAs run
     if (lane == 0 && go) go = mbar_wait(c.tfull, 0);
     if (__shfl_sync(0xffffffffu, go, 0)) {
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int quarter = warp & 3, col = ((warp - 4) >> 2) * 16;
       uint64_t z[16];
       fold16(quarter, col, z);
-      const int word = word0 + quarter * 32 + lane, left = R - rho0 - col;  // rows there are from column 0 on
-      int g = (rho0 + col) % group;
-      int64_t at = left > 0 ? place(rho0 + col, word) : 0;
-      const auto next = [&] {  // the row after: the group's next head, or the next token's first
-        at += dh;
-        if (++g == group) {
-          g = 0;
-          at += static_cast<int64_t>(s.q_heads - group) * dh;
-        }
-      };
       if (SOLO) {
 #pragma unroll
         for (int x0 = 0; x0 < 16; x0 += 8) {
-          uint64_t c0[8], c1[8];
-          const int g1 = g;
-          const int64_t at1 = at;
-#pragma unroll
-          for (int x = 0; x < 8; x++) {
-            const bool in = x0 + x < left && word < dh;
-            c0[x] = ld_if(o.c[0] + at, in);
-            c1[x] = ld_if(o.c[1] + at, in);
-            next();
-          }
-          g = g1;
-          at = at1;
+          if (x0 > 0) fetch_c(x0);
 #pragma unroll
           for (int x = 0; x < 8; x++) {
             if (x0 + x < left && word < dh) o.out[at] = z[x0 + x] + c0[x] + c1[x] + o.r;
