@@ -262,77 +262,6 @@ __global__ void __launch_bounds__(kThreads, RT == 4 ? 4 : 3) values_rows_kernel(
   }
 }
 
-// ---- scores, many rows of wide heads: 64 x 64 tiles on the integer pipes ----
-constexpr int kT = 64, kTK = 16;
-
-__global__ void __launch_bounds__(kThreads) scores_tile_kernel(const __grid_constant__ AttnSeqs s,
-                                                               const __grid_constant__ AttnOperands o) {
-  __shared__ uint64_t sU[kTK][kT + 1], sD[kTK][kT + 1], sE[kTK][kT + 1], sW[kTK][kT + 1];
-  __shared__ int64_t s_key[kT];
-  const int t = threadIdx.x, dh = s.head_dim, group = s.q_heads / s.kv_heads;
-  const int b = blockIdx.z / s.kv_heads, kh = blockIdx.z % s.kv_heads;
-  SeqInfo q;
-  if (!seq_info(s, b, o.status, q)) return;
-  const int R = group * q.n, rho0 = blockIdx.y * kT, n0 = blockIdx.x * kT;
-  if (rho0 >= R || R <= o.few) return;
-  const int last = (rho0 + kT < R ? rho0 + kT : R) - 1;
-  const int len = row_len(q.n, q.L, s.causal, last / group);
-  if (n0 >= len) return;
-  for (int e = t; e < kT; e += kThreads) s_key[e] = n0 + e < len ? key_off(s, b, kh, n0 + e, o.status) : -1;
-  __syncthreads();
-  const int tx = t % 16, ty = t / 16;
-  uint64_t acc[4][4] = {};
-  for (int k0 = 0; k0 < dh; k0 += kTK) {
-    for (int e = t; e < kT * kTK; e += kThreads) {
-      const int rr = e / kTK, kk = e % kTK, rho = rho0 + rr, k = k0 + kk;
-      uint64_t d = 0, u = 0, ev = 0, wv = 0;
-      if (rho < R && k < dh) {
-        const int64_t at = (static_cast<int64_t>(q.t0 + rho / group) * s.q_heads + kh * group + rho % group) * dh + k;
-        d = o.x[0][at];
-        u = d + o.a[0][at] + o.a[1][at];
-      }
-      if (s_key[rr] >= 0 && k < dh) {
-        const int64_t at = s_key[rr] + k;
-        ev = o.e[at];
-        wv = o.b[0][at] + o.b[1][at];
-      }
-      sU[kk][rr] = u;
-      sD[kk][rr] = d;
-      sE[kk][rr] = ev;
-      sW[kk][rr] = wv;
-    }
-    __syncthreads();
-#pragma unroll 4
-    for (int kk = 0; kk < kTK; kk++) {
-      uint64_t u[4], d[4];
-#pragma unroll
-      for (int y = 0; y < 4; y++) {
-        u[y] = sU[kk][ty * 4 + y];
-        d[y] = sD[kk][ty * 4 + y];
-      }
-#pragma unroll
-      for (int x = 0; x < 4; x++) {
-        const uint64_t e = sE[kk][tx + 16 * x], w = sW[kk][tx + 16 * x];
-#pragma unroll
-        for (int y = 0; y < 4; y++) acc[y][x] += u[y] * e + d[y] * w;
-      }
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int y = 0; y < 4; y++) {
-    const int rho = rho0 + ty * 4 + y, i = rho / group;
-    if (rho >= R) continue;
-#pragma unroll
-    for (int x = 0; x < 4; x++) {
-      const int key = n0 + tx + 16 * x;
-      if (key >= row_len(q.n, q.L, s.causal, i)) continue;
-      const int64_t at = q.base + (kh * group + rho % group) * q.blk + row_off(q.n, q.L, s.causal, i) + key;
-      o.out[at] = acc[y][x] + o.c[0][at] + o.c[1][at] + o.r;
-    }
-  }
-}
-
 // The most rows of a (sequence, key head), and the most the row kernels take
 // (0: every sequence has more): a batch of prompts and single tokens runs both
 // kinds of kernel, each on its own sequences.
@@ -436,7 +365,6 @@ int sufb200_attn_scores_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
   o.status = ctx->d_status;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const Rows rows = rows_of(*seqs);
-  const unsigned z = static_cast<unsigned>(seqs->batch) * seqs->kv_heads;
   if (rows.few > 0) {
     const int rt = rows.few <= 4 ? 4 : 8;
     // rows of 8 x 256 words and 256 keys would pass 48 KB of shared memory
@@ -449,13 +377,9 @@ int sufb200_attn_scores_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
       scores_rows_kernel<8><<<grid, kThreads, smem, st>>>(*seqs, o, chunk);
   }
   o.few = rows.few;
-  if (rows.most > kFewRows && scores_tc_fits(*seqs)) {
+  if (rows.most > kFewRows) {
     const cudaError_t e = launch_scores_tc(ctx, *seqs, o, st);
     if (e != cudaSuccess) return fail(SUFB200_ERR_CUDA, std::string("attn_scores_pair: ") + cudaGetErrorString(e));
-  } else if (rows.most > kFewRows) {
-    // row planes of head sizes above 128 do not fit beside the stages (16 / 4
-    // heads of 128, 2,048 tokens: 3,402 us here against 368 us)
-    scores_tile_kernel<<<dim3((seqs->max_ctx + kT - 1) / kT, (rows.most + kT - 1) / kT, z), kThreads, 0, st>>>(*seqs, o);
   }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? SUFB200_OK : fail(SUFB200_ERR_CUDA, std::string("attn_scores_pair: ") + cudaGetErrorString(e));

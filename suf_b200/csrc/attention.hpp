@@ -143,7 +143,6 @@ struct AttnOperands {
 // The products on the tensor cores (attention_tc.cu), for sequences with many
 // rows per key head.  The values form adds to o.out unless values_tc_solo: then
 // it stores whole results.
-bool scores_tc_fits(const AttnSeqs& s);
 cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st);
 bool values_tc_solo(const sufb200_ctx_s* ctx, const AttnSeqs& s);
 cudaError_t launch_values_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st);

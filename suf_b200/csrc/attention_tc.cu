@@ -21,13 +21,14 @@
 // nowhere else.
 //
 // What bounds them (packed prompts of 2,048, 700 behind 1,024 and one token, 16
-// / 4 heads of 128; 49 M scores): a step's MMAs alone take 1,210 cycles, 211 us
-// in all, with the clock near 1.65 - 1.8 GHz under them.  The scores take 493 us
-// (2.7 TB/s): their epilogue moves 24 bytes a score beside MMAs that use most of
-// the shared memory's bandwidth, and a tile's epilogue is slower than its MMAs.
-// The values take 436 us: 1,580 - 1,600 cycles a step, the tensor core sharing shared
-// memory with the splitting of the shares.  On the integer pipes the two took
-// 5,030 and 5,293 us.
+// / 4 heads of 128; 49 M scores): a step's MMAs alone take 1,170 - 1,210 cycles,
+// 211 us in all, with the clock near 1.65 - 1.8 GHz under them.  The scores take
+// 490 us: without their 24 bytes of C and output a score 411 us, without the
+// keys' copies too 410 us; a tile's hand-over between MMAs and epilogue costs 2,800
+// cycles (tensor memory holds one tile), a CTA's set-up and rows' planes 10 of its
+// 90 us.  The values take 415 us: 1,580 cycles a step, the tensor core's reads of
+// shared memory, the copies into it and the splitting of the shares filling its
+// 128 bytes a cycle.  On the integer pipes the two took 5,030 and 5,293 us.
 #include <atomic>
 
 #include "attention.hpp"
@@ -54,6 +55,7 @@ struct AttnTc {
   uint8_t* planes;
   int64_t tiles;  // blocks (scores: 128 keys; values: 32 keys) per key head in `planes`
   int chunks;     // scores: 32-word chunks of the head; values: 128-word tiles of the head
+  int chunk0, part;  // scores: the chunks of this launch
   int span;       // scores: key tiles per CTA; values: keys per CTA
 };
 
@@ -373,6 +375,9 @@ int64_t row_tiles(const AttnSeqs& s) {
   return s.d_tiles ? s.n_tiles : blocks_of(s.q_heads / s.kv_heads * s.tokens, s.batch, kTN);
 }
 
+// FIRST: the head's first part, which adds C and r; else its second part, which
+// adds to the first one's words (o.c[0] = o.out).
+template <bool FIRST>
 __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_constant__ AttnTc a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const AttnSeqs& s = a.s;
@@ -390,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
     pdl_wait();
     return;
   }
-  const int steps = 2 * a.chunks;
+  const int steps = 2 * a.part;
   const uint32_t sbase = smem_u32(smem);
   const Ctrl c = ctrl_at(smem, kBOff + static_cast<uint32_t>(steps) * kBStage);
   if (t < kTN) {
@@ -403,16 +408,18 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
   if (!ready) {
   } else if (warp == 0) {  // A planes: every step of every key tile
     pdl_wait();  // written by the pre-pass
-    const uint8_t* src = a.planes + (kh * a.tiles + first_block(q.l0, b, kTM) + tile0) * steps * static_cast<int64_t>(kAStage);
-    for (int li = 0; li < tiles * steps; li++) {
-      int go = 1;
-      if (lane == 0) {
-        go = load_a(c, sbase, li, src + static_cast<int64_t>(li) * kAStage);
-        if (!go) *c.err = 1;
+    const int64_t next = 2 * static_cast<int64_t>(a.chunks) * kAStage;  // from a key tile to the one after
+    const uint8_t* src = a.planes + (kh * a.tiles + first_block(q.l0, b, kTM) + tile0) * next + 2 * a.chunk0 * kAStage;
+    int go = 1;
+    for (int tl = 0; tl < tiles && go; tl++, src += next)
+      for (int st = 0; st < steps && go; st++) {
+        if (lane == 0) {
+          go = load_a(c, sbase, copies, src + static_cast<int64_t>(st) * kAStage);
+          if (!go) *c.err = 1;
+        }
+        go = __shfl_sync(0xffffffffu, go, 0);
+        copies += go;
       }
-      if (!__shfl_sync(0xffffffffu, go, 0)) break;
-      copies++;
-    }
   } else if (warp == 1) {  // MMAs
     // The whole warp waits and steps, one elected lane issues: step, stage and
     // descriptors stay warp-uniform.
@@ -445,12 +452,12 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
     if (!go && lane == 0) *c.err = 1;
   } else {
     // the rows' planes [U | D]: the loads of two units, then their splitting
-    const int units = a.chunks * (kTN / 4);
+    const int units = a.part * (kTN / 4);
     for (int u0 = warp - 2; u0 < units; u0 += 2 * (kThreads / 32 - 2)) {
       uint64_t d[2][4], w[2][4], x[2][4];
 #pragma unroll
       for (int y = 0; y < 2; y++) {
-        const int u = u0 + y * (kThreads / 32 - 2), k = u / (kTN / 4) * kTK + 16 * (u & 1) + (lane & 15);
+        const int u = u0 + y * (kThreads / 32 - 2), k = (a.chunk0 + u / (kTN / 4)) * kTK + 16 * (u & 1) + (lane & 15);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const int64_t row = c.row[u % (kTN / 4) / 2 * 8 + 2 * j + (lane >> 4)];
@@ -510,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
         for (int x = 0; x < 4; x++) {
           const bool in = x0 + x < rows && key < llen;
           c0[(x0 >> 2) & 1][x] = ld_if(o.c[0] + lat, in);
-          c1[(x0 >> 2) & 1][x] = ld_if(o.c[1] + lat, in);
+          c1[(x0 >> 2) & 1][x] = FIRST ? ld_if(o.c[1] + lat, in) : 0;
           next(lg, llen, lrow, lat);
         }
       };
@@ -532,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
         if (x0 < 12) fetch(x0 + 4);
 #pragma unroll
         for (int x = 0; x < 4; x++) {
-          if (x0 + x < rows && key < slen) o.out[sat] = z[x0 + x] + c0[(x0 >> 2) & 1][x] + c1[(x0 >> 2) & 1][x] + o.r;
+          if (x0 + x < rows && key < slen) o.out[sat] = z[x0 + x] + c0[(x0 >> 2) & 1][x] + c1[(x0 >> 2) & 1][x] + (FIRST ? o.r : 0);
           next(sg, slen, srow, sat);
         }
       }
@@ -728,11 +735,11 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
   stop(c, o.status, warp, lane, copies);
 }
 
-// Launch as the pre-pass's programmatic dependent; the kernel may take all
-// shared memory, said once per kernel and device.
+// Launch, as the pre-pass's programmatic dependent if `after_planes`; the kernel
+// may take all shared memory, said once per kernel and device.
 template <int WHICH>
 cudaError_t launch(const sufb200_ctx_s* ctx, void (*kernel)(AttnTc), dim3 grid, size_t smem, cudaStream_t st,
-                   const AttnTc& a) {
+                   const AttnTc& a, bool after_planes = true) {
   constexpr int kMaxDevices = 64;
   static std::atomic<bool> ready[kMaxDevices];
   const bool known = ctx->device < kMaxDevices;
@@ -741,18 +748,22 @@ cudaError_t launch(const sufb200_ctx_s* ctx, void (*kernel)(AttnTc), dim3 grid, 
     if (e != cudaSuccess) return e;
     if (known) ready[ctx->device].store(true, std::memory_order_release);
   }
-  return launch_pdl(kernel, grid, dim3(kThreads), smem, st, a);
+  if (after_planes) return launch_pdl(kernel, grid, dim3(kThreads), smem, st, a);
+  kernel<<<grid, kThreads, smem, st>>>(a);
+  return cudaGetLastError();
 }
 
-}  // namespace
+// Most chunks of the head whose row planes stay in shared memory beside three A
+// stages; wider heads take a second launch that adds to the first one's words
+// (2,048 tokens, 16 / 4 heads of 256: 646 us, 6,527 on the integer pipes).
+constexpr int kMostChunks = 4;
 
-// Head sizes whose row planes stay in shared memory beside three A stages.
-bool scores_tc_fits(const AttnSeqs& s) { return s.head_dim <= 128; }
+}  // namespace
 
 cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st) {
   const int64_t rts = row_tiles(s);
   const int nt = (s.max_ctx + kTM - 1) / kTM;
-  AttnTc a{s, o, nullptr, blocks_of(s.cached, s.batch, kTM), (s.head_dim + kTK - 1) / kTK, 0};
+  AttnTc a{s, o, nullptr, blocks_of(s.cached, s.batch, kTM), (s.head_dim + kTK - 1) / kTK, 0, 0, 0};
   const int64_t bytes = a.tiles * s.kv_heads * a.chunks * 2 * static_cast<int64_t>(kAStage);
   cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&a.planes), bytes, ctx->pool, st);
   if (e != cudaSuccess) return e;
@@ -764,9 +775,14 @@ cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const 
   a.span = static_cast<int>(want < 1 ? 1 : (want > 16 ? 16 : want));
   cache_planes_kernel<true><<<dim3(static_cast<unsigned>(a.tiles), a.chunks, s.kv_heads), 256, 0, st>>>(a);
   e = cudaGetLastError();
-  const size_t smem = kBOff + static_cast<size_t>(2 * a.chunks) * kBStage + kCtrlBytes;
   const dim3 grid(static_cast<unsigned>(rts * s.kv_heads), (nt + a.span - 1) / a.span);
-  if (e == cudaSuccess) e = launch<0>(ctx, scores_tc_kernel, grid, smem, st, a);
+  for (a.chunk0 = 0; a.chunk0 < a.chunks && e == cudaSuccess; a.chunk0 += a.part) {
+    a.part = a.chunks - a.chunk0 < kMostChunks ? a.chunks - a.chunk0 : kMostChunks;
+    const size_t smem = kBOff + static_cast<size_t>(2 * a.part) * kBStage + kCtrlBytes;
+    e = a.chunk0 == 0 ? launch<0>(ctx, scores_tc_kernel<true>, grid, smem, st, a)
+                      : launch<3>(ctx, scores_tc_kernel<false>, grid, smem, st, a, false);
+    a.o.c[0] = o.out;
+  }
   const cudaError_t f = cudaFreeAsync(a.planes, st);
   return e == cudaSuccess ? f : e;
 }
@@ -786,7 +802,7 @@ int values_span(const sufb200_ctx_s* ctx, const AttnSeqs& s) {
 bool values_tc_solo(const sufb200_ctx_s* ctx, const AttnSeqs& s) { return values_span(ctx, s) >= s.max_ctx; }
 
 cudaError_t launch_values_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st) {
-  AttnTc a{s, o, nullptr, blocks_of(s.cached, s.batch, kTK), (s.head_dim + kTM - 1) / kTM, values_span(ctx, s)};
+  AttnTc a{s, o, nullptr, blocks_of(s.cached, s.batch, kTK), (s.head_dim + kTM - 1) / kTM, 0, 0, values_span(ctx, s)};
   const int64_t bytes = a.tiles * s.kv_heads * a.chunks * 2 * static_cast<int64_t>(kAStage);
   cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&a.planes), bytes, ctx->pool, st);
   if (e != cudaSuccess) return e;

@@ -661,3 +661,18 @@ def test_attention_reports_bad_lengths(ctx, torch_cuda, which, case):
     got = call(ctx, *args)
     ctx.sync()
     assert (from_dev(got) == want).all()
+
+
+@pytest.mark.parametrize("case", [([(70, 150), (33, 20)], 4, 2, 134, 16, True), ([(150, 300), (0, 3)], 2, 1, 256, 64, True),
+                                  ([(20, 5), (1, 40)], 3, 1, 130, 7, True), ([(24, 131)], 2, 2, 224, 32, False)])
+def test_scores_of_wide_heads_in_two_parts(ctx, torch_cuda, case):
+    """Heads above 128 words: the second part adds to the first one's words, and
+    leaves what is behind the last row alone."""
+    from suf_b200 import attention as at
+
+    A = _Attn(ctx, torch_cuda, case, 35)
+    args, want = A.scores()
+    buf, out = _guarded(torch_cuda, want)
+    at.attn_scores_pair(ctx, *args, out=out)
+    ctx.sync()
+    assert (from_dev(out) == want).all() and (buf[want.size:] == 77).all()
