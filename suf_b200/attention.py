@@ -55,10 +55,13 @@ def _stream(ctx: Context, stream) -> int | None:
     return stream.cuda_stream or None
 
 
-def _empty(ctx: Context, shape, stream=None):
+def _empty(ctx: Context, shape, stream=None, like=None):
     """Words on the context's device, allocated on the stream that writes them
-    and kept until the caller's current stream has passed its use of them."""
+    and kept until the caller's current stream has passed its use of them.
+    like: a checked tensor of words there (half the host's time of a new one)."""
     if stream is None:
+        if like is not None:
+            return like.new_empty(shape)
         return torch.empty(shape, dtype=torch.int64, device=ctx.device)
     now = torch.cuda.current_stream(ctx.device)
     if isinstance(stream, int):
@@ -102,6 +105,13 @@ def _pair(ctx: Context, name: str, ts, shape: tuple):
     if not isinstance(ts, (tuple, list)) or len(ts) != 2:
         raise ValueError(f"{name}: expected both parties' tensors")
     x, y = ts
+    try:
+        device, word = ctx.device, torch.int64
+        if (x.dtype is word and y.dtype is word and x.get_device() == device and y.get_device() == device and
+                x.shape == shape and y.shape == shape and x.is_contiguous() and y.is_contiguous()):
+            return _Two(x.data_ptr(), y.data_ptr())
+    except AttributeError:
+        pass
     return _Two(_want(ctx, name, x, shape), _want(ctx, name, y, shape))
 
 
@@ -269,7 +279,7 @@ def rope_append_pair(ctx: Context, q, k, v, positions, slots, cos, sin, trunc: T
         args.d_q, args.q_ts, args.q_hs = _strided(ctx, "q", q, shape)
         args.d_a = _pair(ctx, "a", a, shape)
         if d_q is None:
-            d_q = _empty(ctx, shape, stream)
+            d_q = _empty(ctx, shape, stream, q[0])
         args.d_dq, args.q_heads = _want(ctx, "d_q", d_q, shape), heads
     args.d_slots = _want(ctx, "slots", slots, (tokens,))
     if trunc is not None:
@@ -390,7 +400,7 @@ def attn_scores_pair(ctx: Context, d_q, a, c, r, ek, bk, layout: AttnLayout, out
     seqs, e, b = layout._for_pool(ctx, "ek", ek, bk)
     shape, packed = (layout.tokens, layout.q_heads, seqs.head_dim), (layout.packed,)
     if out is None:
-        out = _empty(ctx, packed, stream)
+        out = _empty(ctx, layout.packed, stream, ek)
     check(ctx._L.sufb200_attn_scores_pair(ctx.h, C.byref(seqs), _want(ctx, "d_q", d_q, shape),
                                           _pair(ctx, "a", a, shape), _pair(ctx, "c", c, packed), _masks(r), e, b,
                                           _want(ctx, "out", out, packed), _stream(ctx, stream)))
@@ -405,7 +415,7 @@ def attn_values_pair(ctx: Context, p, a, c, r, ev, bv, layout: AttnLayout, out=N
     seqs, e, b = layout._for_pool(ctx, "ev", ev, bv)
     shape, packed = (layout.tokens, layout.q_heads, seqs.head_dim), (layout.packed,)
     if out is None:
-        out = _empty(ctx, shape, stream)
+        out = _empty(ctx, shape, stream, ev)
     check(ctx._L.sufb200_attn_values_pair(ctx.h, C.byref(seqs), _pair(ctx, "p", p, packed),
                                           _pair(ctx, "a", a, packed), _pair(ctx, "c", c, shape), _masks(r), e, b,
                                           _want(ctx, "out", out, shape), _stream(ctx, stream)))
@@ -441,11 +451,12 @@ class RowMaxPlan:
 def rowmax_open_pair(ctx: Context, plan: RowMaxPlan, c, r, out=None, stream=None):
     """x^ [pairs[0]]: the opened differences of the first round's pairs of c (packed shares)."""
     n = plan.pairs[0] if plan.rounds else 0
+    words = _pair(ctx, "c", c, (plan.values[0],))
     if out is None:
-        out = _empty(ctx, (n,), stream)
-    c, o = _pair(ctx, "c", c, (plan.values[0],)), _want(ctx, "out", out, (n,))
+        out = _empty(ctx, n, stream, c[0])
+    o = _want(ctx, "out", out, (n,))
     if n:
-        check(ctx._L.sufb200_rowmax_open_pair(ctx.h, c, plan.rows, plan.widths[0], plan._off[0], plan._off[1],
+        check(ctx._L.sufb200_rowmax_open_pair(ctx.h, words, plan.rows, plan.widths[0], plan._off[0], plan._off[1],
                                               _masks(r), o, _stream(ctx, stream)))
     return out
 
@@ -456,36 +467,36 @@ def rowmax_round_pair(ctx: Context, plan: RowMaxPlan, k: int, c, relu, r_next=No
     differences.  Returns ((next_0, next_1), x^ or None)."""
     if not 0 <= k < plan.rounds:
         raise ValueError(f"rowmax: round {k} of {plan.rounds}")
-    n, more = (plan.values[k + 1],), k + 1 < plan.rounds
+    n, more = plan.values[k + 1], k + 1 < plan.rounds
+    words, gates = _pair(ctx, "c", c, (plan.values[k],)), _pair(ctx, "relu", relu, (plan.pairs[k],))
     if nxt is None:
-        nxt = _empty(ctx, n, stream), _empty(ctx, n, stream)
+        nxt = _empty(ctx, n, stream, c[0]), _empty(ctx, n, stream, c[0])
         to = _Two(nxt[0].data_ptr(), nxt[1].data_ptr())
     else:
-        to = _pair(ctx, "next", nxt, n)
+        to = _pair(ctx, "next", nxt, (n,))
     o = off2 = r = None
     if r_next is not None:
         if not more:
             raise ValueError("rowmax: the last round has no further differences to open")
-        pairs = (plan.pairs[k + 1],)
         if out is None:
-            out = _empty(ctx, pairs, stream)
+            out = _empty(ctx, plan.pairs[k + 1], stream, c[0])
             o = out.data_ptr()
         else:
-            o = _want(ctx, "out", out, pairs)
+            o = _want(ctx, "out", out, (plan.pairs[k + 1],))
         off2, r = plan._off[k + 2], _masks(r_next)
     check(ctx._L.sufb200_rowmax_round_pair(
-        ctx.h, _pair(ctx, "c", c, (plan.values[k],)), _pair(ctx, "relu", relu, (plan.pairs[k],)), plan.rows,
-        plan.widths[k], plan._off[k], plan._off[k + 1], off2, r, to, o, _stream(ctx, stream)))
+        ctx.h, words, gates, plan.rows, plan.widths[k], plan._off[k], plan._off[k + 1], off2, r, to, o,
+        _stream(ctx, stream)))
     return nxt, out if r_next is not None else None
 
 
 def maxdiff_ragged_pair(ctx: Context, plan: RowMaxPlan, m, s, out=None, stream=None):
     """t_p = max_p[row] - s_p over the packed rows: m the last round's values, s the first's."""
     n = (plan.values[0],)
+    top, words = _pair(ctx, "max", m, (plan.values[-1],)), _pair(ctx, "s", s, n)
     if out is None:
-        out = _empty(ctx, n, stream), _empty(ctx, n, stream)
-    check(ctx._L.sufb200_maxdiff_ragged_pair(ctx.h, _pair(ctx, "max", m, (plan.values[-1],)), _pair(ctx, "s", s, n),
-                                             plan.rows, plan.widths[0], plan._off[0], plan._off[-1],
+        out = _empty(ctx, n, stream, s[0]), _empty(ctx, n, stream, s[0])
+    check(ctx._L.sufb200_maxdiff_ragged_pair(ctx.h, top, words, plan.rows, plan.widths[0], plan._off[0], plan._off[-1],
                                              _pair(ctx, "out", out, n), _stream(ctx, stream)))
     return out
 
