@@ -489,8 +489,9 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
     // The MMAs take most of the shared-memory bandwidth and every multiply of
     // an address would stand in this warp's chain, so the rows' places are
     // stepped from one row to the next (row_off, row_len by differences).  C is
-    // fetched four rows ahead of the stores, the first four while the tile's
-    // MMAs still run; more in flight would spill.
+    // fetched eight rows ahead of the stores, the first eight while the tile's
+    // MMAs still run (four rows ahead: 16 heads of 64 402 us, eight 384; more in
+    // flight would spill).
     const int quarter = warp & 3, col = ((warp - 4) >> 2) * 16;
     const int i0 = (rho0 + col) / group, g0 = (rho0 + col) % group;  // the first row's query and head of the group
     const int rows = R - rho0 - col;                                 // rows there are, from there on
@@ -499,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
     for (int tl = 0; tl < tiles; tl++) {
       const int key = (tile0 + tl) * kTM + quarter * 32 + lane;
       // this query's row of the group's first head, and this row: one walk for
-      // the loads of C, four rows ahead, one for the stores
+      // the loads of C, eight rows ahead, one for the stores
       int lg = g0, llen = len0, sg = g0, slen = len0;
       int64_t lrow = at0 + key, lat = lrow + g0 * q.blk, srow = lrow, sat = lat;
       const auto next = [&](int& g, int& len, int64_t& row, int64_t& at) {
@@ -522,6 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
         }
       };
       fetch(0);
+      fetch(4);
       int go = 1;
       if (lane == 0) go = mbar_wait(c.tfull, static_cast<uint32_t>(tl & 1));
       if (!__shfl_sync(0xffffffffu, go, 0)) {
@@ -536,12 +538,12 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
       if (lane == 0) mbar_arrive(c.tempty);
 #pragma unroll
       for (int x0 = 0; x0 < 16; x0 += 4) {
-        if (x0 < 12) fetch(x0 + 4);
 #pragma unroll
         for (int x = 0; x < 4; x++) {
           if (x0 + x < rows && key < slen) o.out[sat] = z[x0 + x] + c0[(x0 >> 2) & 1][x] + c1[(x0 >> 2) & 1][x] + (FIRST ? o.r : 0);
           next(sg, slen, srow, sat);
         }
+        if (x0 < 8) fetch(x0 + 8);
       }
     }
   }
