@@ -239,10 +239,14 @@ def _strided(ctx: Context, name: str, ts, shape: tuple):
     if not isinstance(ts, (tuple, list)) or len(ts) != 2:
         raise ValueError(f"{name}: expected both parties' tensors")
     x, y = ts
-    for t in (x, y):
-        if (not isinstance(t, torch.Tensor) or t.dtype is not torch.int64 or t.get_device() != ctx.device or
-                t.shape != shape):
-            _refuse(ctx, name, t, shape, torch.int64)
+    word, device = torch.int64, ctx.device
+    for t in ts:
+        try:
+            if t.dtype is word and t.get_device() == device and t.shape == shape:
+                continue
+        except AttributeError:
+            pass
+        _refuse(ctx, name, t, shape, word)
     ld = x.stride()
     if ld != y.stride():
         raise ValueError(f"{name}: the parties' strides differ")
@@ -276,9 +280,10 @@ def rope_append_pair(ctx: Context, q, k, v, positions, slots, cos, sin, trunc: T
         args.d_dq, args.q_heads = _want(ctx, "d_q", d_q, shape), heads
     args.d_slots = _want(ctx, "slots", slots, (tokens,))
     if trunc is not None:
-        args.d_cos = _want(ctx, "cos", cos, (None, None), torch.int32)
-        args.max_pos, half = cos.shape
-        args.d_sin = _want(ctx, "sin", sin, (args.max_pos, half), torch.int32)
+        table = cos.shape if isinstance(cos, torch.Tensor) and cos.dim() == 2 else (None, None)
+        args.d_cos = _want(ctx, "cos", cos, table, torch.int32)
+        args.d_sin = _want(ctx, "sin", sin, table, torch.int32)
+        args.max_pos, half = table
         args.rot_dim = 2 * half
         if 2 * half > dim:
             raise ValueError(f"the tables turn {2 * half} words of a head of {dim}")

@@ -676,3 +676,42 @@ def test_scores_of_wide_heads_in_two_parts(ctx, torch_cuda, case):
     at.attn_scores_pair(ctx, *args, out=out)
     ctx.sync()
     assert (from_dev(out) == want).all() and (buf[want.size:] == 77).all()
+
+
+def test_two_streams_and_two_graphs_at_once(ctx, torch_cuda):
+    """Calls in flight on two streams, and two captured graphs replayed beside
+    one another, share no workspace: every result as if alone."""
+    from suf_b200 import attention as at
+
+    torch = torch_cuda
+    jobs = []
+    for i, case in enumerate([([(600, 900), (1, 700)], 8, 2, 64, 64, True), ([(300, 1000)], 4, 2, 160, 16, True)]):
+        A = _Attn(ctx, torch, case, 40 + i)
+        for which in ("scores", "values"):
+            call, (args, _) = getattr(at, f"attn_{which}_pair"), getattr(A, which)()
+            jobs.append((A, call, args, call(ctx, *args)))
+    ctx.sync()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(3):
+        outs = [torch.empty_like(want) for *_, want in jobs]
+        torch.cuda.synchronize()
+        for st, out, (_, call, args, _) in zip(streams, outs, jobs):
+            call(ctx, *args, out=out, stream=st)
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for out, (*_, want) in zip(outs, jobs))
+    graphs = []
+    for st, out, (_, call, args, _) in zip(streams, outs, jobs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            call(ctx, *args, out=out, stream=st)
+        graphs.append(g)
+    for _ in range(3):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for st, g in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for out, (*_, want) in zip(outs, jobs))
+    ctx.sync()
