@@ -339,11 +339,17 @@ int keys_per_cta(const sufb200_ctx_s* ctx, const AttnSeqs& s, int least, int mos
 
 }  // namespace
 
+int attn_result(const char* who, cudaError_t e) {
+  if (e == cudaSuccess) return SUFB200_OK;
+  cudaGetLastError();
+  return fail(SUFB200_ERR_CUDA, std::string(who) + ": " + cudaGetErrorString(e));
+}
+
 int attn_check_ctx(sufb200_ctx ctx) {
   if (!ctx) return fail(SUFB200_ERR_INVALID, "null context");
   if (ctx->device < 0) return fail(SUFB200_ERR_UNSUPPORTED, "host-only context: no device to evaluate on");
   const cudaError_t e = cudaSetDevice(ctx->device);
-  return e == cudaSuccess ? SUFB200_OK : fail(SUFB200_ERR_CUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(e));
+  return attn_result("cudaSetDevice", e);
 }
 
 }  // namespace sufb200
@@ -379,10 +385,9 @@ int sufb200_attn_scores_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
   o.few = rows.few;
   if (rows.most > kFewRows) {
     const cudaError_t e = launch_scores_tc(ctx, *seqs, o, st);
-    if (e != cudaSuccess) return fail(SUFB200_ERR_CUDA, std::string("attn_scores_pair: ") + cudaGetErrorString(e));
+    if (e != cudaSuccess) return attn_result("attn_scores_pair", e);
   }
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? SUFB200_OK : fail(SUFB200_ERR_CUDA, std::string("attn_scores_pair: ") + cudaGetErrorString(e));
+  return attn_result("attn_scores_pair", cudaGetLastError());
 }
 
 int sufb200_attn_values_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, const uint64_t* const* d_p,
@@ -424,10 +429,9 @@ int sufb200_attn_values_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
   o.few = rows.few;
   if (any && rows.most > kFewRows) {
     const cudaError_t e = launch_values_tc(ctx, *seqs, o, st);
-    if (e != cudaSuccess) return fail(SUFB200_ERR_CUDA, std::string("attn_values_pair: ") + cudaGetErrorString(e));
+    if (e != cudaSuccess) return attn_result("attn_values_pair", e);
   }
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? SUFB200_OK : fail(SUFB200_ERR_CUDA, std::string("attn_values_pair: ") + cudaGetErrorString(e));
+  return attn_result("attn_values_pair", cudaGetLastError());
 }
 
 }  // extern "C"

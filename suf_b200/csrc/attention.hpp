@@ -125,6 +125,11 @@ __device__ __forceinline__ uint64_t ld_if(const uint64_t* p, bool in) {
 // Context check of the entry points (null, host-only, device made current).
 int attn_check_ctx(sufb200_ctx ctx);
 
+// An entry point's result: OK, or the CUDA error reported (and taken out of the
+// runtime's own last error: a workspace that could not be had is not an error
+// of the calls after it).
+int attn_result(const char* who, cudaError_t e);
+
 inline bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // The operands of one attention product, both parties.

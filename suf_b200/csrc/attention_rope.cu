@@ -275,5 +275,5 @@ extern "C" int sufb200_rope_append_pair(sufb200_ctx ctx, const sufb200_rope_appe
       if (e == cudaSuccess) e = f;
     }
   }
-  return e == cudaSuccess ? SUFB200_OK : fail(SUFB200_ERR_CUDA, std::string("rope_append_pair: ") + cudaGetErrorString(e));
+  return attn_result("rope_append_pair", e);
 }

@@ -130,11 +130,6 @@ int check_words(std::initializer_list<const void*> ps, const char* who) {
   return SUFB200_OK;
 }
 
-int launched(const char* who) {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? SUFB200_OK : fail(SUFB200_ERR_CUDA, std::string(who) + ": " + cudaGetErrorString(e));
-}
-
 }  // namespace
 
 }  // namespace sufb200
@@ -154,7 +149,7 @@ int sufb200_rowmax_open_pair(sufb200_ctx ctx, const uint64_t* const* d_c, int ro
   const Shape s = shape_for(ctx, rows, max_width);
   rowmax_round_kernel<false><<<s.grid, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
       d_c[0], d_c[1], nullptr, nullptr, rows, d_off, d_off1, nullptr, r[0] + r[1], nullptr, nullptr, d_xhat, s.tpr);
-  return launched("rowmax_open_pair");
+  return attn_result("rowmax_open_pair", cudaGetLastError());
 }
 
 int sufb200_rowmax_round_pair(sufb200_ctx ctx, const uint64_t* const* d_c, const uint64_t* const* d_relu, int rows,
@@ -173,7 +168,7 @@ int sufb200_rowmax_round_pair(sufb200_ctx ctx, const uint64_t* const* d_c, const
   rowmax_round_kernel<true><<<s.grid, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
       d_c[0], d_c[1], d_relu[0], d_relu[1], rows, d_off, d_off1, d_off2, d_xhat ? r[0] + r[1] : 0, d_next[0], d_next[1],
       d_xhat, s.tpr);
-  return launched("rowmax_round_pair");
+  return attn_result("rowmax_round_pair", cudaGetLastError());
 }
 
 int sufb200_maxdiff_ragged_pair(sufb200_ctx ctx, const uint64_t* const* d_max, const uint64_t* const* d_s, int rows,
@@ -187,7 +182,7 @@ int sufb200_maxdiff_ragged_pair(sufb200_ctx ctx, const uint64_t* const* d_max, c
   const Shape s = shape_for(ctx, rows, max_width);
   maxdiff_ragged_kernel<<<s.grid, kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
       d_max[0], d_max[1], d_s[0], d_s[1], rows, d_off, d_max_off, d_t[0], d_t[1], s.tpr);
-  return launched("maxdiff_ragged_pair");
+  return attn_result("maxdiff_ragged_pair", cudaGetLastError());
 }
 
 }  // extern "C"

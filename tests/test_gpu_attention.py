@@ -715,3 +715,22 @@ def test_two_streams_and_two_graphs_at_once(ctx, torch_cuda):
         torch.cuda.synchronize()
         assert all(torch.equal(out, want) for out, (*_, want) in zip(outs, jobs))
     ctx.sync()
+
+
+@pytest.mark.parametrize("which", ["scores", "values"])
+def test_a_workspace_that_cannot_be_had_is_this_calls_error_only(ctx, torch_cuda, which):
+    """More cached tokens than any memory holds planes for: refused by the
+    allocator, and the calls after it work."""
+    from suf_b200 import SufB200Error
+    from suf_b200 import attention as at
+
+    A = _Attn(ctx, torch_cuda, ([(20, 40)], 64, 64, 2, 16, True), 50)
+    args, want = getattr(A, which)()
+    call, cached = getattr(at, f"attn_{which}_pair"), A.layout._seqs.cached
+    A.layout._seqs.cached = 2**30  # terabytes of planes
+    with pytest.raises(SufB200Error):
+        call(ctx, *args)
+    A.layout._seqs.cached = cached
+    got = call(ctx, *args)
+    ctx.sync()
+    assert (from_dev(got) == want).all()
