@@ -770,11 +770,11 @@ cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const 
   cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&a.planes), bytes, ctx->pool, st);
   if (e != cudaSuccess) return e;
   // key tiles per CTA: long runs reuse the rows' planes and hide the epilogue
-  // behind the next tile, as long as every SM has a few CTAs to take (a
-  // 2,048-token prompt, 16 / 4 heads of 128, first form: 738 us for runs of one
-  // tile, 510 of two, 410 of four, 363 of eight, 346 of sixteen)
-  const int64_t all = nt * rts * s.kv_heads, want = all / (static_cast<int64_t>(ctx->sm_count) * 4);
-  a.span = static_cast<int>(want < 1 ? 1 : (want > 16 ? 16 : want));
+  // behind the next tile; two CTAs an SM in all even out, more cost more set-ups
+  // (16 / 4 heads of 128, 1,024 tokens: 112 us, 141 by four an SM; 256 behind
+  // 4,096: 192 and 224 us; 64 behind 8,000, 32 / 8 heads: 214 and 259 us)
+  const int64_t all = nt * rts * s.kv_heads, two = static_cast<int64_t>(ctx->sm_count) * 2;
+  a.span = static_cast<int>((all + two - 1) / two < nt ? (all + two - 1) / two : nt);
   cache_planes_kernel<true><<<dim3(static_cast<unsigned>(a.tiles), a.chunks, s.kv_heads), 256, 0, st>>>(a);
   e = cudaGetLastError();
   const dim3 grid(static_cast<unsigned>(rts * s.kv_heads), (nt + a.span - 1) / a.span);
@@ -793,11 +793,13 @@ cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const 
 int values_span(const sufb200_ctx_s* ctx, const AttnSeqs& s) {
   const int nch = (s.max_ctx + kTK - 1) / kTK, words = (s.head_dim + kTM - 1) / kTM;
   const int64_t units = row_tiles(s) * words * s.kv_heads;
-  // at most the exact depth; shorter, down to eight chunks, while that leaves SMs idle
-  int64_t parts = (static_cast<int64_t>(ctx->sm_count) * 4 + units - 1) / units;
-  const int64_t most = (nch + 7) / 8;
-  parts = parts > most ? most : (parts < 1 ? 1 : parts);
-  const int span = static_cast<int>((nch + parts - 1) / parts) * kTK;
+  // whole rows where there is more than one row tile an SM (no pass that starts
+  // the output from C: 16 / 4 heads of 128, 1,024 tokens 83 us, 94 split), else
+  // two CTAs an SM in all, of eight chunks at least (256 behind 4,096: 154 us, 162
+  // by equal parts, 180 by four CTAs an SM); at most the exact depth
+  const int64_t two = static_cast<int64_t>(ctx->sm_count) * 2, even = (units * nch + two - 1) / two;
+  const int64_t want = two / units < 2 ? nch : (even < 8 ? 8 : even);
+  const int span = static_cast<int>(want < nch ? want : nch) * kTK;
   return span > kMaxDepthKeys ? kMaxDepthKeys : span;
 }
 
