@@ -24,11 +24,11 @@
 // / 4 heads of 128; 49 M scores): a step's MMAs alone take 1,170 - 1,210 cycles,
 // 211 us in all, with the clock near 1.65 - 1.8 GHz under them.  The scores take
 // 490 us: without their 24 bytes of C and output a score 411 us, without the
-// keys' copies too 410 us; a tile's hand-over between MMAs and epilogue costs 2,800
-// cycles (tensor memory holds one tile), a CTA's set-up and rows' planes 10 of its
-// 90 us.  The values take 415 us: 1,580 cycles a step, the tensor core's reads of
-// shared memory, the copies into it and the splitting of the shares filling its
-// 128 bytes a cycle.  On the integer pipes the two took 5,030 and 5,293 us.
+// keys' copies too 410 us; the MMAs alone, one tile in tensor memory at a time, take
+// 1,530 cycles a step, a CTA's set-up and rows' planes 11 of its 90 us.  The values
+// take 415 us: 1,580 cycles a step, the tensor core's reads of shared memory (123
+// KB), the copies into it and the splitting of the shares filling its 128 bytes a
+// cycle.  On the integer pipes the two took 5,030 and 5,293 us.
 #include <atomic>
 
 #include "attention.hpp"
