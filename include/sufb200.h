@@ -772,10 +772,11 @@ int sufb200_rope_append_pair(sufb200_ctx ctx, const sufb200_rope_append* args, v
  *   len = causal ? max(0, ctx - n + i + 1) : ctx
  * words, and sequence b's rows start at word d_row_base[b].  max_q and max_ctx
  * bound the lengths, min_q the new tokens of the sequences that have any (from
- * below: short and long ones are computed by different kernels); tokens, cached and packed the sums of the new tokens, the
- * cached tokens and the words (workspaces are sized by them).  At most 2^26
- * cached tokens in a sequence, 65,535 (sequence, key head) pairs and 2^20 rows
- * (queries of its heads) per pair. */
+ * below: short and long ones are computed by different kernels); tokens, cached
+ * and packed are the sums of the new tokens, the cached tokens and the words
+ * (workspaces are sized by them).  At most 2^26 cached tokens in a sequence,
+ * 65,535 (sequence, key head) pairs and 2^20 rows (queries of its heads) per
+ * pair. */
 #define SUFB200_ATTN_FEW_ROWS 8  /* rows of a (sequence, key head) up to which it counts as short */
 #define SUFB200_ATTN_ROW_TILE 64 /* rows of a row tile */
 typedef struct sufb200_attn_seqs {
