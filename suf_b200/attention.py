@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 
 import numpy as np
 import torch
@@ -252,7 +253,12 @@ def _strided(ctx: Context, name: str, ts, shape: tuple):
         raise ValueError(f"{name}: the parties' strides differ")
     if ld[2] != 1 and x.numel():
         raise ValueError(f"{name}: the head's words must be adjacent")
-    return _Two(x.data_ptr(), y.data_ptr()), ld[0], ld[1]
+    return x.data_ptr(), y.data_ptr(), ld[0], ld[1]
+
+
+# sufb200_rope_append up to d_ek: the shares' addresses and strides, positions,
+# slots, cosines, sines, the queries' masks and output
+_ROPE_FRONT = struct.Struct("=6Q6q7Q")
 
 
 def rope_append_pair(ctx: Context, q, k, v, positions, slots, cos, sin, trunc: TruncPair | None, a, cache: ShareCache,
@@ -268,29 +274,32 @@ def rope_append_pair(ctx: Context, q, k, v, positions, slots, cos, sin, trunc: T
         raise ValueError(f"the cache is on cuda:{cache.device}, the context on cuda:{ctx.device}")
     tokens, kv, dim = k[0].shape[0], cache.kv_heads, cache.head_dim
     args = RopeAppend.from_buffer_copy(cache._args)
-    args.d_k, args.k_ts, args.k_hs = _strided(ctx, "k", k, (tokens, kv, dim))
-    args.d_v, args.v_ts, args.v_hs = _strided(ctx, "v", v, (tokens, kv, dim))
+    k0, k1, k_ts, k_hs = _strided(ctx, "k", k, (tokens, kv, dim))
+    v0, v1, v_ts, v_hs = _strided(ctx, "v", v, (tokens, kv, dim))
+    q0 = q1 = q_ts = q_hs = a0 = a1 = out = 0
     if q is not None:
         heads = q[0].shape[1]
         shape = (tokens, heads, dim)
-        args.d_q, args.q_ts, args.q_hs = _strided(ctx, "q", q, shape)
-        args.d_a = _pair(ctx, "a", a, shape)
+        q0, q1, q_ts, q_hs = _strided(ctx, "q", q, shape)
+        a0, a1 = _pair(ctx, "a", a, shape)
         if d_q is None:
             d_q = _empty(ctx, shape, stream, q[0])
-        args.d_dq, args.q_heads = _want(ctx, "d_q", d_q, shape), heads
-    args.d_slots = _want(ctx, "slots", slots, (tokens,))
+        out, args.q_heads = _want(ctx, "d_q", d_q, shape), heads
+    at_pos = at_cos = at_sin = 0
     if trunc is not None:
         table = cos.shape if isinstance(cos, torch.Tensor) and cos.dim() == 2 else (None, None)
-        args.d_cos = _want(ctx, "cos", cos, table, torch.int32)
-        args.d_sin = _want(ctx, "sin", sin, table, torch.int32)
+        at_cos = _want(ctx, "cos", cos, table, torch.int32)
+        at_sin = _want(ctx, "sin", sin, table, torch.int32)
+        at_pos = _want(ctx, "positions", positions, (tokens,), torch.int32)
         args.max_pos, half = table
         args.rot_dim = 2 * half
         if 2 * half > dim:
             raise ValueError(f"the tables turn {2 * half} words of a head of {dim}")
-        args.d_positions = _want(ctx, "positions", positions, (tokens,), torch.int32)
         args.trunc, args.d_tables, args.r = trunc._args
     elif cos is not None or sin is not None:
         raise ValueError("rotation needs the truncation bundle")
+    _ROPE_FRONT.pack_into(args, 0, q0, q1, k0, k1, v0, v1, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, at_pos,
+                          _want(ctx, "slots", slots, (tokens,)), at_cos, at_sin, a0 or 0, a1 or 0, out)
     args.tokens, args.interleaved = tokens, 1 if interleaved else 0
     check(ctx._L.sufb200_rope_append_pair(ctx.h, C.byref(args), _stream(ctx, stream)))
     return d_q

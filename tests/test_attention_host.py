@@ -362,3 +362,17 @@ def test_rowmax_refuses_rows_whose_steps_pass_32_bits(host):
     for lens in ([2**30 + 1], [3, -1], [2**30, 2**30]):
         with pytest.raises(ValueError, match="row lengths"):
             at.RowMaxPlan(_Ctx, lens)
+
+
+def test_the_appends_packed_arguments_are_the_structs():
+    """What the wrapper packs in one piece lies where the struct's fields are."""
+    from suf_b200 import attention as at
+    from suf_b200._lib import RopeAppend
+
+    args = RopeAppend()
+    at._ROPE_FRONT.pack_into(args, 0, *range(1, 13), *range(13, 20))
+    assert at._ROPE_FRONT.size == RopeAppend.d_ek.offset
+    assert [v for f in (args.d_q, args.d_k, args.d_v) for v in f] == list(range(1, 7))
+    assert [args.q_ts, args.q_hs, args.k_ts, args.k_hs, args.v_ts, args.v_hs] == list(range(7, 13))
+    assert [args.d_positions, args.d_slots, args.d_cos, args.d_sin] == list(range(13, 17))
+    assert list(args.d_a) == [17, 18] and args.d_dq == 19
