@@ -223,10 +223,9 @@ class ShareCache:
         args.d_bk, args.d_bv = _pair(ctx, "bk", bk, shape), _pair(ctx, "bv", bv, shape)
         self._pools, self.device = (ek, tuple(bk), ev, tuple(bv)), ctx.device
         self.pages, self.kv_heads, self.page_size, self.head_dim = shape
-        if min(shape) < 1 or self.head_dim % 2 or self.head_dim > 256:
-            raise ValueError("cache: empty, or a head size that is not even, 2..256")
+        if min(shape) < 1 or max(shape) >= 2**31 or self.head_dim % 2 or self.head_dim > 256:
+            raise ValueError("cache: empty, past 2^31 pages, or a head size that is not even, 2..256")
         args.pages, args.kv_heads, args.page_size, args.head_dim = shape
-
 
     # the pools are fixed: appends keep their addresses
     ek = property(lambda self: self._pools[0])
@@ -273,6 +272,8 @@ def rope_append_pair(ctx: Context, q, k, v, positions, slots, cos, sin, trunc: T
     if cache.device != ctx.device:
         raise ValueError(f"the cache is on cuda:{cache.device}, the context on cuda:{ctx.device}")
     tokens, kv, dim = k[0].shape[0], cache.kv_heads, cache.head_dim
+    if tokens >= 2**31:
+        raise ValueError("more than 2^31 tokens in one call")
     args = RopeAppend.from_buffer_copy(cache._args)
     k0, k1, k_ts, k_hs = _strided(ctx, "k", k, (tokens, kv, dim))
     v0, v1, v_ts, v_hs = _strided(ctx, "v", v, (tokens, kv, dim))
@@ -323,7 +324,7 @@ class AttnLayout:
         q, L = np.asarray(q_lens, dtype=np.int64).reshape(-1), np.asarray(ctx_lens, dtype=np.int64).reshape(-1)
         if q.size != L.size or (q < 0).any() or (L < 0).any():
             raise ValueError("layout: one non-negative query and context length per sequence")
-        if kv_heads < 1 or q_heads < kv_heads or q_heads % kv_heads or page_size < 1:
+        if kv_heads < 1 or q_heads < kv_heads or q_heads % kv_heads or page_size < 1 or max(q_heads, page_size) >= 2**31:
             raise ValueError("layout: query heads must be a multiple of key heads, the page size positive")
         if not isinstance(block_table, torch.Tensor):
             rows = [list(r) for r in block_table]

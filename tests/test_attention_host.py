@@ -376,3 +376,21 @@ def test_the_appends_packed_arguments_are_the_structs():
     assert [args.q_ts, args.q_hs, args.k_ts, args.k_hs, args.v_ts, args.v_hs] == list(range(7, 13))
     assert [args.d_positions, args.d_slots, args.d_cos, args.d_sin] == list(range(13, 17))
     assert list(args.d_a) == [17, 18] and args.d_dq == 19
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Sizes the entry points hold in 32 bits: refused, not cut off."""
+    import types
+
+    import torch
+
+    from suf_b200 import attention as at
+
+    for kw in (dict(q_heads=2**32 + 4), dict(page_size=2**32 + 16)):
+        with pytest.raises(ValueError, match="multiple of key heads"):
+            at.AttnLayout(_Ctx, **{**dict(q_lens=[1], ctx_lens=[3], block_table=[[0]], page_size=16, q_heads=4,
+                                          kv_heads=2), **kw})
+    k = (torch.zeros(1, 1, 2, dtype=torch.int64).expand(2**32 + 1, 1, 2),) * 2
+    cache = types.SimpleNamespace(device=0, kv_heads=1, head_dim=2)
+    with pytest.raises(ValueError, match="2\\^31 tokens"):
+        at.rope_append_pair(_Ctx, None, k, k, None, None, None, None, None, None, cache)
