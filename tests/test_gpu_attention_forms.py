@@ -1,0 +1,107 @@
+"""The forms of the tensor-core products that whole prompts take, against the
+definition in 64-bit words (tolerance zero): several key tiles a CTA, whole
+rows of values of more than eight chunks, ranges cut at the exact depth, and
+short sequences beside them.  Which form a case takes follows from the launch
+rule restated here, and every case says which one it is for."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from tests.conftest import from_dev
+from tests.test_gpu_attention import GUARD, U, _Attn, _guarded
+
+pytestmark = pytest.mark.gpu
+
+
+def _ceil(a, b):
+    return -(-a // b)
+
+
+def _launch(ctx, A):
+    """(key tiles per CTA of the scores, keys per CTA of the values, longest
+    context) of the sequences with more than eight rows per key head."""
+    group = A.hq // A.hkv
+    long_ = [(n, L) for n, L in zip(A.q, A.L) if n * group > 8]
+    tiles, ctx_len = sum(_ceil(n * group, 64) for n, _ in long_), max(L for _, L in long_)
+    two = 2 * ctx.sm_count
+    nt, nch = _ceil(ctx_len, 128), _ceil(ctx_len, 32)
+    span = min(_ceil(nt * tiles * A.hkv, two), nt)
+    units = tiles * _ceil(A.dh, 128) * A.hkv
+    keys = min(nch if units > ctx.sm_count else max(8, _ceil(units * nch, two)), nch) * 32
+    return span, min(keys, 4096), ctx_len
+
+
+SCORES = [  # (case, least key tiles a CTA); the last tile and the last row tile are ragged
+    (([(200, 1290)], 16, 16, 16, 64, True), 3),
+    (([(128, 2000), (1, 300)], 32, 32, 8, 32, True), 4),
+    (([(77, 1500), (130, 140)], 40, 20, 34, 16, False), 2),
+    (([(100, 1100)], 24, 24, 130, 64, True), 2),  # a wide head: both parts walk several tiles
+    (([(60, 50), (90, 1000), (3, 700)], 60, 20, 40, 100, True), 2),
+]
+
+
+@pytest.mark.parametrize("case,least", SCORES)
+def test_scores_of_several_key_tiles_a_cta(ctx, torch_cuda, case, least):
+    from suf_b200.attention import attn_scores_pair
+
+    A = _Attn(ctx, torch_cuda, case, 61)
+    assert _launch(ctx, A)[0] >= least
+    args, want = A.scores()
+    buf, out = _guarded(torch_cuda, want)
+    for _ in range(2):
+        out.fill_(5)
+        attn_scores_pair(ctx, *args, out=out)
+        ctx.sync()
+        assert (from_dev(out) == want).all() and (buf[want.size:] == 77).all()
+
+
+VALUES = [  # (case, whole rows)
+    (([(256, 600)], 40, 40, 8, 64, True), True),
+    (([(256, 600), (1, 400), (2, 300)], 40, 40, 8, 64, True), True),  # the short ones start from C, the prompt does not
+    (([(1, 290), (70, 400), (0, 33), (64, 333)], 60, 60, 18, 16, False), True),
+    (([(40, 30), (100, 400), (1, 380)], 40, 20, 130, 32, True), True),  # two tiles of words, queries without keys
+    (([(12, 5000)], 150, 150, 2, 64, True), False),  # whole rows would pass the exact depth
+    (([(16, 4500), (1, 4200)], 160, 160, 2, 64, False), False),
+    (([(70, 3000), (1, 700)], 16, 16, 24, 64, True), False),  # ranges of more than eight chunks
+]
+
+
+@pytest.mark.parametrize("case,whole", VALUES)
+def test_values_of_whole_rows_and_of_ranges(ctx, torch_cuda, case, whole):
+    from suf_b200.attention import attn_values_pair
+
+    A = _Attn(ctx, torch_cuda, case, 62)
+    _, keys, longest = _launch(ctx, A)
+    assert (keys >= longest) == whole and keys > 256
+    args, want = A.values()
+    buf, out = _guarded(torch_cuda, want)
+    for _ in range(2):
+        out.fill_(5)
+        attn_values_pair(ctx, *args, out=out)
+        ctx.sync()
+        assert (from_dev(out) == want).all() and (buf[want.size:] == 77).all()
+
+
+@pytest.mark.parametrize("L,keys", [(4096, 4096), (5000, 4096)])
+def test_values_are_exact_over_4096_keys_a_cta(ctx, torch_cuda, L, keys):
+    """Every word all ones, and more row tiles than SMs, so that one CTA adds up
+    4,096 keys: 8,192 products of 255 x 255 on every limb pair, eight pairs on the
+    highest diagonal, 8 * 8,192 * 255^2 = 4,261,478,400 < 2^32."""
+    from suf_b200.attention import AttnLayout, attn_values_pair
+
+    torch = torch_cuda
+    n, h, dh, page = 12, ctx.sm_count + 2, 32, 64
+    pages = _ceil(L, page)
+    lay = AttnLayout(ctx, [n], [L], [list(range(pages))], page, h, h, causal=False)
+    units, nch = h, _ceil(L, 32)
+    assert units > ctx.sm_count and min(nch * 32, 4096) == keys
+    ones = torch.full((pages, h, page, dh), -1, dtype=torch.int64, device="cuda")
+    pool = (ones, (ones, torch.zeros_like(ones)))  # E and W all ones
+    z_p = torch.zeros(lay.packed, dtype=torch.int64, device="cuda")
+    z_q = torch.zeros((n, h, dh), dtype=torch.int64, device="cuda")
+    buf = torch.full((z_q.numel() + GUARD,), 77, dtype=torch.int64, device="cuda")
+    out = buf[:z_q.numel()].view(z_q.shape)
+    attn_values_pair(ctx, (z_p - 1, z_p), (z_p, z_p), (z_q, z_q), (0, 0), *pool, lay, out=out)
+    ctx.sync()
+    assert (from_dev(out) == U(2 * L)).all() and (buf[z_q.numel():] == 77).all()  # (-1)(-1) twice per key
