@@ -75,6 +75,10 @@ def _empty(ctx: Context, shape, stream=None, like=None):
     return t
 
 
+def _elsewhere(ctx: Context, name: str, device: int):
+    raise ValueError(f"the {name} is on cuda:{device}, the context on cuda:{ctx.device}")
+
+
 def _refuse(ctx: Context, name: str, t, shape, dtype):
     if not isinstance(t, torch.Tensor) or t.dtype != dtype:
         raise ValueError(f"{name}: expected a {dtype} tensor")
@@ -161,7 +165,7 @@ class TruncPair(_Trunc):
             raise ValueError("TruncPair: 1..16 fractional bits")
         dev = torch.device("cuda", ctx.device)
         super().__init__(ctx, np.random.default_rng(seed), frac_bits, dev)
-        self.frac_bits = frac_bits
+        self.frac_bits, self.device = frac_bits, ctx.device
         self._full = TruncTables(self.bundles(), dev)
         if self._full.any():
             self._full.fill(ctx, _stream(ctx, stream) or 0)
@@ -174,6 +178,8 @@ class TruncPair(_Trunc):
     def eval_pair(self, ctx: Context, d_xhat, d_y0, d_y1, stream=None):
         """Both parties' truncated shares of the opened x^: lookups in the
         tables (a bundle without queries has none and is evaluated as it is)."""
+        if self.device != ctx.device:
+            _elsewhere(ctx, "truncation bundle", self.device)
         shape = d_xhat.shape
         for name, t in (("x^", d_xhat), ("y0", d_y0), ("y1", d_y1)):
             _want(ctx, name, t, shape)
@@ -270,7 +276,9 @@ def rope_append_pair(ctx: Context, q, k, v, positions, slots, cos, sin, trunc: T
     others distinct), queries opened against the mask shares a into d_q [tokens]
     [q_heads][head_dim], which is returned.  q, a None: append only."""
     if cache.device != ctx.device:
-        raise ValueError(f"the cache is on cuda:{cache.device}, the context on cuda:{ctx.device}")
+        _elsewhere(ctx, "cache", cache.device)
+    if trunc is not None and trunc.device != ctx.device:
+        _elsewhere(ctx, "truncation bundle", trunc.device)
     tokens, kv, dim = k[0].shape[0], cache.kv_heads, cache.head_dim
     if tokens >= 2**31:
         raise ValueError("more than 2^31 tokens in one call")
@@ -320,6 +328,7 @@ class AttnLayout:
 
     def __init__(self, ctx: Context, q_lens, ctx_lens, block_table, page_size: int, q_heads: int, kv_heads: int,
                  causal: bool = True):
+        self.device = ctx.device
         dev = torch.device("cuda", ctx.device)
         q, L = np.asarray(q_lens, dtype=np.int64).reshape(-1), np.asarray(ctx_lens, dtype=np.int64).reshape(-1)
         if q.size != L.size or (q < 0).any() or (L < 0).any():
@@ -393,6 +402,8 @@ class AttnLayout:
 
     def _for_pool(self, ctx, name, e, b):
         """(the sequences with the pool's sizes, the pool's address, its masks' addresses)"""
+        if self.device != ctx.device:
+            _elsewhere(ctx, "layout", self.device)
         e_ptr = _want(ctx, name, e, (None, self.kv_heads, self.page_size, None))
         shape = e.shape
         s = AttnSeqs.from_buffer_copy(self._seqs)
@@ -438,6 +449,7 @@ class RowMaxPlan:
     values[k] its packed values, `rounds` how often the longest row halves."""
 
     def __init__(self, ctx: Context, row_lengths):
+        self.device = ctx.device
         dev = torch.device("cuda", ctx.device)
         w = np.asarray(row_lengths, dtype=np.int64).reshape(-1)
         if (w < 0).any() or int(w.max(initial=0)) > 2**30 or int(w.sum()) >= 2**31:
@@ -458,6 +470,8 @@ class RowMaxPlan:
 
 def rowmax_open_pair(ctx: Context, plan: RowMaxPlan, c, r, out=None, stream=None):
     """x^ [pairs[0]]: the opened differences of the first round's pairs of c (packed shares)."""
+    if plan.device != ctx.device:
+        _elsewhere(ctx, "row max plan", plan.device)
     n = plan.pairs[0] if plan.rounds else 0
     words = _pair(ctx, "c", c, (plan.values[0],))
     if out is None:
@@ -473,6 +487,8 @@ def rowmax_round_pair(ctx: Context, plan: RowMaxPlan, k: int, c, relu, r_next=No
     """Round k: its values c (packed shares) and the gate's shares relu of its
     pairs to the next round's values, and, with r_next, the open of their
     differences.  Returns ((next_0, next_1), x^ or None)."""
+    if plan.device != ctx.device:
+        _elsewhere(ctx, "row max plan", plan.device)
     if not 0 <= k < plan.rounds:
         raise ValueError(f"rowmax: round {k} of {plan.rounds}")
     n, more = plan.values[k + 1], k + 1 < plan.rounds
@@ -500,6 +516,8 @@ def rowmax_round_pair(ctx: Context, plan: RowMaxPlan, k: int, c, relu, r_next=No
 
 def maxdiff_ragged_pair(ctx: Context, plan: RowMaxPlan, m, s, out=None, stream=None):
     """t_p = max_p[row] - s_p over the packed rows: m the last round's values, s the first's."""
+    if plan.device != ctx.device:
+        _elsewhere(ctx, "row max plan", plan.device)
     n = (plan.values[0],)
     top, words = _pair(ctx, "max", m, (plan.values[-1],)), _pair(ctx, "s", s, n)
     if out is None:
@@ -525,6 +543,9 @@ class CachedAttentionPair:
 
     def __init__(self, ctx: Context, cache: ShareCache, layout: AttnLayout, seed: int = 1,
                  score_shift: int | None = None, rope: tuple | None = None, interleaved: bool = False):
+        for name, what in (("cache", cache), ("layout", layout)):
+            if what.device != ctx.device:
+                _elsewhere(ctx, name, what.device)
         if layout.kv_heads != cache.kv_heads or layout.page_size != cache.page_size:
             raise ValueError("attention: the layout's heads or pages are not the cache's")
         dim = cache.head_dim

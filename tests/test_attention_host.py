@@ -394,3 +394,36 @@ def test_sizes_past_32_bits_are_refused():
     cache = types.SimpleNamespace(device=0, kv_heads=1, head_dim=2)
     with pytest.raises(ValueError, match="2\\^31 tokens"):
         at.rope_append_pair(_Ctx, None, k, k, None, None, None, None, None, None, cache)
+
+
+def test_plans_of_another_device_are_refused():
+    """Layouts, row max plans, truncation bundles and caches hold addresses of the
+    device they were made on: a context of another one takes none of them."""
+    import types
+
+    from suf_b200 import attention as at
+
+    def made(cls, **kw):
+        x = cls.__new__(cls)
+        x.__dict__.update(device=1, **kw)
+        return x
+
+    layout = made(at.AttnLayout, tokens=1, packed=1, q_heads=1, kv_heads=1, page_size=1)
+    plan = made(at.RowMaxPlan, rows=1, rounds=1, pairs=[1], values=[2, 1], widths=[2, 1])
+    trunc, cache = made(at.TruncPair, frac_bits=12), made(at.ShareCache, kv_heads=1, page_size=1, head_dim=4)
+    here = types.SimpleNamespace(device=0, kv_heads=1, page_size=1, head_dim=4)
+    none = (None, None)
+    for said, call in [
+            ("layout", lambda: at.attn_scores_pair(_Ctx, None, none, none, (1, 2), None, none, layout)),
+            ("layout", lambda: at.attn_values_pair(_Ctx, none, none, none, (1, 2), None, none, layout)),
+            ("row max plan", lambda: at.rowmax_open_pair(_Ctx, plan, none, (1, 2))),
+            ("row max plan", lambda: at.rowmax_round_pair(_Ctx, plan, 0, none, none)),
+            ("row max plan", lambda: at.maxdiff_ragged_pair(_Ctx, plan, none, none)),
+            ("truncation bundle", lambda: trunc.eval_pair(_Ctx, None, None, None)),
+            ("truncation bundle", lambda: at.rope_append_pair(_Ctx, None, none, none, None, None, None, None, trunc, None,
+                                                              here)),
+            ("cache", lambda: at.rope_append_pair(_Ctx, None, none, none, None, None, None, None, None, None, cache)),
+            ("cache", lambda: at.CachedAttentionPair(_Ctx, cache, layout)),
+            ("layout", lambda: at.CachedAttentionPair(_Ctx, here, layout))]:
+        with pytest.raises(ValueError, match=f"the {said} is on cuda:1, the context on cuda:0"):
+            call()
