@@ -773,12 +773,12 @@ int sufb200_rope_append_pair(sufb200_ctx ctx, const sufb200_rope_append* args, v
  * words, and sequence b's rows start at word d_row_base[b].  max_q and max_ctx
  * bound the lengths, min_q the new tokens of the sequences that have any (from
  * below: short and long ones are computed by different kernels); tokens, cached
- * and packed are the sums of the new tokens, the cached tokens and the words
- * (workspaces are sized by them).  At most 2^26 cached tokens in a sequence,
+ * and packed are the sums of the new tokens, the cached tokens and the words.  At most 2^26 cached tokens in a sequence,
  * 65,535 (sequence, key head) pairs and 2^20 rows (queries of its heads) per
  * pair. */
 #define SUFB200_ATTN_FEW_ROWS 8  /* rows of a (sequence, key head) up to which it counts as short */
 #define SUFB200_ATTN_ROW_TILE 64 /* rows of a row tile */
+#define SUFB200_ATTN_KEY_TILE 128 /* cached tokens of a key tile */
 typedef struct sufb200_attn_seqs {
   const int32_t* d_cu_q;        /* [batch + 1] */
   const int32_t* d_cu_ctx;      /* [batch + 1] */
@@ -791,6 +791,13 @@ typedef struct sufb200_attn_seqs {
   const int32_t* d_tiles; /* [n_tiles][2] */
   int64_t tokens, cached, packed;
   int32_t batch, max_pages, page_size, pages, q_heads, kv_heads, head_dim, causal, min_q, max_q, max_ctx, n_tiles;
+  /* (since 1.1) Where a long sequence's cached tokens lie in the products'
+   * workspace, or NULL (room for all `cached` tokens of the call): [batch + 1], from
+   * 0 on, every sequence with more than SUFB200_ATTN_FEW_ROWS rows per key head taking
+   * its cached tokens rounded up to SUFB200_ATTN_KEY_TILE, the others nothing.
+   * plane_keys, a positive multiple of SUFB200_ATTN_KEY_TILE, bounds the last entry. */
+  const int32_t* d_plane_keys;
+  int64_t plane_keys;
 } sufb200_attn_seqs;
 
 /* Scores: x^ = sum_p (C_p + D B_p + A_p E (+ D E for party 0) + r[p]) for every

@@ -30,6 +30,7 @@ TRUNC_GAPARS = 2
 
 ATTN_FEW_ROWS = 8  # SUFB200_ATTN_FEW_ROWS
 ATTN_ROW_TILE = 64  # SUFB200_ATTN_ROW_TILE
+ATTN_KEY_TILE = 128  # SUFB200_ATTN_KEY_TILE
 
 NOALLOC_KEY_BYTES = 16384  # SUFB200_NOALLOC_KEY_BYTES
 
@@ -80,6 +81,7 @@ class AttnSeqs(C.Structure):
         ("batch", C.c_int32), ("max_pages", C.c_int32), ("page_size", C.c_int32), ("pages", C.c_int32),
         ("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("causal", C.c_int32),
         ("min_q", C.c_int32), ("max_q", C.c_int32), ("max_ctx", C.c_int32), ("n_tiles", C.c_int32),
+        ("d_plane_keys", C.c_void_p), ("plane_keys", C.c_int64),
     ]
 
 

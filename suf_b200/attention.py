@@ -378,6 +378,10 @@ class AttnLayout:
         if len(tiles):
             self._tiles = torch.from_numpy(tiles).to(dev)
             s.d_tiles, s.n_tiles = self._tiles.data_ptr(), len(tiles)
+            places = self._plane_keys()
+            if places is not None:
+                self._places = torch.from_numpy(places).to(dev)
+                s.d_plane_keys, s.plane_keys = self._places.data_ptr(), max(int(places[-1]), _lib.ATTN_KEY_TILE)
 
     def _tile_list(self) -> np.ndarray:
         """(sequence, row tile) of the sequences with many rows, the longest rows first."""
@@ -393,6 +397,16 @@ class AttnLayout:
         length = self.ctx_lens[seq] + (last + 1 - self.q_lens[seq] if self.causal else 0)
         order = np.argsort(-length, kind="stable")
         return np.stack([seq, tile], axis=1)[order].astype(np.int32)
+
+    def _plane_keys(self) -> np.ndarray | None:
+        """Where the cached tokens of the sequences with many rows lie in the products' workspace (prefix
+        sums, whole key tiles); None where those are all sequences there are, or past 32 bits."""
+        long_ = self.q_lens * (self.q_heads // self.kv_heads) > _lib.ATTN_FEW_ROWS
+        if not self.ctx_lens[~long_].any():
+            return None
+        tile = _lib.ATTN_KEY_TILE
+        at = np.concatenate([[0], np.cumsum(np.where(long_, -(-self.ctx_lens // tile) * tile, 0))])
+        return at.astype(np.int32) if at[-1] < 2**31 - tile else None
 
     def row_lengths(self) -> np.ndarray:
         """Keys of every row, in (sequence, head, query) order."""

@@ -302,6 +302,9 @@ int check_seqs(const sufb200_attn_seqs* s, const char* who) {
     return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^60 packed words");
   if (s->n_tiles < 0 || (s->n_tiles > 0) != (s->d_tiles != nullptr))
     return fail(SUFB200_ERR_INVALID, at + "null or empty tile list");
+  if ((s->plane_keys > 0) != (s->d_plane_keys != nullptr) || s->plane_keys < 0 || s->plane_keys > INT32_MAX ||
+      s->plane_keys % SUFB200_ATTN_KEY_TILE)
+    return fail(SUFB200_ERR_INVALID, at + "null or empty list of places, or not in whole key tiles");
   if (s->batch > 0 && (!s->d_cu_q || !s->d_cu_ctx || !s->d_row_base || (s->max_ctx > 0 && !s->d_block_table)))
     return fail(SUFB200_ERR_INVALID, at + "null sequence array");
   return SUFB200_OK;

@@ -47,6 +47,18 @@ SUFB200_HD int64_t row_off(int n, int L, int causal, int i) {
 SUFB200_HD int64_t first_block(int64_t c, int b, int per) { return c / per + b; }
 inline int64_t blocks_of(int64_t items, int batch, int per) { return items / per + batch; }
 
+// The long sequences' places in the planes' workspace: from the list where the
+// call has one, else every sequence's cached tokens have room.
+inline int64_t plane_blocks(const AttnSeqs& s, int per) {
+  return s.d_plane_keys ? s.plane_keys / per : blocks_of(s.cached, s.batch, per);
+}
+
+// Whether the list's entries p0, p1 of a sequence of L cached tokens give it
+// room inside the workspace, from a whole key tile on.
+SUFB200_HD bool plane_fits(const AttnSeqs& s, int p0, int p1, int L) {
+  return p0 >= 0 && p0 % SUFB200_ATTN_KEY_TILE == 0 && p1 <= s.plane_keys && p1 >= p0 && p1 - p0 >= L;
+}
+
 // Whether a sequence's lengths and rows lie inside what the host arguments
 // say (so every address formed from them does too); fills q.
 SUFB200_HD bool seq_fits(const AttnSeqs& s, int c0, int c1, int l0, int l1, int64_t base, SeqInfo& q) {
@@ -70,14 +82,14 @@ SUFB200_HD int64_t page_word(const AttnSeqs& s, int pg, int kh, int j) {
 
 #if defined(__CUDACC__)
 // The sequence block g of the list belongs to (m items per entry of cu, [batch
-// + 1]): the last one that starts at or before g.  A whole warp searches, 32
-// sequences a round.
-__device__ __forceinline__ int block_seq(const int32_t* cu, int batch, int m, int per, int64_t g) {
+// + 1]; room = 0: sequences fill whole blocks and none is left between them): the
+// last one that starts at or before g.  A whole warp searches, 32 sequences a round.
+__device__ __forceinline__ int block_seq(const int32_t* cu, int batch, int m, int per, int64_t g, int room = 1) {
   const int lane = threadIdx.x & 31;
   int lo = 0, hi = batch;
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32, i = lo + (lane + 1) * step;
-    const bool before = i < hi && first_block(static_cast<int64_t>(m) * cu[i], i, per) <= g;
+    const bool before = i < hi && first_block(static_cast<int64_t>(m) * cu[i], i * room, per) <= g;
     lo += __popc(__ballot_sync(0xffffffffu, before)) * step;
     hi = lo + step < hi ? lo + step : hi;
   }
@@ -90,6 +102,16 @@ __device__ __forceinline__ bool seq_info(const AttnSeqs& s, int b, uint32_t* sta
   const bool ok = seq_fits(s, s.d_cu_q[b], s.d_cu_q[b + 1], s.d_cu_ctx[b], s.d_cu_ctx[b + 1], s.d_row_base[b], q);
   if (!ok) atomicOr(status, kStatusBadArgument);
   return ok;
+}
+
+// First block of `per` keys of sequence b in the planes; -1 (and the status word
+// flagged) when the list of places does not hold it.
+__device__ __forceinline__ int64_t plane_first(const AttnSeqs& s, int b, const SeqInfo& q, int per, uint32_t* status) {
+  if (!s.d_plane_keys) return first_block(q.l0, b, per);
+  const int p0 = s.d_plane_keys[b], p1 = s.d_plane_keys[b + 1];
+  if (plane_fits(s, p0, p1, q.L)) return p0 / per;
+  atomicOr(status, kStatusBadArgument);
+  return -1;
 }
 
 // Word offset of cached token j of sequence b, key head kh; -1 (and the

@@ -15,7 +15,8 @@
 //
 // The cached operand is read by every row tile of its group of heads, so a
 // pre-pass writes its byte planes once, one contiguous 32 KB block per step
-// (bulk copies, no multicast).  The rows' planes are made inside: for the
+// (bulk copies, no multicast); a list of places keeps room for the long
+// sequences alone.  The rows' planes are made inside: for the
 // scores once per CTA (they stay in shared memory while the keys stream past),
 // for the values chunk by chunk from the packed shares, which are read
 // nowhere else.
@@ -38,7 +39,7 @@ namespace sufb200 {
 
 namespace {
 
-static_assert(kTN == SUFB200_ATTN_ROW_TILE, "row tile");
+static_assert(kTN == SUFB200_ATTN_ROW_TILE && kTM == SUFB200_ATTN_KEY_TILE && kTM % kTK == 0, "tiles");
 constexpr int kThreads = 640;  // warp 0 copies A, warp 1 issues MMAs, warps 4-19 make B planes and store
 constexpr int kWorkers = 512;
 constexpr uint32_t kAStage = 8 * kPlaneX;  // 32 KB: A planes of one step
@@ -118,11 +119,13 @@ __global__ void __launch_bounds__(256) cache_planes_kernel(const __grid_constant
   __shared__ int64_t s_key[kTM];
   const AttnSeqs& s = a.s;
   constexpr int kPer = KEYS ? kTM : kTK;
-  const int t = threadIdx.x, b = block_seq(s.d_cu_ctx, s.batch, 1, kPer, blockIdx.x), kh = blockIdx.z;
+  const int t = threadIdx.x, kh = blockIdx.z;
+  const int b = s.d_plane_keys ? block_seq(s.d_plane_keys, s.batch, 1, kPer, blockIdx.x, 0)
+                               : block_seq(s.d_cu_ctx, s.batch, 1, kPer, blockIdx.x);
   SeqInfo q;
   if (!seq_info(s, b, a.o.status, q) || s.q_heads / s.kv_heads * q.n <= a.o.few) return;
-  const int64_t first = blockIdx.x - first_block(q.l0, b, kPer);  // this block in its sequence
-  if (first < 0 || first * kPer >= q.L) return;
+  const int64_t plane = plane_first(s, b, q, kPer, a.o.status), first = blockIdx.x - plane;  // this block in its sequence
+  if (plane < 0 || first < 0 || first * kPer >= q.L) return;
   const int j0 = static_cast<int>(first) * kPer;
   for (int e = t; e < kPer; e += 256) s_key[e] = j0 + e < q.L ? key_off(s, b, kh, j0 + e, a.o.status) : -1;
   __syncthreads();
@@ -391,7 +394,8 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
   const int len = rho0 >= 0 && rho0 < R ? row_len(q.n, q.L, s.causal, last / group) : 0;
   const int nt = (len + kTM - 1) / kTM, tile0 = blockIdx.y * a.span;
   const int tiles = nt - tile0 < a.span ? nt - tile0 : a.span;
-  if (tiles <= 0) {
+  const int64_t plane = tiles > 0 ? plane_first(s, b, q, kTM, o.status) : -1;
+  if (plane < 0) {
     pdl_wait();
     return;
   }
@@ -409,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
   } else if (warp == 0) {  // A planes: every step of every key tile
     pdl_wait();  // written by the pre-pass
     const int64_t next = 2 * static_cast<int64_t>(a.chunks) * kAStage;  // from a key tile to the one after
-    const uint8_t* src = a.planes + (kh * a.tiles + first_block(q.l0, b, kTM) + tile0) * next + 2 * a.chunk0 * kAStage;
+    const uint8_t* src = a.planes + (kh * a.tiles + plane + tile0) * next + 2 * a.chunk0 * kAStage;
     int go = 1;
     for (int tl = 0; tl < tiles && go; tl++, src += next)
       for (int st = 0; st < steps && go; st++) {
@@ -580,6 +584,11 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
       }
     return;
   }
+  const int64_t plane = plane_first(s, b, q, kTK, o.status);
+  if (plane < 0) {
+    pdl_wait();
+    return;
+  }
   const uint32_t sbase = smem_u32(smem);
   const Ctrl c = ctrl_at(smem, kBOff + kBStages * kBStage);
   if (t < kTN) {
@@ -594,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1) values_tc_kernel(const __grid_con
   if (!ready) {
   } else if (warp == 0) {
     pdl_wait();
-    const int64_t block0 = kh * a.tiles + first_block(q.l0, b, kTK) + beg / kTK;
+    const int64_t block0 = kh * a.tiles + plane + beg / kTK;
     for (int li = 0; li < 2 * nch; li++) {
       int go = 1;
       if (lane == 0) {
@@ -765,7 +774,7 @@ constexpr int kMostChunks = 4;
 cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st) {
   const int64_t rts = row_tiles(s);
   const int nt = (s.max_ctx + kTM - 1) / kTM;
-  AttnTc a{s, o, nullptr, blocks_of(s.cached, s.batch, kTM), (s.head_dim + kTK - 1) / kTK, 0, 0, 0};
+  AttnTc a{s, o, nullptr, plane_blocks(s, kTM), (s.head_dim + kTK - 1) / kTK, 0, 0, 0};
   const int64_t bytes = a.tiles * s.kv_heads * a.chunks * 2 * static_cast<int64_t>(kAStage);
   cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&a.planes), bytes, ctx->pool, st);
   if (e != cudaSuccess) return e;
@@ -806,7 +815,7 @@ int values_span(const sufb200_ctx_s* ctx, const AttnSeqs& s) {
 bool values_tc_solo(const sufb200_ctx_s* ctx, const AttnSeqs& s) { return values_span(ctx, s) >= s.max_ctx; }
 
 cudaError_t launch_values_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st) {
-  AttnTc a{s, o, nullptr, blocks_of(s.cached, s.batch, kTK), (s.head_dim + kTM - 1) / kTM, 0, 0, values_span(ctx, s)};
+  AttnTc a{s, o, nullptr, plane_blocks(s, kTK), (s.head_dim + kTM - 1) / kTM, 0, 0, values_span(ctx, s)};
   const int64_t bytes = a.tiles * s.kv_heads * a.chunks * 2 * static_cast<int64_t>(kAStage);
   cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&a.planes), bytes, ctx->pool, st);
   if (e != cudaSuccess) return e;

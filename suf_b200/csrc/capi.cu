@@ -166,7 +166,7 @@ cudaError_t probe_dyn_smem_base(uint32_t* d_out, cudaStream_t st) {
 
 extern "C" {
 
-int sufb200_version(void) { return 10000; }
+int sufb200_version(void) { return 10100; }
 
 const char* sufb200_last_error(void) { return g_err.c_str(); }
 

@@ -24,3 +24,4 @@ size_t emu_sizeof(int which) { return which == 0 ? sizeof(sufb200_rope_append) :
 
 extern "C" int64_t emu_first_block(int64_t c, int b, int per) { return first_block(c, b, per); }
 extern "C" int64_t emu_blocks_of(int64_t items, int batch, int per) { return blocks_of(items, batch, per); }
+extern "C" int emu_plane_fits(const sufb200_attn_seqs* s, int p0, int p1, int L) { return plane_fits(*s, p0, p1, L); }

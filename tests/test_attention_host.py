@@ -427,3 +427,41 @@ def test_plans_of_another_device_are_refused():
             ("layout", lambda: at.CachedAttentionPair(_Ctx, here, layout))]:
         with pytest.raises(ValueError, match=f"the {said} is on cuda:1, the context on cuda:0"):
             call()
+
+
+def _layout(q, L, q_heads, kv_heads, causal=True):
+    """An AttnLayout's lengths, without its device side."""
+    from suf_b200 import attention as at
+
+    lay = at.AttnLayout.__new__(at.AttnLayout)
+    lay.q_lens, lay.ctx_lens, lay.causal = np.asarray(q, dtype=np.int64), np.asarray(L, dtype=np.int64), causal
+    lay.q_heads, lay.kv_heads = q_heads, kv_heads
+    return lay
+
+
+def test_workspace_places_of_long_sequences(emu):
+    """Only sequences with more than eight rows per key head take room, in whole
+    key tiles, each disjoint from the others; a batch of long ones alone needs no list."""
+    q, L = [2048, 1, 0, 3, 2, 9, 1], [2048, 16384, 777, 300, 500, 0, 0]
+    at = _layout(q, L, 8, 2)._plane_keys()  # groups of four: nine rows from three tokens on
+    assert at.tolist() == [0, 2048, 2048, 2048, 2048 + 384, 2048 + 384, 2048 + 384, 2048 + 384] and at.dtype == np.int32
+    assert _layout([3, 40], [5, 900], 8, 2)._plane_keys() is None
+    assert _layout([3, 1], [5, 0], 8, 2)._plane_keys() is None  # the short one has nothing cached
+    assert _layout([64] * 40 + [1], [2**26] * 40 + [5], 1, 1)._plane_keys() is None  # past 32 bits
+    s = _seqs(plane_keys=2432)
+    for p0, p1, n in [(0, 2048, 2048), (2048, 2432, 300), (2432, 2432, 0), (0, 2432, 1)]:
+        assert emu.emu_plane_fits(C.byref(s), p0, p1, n)
+    for p0, p1, n in [(-128, 128, 5), (0, 128, 129), (64, 256, 5), (2048, 2433, 300), (128, 0, 0), (2**31 - 128, 2**31 - 1, 5),
+                      (0, -2**31, 5), (-2**31, 2**31 - 1, 5)]:
+        assert not emu.emu_plane_fits(C.byref(s), p0, p1, n), (p0, p1, n)
+
+
+@pytest.mark.parametrize("which", ["scores", "values"])
+def test_wrong_workspace_places_are_refused(host, which):
+    from suf_b200 import _lib
+
+    assert _attn(host, which, _seqs(**PTRS, d_plane_keys=P16, plane_keys=256)) == _lib.ERR_UNSUPPORTED
+    assert b"host-only" in _lib.lib().sufb200_last_error()
+    for kw in [dict(plane_keys=128), dict(d_plane_keys=P16), dict(d_plane_keys=P16, plane_keys=-128),
+               dict(d_plane_keys=P16, plane_keys=130), dict(d_plane_keys=P16, plane_keys=2**31)]:
+        assert _attn(host, which, _seqs(**PTRS, **kw)) == _lib.ERR_INVALID, kw

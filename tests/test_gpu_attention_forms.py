@@ -105,3 +105,62 @@ def test_values_are_exact_over_4096_keys_a_cta(ctx, torch_cuda, L, keys):
     attn_values_pair(ctx, (z_p - 1, z_p), (z_p, z_p), (z_q, z_q), (0, 0), *pool, lay, out=out)
     ctx.sync()
     assert (from_dev(out) == U(2 * L)).all() and (buf[z_q.numel():] == 77).all()  # (-1)(-1) twice per key
+
+
+@pytest.mark.parametrize("which", ["scores", "values"])
+def test_workspace_follows_the_prompts_and_not_the_batch(ctx, torch_cuda, which):
+    """A prompt of 40 tokens beside 300 idle caches of 2^22 tokens (all on the same
+    pages: nothing reads them): planes of all of them would take 640 GB."""
+    from suf_b200 import attention as at
+
+    A = _Attn(ctx, torch_cuda, ([(20, 40)], 2, 2, 2, 65536, True), 63)
+    args, want = getattr(A, which)()
+    idle = [A.table[0] * 64] * 300
+    lay = at.AttnLayout(ctx, A.q + [0] * 300, A.L + [2**22] * 300, A.table + idle, A.page, A.hq, A.hkv)
+    got = getattr(at, f"attn_{which}_pair")(ctx, *args[:-1], lay)
+    ctx.sync()
+    assert (from_dev(got) == want).all()
+
+
+MIXED = [  # long sequences between short ones, idle ones and empty caches
+    ([(1, 300), (70, 130), (0, 200), (1, 0), (33, 257), (2, 77), (20, 5)], 4, 2, 66, 16, True),
+    ([(12, 0), (1, 500), (1, 129)], 2, 1, 32, 64, True),  # the long sequence has no keys: nothing takes room
+    ([(1, 40), (24, 300), (1, 128), (130, 128)], 3, 1, 160, 32, False),
+]
+
+
+@pytest.mark.parametrize("which", ["scores", "values"])
+@pytest.mark.parametrize("case", MIXED)
+def test_long_and_short_sequences_with_and_without_places(ctx, torch_cuda, which, case):
+    from suf_b200 import attention as at
+
+    A = _Attn(ctx, torch_cuda, case, 64)
+    args, want = getattr(A, which)()
+    call = getattr(at, f"attn_{which}_pair")
+    assert A.layout._seqs.plane_keys > 0
+    for places in (True, False):
+        if not places:
+            A.layout._seqs.d_plane_keys, A.layout._seqs.plane_keys = None, 0
+        buf, out = _guarded(torch_cuda, want)
+        call(ctx, *args, out=out)
+        ctx.sync()
+        assert (from_dev(out) == want).all() and (buf[want.size:] == 77).all()
+
+
+@pytest.mark.parametrize("which", ["scores", "values"])
+def test_attention_reports_bad_places(ctx, torch_cuda, which):
+    from suf_b200 import SufB200Error
+    from suf_b200 import attention as at
+
+    A = _Attn(ctx, torch_cuda, MIXED[0], 65)
+    args, want = getattr(A, which)()
+    call, good = getattr(at, f"attn_{which}_pair"), A.layout._places.clone()
+    for i, bad in [(1, -128), (1, 64), (2, 128), (5, 2**31 - 1), (4, 2**31 - 128), (4, -2**31)]:
+        A.layout._places[i] = bad
+        call(ctx, *args)
+        with pytest.raises(SufB200Error):
+            ctx.sync()
+        A.layout._places.copy_(good)
+    got = call(ctx, *args)
+    ctx.sync()
+    assert (from_dev(got) == want).all()
