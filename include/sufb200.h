@@ -798,6 +798,11 @@ typedef struct sufb200_attn_seqs {
    * plane_keys, a positive multiple of SUFB200_ATTN_KEY_TILE, bounds the last entry. */
   const int32_t* d_plane_keys;
   int64_t plane_keys;
+  /* (since 1.1) Bounds by which the work of long and short sequences is dealt out,
+   * each for itself, or 0 (max_ctx, and SUFB200_ATTN_FEW_ROWS rows): the most cached
+   * tokens of a sequence with more than SUFB200_ATTN_FEW_ROWS rows per key head, and the
+   * most rows of the others. */
+  int32_t long_ctx, short_rows;
 } sufb200_attn_seqs;
 
 /* Scores: x^ = sum_p (C_p + D B_p + A_p E (+ D E for party 0) + r[p]) for every

@@ -81,7 +81,7 @@ class AttnSeqs(C.Structure):
         ("batch", C.c_int32), ("max_pages", C.c_int32), ("page_size", C.c_int32), ("pages", C.c_int32),
         ("q_heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("causal", C.c_int32),
         ("min_q", C.c_int32), ("max_q", C.c_int32), ("max_ctx", C.c_int32), ("n_tiles", C.c_int32),
-        ("d_plane_keys", C.c_void_p), ("plane_keys", C.c_int64),
+        ("d_plane_keys", C.c_void_p), ("plane_keys", C.c_int64), ("long_ctx", C.c_int32), ("short_rows", C.c_int32),
     ]
 
 

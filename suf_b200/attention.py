@@ -374,6 +374,7 @@ class AttnLayout:
         s.page_size, s.q_heads, s.kv_heads, s.causal = self.page_size, self.q_heads, self.kv_heads, int(self.causal)
         s.min_q, s.max_q, s.max_ctx = int(q[q > 0].min(initial=2**31 - 1)), int(q.max(initial=0)), int(L.max(initial=0))
         s.min_q = min(s.min_q, s.max_q)
+        s.long_ctx, s.short_rows = self._bounds()
         tiles = self._tile_list()
         if len(tiles):
             self._tiles = torch.from_numpy(tiles).to(dev)
@@ -397,6 +398,12 @@ class AttnLayout:
         length = self.ctx_lens[seq] + (last + 1 - self.q_lens[seq] if self.causal else 0)
         order = np.argsort(-length, kind="stable")
         return np.stack([seq, tile], axis=1)[order].astype(np.int32)
+
+    def _bounds(self) -> tuple[int, int]:
+        """The longest context of the sequences with many rows, the most rows of the others."""
+        rows = self.q_lens * (self.q_heads // self.kv_heads)
+        many = rows > _lib.ATTN_FEW_ROWS
+        return int(self.ctx_lens[many].max(initial=0)), int(rows[~many].max(initial=0))
 
     def _plane_keys(self) -> np.ndarray | None:
         """Where the cached tokens of the sequences with many rows lie in the products' workspace (prefix

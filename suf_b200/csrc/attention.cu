@@ -272,7 +272,7 @@ struct Rows {
 Rows rows_of(const AttnSeqs& s) {
   const int group = s.q_heads / s.kv_heads;
   Rows r{group * s.max_q, 0};
-  if (group * s.min_q <= kFewRows) r.few = r.most <= kFewRows ? r.most : kFewRows;
+  if (group * s.min_q <= kFewRows) r.few = s.short_rows > 0 ? s.short_rows : (r.most <= kFewRows ? r.most : kFewRows);
   return r;
 }
 
@@ -300,6 +300,8 @@ int check_seqs(const sufb200_attn_seqs* s, const char* who) {
     return fail(SUFB200_ERR_INVALID, at + "max_ctx is more than the block table's pages hold");
   if (static_cast<__int128>(s->q_heads) * s->max_q * s->max_ctx >= (static_cast<__int128>(1) << 60))
     return fail(SUFB200_ERR_UNSUPPORTED, at + "more than 2^60 packed words");
+  if (s->long_ctx < 0 || s->long_ctx > s->max_ctx || s->short_rows < 0 || s->short_rows > kFewRows)
+    return fail(SUFB200_ERR_INVALID, at + "bounds of the long or short sequences");
   if (s->n_tiles < 0 || (s->n_tiles > 0) != (s->d_tiles != nullptr))
     return fail(SUFB200_ERR_INVALID, at + "null or empty tile list");
   if ((s->plane_keys > 0) != (s->d_plane_keys != nullptr) || s->plane_keys < 0 || s->plane_keys > INT32_MAX ||
@@ -385,7 +387,7 @@ int sufb200_attn_scores_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
     else
       scores_rows_kernel<8><<<grid, kThreads, smem, st>>>(*seqs, o, chunk);
   }
-  o.few = rows.few;
+  o.few = rows.few > 0 ? kFewRows : 0;
   if (rows.most > kFewRows) {
     const cudaError_t e = launch_scores_tc(ctx, *seqs, o, st);
     if (e != cudaSuccess) return attn_result("attn_scores_pair", e);
@@ -429,7 +431,7 @@ int sufb200_attn_values_pair(sufb200_ctx ctx, const sufb200_attn_seqs* seqs, con
                                       : (few_solo ? values_rows_kernel<8, true> : values_rows_kernel<8, false>);
     kernel<<<grid, kThreads, 0, st>>>(*seqs, o, range);
   }
-  o.few = rows.few;
+  o.few = rows.few > 0 ? kFewRows : 0;
   if (any && rows.most > kFewRows) {
     const cudaError_t e = launch_values_tc(ctx, *seqs, o, st);
     if (e != cudaSuccess) return attn_result("attn_values_pair", e);

@@ -69,6 +69,8 @@ SUFB200_HD bool seq_fits(const AttnSeqs& s, int c0, int c1, int l0, int l1, int6
       L > static_cast<int64_t>(s.max_pages) * s.page_size || base < 0 || base > s.packed)
     return false;
   q.n = c1 - c0;
+  const int rows = s.q_heads / s.kv_heads * q.n;  // of a key head
+  if (rows > SUFB200_ATTN_FEW_ROWS ? s.long_ctx > 0 && L > s.long_ctx : s.short_rows > 0 && rows > s.short_rows) return false;
   q.blk = row_off(q.n, L, s.causal, q.n);
   return q.blk * s.q_heads <= s.packed - base;
 }
@@ -151,6 +153,9 @@ int attn_check_ctx(sufb200_ctx ctx);
 // runtime's own last error: a workspace that could not be had is not an error
 // of the calls after it).
 int attn_result(const char* who, cudaError_t e);
+
+// The longest context of the sequences on the tensor cores.
+inline int long_ctx(const AttnSeqs& s) { return s.long_ctx > 0 ? s.long_ctx : s.max_ctx; }
 
 inline bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 

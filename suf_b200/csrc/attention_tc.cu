@@ -773,7 +773,7 @@ constexpr int kMostChunks = 4;
 
 cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st) {
   const int64_t rts = row_tiles(s);
-  const int nt = (s.max_ctx + kTM - 1) / kTM;
+  const int nt = (long_ctx(s) + kTM - 1) / kTM;
   AttnTc a{s, o, nullptr, plane_blocks(s, kTM), (s.head_dim + kTK - 1) / kTK, 0, 0, 0};
   const int64_t bytes = a.tiles * s.kv_heads * a.chunks * 2 * static_cast<int64_t>(kAStage);
   cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&a.planes), bytes, ctx->pool, st);
@@ -800,7 +800,7 @@ cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const 
 
 // Keys per CTA of the values form, and whether one CTA takes whole rows.
 int values_span(const sufb200_ctx_s* ctx, const AttnSeqs& s) {
-  const int nch = (s.max_ctx + kTK - 1) / kTK, words = (s.head_dim + kTM - 1) / kTM;
+  const int nch = (long_ctx(s) + kTK - 1) / kTK, words = (s.head_dim + kTM - 1) / kTM;
   const int64_t units = row_tiles(s) * words * s.kv_heads;
   // whole rows where there is more than one row tile an SM (no pass that starts
   // the output from C: 16 / 4 heads of 128, 1,024 tokens 83 us, 94 split), else
@@ -812,7 +812,7 @@ int values_span(const sufb200_ctx_s* ctx, const AttnSeqs& s) {
   return span > kMaxDepthKeys ? kMaxDepthKeys : span;
 }
 
-bool values_tc_solo(const sufb200_ctx_s* ctx, const AttnSeqs& s) { return values_span(ctx, s) >= s.max_ctx; }
+bool values_tc_solo(const sufb200_ctx_s* ctx, const AttnSeqs& s) { return values_span(ctx, s) >= long_ctx(s); }
 
 cudaError_t launch_values_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const AttnOperands& o, cudaStream_t st) {
   AttnTc a{s, o, nullptr, plane_blocks(s, kTK), (s.head_dim + kTM - 1) / kTM, 0, 0, values_span(ctx, s)};
@@ -822,9 +822,9 @@ cudaError_t launch_values_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const 
   cache_planes_kernel<false><<<dim3(static_cast<unsigned>(a.tiles), a.chunks, s.kv_heads), 256, 0, st>>>(a);
   e = cudaGetLastError();
   const size_t smem = kBOff + kBStages * kBStage + kCtrlBytes;
-  const dim3 grid(static_cast<unsigned>(row_tiles(s) * a.chunks * s.kv_heads), (s.max_ctx + a.span - 1) / a.span);
+  const dim3 grid(static_cast<unsigned>(row_tiles(s) * a.chunks * s.kv_heads), (long_ctx(s) + a.span - 1) / a.span);
   if (e == cudaSuccess)
-    e = a.span >= s.max_ctx ? launch<1>(ctx, values_tc_kernel<true>, grid, smem, st, a)
+    e = a.span >= long_ctx(s) ? launch<1>(ctx, values_tc_kernel<true>, grid, smem, st, a)
                             : launch<2>(ctx, values_tc_kernel<false>, grid, smem, st, a);
   const cudaError_t f = cudaFreeAsync(a.planes, st);
   return e == cudaSuccess ? f : e;

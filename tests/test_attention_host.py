@@ -465,3 +465,33 @@ def test_wrong_workspace_places_are_refused(host, which):
     for kw in [dict(plane_keys=128), dict(d_plane_keys=P16), dict(d_plane_keys=P16, plane_keys=-128),
                dict(d_plane_keys=P16, plane_keys=130), dict(d_plane_keys=P16, plane_keys=2**31)]:
         assert _attn(host, which, _seqs(**PTRS, **kw)) == _lib.ERR_INVALID, kw
+
+
+def test_long_and_short_sequences_are_bounded_each_for_itself(emu):
+    """What deals out the work of whole prompts (the longest of their contexts) and
+    of single tokens (the most rows of theirs) comes from those sequences alone,
+    and a sequence outside its bound is refused like any other wrong length."""
+    q, L = [64, 1, 2, 0, 3], [4096, 65536, 70000, 80000, 100]
+    assert _layout(q, L, 32, 8)._bounds() == (4096, 8)
+    assert _layout([64, 1, 1], [300, 9000, 5], 32, 8)._bounds() == (300, 4)
+    assert _layout([1, 2], [300, 9000], 4, 4)._bounds() == (0, 2) and _layout([20], [9], 4, 4)._bounds() == (9, 0)
+    blk = C.c_int64()
+    s = _seqs(long_ctx=12, short_rows=4)  # groups of two: long from five tokens on
+
+    def fits(n, ctx):
+        return emu.emu_seq_fits(C.byref(s), 0, n, 0, ctx, 0, C.byref(blk))
+
+    assert fits(5, 12) and fits(2, 30) and fits(0, 30) and not fits(5, 13) and not fits(3, 5) and not fits(4, 5)
+    s.long_ctx = s.short_rows = 0
+    assert fits(5, 13) and fits(3, 5) and fits(4, 30)
+
+
+@pytest.mark.parametrize("which", ["scores", "values"])
+def test_wrong_bounds_of_long_and_short_sequences_are_refused(host, which):
+    from suf_b200 import _lib
+
+    for kw in [dict(long_ctx=30), dict(short_rows=8)]:
+        assert _attn(host, which, _seqs(**PTRS, **kw)) == _lib.ERR_UNSUPPORTED
+        assert b"host-only" in _lib.lib().sufb200_last_error()
+    for kw in [dict(long_ctx=31), dict(long_ctx=-1), dict(short_rows=9), dict(short_rows=-1)]:
+        assert _attn(host, which, _seqs(**PTRS, **kw)) == _lib.ERR_INVALID, kw

@@ -164,3 +164,50 @@ def test_attention_reports_bad_places(ctx, torch_cuda, which):
     got = call(ctx, *args)
     ctx.sync()
     assert (from_dev(got) == want).all()
+
+
+BESIDE = [  # a short sequence whose cache is longer than the prompts': theirs alone decide how they are split
+    (([(200, 1290), (1, 4000)], 16, 16, 16, 64, True), 3),
+    (([(256, 600), (1, 3000), (4, 700)], 40, 40, 8, 64, True), 3),   # whole rows of values
+    (([(1, 5000), (60, 90), (2, 3), (90, 1000)], 60, 20, 40, 100, True), 2),
+    (([(1, 2000), (40, 300), (1, 65)], 8, 2, 130, 16, False), 1),    # groups of four: four rows beside a prompt
+]
+
+
+@pytest.mark.parametrize("which", ["scores", "values"])
+@pytest.mark.parametrize("case,span", BESIDE)
+def test_prompts_beside_longer_caches(ctx, torch_cuda, which, case, span):
+    from suf_b200 import attention as at
+
+    A = _Attn(ctx, torch_cuda, case, 66)
+    assert _launch(ctx, A)[0] >= span and _launch(ctx, A)[2] == A.layout._seqs.long_ctx < max(A.L)
+    args, want = getattr(A, which)()
+    call = getattr(at, f"attn_{which}_pair")
+    for given in (True, False):  # without the bounds: the batch's longest context, eight rows
+        if not given:
+            A.layout._seqs.long_ctx = A.layout._seqs.short_rows = 0
+        buf, out = _guarded(torch_cuda, want)
+        call(ctx, *args, out=out)
+        ctx.sync()
+        assert (from_dev(out) == want).all() and (buf[want.size:] == 77).all()
+
+
+@pytest.mark.parametrize("which", ["scores", "values"])
+def test_attention_reports_sequences_past_their_bounds(ctx, torch_cuda, which):
+    from suf_b200 import SufB200Error
+    from suf_b200 import attention as at
+
+    A = _Attn(ctx, torch_cuda, BESIDE[3][0], 67)
+    args, _ = getattr(A, which)()
+    call, s = getattr(at, f"attn_{which}_pair"), A.layout._seqs
+    for kw in (dict(long_ctx=299), dict(short_rows=3)):
+        old = {k: getattr(s, k) for k in kw}
+        for k, v in kw.items():
+            setattr(s, k, v)
+        call(ctx, *args)
+        with pytest.raises(SufB200Error):
+            ctx.sync()
+        for k, v in old.items():
+            setattr(s, k, v)
+    call(ctx, *args)
+    ctx.sync()
