@@ -110,6 +110,21 @@ __device__ __forceinline__ void ld2_if(const uint64_t* p, bool in, uint64_t& x, 
       : "l"(p), "r"(static_cast<int>(in)));
 }
 
+// *p where `in`, else 0: a word of a buffer that the same kernel writes (ld_if's
+// loads are for memory that nothing writes while the kernel runs).
+__device__ __forceinline__ uint64_t ld_written_if(const uint64_t* p, bool in) {
+  uint64_t v;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %2, 0;\n\t"
+      "mov.u64 %0, 0;\n\t"
+      "@p ld.global.u64 %0, [%1];\n\t}"
+      : "=l"(v)
+      : "l"(p), "r"(static_cast<int>(in))
+      : "memory");
+  return v;
+}
+
 // The cached operand's byte planes.  KEYS: block (128-key tile, chunk of 32
 // words), rows = keys; else block (32 keys, 128-word tile), rows = words of
 // the head.  Out-of-range rows and depths are zero.
@@ -379,7 +394,7 @@ int64_t row_tiles(const AttnSeqs& s) {
 }
 
 // FIRST: the head's first part, which adds C and r; else its second part, which
-// adds to the first one's words (o.c[0] = o.out).
+// adds to the first one's words in o.out.
 template <bool FIRST>
 __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_constant__ AttnTc a) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -521,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) scores_tc_kernel(const __grid_con
 #pragma unroll
         for (int x = 0; x < 4; x++) {
           const bool in = x0 + x < rows && key < llen;
-          c0[(x0 >> 2) & 1][x] = ld_if(o.c[0] + lat, in);
+          c0[(x0 >> 2) & 1][x] = FIRST ? ld_if(o.c[0] + lat, in) : ld_written_if(o.out + lat, in);
           c1[(x0 >> 2) & 1][x] = FIRST ? ld_if(o.c[1] + lat, in) : 0;
           next(lg, llen, lrow, lat);
         }
@@ -792,7 +807,6 @@ cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const 
     const size_t smem = kBOff + static_cast<size_t>(2 * a.part) * kBStage + kCtrlBytes;
     e = a.chunk0 == 0 ? launch<0>(ctx, scores_tc_kernel<true>, grid, smem, st, a)
                       : launch<3>(ctx, scores_tc_kernel<false>, grid, smem, st, a, false);
-    a.o.c[0] = o.out;
   }
   const cudaError_t f = cudaFreeAsync(a.planes, st);
   return e == cudaSuccess ? f : e;

@@ -495,3 +495,16 @@ def test_wrong_bounds_of_long_and_short_sequences_are_refused(host, which):
         assert b"host-only" in _lib.lib().sufb200_last_error()
     for kw in [dict(long_ctx=31), dict(long_ctx=-1), dict(short_rows=9), dict(short_rows=-1)]:
         assert _attn(host, which, _seqs(**PTRS, **kw)) == _lib.ERR_INVALID, kw
+
+
+def test_words_that_a_kernel_writes_are_not_read_as_read_only():
+    """The second part of wide heads adds to the words it stores: no read-only load
+    (ld.global.nc, __ldg) may be given the output."""
+    import re
+
+    for name in ("attention.cu", "attention_tc.cu", "attention_rope.cu", "rowmax.cu"):
+        src = (ROOT / "suf_b200" / "csrc" / name).read_text()
+        assert not re.search(r"\bc\[\d\] = \S*out\b", src), name  # the output under an input's name
+        assert not re.search(r"\b(ld_if|ld2_if|ld_stream|__ldg)\(&?(a\.)?(o\.)?out\b", src), name
+    plain = re.search(r"uint64_t ld_written_if.*?\n}", (ROOT / "suf_b200" / "csrc" / "attention_tc.cu").read_text(), re.S)
+    assert "ld.global.u64" in plain.group() and ".nc" not in plain.group()
