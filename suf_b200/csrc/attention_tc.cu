@@ -244,6 +244,7 @@ __device__ __forceinline__ bool start(const Ctrl& c, int warp, int t, int bwarps
     mbar_init(c.tfull, 1);
     mbar_init(c.tempty, kWorkers / 32);
     mbar_init(c.done, 1);
+    mbar_init_fence();
     *c.err = 0;
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

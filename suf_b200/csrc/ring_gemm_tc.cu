@@ -351,6 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1) ring_gemm_tc_kernel(const RingGem
       mbar_init(empty0 + 8 * i, 1);
     }
     mbar_init(done, 1);
+    mbar_init_fence();
     *err = 0;
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -541,6 +542,7 @@ __global__ void __launch_bounds__(kFThreads, 1)
       mbar_init(rempty0 + 8 * i, kFConvWarps);
     }
     mbar_init(done, 1);
+    mbar_init_fence();
     *err = 0;
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

@@ -33,6 +33,11 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
 
+// After a thread's last mbar_init, before the CTA's barrier: bulk copies and the
+// tensor core's commits complete phases through the async proxy, which must see
+// the initialised barriers.
+__device__ __forceinline__ void mbar_init_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 __device__ __forceinline__ uint64_t global_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));

@@ -508,3 +508,17 @@ def test_words_that_a_kernel_writes_are_not_read_as_read_only():
         assert not re.search(r"\b(ld_if|ld2_if|ld_stream|__ldg)\(&?(a\.)?(o\.)?out\b", src), name
     plain = re.search(r"uint64_t ld_written_if.*?\n}", (ROOT / "suf_b200" / "csrc" / "attention_tc.cu").read_text(), re.S)
     assert "ld.global.u64" in plain.group() and ".nc" not in plain.group()
+
+
+@pytest.mark.parametrize("name", ["attention_tc.cu", "ring_gemm_tc.cu"])
+def test_barriers_are_fenced_between_their_init_and_the_first_use(name):
+    """Copies and commits complete mbarriers through the async proxy: the fence
+    that shows it their initialisation stands before the CTA's barrier."""
+    src = (ROOT / "suf_b200" / "csrc" / name).read_text()
+    parts = src.split("mbar_init(")[1:]
+    assert parts
+    for part in parts:  # up to the next init, or (the last of a group) up to the barrier
+        if "__syncthreads();" in part:
+            assert "mbar_init_fence();" in part.split("__syncthreads();")[0]
+    fence = (ROOT / "suf_b200" / "csrc" / "umma_i8.cuh").read_text().split("void mbar_init_fence()")[1].split("\n")[0]
+    assert "fence.proxy.async.shared::cta" in fence
