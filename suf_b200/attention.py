@@ -241,7 +241,8 @@ class ShareCache:
 
 
 def _strided(ctx: Context, name: str, ts, shape: tuple):
-    """Both parties' addresses and the common strides of [tokens][heads][dim] views (the last axis dense)."""
+    """Both parties' addresses and the common strides of [tokens][heads][dim] views (the last axis dense;
+    an axis of one entry has any stride)."""
     if not isinstance(ts, (tuple, list)) or len(ts) != 2:
         raise ValueError(f"{name}: expected both parties' tensors")
     x, y = ts
@@ -255,7 +256,9 @@ def _strided(ctx: Context, name: str, ts, shape: tuple):
         _refuse(ctx, name, t, shape, word)
     ld = x.stride()
     if ld != y.stride():
-        raise ValueError(f"{name}: the parties' strides differ")
+        ld = tuple(s if n > 1 else 0 for s, n in zip(ld, shape))
+        if x.numel() and ld != tuple(s if n > 1 else 0 for s, n in zip(y.stride(), shape)):
+            raise ValueError(f"{name}: the parties' strides differ")
     if ld[2] != 1 and x.numel():
         raise ValueError(f"{name}: the head's words must be adjacent")
     return x.data_ptr(), y.data_ptr(), ld[0], ld[1]

@@ -522,3 +522,31 @@ def test_barriers_are_fenced_between_their_init_and_the_first_use(name):
             assert "mbar_init_fence();" in part.split("__syncthreads();")[0]
     fence = (ROOT / "suf_b200" / "csrc" / "umma_i8.cuh").read_text().split("void mbar_init_fence()")[1].split("\n")[0]
     assert "fence.proxy.async.shared::cta" in fence
+
+
+def test_strides_of_single_entries_do_not_count():
+    """One token (or one head) has no step to the next: views that differ in that
+    stride alone are taken; others are refused."""
+    import types
+
+    import torch
+
+    from suf_b200 import attention as at
+
+    cpu = types.SimpleNamespace(device=-1)  # what get_device() says of CPU tensors
+    wide, tight = torch.zeros(3, 50, dtype=torch.int64), torch.zeros(3, 16, dtype=torch.int64)
+
+    def views(tokens, heads, dim=4):
+        return tuple(t[:tokens, :heads * dim].unflatten(1, (heads, dim)) for t in (wide, tight))
+
+    assert at._strided(cpu, "k", views(1, 4), (1, 4, 4))[3] == 4
+    assert at._strided(cpu, "k", views(1, 1), (1, 1, 4))[:2] == (wide.data_ptr(), tight.data_ptr())
+    assert at._strided(cpu, "k", views(0, 4), (0, 4, 4))
+    per_head = tuple(torch.zeros(2, 3, n, 4, dtype=torch.int64)[:, :, 0] for n in (1, 2))
+    assert at._strided(cpu, "k", tuple(t[:, :1].as_strided((2, 1, 4), (12, s, 1)) for t, s in zip(per_head, (4, 8))),
+                       (2, 1, 4))[2] == 12
+    for bad, shape in [(views(2, 4), (2, 4, 4)), (per_head, (2, 3, 4))]:
+        with pytest.raises(ValueError, match="strides differ"):
+            at._strided(cpu, "k", bad, shape)
+    with pytest.raises(ValueError, match="adjacent"):
+        at._strided(cpu, "k", (torch.zeros(1, 4, 8, dtype=torch.int64)[..., ::2],) * 2, (1, 4, 4))

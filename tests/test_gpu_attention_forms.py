@@ -211,3 +211,17 @@ def test_attention_reports_sequences_past_their_bounds(ctx, torch_cuda, which):
             setattr(s, k, v)
     call(ctx, *args)
     ctx.sync()
+
+
+def test_one_token_of_views_with_different_strides(ctx, torch_cuda):
+    """The parties' shares of one token, one in a fused row and one by itself."""
+    from suf_b200.attention import rope_append_pair
+    from tests.test_gpu_attention import _rope_case
+
+    for case in [(1, 12, 4, 64, 64, False, 64, 12, 40, 0), (1, 3, 1, 18, 6, True, 3, 15, 40, 0)]:
+        args, kw, want, got, _ = _rope_case(ctx, torch_cuda, case, seed=9)
+        q, k, v = ((x, y.clone(memory_format=torch_cuda.contiguous_format)) for x, y in args[:3])
+        assert q[0].stride() != q[1].stride()
+        rope_append_pair(ctx, q, k, v, *args[3:], **kw)
+        ctx.sync()
+        assert all((from_dev(g) == w).all() for w, g in zip(want, got))
