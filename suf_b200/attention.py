@@ -283,14 +283,16 @@ def rope_append_pair(ctx: Context, q, k, v, positions, slots, cos, sin, trunc: T
     if trunc is not None and trunc.device != ctx.device:
         _elsewhere(ctx, "truncation bundle", trunc.device)
     tokens, kv, dim = k[0].shape[0], cache.kv_heads, cache.head_dim
+    heads = 0 if q is None else q[0].shape[1]
     if tokens >= 2**31:
         raise ValueError("more than 2^31 tokens in one call")
+    if heads + 2 * kv >= 2**31:
+        raise ValueError("more than 2^31 heads of a token")
     args = RopeAppend.from_buffer_copy(cache._args)
     k0, k1, k_ts, k_hs = _strided(ctx, "k", k, (tokens, kv, dim))
     v0, v1, v_ts, v_hs = _strided(ctx, "v", v, (tokens, kv, dim))
     q0 = q1 = q_ts = q_hs = a0 = a1 = out = 0
     if q is not None:
-        heads = q[0].shape[1]
         shape = (tokens, heads, dim)
         q0, q1, q_ts, q_hs = _strided(ctx, "q", q, shape)
         a0, a1 = _pair(ctx, "a", a, shape)
@@ -303,10 +305,12 @@ def rope_append_pair(ctx: Context, q, k, v, positions, slots, cos, sin, trunc: T
         at_cos = _want(ctx, "cos", cos, table, torch.int32)
         at_sin = _want(ctx, "sin", sin, table, torch.int32)
         at_pos = _want(ctx, "positions", positions, (tokens,), torch.int32)
-        args.max_pos, half = table
-        args.rot_dim = 2 * half
+        half = table[1]
+        if table[0] >= 2**31:
+            raise ValueError("tables of more than 2^31 positions")
         if 2 * half > dim:
             raise ValueError(f"the tables turn {2 * half} words of a head of {dim}")
+        args.max_pos, args.rot_dim = table[0], 2 * half
         args.trunc, args.d_tables, args.r = trunc._args
     elif cos is not None or sin is not None:
         raise ValueError("rotation needs the truncation bundle")
@@ -363,8 +367,8 @@ class AttnLayout:
         self.packed = int(base[-1])
         if self.batch and int(L.max()) > block_table.shape[1] * page_size:
             raise ValueError("layout: a sequence is longer than its pages")
-        if max(self.tokens, self.batch, int(L.sum())) >= 2**31:
-            raise ValueError("layout: more than 2^31 tokens")
+        if max(self.tokens, self.batch, int(L.sum()), block_table.shape[1]) >= 2**31:
+            raise ValueError("layout: more than 2^31 tokens, or pages of a sequence")
         self._cu = torch.from_numpy(np.concatenate([[0], np.cumsum(q)]).astype(np.int32)).to(dev)
         self._ctx = torch.from_numpy(np.concatenate([[0], np.cumsum(L)]).astype(np.int32)).to(dev)
         self._base = torch.from_numpy(base[:-1].astype(np.int64)).to(dev)
@@ -430,6 +434,8 @@ class AttnLayout:
             _elsewhere(ctx, "layout", self.device)
         e_ptr = _want(ctx, name, e, (None, self.kv_heads, self.page_size, None))
         shape = e.shape
+        if max(shape) >= 2**31:
+            raise ValueError(f"{name}: past 2^31 pages")
         s = AttnSeqs.from_buffer_copy(self._seqs)
         s.pages, s.head_dim = shape[0], shape[3]
         return s, e_ptr, _pair(ctx, f"{name}'s masks", b, shape)

@@ -169,6 +169,8 @@ int check_rope(const sufb200_rope_append* a) {
     return fail(SUFB200_ERR_INVALID, "rope_append_pair: bad token, head or page count");
   if (a->head_dim < 2 || a->head_dim > 256 || a->head_dim % 2)
     return fail(SUFB200_ERR_UNSUPPORTED, "rope_append_pair: head size must be even, 2..256");
+  if (a->q_heads + 2 * static_cast<int64_t>(a->kv_heads) > INT32_MAX)
+    return fail(SUFB200_ERR_UNSUPPORTED, "rope_append_pair: more than 2^31 heads of a token");
   if (a->rot_dim < 0 || a->rot_dim > a->head_dim || a->rot_dim % 2)
     return fail(SUFB200_ERR_INVALID, "rope_append_pair: the rotated part must be even and within the head");
   if (a->tokens == 0) return SUFB200_OK;

@@ -550,3 +550,37 @@ def test_strides_of_single_entries_do_not_count():
             at._strided(cpu, "k", bad, shape)
     with pytest.raises(ValueError, match="adjacent"):
         at._strided(cpu, "k", (torch.zeros(1, 4, 8, dtype=torch.int64)[..., ::2],) * 2, (1, 4, 4))
+
+
+def test_sizes_past_32_bits_in_any_argument_are_refused(host):
+    """Heads, positions, pages and the pages of a sequence are 32-bit fields of the
+    C structs: larger sizes are refused, not cut off (tensors without elements
+    stand for large ones)."""
+    import types
+
+    import torch
+
+    from suf_b200 import _lib
+    from suf_b200 import attention as at
+
+    cpu = types.SimpleNamespace(device=-1)
+    cache = types.SimpleNamespace(device=-1, kv_heads=1, head_dim=2, _args=_lib.RopeAppend())
+    k = (torch.zeros(1, 1, 2, dtype=torch.int64),) * 2
+    q = (torch.zeros(1, 1, 2, dtype=torch.int64).expand(1, 2**32 + 4, 2),) * 2
+    with pytest.raises(ValueError, match="2\\^31 heads"):
+        at.rope_append_pair(cpu, q, k, k, None, None, None, None, None, q, cache)
+    table = torch.zeros(2**32 + 5, 0, dtype=torch.int32)
+    pos = torch.zeros(1, dtype=torch.int32)
+    trunc = types.SimpleNamespace(device=-1, _args=(_lib.TruncDesc * 2)())
+    with pytest.raises(ValueError, match="2\\^31 positions"):
+        at.rope_append_pair(cpu, None, k, k, pos, pos.long(), table, table, trunc, None, cache)
+    lay = at.AttnLayout.__new__(at.AttnLayout)
+    lay.device, lay.kv_heads, lay.page_size, lay._seqs, lay.tokens, lay.packed, lay.q_heads = -1, 1, 1, _lib.AttnSeqs(), 0, 0, 1
+    pool = torch.zeros(2**32 + 3, 1, 1, 0, dtype=torch.int64)
+    with pytest.raises(ValueError, match="2\\^31 pages"):
+        at.attn_scores_pair(cpu, None, None, None, (1, 2), pool, (pool, pool), lay)
+    L = _lib.lib()
+    for heads, said in [((2**31 - 5, 2), b"host-only"), ((2**31 - 4, 2), b"2^31 heads"), ((0, 2**30), b"2^31 heads")]:
+        a = _rope(q_heads=heads[0], kv_heads=heads[1])
+        assert L.sufb200_rope_append_pair(host, C.byref(a), None) == _lib.ERR_UNSUPPORTED
+        assert said in L.sufb200_last_error()
