@@ -114,9 +114,11 @@ def _pair(ctx: Context, name: str, ts, shape: tuple):
 
 
 def _masks(r):
-    if len(r) != 2:
-        raise ValueError("r: expected both parties' shares of the mask")
-    return _TwoWords(int(r[0]) & M64, int(r[1]) & M64)
+    try:
+        r0, r1 = r
+        return _TwoWords(int(r0) & M64, int(r1) & M64)
+    except (TypeError, ValueError):
+        raise ValueError("r: expected both parties' shares of the mask") from None
 
 
 # -- rotary tables --------------------------------------------------------------
@@ -282,8 +284,11 @@ def rope_append_pair(ctx: Context, q, k, v, positions, slots, cos, sin, trunc: T
         _elsewhere(ctx, "cache", cache.device)
     if trunc is not None and trunc.device != ctx.device:
         _elsewhere(ctx, "truncation bundle", trunc.device)
-    tokens, kv, dim = k[0].shape[0], cache.kv_heads, cache.head_dim
-    heads = 0 if q is None else q[0].shape[1]
+    try:
+        tokens, kv, dim = k[0].shape[0], cache.kv_heads, cache.head_dim
+        heads = 0 if q is None else q[0].shape[1]
+    except (TypeError, IndexError, AttributeError):
+        raise ValueError("q, k: expected both parties' tensors [tokens][heads][head_dim]") from None
     if tokens >= 2**31:
         raise ValueError("more than 2^31 tokens in one call")
     if heads + 2 * kv >= 2**31:

@@ -584,3 +584,20 @@ def test_sizes_past_32_bits_in_any_argument_are_refused(host):
         a = _rope(q_heads=heads[0], kv_heads=heads[1])
         assert L.sufb200_rope_append_pair(host, C.byref(a), None) == _lib.ERR_UNSUPPORTED
         assert said in L.sufb200_last_error()
+
+
+def test_malformed_shares_are_refused_as_such():
+    import types
+
+    import torch
+
+    from suf_b200 import attention as at
+
+    cache = types.SimpleNamespace(device=0, kv_heads=1, head_dim=2)
+    k = (torch.zeros(1, 1, 2, dtype=torch.int64),) * 2
+    for q, kk in [(None, None), (None, ()), (None, 3), ((k[0][0, 0],) * 2, k), (k[0][0], None), ((1, 2), k)]:
+        with pytest.raises(ValueError, match="both parties"):
+            at.rope_append_pair(_Ctx, q, kk, k, None, None, None, None, None, None, cache)
+    for r in (None, 5, (1,), (1, 2, 3)):
+        with pytest.raises(ValueError, match="both parties"):
+            at._masks(r)
