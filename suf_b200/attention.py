@@ -202,7 +202,9 @@ class TruncPair(_Trunc):
 class ShareCache:
     """The paged cache of one layer: opened pools ek, ev and the masks' shares
     bk, bv (pairs), each [pages][kv_heads][page_size][head_dim].  Slot = page *
-    page_size + place.  The constructor deals fresh masks for every slot."""
+    page_size + place.  The constructor deals fresh masks for every slot; a page
+    that is to be written again takes fresh_masks first, or the two openings
+    under one mask give away the difference of the rows."""
 
     def __init__(self, ctx: Context, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, seed: int = 1):
         dev = torch.device("cuda", ctx.device)
@@ -215,13 +217,37 @@ class ShareCache:
 
         self._set(ctx, torch.zeros(shape, dtype=torch.int64, device=dev), (words(), words()),
                   torch.zeros(shape, dtype=torch.int64, device=dev), (words(), words()))
+        self._dealer = g
 
     @classmethod
     def from_tensors(cls, ctx: Context, ek, bk, ev, bv) -> "ShareCache":
-        """A cache over pools the caller holds."""
+        """A cache over pools the caller holds, and whose masks they deal."""
         self = cls.__new__(cls)
         self._set(ctx, ek, bk, ev, bv)
+        self._dealer = None
         return self
+
+    def fresh_masks(self, pages, seed: int | None = None):
+        """New masks for every slot of the given pages (numbers), on the current
+        stream: what was cached there is gone, and so is material dealt for it
+        (CachedAttentionPair's triples).  The constructor's dealer goes on from where
+        it was; a cache over the caller's pools takes a seed, another one every time."""
+        at = np.unique(np.asarray(pages, dtype=np.int64).reshape(-1))
+        if at.size and not 0 <= at[0] <= at[-1] < self.pages:
+            raise ValueError(f"fresh_masks: pages are numbers from 0 to {self.pages - 1}")
+        dev = self.ek.device
+        g = self._dealer
+        if seed is not None:
+            g = torch.Generator(device=dev)
+            g.manual_seed(seed)
+        if g is None:
+            raise ValueError("fresh_masks: a cache over the caller's pools takes a seed")
+        at = torch.from_numpy(at).to(dev)
+        shape = (at.numel(), self.kv_heads, self.page_size, self.head_dim)
+        for pool in (*self.bk, *self.bv):
+            pool[at] = torch.randint(-(2**63), 2**63 - 1, shape, dtype=torch.int64, device=dev, generator=g)
+        for pool in (self.ek, self.ev):
+            pool[at] = 0
 
     def _set(self, ctx, ek, bk, ev, bv):
         args = self._args = RopeAppend()  # what every append into this cache passes

@@ -601,3 +601,40 @@ def test_malformed_shares_are_refused_as_such():
     for r in (None, 5, (1,), (1, 2, 3)):
         with pytest.raises(ValueError, match="both parties"):
             at._masks(r)
+
+
+def test_pages_take_fresh_masks_before_they_are_written_again():
+    """New masks for the given pages alone, others each time, and nothing left of
+    what was opened there."""
+    import types
+
+    import torch
+
+    from suf_b200 import attention as at
+
+    cpu = types.SimpleNamespace(device=-1)
+    pools = [torch.arange(5 * 2 * 3 * 4).view(5, 2, 3, 4) * (i + 1) + 1 for i in range(6)]
+    cache = at.ShareCache.from_tensors(cpu, pools[0], pools[1:3], pools[3], pools[4:6])
+    old = [p.clone() for p in pools]
+    seen = [p[[1, 3]].clone() for p in pools]
+    with pytest.raises(ValueError, match="seed"):
+        cache.fresh_masks([1])
+    for bad in ([5], [-1, 2], [0, 1 << 40]):
+        with pytest.raises(ValueError, match="0 to 4"):
+            cache.fresh_masks(bad, seed=1)
+    assert all(torch.equal(p, o) for p, o in zip(pools, old))
+    for seed in (7, 8):
+        cache.fresh_masks([3, 1, 3], seed=seed)
+        for i, (p, o) in enumerate(zip(pools, old)):
+            assert torch.equal(p[[0, 2, 4]], o[[0, 2, 4]])
+            if i in (0, 3):
+                assert (p[[1, 3]] == 0).all()
+            else:
+                assert (p[[1, 3]] != seen[i]).all()
+                seen[i] = p[[1, 3]].clone()
+    cache._dealer = torch.Generator()  # as the constructor leaves it
+    cache.fresh_masks(torch.tensor([2]))
+    first = pools[1][2].clone()
+    cache.fresh_masks([2])
+    assert (pools[1][2] != first).all()
+    cache.fresh_masks([])

@@ -225,3 +225,23 @@ def test_one_token_of_views_with_different_strides(ctx, torch_cuda):
         rope_append_pair(ctx, q, k, v, *args[3:], **kw)
         ctx.sync()
         assert all((from_dev(g) == w).all() for w, g in zip(want, got))
+
+
+def test_a_page_written_again_under_fresh_masks(ctx, torch_cuda):
+    """The same rows appended twice into one page: under fresh masks the two
+    openings share no word, and each opens to the rows."""
+    from suf_b200.attention import ShareCache, rope_append_pair
+
+    torch = torch_cuda
+    cache = ShareCache(ctx, 3, 2, 16, 8, seed=4)
+    x = [torch.randint(-(2**63), 2**63 - 1, (8, 2, 16), dtype=torch.int64, device="cuda") for _ in range(4)]
+    slots = torch.arange(8, 16, dtype=torch.int64, device="cuda")
+    opened = []
+    for _ in range(2):
+        rope_append_pair(ctx, None, (x[0], x[1]), (x[2], x[3]), None, slots, None, None, None, None, cache)
+        ctx.sync()
+        opened.append((cache.ek[1].clone(), cache.ev[1].clone()))
+        for e, b, s in ((cache.ek, cache.bk, x[:2]), (cache.ev, cache.bv, x[2:])):
+            assert torch.equal((e[1] + b[0][1] + b[1][1]).transpose(0, 1), s[0] + s[1])
+        cache.fresh_masks([1])
+    assert (opened[0][0] != opened[1][0]).all() and (opened[0][1] != opened[1][1]).all()
