@@ -8,8 +8,8 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from tests.conftest import from_dev
-from tests.test_gpu_attention import GUARD, U, _Attn, _guarded
+from tests.conftest import from_dev, rand_u64, to_dev
+from tests.test_gpu_attention import GUARD, U, _Attn, _guarded, _model, _rope_case, test_rowmax_rounds_match_definition as _rowmax
 
 pytestmark = pytest.mark.gpu
 
@@ -216,7 +216,6 @@ def test_attention_reports_sequences_past_their_bounds(ctx, torch_cuda, which):
 def test_one_token_of_views_with_different_strides(ctx, torch_cuda):
     """The parties' shares of one token, one in a fused row and one by itself."""
     from suf_b200.attention import rope_append_pair
-    from tests.test_gpu_attention import _rope_case
 
     for case in [(1, 12, 4, 64, 64, False, 64, 12, 40, 0), (1, 3, 1, 18, 6, True, 3, 15, 40, 0)]:
         args, kw, want, got, _ = _rope_case(ctx, torch_cuda, case, seed=9)
@@ -245,3 +244,114 @@ def test_a_page_written_again_under_fresh_masks(ctx, torch_cuda):
             assert torch.equal((e[1] + b[0][1] + b[1][1]).transpose(0, 1), s[0] + s[1])
         cache.fresh_masks([1])
     assert (opened[0][0] != opened[1][0]).all() and (opened[0][1] != opened[1][1]).all()
+
+
+@pytest.mark.parametrize("new", [[(1, 1)], [(1, 1), (1, 1), (1, 1)], [(5, 3), (1, 1)], [(9, 2), (1, 12), (4, 1)], [(3, 0), (2, 2)]])
+def test_block_with_single_keys_and_rows_that_see_nothing(ctx, torch_cuda, new):
+    """First tokens (one key: no row max round) and queries in front of what is
+    cached (empty rows through the row max and the softmax block), against the
+    plaintext model word for word; an empty row gives zero."""
+    from oracle.layer_model import load_layer_tables
+    from oracle.softmax_model import load_tables
+    from suf_b200.attention import AttnLayout, CachedAttentionPair, ShareCache
+
+    torch = torch_cuda
+    hq, hkv, dh, page = 4, 2, 16, 4
+    rng = np.random.default_rng(17)
+    cache = ShareCache(ctx, 16, hkv, dh, page, seed=8)
+    q_lens, ctx_lens = [n for n, _ in new], [L for _, L in new]
+    tables = [[3 * b + j for j in range(3)] for b in range(len(new))]
+    blk = CachedAttentionPair(ctx, cache, AttnLayout(ctx, q_lens, ctx_lens, tables, page, hq, hkv), seed=19)
+    T = sum(q_lens)
+    x = np.rint(rng.normal(0.0, 1.0, (T, hq + 2 * hkv, dh)) * 4096).astype(np.int64)
+    old = [np.rint(rng.normal(0.0, 1.0, (2, max(L - n, 0), hkv, dh)) * 4096).astype(np.int64) for n, L in new]
+    slots, t0, spare = [], 0, 12 * page
+    for b, (n, L) in enumerate(new):
+        for j in range(max(L - n, 0)):  # what was cached before
+            pg, at = tables[b][j // page], j % page
+            for pool, m, y in ((cache.ek, cache.bk, old[b][0]), (cache.ev, cache.bv, old[b][1])):
+                pool[pg, :, at] = torch.from_numpy(y[j]).cuda() - m[0][pg, :, at] - m[1][pg, :, at]
+        for i in range(n):
+            j = L - n + i
+            slots.append(tables[b][j // page] * page + j % page if j >= 0 else spare)
+            spare += j < 0
+    s0 = rand_u64(rng, x.size).reshape(x.shape)
+    sh = [to_dev(torch, s0), to_dev(torch, x.view(U) - s0)]
+    o = blk.run(tuple(s[:, :hq] for s in sh), tuple(s[:, hq:hq + hkv] for s in sh), tuple(s[:, hq + hkv:] for s in sh),
+                None, torch.tensor(slots, dtype=torch.int64, device="cuda"))
+    ctx.sync()
+    got = from_dev(o[0]) + from_dev(o[1])
+    relu, sm = load_layer_tables()["relu"], load_tables()
+    for b, (n, L) in enumerate(new):
+        k, v = (np.concatenate([old[b][w], x[t0 + max(n - L, 0):t0 + n, hq + w * hkv:hq + (w + 1) * hkv]]).view(U)
+                for w in (0, 1))
+        assert len(k) == L
+        want = _model(x[t0:t0 + n, :hq].view(U), k, v, lambda i: max(0, L - n + i + 1), hq // hkv, 12, 2, relu, sm)
+        assert (got[t0:t0 + n] == want).all(), b
+        t0 += n
+
+
+def test_append_of_a_prompt_on_a_side_stream_and_in_a_graph(ctx, torch_cuda):
+    """Enough turned words for the packed carries: their table is the call's own,
+    also where two captured appends replay beside one another."""
+    from suf_b200.attention import rope_append_pair
+
+    torch = torch_cuda
+    jobs, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    for inter, st in zip((False, True), streams):
+        args, kw, want, got, _ = _rope_case(ctx, torch, (300, 32, 8, 128, 128, inter, 64, 12, 44, 2), 70 + inter)
+        before = [g.clone() for g in got]
+        torch.cuda.synchronize()
+        rope_append_pair(ctx, *args, **kw, stream=st)
+        ctx.sync(st)
+        assert all((from_dev(g) == w).all() for w, g in zip(want, got))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st, capture_error_mode="relaxed"):
+            rope_append_pair(ctx, *args, **kw, stream=st)
+        jobs.append((graph, st, before, want, got, args))
+    for _ in range(3):
+        for _, _, before, _, got, _ in jobs:
+            for g, b in zip(got, before):
+                g.copy_(b)
+        torch.cuda.synchronize()
+        for graph, st, *_ in jobs:
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        ctx.sync()
+        for _, _, _, want, got, _ in jobs:
+            assert all((from_dev(g) == w).all() for w, g in zip(want, got))
+
+
+def test_append_of_more_rows_than_the_grid_has_warps(ctx, torch_cuda):
+    """100,000 tokens of 96 heads: 9.6 million rows on 2^20 blocks of eight."""
+    from suf_b200.attention import ShareCache, TruncPair, rope_append_pair, rope_tables
+
+    torch = torch_cuda
+    T, hq, hkv, dh, page, f = 100_000, 60, 18, 2, 64, 12
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    x = torch.randint(-(2**40), 2**40, (T, hq + 2 * hkv, dh), dtype=torch.int64, device="cuda", generator=g)
+    s = torch.randint(-(2**63), 2**63 - 1, x.shape, dtype=torch.int64, device="cuda", generator=g)
+    sh = (s, x - s)
+    q, k, v = (tuple(t[:, i:j] for t in sh) for i, j in ((0, hq), (hq, hq + hkv), (hq + hkv, hq + 2 * hkv)))
+    cache = ShareCache(ctx, -(-T // page), hkv, dh, page, seed=5)
+    slots = torch.randperm(cache.pages * page, device="cuda", generator=g)[:T]
+    pos = torch.randint(0, 4096, (T,), device="cuda", generator=g).to(torch.int32)
+    cos, sin = rope_tables(ctx, 4096, dh, f)
+    a = tuple(torch.randint(-(2**63), 2**63 - 1, (T, hq, dh), dtype=torch.int64, device="cuda", generator=g) for _ in range(2))
+    d_q = rope_append_pair(ctx, q, k, v, pos, slots, cos, sin, TruncPair(ctx, f, seed=6), a, cache)
+    ctx.sync()
+    c, n = (t[pos.long(), 0].long()[:, None] for t in (cos, sin))
+    y = x.clone()
+    y[:, :hq + hkv, 0] = (x[:, :hq + hkv, 0] * c - x[:, :hq + hkv, 1] * n) >> f
+    y[:, :hq + hkv, 1] = (x[:, :hq + hkv, 1] * c + x[:, :hq + hkv, 0] * n) >> f
+    assert torch.equal(d_q, y[:, :hq] - a[0] - a[1])
+    for e, b, rows in ((cache.ek, cache.bk, y[:, hq:hq + hkv]), (cache.ev, cache.bv, y[:, hq + hkv:])):
+        assert torch.equal((e + b[0] + b[1]).transpose(1, 2).reshape(-1, hkv, dh)[slots], rows)
+
+
+@pytest.mark.parametrize("rows,most", [(100_000, 9), (20_000, 40), (3_000, 900)])
+def test_rowmax_of_more_rows_than_the_grid_takes_at_once(ctx, torch_cuda, rows, most):
+    rng = np.random.default_rng(rows)
+    _rowmax(ctx, torch_cuda, rng.integers(0, most + 1, rows).tolist())
