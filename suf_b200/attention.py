@@ -412,7 +412,9 @@ class AttnLayout:
         s.page_size, s.q_heads, s.kv_heads, s.causal = self.page_size, self.q_heads, self.kv_heads, int(self.causal)
         s.min_q, s.max_q, s.max_ctx = int(q[q > 0].min(initial=2**31 - 1)), int(q.max(initial=0)), int(L.max(initial=0))
         s.min_q = min(s.min_q, s.max_q)
-        s.long_ctx, s.short_rows = self._bounds()
+        longest, most = self._bounds()
+        if longest and most:  # of one kind alone, max_ctx and max_q say the same
+            s.long_ctx, s.short_rows = longest, most
         tiles = self._tile_list()
         if len(tiles):
             self._tiles = torch.from_numpy(tiles).to(dev)
@@ -465,10 +467,11 @@ class AttnLayout:
             _elsewhere(ctx, "layout", self.device)
         e_ptr = _want(ctx, name, e, (None, self.kv_heads, self.page_size, None))
         shape = e.shape
-        if max(shape) >= 2**31:
+        pages, _, _, dim = shape
+        if pages >= 2**31 or dim >= 2**31:
             raise ValueError(f"{name}: past 2^31 pages")
         s = AttnSeqs.from_buffer_copy(self._seqs)
-        s.pages, s.head_dim = shape[0], shape[3]
+        s.pages, s.head_dim = pages, dim
         return s, e_ptr, _pair(ctx, f"{name}'s masks", b, shape)
 
 

@@ -69,8 +69,10 @@ SUFB200_HD bool seq_fits(const AttnSeqs& s, int c0, int c1, int l0, int l1, int6
       L > static_cast<int64_t>(s.max_pages) * s.page_size || base < 0 || base > s.packed)
     return false;
   q.n = c1 - c0;
-  const int rows = s.q_heads / s.kv_heads * q.n;  // of a key head
-  if (rows > SUFB200_ATTN_FEW_ROWS ? s.long_ctx > 0 && L > s.long_ctx : s.short_rows > 0 && rows > s.short_rows) return false;
+  if (s.long_ctx > 0 || s.short_rows > 0) {
+    const int rows = s.q_heads / s.kv_heads * q.n;  // of a key head
+    if (rows > SUFB200_ATTN_FEW_ROWS ? s.long_ctx > 0 && L > s.long_ctx : s.short_rows > 0 && rows > s.short_rows) return false;
+  }
   q.blk = row_off(q.n, L, s.causal, q.n);
   return q.blk * s.q_heads <= s.packed - base;
 }

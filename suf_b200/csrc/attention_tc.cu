@@ -135,8 +135,8 @@ __global__ void __launch_bounds__(256) cache_planes_kernel(const __grid_constant
   const AttnSeqs& s = a.s;
   constexpr int kPer = KEYS ? kTM : kTK;
   const int t = threadIdx.x, kh = blockIdx.z;
-  const int b = s.d_plane_keys ? block_seq(s.d_plane_keys, s.batch, 1, kPer, blockIdx.x, 0)
-                               : block_seq(s.d_cu_ctx, s.batch, 1, kPer, blockIdx.x);
+  const bool places = s.d_plane_keys != nullptr;
+  const int b = block_seq(places ? s.d_plane_keys : s.d_cu_ctx, s.batch, 1, kPer, blockIdx.x, places ? 0 : 1);
   SeqInfo q;
   if (!seq_info(s, b, a.o.status, q) || s.q_heads / s.kv_heads * q.n <= a.o.few) return;
   const int64_t plane = plane_first(s, b, q, kPer, a.o.status), first = blockIdx.x - plane;  // this block in its sequence
