@@ -309,6 +309,9 @@ int check_seqs(const sufb200_attn_seqs* s, const char* who) {
     return fail(SUFB200_ERR_INVALID, at + "null or empty list of places, or not in whole key tiles");
   if (s->batch > 0 && (!s->d_cu_q || !s->d_cu_ctx || !s->d_row_base || (s->max_ctx > 0 && !s->d_block_table)))
     return fail(SUFB200_ERR_INVALID, at + "null sequence array");
+  for (const void* p : {s->d_cu_q, s->d_cu_ctx, s->d_block_table, s->d_tiles, s->d_plane_keys})
+    if (!aligned_to(p, 4)) return fail(SUFB200_ERR_INVALID, at + "misaligned sequence array");
+  if (!aligned_to(s->d_row_base, 8)) return fail(SUFB200_ERR_INVALID, at + "misaligned sequence array");
   return SUFB200_OK;
 }
 

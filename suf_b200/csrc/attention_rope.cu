@@ -174,7 +174,8 @@ int check_rope(const sufb200_rope_append* a) {
   if (a->rot_dim < 0 || a->rot_dim > a->head_dim || a->rot_dim % 2)
     return fail(SUFB200_ERR_INVALID, "rope_append_pair: the rotated part must be even and within the head");
   if (a->tokens == 0) return SUFB200_OK;
-  if (!a->d_slots) return fail(SUFB200_ERR_INVALID, "rope_append_pair: null slots");
+  if (!a->d_slots || !aligned_to(a->d_slots, 8))
+    return fail(SUFB200_ERR_INVALID, "rope_append_pair: null or misaligned slots");
   for (int p = 0; p < 2; p++) {
     if (!a->d_k[p] || !a->d_v[p] || !a->d_bk[p] || !a->d_bv[p] || (a->q_heads > 0 && (!a->d_q[p] || !a->d_a[p])))
       return fail(SUFB200_ERR_INVALID, "rope_append_pair: null share or mask pointer");
@@ -190,6 +191,8 @@ int check_rope(const sufb200_rope_append* a) {
   if (a->rot_dim > 0) {
     if (!a->d_positions || !a->d_cos || !a->d_sin || a->max_pos < 1)
       return fail(SUFB200_ERR_INVALID, "rope_append_pair: positions or cosine and sine tables missing");
+    if (!aligned_to(a->d_positions, 4) || !aligned_to(a->d_cos, 4) || !aligned_to(a->d_sin, 4))
+      return fail(SUFB200_ERR_INVALID, "rope_append_pair: misaligned positions or tables");
     for (int p = 0; p < 2; p++) {
       const sufb200_trunc_desc& d = a->trunc[p];
       if (d.kind != SUFB200_TRUNC_GAPARS || d.party != p || d.frac_bits < 1 || d.frac_bits > 16 ||

@@ -124,6 +124,12 @@ int check_rows(int rows, int max_width, const char* who) {
   return SUFB200_OK;
 }
 
+int check_offsets(std::initializer_list<const void*> ps, const char* who) {
+  for (const void* p : ps)
+    if (!aligned_to(p, 4)) return fail(SUFB200_ERR_INVALID, std::string(who) + ": misaligned offsets");
+  return SUFB200_OK;
+}
+
 int check_words(std::initializer_list<const void*> ps, const char* who) {
   for (const void* p : ps)
     if (!p || !aligned_to(p, 8)) return fail(SUFB200_ERR_INVALID, std::string(who) + ": null or misaligned device pointer");
@@ -144,6 +150,7 @@ int sufb200_rowmax_open_pair(sufb200_ctx ctx, const uint64_t* const* d_c, int ro
   if (int rc = check_rows(rows, max_width, "rowmax_open_pair")) return rc;
   if (rows == 0 || max_width < 2) return SUFB200_OK;
   if (!d_c || !r || !d_off || !d_off1) return fail(SUFB200_ERR_INVALID, "rowmax_open_pair: null argument");
+  if (int rc = check_offsets({d_off, d_off1}, "rowmax_open_pair")) return rc;
   if (int rc = check_words({d_c[0], d_c[1], d_xhat}, "rowmax_open_pair")) return rc;
   if (int rc = attn_check_ctx(ctx)) return rc;
   const Shape s = shape_for(ctx, rows, max_width);
@@ -158,6 +165,7 @@ int sufb200_rowmax_round_pair(sufb200_ctx ctx, const uint64_t* const* d_c, const
   if (int rc = check_rows(rows, max_width, "rowmax_round_pair")) return rc;
   if (rows == 0 || max_width == 0) return SUFB200_OK;
   if (!d_c || !d_relu || !d_off || !d_off1 || !d_next) return fail(SUFB200_ERR_INVALID, "rowmax_round_pair: null argument");
+  if (int rc = check_offsets({d_off, d_off1, d_off2}, "rowmax_round_pair")) return rc;
   if (int rc = check_words({d_c[0], d_c[1], d_next[0], d_next[1]}, "rowmax_round_pair")) return rc;
   if (max_width > 1)
     if (int rc = check_words({d_relu[0], d_relu[1]}, "rowmax_round_pair")) return rc;
@@ -177,6 +185,7 @@ int sufb200_maxdiff_ragged_pair(sufb200_ctx ctx, const uint64_t* const* d_max, c
   if (int rc = check_rows(rows, max_width, "maxdiff_ragged_pair")) return rc;
   if (rows == 0 || max_width == 0) return SUFB200_OK;
   if (!d_max || !d_s || !d_t || !d_off || !d_max_off) return fail(SUFB200_ERR_INVALID, "maxdiff_ragged_pair: null argument");
+  if (int rc = check_offsets({d_off, d_max_off}, "maxdiff_ragged_pair")) return rc;
   if (int rc = check_words({d_max[0], d_max[1], d_s[0], d_s[1], d_t[0], d_t[1]}, "maxdiff_ragged_pair")) return rc;
   if (int rc = attn_check_ctx(ctx)) return rc;
   const Shape s = shape_for(ctx, rows, max_width);

@@ -638,3 +638,26 @@ def test_pages_take_fresh_masks_before_they_are_written_again():
     cache.fresh_masks([2])
     assert (pools[1][2] != first).all()
     cache.fresh_masks([])
+
+
+def test_misaligned_index_arrays_are_refused(host):
+    """An array of 4- or 8-byte entries at an odd address would fault the GPU."""
+    from suf_b200 import _lib
+
+    L, r, g = _lib.lib(), (C.c_uint64 * 2)(1, 2), _arr(P16, P16)
+    P2 = 0x10002
+    for which in ("scores", "values"):
+        for kw in [dict(d_cu_q=P2), dict(d_cu_ctx=P2), dict(d_block_table=P2), dict(d_row_base=P4),
+                   dict(d_tiles=P2, n_tiles=1), dict(d_plane_keys=P2, plane_keys=128)]:
+            assert _attn(host, which, _seqs(**{**PTRS, **kw})) == _lib.ERR_INVALID, kw
+            assert b"misaligned sequence" in L.sufb200_last_error()
+    for kw in [dict(d_slots=P4), dict(d_positions=P2), dict(d_cos=P2), dict(d_sin=P2)]:
+        assert L.sufb200_rope_append_pair(host, C.byref(_rope(**kw)), None) == _lib.ERR_INVALID, kw
+        assert b"misaligned" in L.sufb200_last_error()
+    for a, b, c in [(P2, P16, P16), (P16, P2, P16), (P16, P16, P2)]:
+        assert L.sufb200_rowmax_round_pair(host, g, g, 4, 9, a, b, c, r, g, P16, None) == _lib.ERR_INVALID
+        if c == P16:
+            assert L.sufb200_rowmax_open_pair(host, g, 4, 9, a, b, r, P16, None) == _lib.ERR_INVALID
+            assert L.sufb200_maxdiff_ragged_pair(host, g, g, 4, 9, a, b, g, None) == _lib.ERR_INVALID
+        assert b"misaligned offsets" in L.sufb200_last_error()
+    assert _attn(host, "scores", _seqs(**{**PTRS, "d_cu_q": P4})) == _lib.ERR_UNSUPPORTED  # four bytes will do
