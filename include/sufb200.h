@@ -740,7 +740,8 @@ int sufb200_beaver_open_pair(const uint64_t* const* d_x, size_t sx, int ldx, con
  * of it is written, its row of d_dq neither.  The slots of a call are
  * distinct.  Shares of (t, h, d) at base + t * ts + h * hs + d.  q_heads = 0
  * appends only (d_q, d_a, d_dq may be NULL); rot_dim = 0 rotates nothing
- * (positions, tables and bundle unused).  Asynchronous; one launch. */
+ * (positions, tables and bundle unused).  Asynchronous; one launch, two and a
+ * table from the context's pool from 2^19 turned words on. */
 typedef struct sufb200_rope_append {
   const uint64_t* d_q[2];
   const uint64_t* d_k[2];
@@ -776,7 +777,7 @@ int sufb200_rope_append_pair(sufb200_ctx ctx, const sufb200_rope_append* args, v
  * and packed are the sums of the new tokens, the cached tokens and the words.  At most 2^26 cached tokens in a sequence,
  * 65,535 (sequence, key head) pairs and 2^20 rows (queries of its heads) per
  * pair. */
-#define SUFB200_ATTN_FEW_ROWS 8  /* rows of a (sequence, key head) up to which it counts as short */
+#define SUFB200_ATTN_FEW_ROWS 8  /* rows of a (sequence, key head) up to which it counts as short (callers' lists are made by it: fixed) */
 #define SUFB200_ATTN_ROW_TILE 64 /* rows of a row tile */
 #define SUFB200_ATTN_KEY_TILE 128 /* cached tokens of a key tile */
 typedef struct sufb200_attn_seqs {

@@ -23,7 +23,8 @@
 //
 // What bounds them (packed prompts of 2,048, 700 behind 1,024 and one token, 16
 // / 4 heads of 128; 49 M scores): a step's MMAs alone take 1,170 - 1,210 cycles,
-// 211 us in all, with the clock near 1.65 - 1.8 GHz under them.  The scores take
+// 211 us in all, with the clock near 1.65 - 1.8 GHz under them.  On one set of
+// inputs (548 and 487 us with inputs that change from pass to pass) the scores take
 // 490 us: without their 24 bytes of C and output a score 411 us, without the
 // keys' copies too 410 us; the MMAs alone, one tile in tensor memory at a time, take
 // 1,530 cycles a step, a CTA's set-up and rows' planes 11 of its 90 us.  The values
@@ -794,7 +795,9 @@ cudaError_t launch_scores_tc(const sufb200_ctx_s* ctx, const AttnSeqs& s, const 
   const int64_t bytes = a.tiles * s.kv_heads * a.chunks * 2 * static_cast<int64_t>(kAStage);
   cudaError_t e = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&a.planes), bytes, ctx->pool, st);
   if (e != cudaSuccess) return e;
-  // key tiles per CTA: long runs reuse the rows' planes and hide the epilogue
+  // key tiles per CTA, by the longest of these sequences' own contexts (by the
+  // batch's, 64 tokens behind 4,096 beside a single one with 65,536 cached, 32 / 8
+  // heads, took 717 us, 457 now; the values 703 and 449): long runs reuse the rows' planes and hide the epilogue
   // behind the next tile; two CTAs an SM in all even out, more cost more set-ups
   // (16 / 4 heads of 128, 1,024 tokens: 112 us, 141 by four an SM; 256 behind
   // 4,096: 192 and 224 us; 64 behind 8,000, 32 / 8 heads: 214 and 259 us)
