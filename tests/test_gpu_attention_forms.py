@@ -2,7 +2,9 @@
 definition in 64-bit words (tolerance zero): several key tiles a CTA, whole
 rows of values of more than eight chunks, ranges cut at the exact depth, and
 short sequences beside them.  Which form a case takes follows from the launch
-rule restated here, and every case says which one it is for."""
+rule restated here, and every case says which one it is for.  Then workspaces and
+bounds of mixed batches, appends and row maxima past one grid, and the block's
+rows with one key or none."""
 from __future__ import annotations
 
 import numpy as np
